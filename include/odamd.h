@@ -365,6 +365,93 @@ int odamd_adam_ema_step(float* param, const float* grad, float* exp_avg, float* 
                         double ema_decay, double grad_scale, void* stream);
 int odamd_ema_update(float* ema, const float* src, size_t n, double decay, void* stream);
 
+/* odamd_adam_ema_step over ranges of the buffers: elements [offset, offset + len) of each, nothing between them is read or
+ * written.  The table is a HOST array and is read before the call returns. */
+typedef struct {
+    long long offset; /* >= 0 */
+    long long len;    /* 1 .. 2^31 - 1025 */
+} odamd_range;
+int odamd_adam_ema_ranges_step(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, float* ema,
+                               const odamd_range* ranges_host, int n_ranges, double lr, double beta1, double beta2, double eps,
+                               double weight_decay, int step, double ema_decay, double grad_scale, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Matrix operators (no counterpart in the reference).
+ *
+ * Orthogonalisation by Newton-Schulz products.  x: (batch, rows, cols), contiguous, `dtype`; out: the same shape and type,
+ * may be x itself.  Per matrix G:
+ *   X = G / (|G|_F + eps), transposed while rows > cols;
+ *   `steps` times (1 .. 32):  A = X X^T,  X = a X + (b A + c A A) X,  (a, b, c) = (3.4445, -4.7750, 2.0315);
+ *   out = X, transposed back.
+ * Products carry 22 bits per factor and sum in float32, whatever dtype is; out is rounded once.  A matrix that holds a NaN
+ * or an infinity gives NaN throughout, a zero matrix zeros.  Values of X under 2^-36 count as zero: a matrix whose norm lies
+ * far under eps comes out as zero.  rows * cols < 2^31.  The workspace is 256-byte aligned. */
+size_t odamd_orthogonalize_workspace_bytes(int batch, int rows, int cols);
+int odamd_orthogonalize(const void* x, void* out, int batch, int rows, int cols, int steps, double eps, int dtype,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* Optimizer step with orthogonalised momentum over matrices of flat float32 buffers (the layout of odamd_adam_ema_step).
+ * For each matrix of the HOST array (read before the call returns), rows x cols row-major from element `offset` on:
+ *   m = momentum_decay m + grad_scale g;   u = nesterov ? grad_scale g + momentum_decay m : m;
+ *   p = p (1 - lr weight_decay) - lr 0.2 sqrt(max(rows, cols)) O,   O = u orthogonalised as above;
+ *   ema = ema_decay ema + (1 - ema_decay) p   where ema != NULL.
+ * 0.2 sqrt(max(rows, cols)) gives the update the root mean square of an Adam step, so that one learning rate and one weight
+ * decay serve both.  Elements outside the matrices are neither read nor written; matrices must not overlap.  The workspace
+ * is 256-byte aligned. */
+typedef struct {
+    long long offset; /* >= 0 */
+    int rows, cols;   /* rows * cols < 2^31 */
+} odamd_matrix;
+size_t odamd_muon_workspace_bytes(const odamd_matrix* matrices_host, int n_matrices);
+int odamd_muon_ema_step(float* param, const float* grad, float* momentum, float* ema, const odamd_matrix* matrices_host,
+                        int n_matrices, double lr, double momentum_decay, int nesterov, double weight_decay, int steps,
+                        double eps, double ema_decay, double grad_scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Dense layer with its epilogue in one product: y = act(x W^T + b) + r.  x: m rows of k values, x_ld elements apart; w: n rows
+ * of k; bias: n values or NULL; residual, y, z: m rows of n.  All of them of `dtype`, rows contiguous, row strides in elements
+ * and at least the row's length.  z != NULL also receives x W^T + b, which the backward pass of an activation needs.  r may be
+ * y itself; no other operand may overlap an output.  Sums are float32 and y is rounded once; float32 products carry 22 bits
+ * of each value, counted from the largest magnitude of its row of x or w down to 2^-17 of it and with the same absolute
+ * step below.  A float32 row that holds an infinity gives NaN or infinity.
+ * The workspace (256-byte aligned) may be NULL where the query returns 0. */
+#define ODAMD_ACT_NONE 0
+#define ODAMD_ACT_SILU 1
+#define ODAMD_ACT_GELU 2 /* z (1 + erf(z / sqrt 2)) / 2 */
+#define ODAMD_ACT_RELU 3
+typedef struct {
+    const void* x;
+    const void* w;
+    const void* bias;
+    const void* residual;
+    void* y;
+    void* z;
+    long long x_ld, w_ld, r_ld, y_ld, z_ld;
+    int m, k, n;
+    int act;   /* ODAMD_ACT_* */
+    int dtype; /* ODAMD_DTYPE_* */
+} odamd_linear_desc;
+size_t odamd_linear_workspace_bytes(const odamd_linear_desc* d);
+int odamd_linear_forward(const odamd_linear_desc* d, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its backward pass: dz = dy act'(z);  dx = dz W (m x k),  dw = dz^T x (n x k),  db = column sums of dz (n values).  Outputs that
+ * are NULL are not computed; w is needed for dx only, x for dw only, z with an activation only.  dz is rounded to `dtype`
+ * between the two products (bfloat16: as an activation gradient in memory would be); db is summed before that rounding. */
+typedef struct {
+    const void* dy;
+    const void* z;
+    const void* x;
+    const void* w;
+    void* dx;
+    void* dw;
+    void* db;
+    long long dy_ld, z_ld, x_ld, w_ld, dx_ld, dw_ld;
+    int m, k, n;
+    int act;
+    int dtype;
+} odamd_linear_grad_desc;
+size_t odamd_linear_backward_workspace_bytes(const odamd_linear_grad_desc* d);
+int odamd_linear_backward(const odamd_linear_grad_desc* d, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Packs master float32 weights into the kernels' layouts for every convolution at once.
  * table_dev: device array of n_entries descriptors of odamd_pack_desc_bytes() bytes each:
  *   { const float* w; void* fwd; void* bwd; int cout, cin, k, cin_phys, cout_phys, n_seg;

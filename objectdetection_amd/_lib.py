@@ -46,6 +46,20 @@ class PackDesc(C.Structure):
                 ('seg_len', c_int * 8), ('fwd_f32', c_int), ('fwd_frag', c_int), ('bwd_frag', c_int), ('reserved', c_int)]
 
 
+class LinearDesc(C.Structure):
+    """odamd_linear_desc"""
+    _fields_ = [(n, c_void_p) for n in ('x', 'w', 'bias', 'residual', 'y', 'z')] + \
+               [(n, C.c_longlong) for n in ('x_ld', 'w_ld', 'r_ld', 'y_ld', 'z_ld')] + \
+               [(n, c_int) for n in ('m', 'k', 'n', 'act', 'dtype')]
+
+
+class LinearGradDesc(C.Structure):
+    """odamd_linear_grad_desc"""
+    _fields_ = [(n, c_void_p) for n in ('dy', 'z', 'x', 'w', 'dx', 'dw', 'db')] + \
+               [(n, C.c_longlong) for n in ('dy_ld', 'z_ld', 'x_ld', 'w_ld', 'dx_ld', 'dw_ld')] + \
+               [(n, c_int) for n in ('m', 'k', 'n', 'act', 'dtype')]
+
+
 # name -> (restype, argtypes); every symbol include/odamd.h declares must appear here.
 SIGNATURES = {
     'odamd_abi_version': (c_int, []),
@@ -112,6 +126,18 @@ SIGNATURES = {
     'odamd_adam_ema_step': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, C.c_double, C.c_double,
                                     C.c_double, C.c_double, C.c_double, c_int, C.c_double, C.c_double, c_void_p]),
     'odamd_ema_update': (c_int, [c_void_p, c_void_p, c_size_t, C.c_double, c_void_p]),
+    'odamd_adam_ema_ranges_step': (c_int, [c_void_p] * 6 + [c_int] + [C.c_double] * 5 + [c_int, C.c_double, C.c_double,
+                                                                                          c_void_p]),
+    'odamd_orthogonalize_workspace_bytes': (c_size_t, [c_int] * 3),
+    'odamd_orthogonalize': (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, C.c_double, c_int, c_void_p, c_size_t,
+                                    c_void_p]),
+    'odamd_muon_workspace_bytes': (c_size_t, [c_void_p, c_int]),
+    'odamd_muon_ema_step': (c_int, [c_void_p] * 5 + [c_int, C.c_double, C.c_double, c_int, C.c_double, c_int, C.c_double,
+                                                     C.c_double, C.c_double, c_void_p, c_size_t, c_void_p]),
+    'odamd_linear_workspace_bytes': (c_size_t, [C.POINTER(LinearDesc)]),
+    'odamd_linear_forward': (c_int, [C.POINTER(LinearDesc), c_void_p, c_size_t, c_void_p]),
+    'odamd_linear_backward_workspace_bytes': (c_size_t, [C.POINTER(LinearGradDesc)]),
+    'odamd_linear_backward': (c_int, [C.POINTER(LinearGradDesc), c_void_p, c_size_t, c_void_p]),
     'odamd_pack_weights': (c_int, [c_void_p, c_int, c_int, c_void_p]),
     'odamd_pack_desc_bytes': (c_size_t, []),
     'odamd_nchw_to_nhwc': (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),

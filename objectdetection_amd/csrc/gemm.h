@@ -1,0 +1,217 @@
+// Matrix product core of the dense layer and of the Newton-Schulz products: C[m][n] = sum_k A[m][k] B[n][k], both operands
+// with the reduction contiguous.  Included by linear.hip and orthogonalize.hip inside their anonymous namespaces.
+//
+// Two operand forms, one data path:
+//   PL = 1: bf16 values, one v_mfma_f32_32x32x16_bf16 per 32 x 32 x 16 block;
+//   PL = 2: every value as a pair of fp16 numbers, v = (hi + lo) 2^-s; 32 hi and then their 32 lo lie side by side.  hi holds the upper 11 bits of v, lo the
+//           next 11, so hi_a hi_b + hi_a lo_b + lo_a hi_b (three v_mfma_f32_32x32x16_f16) carries a product to 2^-22, the
+//           dropped lo_a lo_b.  Float32 operands run at a third of the half-precision matrix rate this way, which is five
+//           times the rate of the float32 matrix instructions; 2^s is a power of two, so it costs no rounding.  fp16
+//           has no more exponents than its scale gives it: the caller's scale keeps the largest value under 65504, and the
+//           smallest step, 2^-24, lies 2^-39 or less under it.
+//
+// A workgroup holds a TM x TN tile of C in registers (WGM x WGN waves) and walks K in chunks of 128 bytes per row (64
+// bf16 values, or 32 pairs).  A chunk of A and B goes global -> LDS without passing registers
+// (global_load_lds_dwordx4), into the buffer that the chunk before the last one left; one barrier per chunk.  An LDS row is
+// eight 16-byte pieces; piece p of row r lies in slot p ^ (r & 7), so the eight lanes that read the same piece of eight
+// consecutive rows touch eight different slots.  The DMA writes LDS in lane order: the exchange of the slots is in the global
+// address each lane reads.
+#ifndef ODAMD_GEMM_H
+#define ODAMD_GEMM_H
+
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16v8_t;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+
+__device__ __attribute__((aligned(16))) const unsigned char g_gemm_zero[16] = {};   // 16 bytes of zeros: the source of pieces past the end of K
+
+__device__ __forceinline__ void gemm_dma16(const char* g, char* l) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                     (__attribute__((address_space(3))) void*)l, 16, 0, 0);
+}
+
+// Blocks that run on one XCD (block index modulo 8) take neighbouring tiles: they share operand rows in that XCD's L2.
+__device__ __forceinline__ int gemm_xcd_remap(int bid, int n) {
+    const int q = n >> 3, r = n & 7, xcd = bid & 7, slot = bid >> 3;
+    return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + slot;
+}
+
+// Tile `t` of an mt x nt grid, walked in bands of 8 tile rows: the tiles in flight share 8 row blocks of A and few of B.
+__device__ __forceinline__ void gemm_tile_at(int t, int mt, int nt, int& ti, int& tj) {
+    const int band = t / (8 * nt), left = t - band * 8 * nt;
+    const int rows = min(8, mt - band * 8);
+    tj = left / rows;
+    ti = band * 8 + left - tj * rows;
+}
+
+// Tile `t` of the upper triangle (ti <= tj) of an nt x nt grid, column by column.
+__device__ __forceinline__ void gemm_triangle_at(int t, int& ti, int& tj) {
+    int j = (int)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
+    while ((j + 1) * (j + 2) / 2 <= t) ++j;
+    while (j * (j + 1) / 2 > t) --j;
+    tj = j;
+    ti = t - j * (j + 1) / 2;
+}
+
+struct GemmOperand {
+    const char* p;     // row 0 of the operand
+    long long ld;      // bytes per row, a multiple of 16
+    int rows;          // rows past the last one are read as the last one; their results are not stored
+};
+
+template <int PL, bool F16>
+__device__ __forceinline__ f32x16_t gemm_mma(u32x4 a, u32x4 b, f32x16_t c) {
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16v8_t, a), __builtin_bit_cast(bf16v8_t, b), c, 0, 0, 0);
+}
+
+template <int PL_, bool F16_, int TM_, int TN_, int WGM_, int WGN_>
+struct GemmTile {
+    static constexpr int PL = PL_, TM = TM_, TN = TN_, WGM = WGM_, WGN = WGN_;
+    static constexpr bool F16 = F16_;
+    static constexpr int NW = WGM * WGN, THREADS = 64 * NW;
+    static constexpr int WTM = TM / WGM, WTN = TN / WGN, FM = WTM / 32, FN = WTN / 32;
+    static constexpr int BK = PL == 1 ? 64 : 32;                    // values of K per chunk
+    static constexpr int BUF = (TM + TN) * 128;                     // bytes of one LDS buffer
+    static constexpr int SLAB_LD = WTN + 4;                         // floats per row of a wave's epilogue slab
+    static constexpr int SLAB = 32 * SLAB_LD * 4;
+    static constexpr int LDS = 2 * BUF > NW * SLAB ? 2 * BUF : NW * SLAB;
+    static constexpr int NI = (TM + TN) / 8 / NW;                   // DMA instructions per wave and chunk
+    static_assert((TM + TN) % (8 * NW) == 0 && TM % 8 == 0, "whole DMA instructions");
+
+    f32x16_t acc[FM][FN];
+
+    // Chunks [c0, c1) of K into acc.  k_len: values of K (PL = 1: a multiple of 8, pieces past it are read as zeros; PL = 2:
+    // the rows are padded to whole chunks).
+    __device__ __forceinline__ void run(const GemmOperand& a, const GemmOperand& b, int m0, int n0, int c0, int c1, int k_len,
+                                        char* lds) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wm = wave / WGN, wn = wave % WGN, r = lane & 31, h = lane >> 5;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+
+        const char* src[NI];
+        const int piece = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            const int row8 = (wave + j * NW) * 8;                   // wave uniform: A and B instructions do not mix
+            const bool is_a = row8 < TM;
+            const int row = is_a ? m0 + row8 + (lane >> 3) : n0 + row8 - TM + (lane >> 3);
+            const GemmOperand& o = is_a ? a : b;
+            src[j] = o.p + (long long)min(row, o.rows - 1) * o.ld + piece * 16;
+        }
+        auto issue = [&](int c, char* buf) {
+            const long long at = (long long)c * 128;
+            if (PL == 2 || (c + 1) * BK <= k_len) {
+#pragma unroll
+                for (int j = 0; j < NI; ++j) gemm_dma16(src[j] + at, buf + (wave + j * NW) * 1024);
+            } else {
+                const bool in = c * BK + piece * 8 < k_len;
+#pragma unroll
+                for (int j = 0; j < NI; ++j) gemm_dma16(in ? src[j] + at : (const char*)g_gemm_zero, buf + (wave + j * NW) * 1024);
+            }
+        };
+        if (c0 >= c1) return;
+        issue(c0, lds);
+        const int a_off = (wm * WTM + r) * 128, b_off = TM * 128 + (wn * WTN + r) * 128, sw = r & 7;
+        for (int c = c0; c < c1; ++c) {
+            char* buf = lds + ((c - c0) & 1) * BUF;
+            // every wave's pieces of chunk c are in LDS, every read of the other buffer has returned
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            if (c + 1 < c1) issue(c + 1, lds + ((c - c0 + 1) & 1) * BUF);
+#pragma unroll
+            for (int s = 0; s < BK / 16; ++s) {
+                u32x4 fa[PL][FM], fb[PL][FN];
+#pragma unroll
+                for (int q = 0; q < PL; ++q) {
+                    const int slot = ((4 * q + 2 * s + h) ^ sw) * 16;
+#pragma unroll
+                    for (int i = 0; i < FM; ++i) fa[q][i] = *(const u32x4*)(buf + a_off + i * 4096 + slot);
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) fb[q][j] = *(const u32x4*)(buf + b_off + j * 4096 + slot);
+                }
+                // B is the instruction's row operand: a lane then holds one row m of C and runs of four columns n
+#pragma unroll
+                for (int q = 0; q < (PL == 1 ? 1 : 3); ++q)
+#pragma unroll
+                    for (int i = 0; i < FM; ++i)
+#pragma unroll
+                        for (int j = 0; j < FN; ++j)
+                            acc[i][j] = gemm_mma<PL, F16>(fb[q == 1 ? PL - 1 : 0][j], fa[q == 2 ? PL - 1 : 0][i], acc[i][j]);
+            }
+        }
+    }
+
+    // Hands the tile out in runs of eight: rows(m, n, v[8]) for C[m][n .. n+7], cols(m, n, v[8]) for C[m .. m+7][n]
+    // (m, n relative to the tile).  Every wave passes 32 rows at a time through a slab of LDS of its own.
+    template <bool ROWS, bool COLS, typename FR, typename FC>
+    __device__ __forceinline__ void hand_out(char* lds, FR&& rows, FC&& cols) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wm = wave / WGN, wn = wave % WGN, r = lane & 31, h = lane >> 5;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();                               // every wave has read its last fragments
+        float* slab = (float*)(lds + wave * SLAB);
+        constexpr int LPR = WTN / 8, RPP = 64 / LPR;                // lanes per row, rows per pass
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *(f32x4_t*)(slab + r * SLAB_LD + j * 32 + q * 8 + h * 4) =
+                        f32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if constexpr (ROWS) {
+#pragma unroll
+                for (int p = 0; p < 32 / RPP; ++p) {
+                    const int row = p * RPP + lane / LPR, col = (lane % LPR) * 8;
+                    const f32x4_t u = *(const f32x4_t*)(slab + row * SLAB_LD + col), w = *(const f32x4_t*)(slab + row * SLAB_LD + col + 4);
+                    float v[8] = {u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]};
+                    rows(wm * WTM + i * 32 + row, wn * WTN + col, v);
+                }
+            }
+            if constexpr (COLS) {
+#pragma unroll
+                for (int p = 0; p < 4 * WTN / 64; ++p) {
+                    const int n = (p * 64 + lane) % WTN, g = (p * 64 + lane) / WTN;
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = slab[(g * 8 + e) * SLAB_LD + n];
+                    cols(wm * WTM + i * 32 + g * 8, wn * WTN + n, v);
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    }
+};
+
+// v (already scaled) as a pair of fp16 numbers.  A value that is no number, or beyond fp16, keeps that in hi alone.
+__device__ __forceinline__ void split_f16(float v, _Float16& hi, _Float16& lo) {
+    hi = (_Float16)v;
+    const float rest = v - (float)hi;
+    lo = fabsf(v) < 65504.0f ? (_Float16)rest : (_Float16)0.0f;
+}
+// Byte of value k's hi within its row; its lo lies 64 bytes on.
+__device__ __forceinline__ int split_at(int k) { return (k >> 5) * 128 + (k & 31) * 2; }
+// Eight of them, from a multiple of eight on.
+__device__ __forceinline__ void store_split8(char* hi_at, const float v[8], float scale) {
+    f16x8_t hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        _Float16 a, b;
+        split_f16(v[e] * scale, a, b);
+        hi[e] = a;
+        lo[e] = b;
+    }
+    *(f16x8_t*)hi_at = hi;
+    *(f16x8_t*)(hi_at + 64) = lo;
+}
+
+#endif

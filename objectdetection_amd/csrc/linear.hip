@@ -1,0 +1,661 @@
+// Dense layer: y = act(x W^T + b) + r, and its backward pass.
+//
+//   dz = dy act'(z),  z = x W^T + b;   dx = dz W,   dW = dz^T x,   db = column sums of dz   (dr = dy, the caller's own)
+// bfloat16 operands run on bf16 matrix instructions as they are; float32 operands as fp16 pairs (gemm.h) with a power of
+// two per row of each operand, so that a row's largest value sits just under 2^15: 22 bits per value down to 2^-17 of the row's
+// largest, and the same absolute step below.  Sums are float32, z and dz are kept in the operands' type.
+// Every product reduces along the contiguous axis of both operands: the backward pass lays W, x and dz out by columns
+// first (one launch for all three), because dx reduces over the outputs and dW over the rows.
+#include "common.h"
+#include "odamd.h"
+
+namespace {
+
+#include "gemm.h"
+
+template <int DT> struct LinType;
+template <> struct LinType<ODAMD_DTYPE_F32> {
+    using T = float;
+    static constexpr int PL = 2;
+    static __device__ __forceinline__ float get(T v) { return v; }
+    static __device__ __forceinline__ T put(float v) { return v; }
+};
+template <> struct LinType<ODAMD_DTYPE_BF16> {
+    using T = uint16_t;
+    static constexpr int PL = 1;
+    static __device__ __forceinline__ float get(T v) { return bf16_to_f32(v); }
+    static __device__ __forceinline__ T put(float v) { return f32_to_bf16(v); }
+};
+
+__host__ __device__ inline long long lin_up(long long v, int to) { return (v + to - 1) / to * to; }
+
+// The float32 forms go through expf / erff: their results are held to float32, not to bfloat16.
+__device__ __forceinline__ float lin_act(float z, int act) {
+    switch (act) {
+        case ODAMD_ACT_SILU: return z / (1.0f + expf(-z));
+        case ODAMD_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        case ODAMD_ACT_RELU: return z < 0.0f ? 0.0f : z;
+        default: return z;
+    }
+}
+__device__ __forceinline__ float lin_slope(float z, int act) {
+    switch (act) {
+        case ODAMD_ACT_SILU: {
+            const float p = 1.0f / (1.0f + expf(-z));
+            return p * (1.0f + z * (1.0f - p));
+        }
+        case ODAMD_ACT_GELU: return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+        case ODAMD_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+        default: return 1.0f;
+    }
+}
+
+// Power of two that brings a row whose largest finite magnitude has these bits just under 2^15
+__device__ __forceinline__ int lin_shift(unsigned max_bits) {
+    return max_bits ? 15 - __builtin_amdgcn_frexp_expf(__uint_as_float(max_bits)) : 0;
+}
+__device__ __forceinline__ unsigned lin_magnitude(float v) {
+    const unsigned b = __float_as_uint(v) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
+}
+
+// ---- what is done with a value of x W^T -----------------------------------------------------------------------------
+struct LinEnd {
+    const void* bias;
+    const void* residual;
+    void* y;
+    void* z;
+    long long r_ld, y_ld, z_ld;
+    int act;
+};
+
+template <int DT>
+__device__ __forceinline__ void lin_load8(const void* base, long long at, int cnt, float v[8]) {
+    using T = typename LinType<DT>::T;
+    const T* s = (const T*)base + at;
+    if (cnt == 8 && ((uintptr_t)s & 15) == 0) {
+        if constexpr (DT == ODAMD_DTYPE_F32) {
+            const f32x4_t a = *(const f32x4_t*)s, b = *(const f32x4_t*)(s + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[e + 4] = b[e]; }
+        } else {
+            const u32x4 a = *(const u32x4*)s;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { v[2 * e] = __uint_as_float(a[e] << 16); v[2 * e + 1] = __uint_as_float(a[e] & 0xffff0000u); }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < cnt ? LinType<DT>::get(s[e]) : 0.0f;
+    }
+}
+template <int DT>
+__device__ __forceinline__ void lin_store8(void* base, long long at, int cnt, const float v[8]) {
+    using T = typename LinType<DT>::T;
+    T* d = (T*)base + at;
+    if (cnt == 8 && ((uintptr_t)d & 15) == 0) {
+        if constexpr (DT == ODAMD_DTYPE_F32) {
+            *(f32x4_t*)d = f32x4_t{v[0], v[1], v[2], v[3]};
+            *(f32x4_t*)(d + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+        } else {
+            *(u32x4*)d = u32x4{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]), f32x2_to_bf16x2(v[4], v[5]), f32x2_to_bf16x2(v[6], v[7])};
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < cnt) d[e] = LinType<DT>::put(v[e]);
+    }
+}
+// Row i, columns j .. j + cnt - 1 (cnt <= 8)
+template <int DT>
+__device__ __forceinline__ void lin_finish8(const LinEnd& p, long long i, int j, int cnt, float v[8]) {
+    if (p.bias) {
+        float b[8];
+        lin_load8<DT>(p.bias, j, cnt, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += b[e];
+    }
+    if (p.z) lin_store8<DT>(p.z, i * p.z_ld + j, cnt, v);
+    if (p.act != ODAMD_ACT_NONE) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = lin_act(v[e], p.act);
+    }
+    if (p.residual) {
+        float r[8];
+        lin_load8<DT>(p.residual, i * p.r_ld + j, cnt, r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += r[e];
+    }
+    lin_store8<DT>(p.y, i * p.y_ld + j, cnt, v);
+}
+
+// ---- a few rows: one wave per output column, W read once from memory, no matrix instructions ------------------------
+struct LinRow {
+    const void* x;
+    const void* w;
+    long long x_ld, w_ld;
+    int m, k, n;
+    LinEnd end;
+};
+template <int DT, int MR, bool WIDE>
+__global__ void __launch_bounds__(256) linear_rows_kernel(LinRow p) {
+    using T = typename LinType<DT>::T;
+    constexpr int V = WIDE ? 16 / (int)sizeof(T) : 1;
+    const int lane = threadIdx.x & 63, col = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (col >= p.n) return;
+    const T* w = (const T*)p.w + col * p.w_ld;
+    const T* x = (const T*)p.x;
+    float acc[MR];
+#pragma unroll
+    for (int i = 0; i < MR; ++i) acc[i] = 0.0f;
+    for (int k = lane * V; k < p.k; k += 64 * V) {
+        T wv[V];
+        if constexpr (WIDE) *(u32x4*)wv = *(const u32x4*)(w + k);
+        else wv[0] = w[k];
+#pragma unroll
+        for (int i = 0; i < MR; ++i) {
+            if (i >= p.m) break;
+            T xv[V];
+            if constexpr (WIDE) *(u32x4*)xv = *(const u32x4*)(x + i * p.x_ld + k);
+            else xv[0] = x[i * p.x_ld + k];
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[i] = fmaf(LinType<DT>::get(xv[e]), LinType<DT>::get(wv[e]), acc[i]);
+        }
+    }
+    float mine = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MR; ++i) {
+        float s = acc[i];
+#pragma unroll
+        for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+        mine = lane == i ? s : mine;
+    }
+    if (lane < p.m) {
+        float v[8] = {mine};
+        lin_finish8<DT>(p.end, lane, col, 1, v);
+    }
+}
+
+// ---- laying operands out ---------------------------------------------------------------------------------------------
+// One matrix (m x n) of the caller's, optionally dz = src act'(z): written by rows and / or by columns with the reduction
+// padded with zeros to whole chunks.
+struct LinJob {
+    const void* src;
+    const void* z;
+    long long ld, z_ld;
+    char* rows;            // [m][n padded]
+    char* cols;            // [n][m padded]
+    unsigned* row_max;     // float32: bits of each row's / column's largest magnitude
+    unsigned* col_max;
+    float* sums;           // [ceil(m / 64)][n] column sums
+    int m, n, act, tile0;
+};
+struct LinJobs { LinJob j[3]; int n; };
+
+__device__ __forceinline__ const LinJob& lin_job(const LinJobs& t, int block) {
+    int i = 0;
+    if (t.n > 1 && block >= t.j[1].tile0) i = 1;
+    if (t.n > 2 && block >= t.j[2].tile0) i = 2;
+    return t.j[i];
+}
+template <int DT>
+__device__ __forceinline__ float lin_value(const LinJob& p, int i, int j) {
+    using T = typename LinType<DT>::T;
+    if (i >= p.m || j >= p.n) return 0.0f;
+    float v = LinType<DT>::get(((const T*)p.src)[(long long)i * p.ld + j]);
+    if (p.z) v *= lin_slope(LinType<DT>::get(((const T*)p.z)[(long long)i * p.z_ld + j]), p.act);
+    return v;
+}
+
+__global__ void __launch_bounds__(256) linear_clear_kernel(unsigned* p, long long n) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) p[i] = 0u;
+}
+
+// Largest magnitudes of rows and columns.  The maximum does not depend on the order of its arguments, so the atomics leave
+// the same result every time.
+__global__ void __launch_bounds__(256) linear_max_kernel(LinJobs t) {
+    __shared__ unsigned best[4][64];
+    const LinJob& p = lin_job(t, blockIdx.x);
+    const int tile = blockIdx.x - p.tile0, nt = (p.n + 63) / 64, i0 = tile / nt * 64, j0 = tile % nt * 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    unsigned mine = 0;
+    for (int q = wave; q < 64; q += 4) {
+        unsigned b = lin_magnitude(lin_value<ODAMD_DTYPE_F32>(p, i0 + q, j0 + lane));
+        mine = b > mine ? b : mine;
+        if (p.row_max) {
+#pragma unroll
+            for (int o = 32; o; o >>= 1) {
+                const unsigned u = __shfl_xor(b, o);
+                b = u > b ? u : b;
+            }
+            if (lane == 0 && b && i0 + q < p.m) atomicMax(p.row_max + i0 + q, b);
+        }
+    }
+    best[wave][lane] = mine;
+    __syncthreads();
+    if (wave == 0 && j0 + lane < p.n) {
+#pragma unroll
+        for (int q = 1; q < 4; ++q) mine = best[q][lane] > mine ? best[q][lane] : mine;
+        if (p.col_max && mine) atomicMax(p.col_max + j0 + lane, mine);
+    }
+}
+
+// Eight values of row `at` from column k on, shifted by a power of two (float32 form only)
+template <int DT>
+__device__ __forceinline__ void lin_lay8(char* base, long long at, int padded, int k, const float v[8], int shift) {
+    if constexpr (DT == ODAMD_DTYPE_F32) {
+        float s[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = ldexpf(v[e], shift);
+        store_split8(base + at * padded * 4 + split_at(k), s, 1.0f);
+    } else {
+        *(u32x4*)(base + (at * padded + k) * 2) = u32x4{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]), f32x2_to_bf16x2(v[4], v[5]), f32x2_to_bf16x2(v[6], v[7])};
+    }
+}
+template <int DT> __host__ __device__ constexpr int lin_chunk() { return DT == ODAMD_DTYPE_F32 ? 32 : 64; }
+
+template <int DT>
+__global__ void __launch_bounds__(256) linear_lay_kernel(LinJobs t) {
+    __shared__ float tile[64][65];
+    const LinJob& p = lin_job(t, blockIdx.x);
+    const int at = blockIdx.x - p.tile0, nt = (p.n + 63) / 64, i0 = at / nt * 64, j0 = at % nt * 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int q = wave; q < 64; q += 4) tile[q][lane] = lin_value<DT>(p, i0 + q, j0 + lane);
+    __syncthreads();
+    if (p.sums && wave == 0 && j0 + lane < p.n) {
+        float s = 0.0f;
+        for (int q = 0; q < 64; ++q) s += tile[q][lane];
+        p.sums[(long long)(i0 / 64) * p.n + j0 + lane] = s;
+    }
+    const int np = (int)lin_up(p.n, lin_chunk<DT>()), mp = (int)lin_up(p.m, lin_chunk<DT>());
+    for (int q = threadIdx.x; q < 512; q += 256) {
+        float v[8];
+        const int r = q >> 3, c = (q & 7) * 8;
+        if (p.rows && i0 + r < p.m && j0 + c < np) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = tile[r][c + e];
+            lin_lay8<DT>(p.rows, i0 + r, np, j0 + c, v, DT == ODAMD_DTYPE_F32 ? lin_shift(p.row_max[i0 + r]) : 0);
+        }
+        if (p.cols && j0 + r < p.n && i0 + c < mp) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = tile[c + e][r];
+            lin_lay8<DT>(p.cols, j0 + r, mp, i0 + c, v, DT == ODAMD_DTYPE_F32 ? lin_shift(p.col_max[j0 + r]) : 0);
+        }
+    }
+}
+
+// By rows only, a wave per row: the row's largest magnitude first, then (out of the caches) its pairs.  bfloat16: a plain copy
+// to aligned, padded rows.
+template <int DT>
+__global__ void __launch_bounds__(256) linear_lay_rows_kernel(LinJobs t) {
+    const LinJob& p = lin_job(t, blockIdx.x);
+    const int row = (blockIdx.x - p.tile0) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (row >= p.m) return;
+    const long long at = (long long)row * p.ld;
+    int shift = 0;
+    if constexpr (DT == ODAMD_DTYPE_F32) {
+        unsigned b = 0;
+        for (int k = lane * 8; k < p.n; k += 512) {
+            float v[8];
+            lin_load8<DT>(p.src, at + k, min(8, p.n - k), v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { const unsigned u = lin_magnitude(v[e]); b = u > b ? u : b; }
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) { const unsigned u = __shfl_xor(b, o); b = u > b ? u : b; }
+        if (lane == 0) p.row_max[row] = b;
+        shift = lin_shift(b);
+    }
+    const int np = (int)lin_up(p.n, lin_chunk<DT>());
+    for (int k = lane * 8; k < np; k += 512) {
+        float v[8];
+        lin_load8<DT>(p.src, at + k, max(0, min(8, p.n - k)), v);
+        lin_lay8<DT>(p.rows, row, np, k, v, shift);
+    }
+}
+
+// ---- the products ----------------------------------------------------------------------------------------------------
+struct LinGemm {
+    GemmOperand a, b;
+    const unsigned* a_max;   // float32: the rows' largest magnitudes
+    const unsigned* b_max;
+    float* part;             // split reduction: [split][m][n]
+    int m, n, k_len, chunks, per, split;   // chunks of K, chunks per split part
+    LinEnd end;
+};
+
+template <typename TILE, int DT, bool PART>
+__global__ void __launch_bounds__(TILE::THREADS) linear_product_kernel(LinGemm p) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int mt = (p.m + TILE::TM - 1) / TILE::TM, nt = (p.n + TILE::TN - 1) / TILE::TN;
+    const int id = gemm_xcd_remap(blockIdx.x, gridDim.x);
+    const int part = PART ? id / (mt * nt) : 0;
+    int ti, tj;
+    gemm_tile_at(PART ? id - part * mt * nt : id, mt, nt, ti, tj);
+    const int i0 = ti * TILE::TM, j0 = tj * TILE::TN;
+    TILE tile;
+    tile.run(p.a, p.b, i0, j0, part * p.per, min(p.chunks, (part + 1) * p.per), p.k_len, lds);
+    auto rows = [&](int i, int j, float v[8]) {
+        i += i0;
+        j += j0;
+        if (i >= p.m || j >= p.n) return;
+        const int cnt = min(8, p.n - j);
+        if constexpr (DT == ODAMD_DTYPE_F32) {
+            const int s = lin_shift(p.a_max[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], -(s + lin_shift(p.b_max[min(j + e, p.n - 1)])));
+        }
+        if constexpr (PART) lin_store8<ODAMD_DTYPE_F32>(p.part, ((long long)part * p.m + i) * p.n + j, cnt, v);
+        else lin_finish8<DT>(p.end, i, j, cnt, v);
+    };
+    tile.template hand_out<true, false>(lds, rows, rows);
+}
+
+// Sums the parts of a split reduction in their order
+template <int DT>
+__global__ void __launch_bounds__(256) linear_join_kernel(LinGemm p) {
+    const int runs = (p.n + 7) / 8;
+    const long long total = (long long)p.m * runs;
+    for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total; q += (long long)gridDim.x * 256) {
+        const long long i = q / runs;
+        const int j = (int)(q - i * runs) * 8, cnt = min(8, p.n - j);
+        float v[8], u[8];
+        lin_load8<ODAMD_DTYPE_F32>(p.part, i * p.n + j, cnt, v);
+        for (int s = 1; s < p.split; ++s) {
+            lin_load8<ODAMD_DTYPE_F32>(p.part, ((long long)s * p.m + i) * p.n + j, cnt, u);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += u[e];
+        }
+        lin_finish8<DT>(p.end, i, j, cnt, v);
+    }
+}
+
+// db from the column sums of 64-row blocks
+template <int DT>
+__global__ void __launch_bounds__(256) linear_bias_grad_kernel(const float* sums, int blocks, int n, void* db) {
+    __shared__ double part[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = blockIdx.x * 64 + lane;
+    double s = 0.0;
+    if (j < n)
+        for (int b = wave; b < blocks; b += 4) s += sums[(long long)b * n + j];
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && j < n) ((typename LinType<DT>::T*)db)[j] = LinType<DT>::put((float)(part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane]));
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+// Workspace as one walk over its regions: with base 0 it measures, with the caller's base it hands out.
+struct LinSpace {
+    char* base;
+    long long at = 0;
+    char* take(long long bytes) {
+        char* p = base + at;
+        at += lin_up(bytes, 256);
+        return p;
+    }
+};
+
+struct LinPlan { int tile, split, per; };
+// The largest tile that still gives every compute unit one; where even 64 x 64 tiles leave units idle, the reduction is cut so
+// that about two workgroups per unit run, four chunks each at least.
+LinPlan lin_plan(int m, int n, int chunks) {
+    const auto tiles = [&](int t) { return ((long long)m + t - 1) / t * (((long long)n + t - 1) / t); };
+    if (tiles(256) >= 256) return {256, 1, chunks};
+    if (tiles(128) >= 256) return {128, 1, chunks};
+    const long long t = tiles(64);
+    int split = 1;
+    if (t < 256) split = (int)((511 + t) / t);
+    if (split > chunks / 4) split = chunks / 4;
+    if (split > 32) split = 32;
+    if (split < 1) split = 1;
+    const int per = (chunks + split - 1) / split;
+    return {64, (chunks + per - 1) / per, per};
+}
+
+template <typename TILE, int DT, bool PART>
+int lin_launch(const LinGemm& g, long long blocks, hipStream_t s) {
+    if (blocks > 0x7fffffffLL) return ODAMD_E_LIMIT;
+    const auto kernel = linear_product_kernel<TILE, DT, PART>;
+    const hipError_t e = odamd_ensure_lds((const void*)kernel, TILE::LDS);
+    if (e != hipSuccess) return (int)e;
+    kernel<<<(int)blocks, TILE::THREADS, TILE::LDS, s>>>(g);
+    return (int)hipGetLastError();
+}
+template <int DT>
+int lin_product(LinGemm g, LinSpace& ws, bool go, hipStream_t s) {
+    constexpr int PL = LinType<DT>::PL;
+    constexpr bool F16 = DT == ODAMD_DTYPE_F32;
+    g.chunks = (g.k_len + lin_chunk<DT>() - 1) / lin_chunk<DT>();
+    const LinPlan plan = lin_plan(g.m, g.n, g.chunks);
+    g.per = plan.per;
+    g.split = plan.split;
+    if (plan.split > 1) g.part = (float*)ws.take((long long)plan.split * g.m * g.n * 4);
+    if (!go) return 0;
+    const long long blocks = (((long long)g.m + plan.tile - 1) / plan.tile) * ((g.n + plan.tile - 1) / plan.tile) * plan.split;
+    if (plan.tile == 256) return lin_launch<GemmTile<PL, F16, 256, 256, 2, 4>, DT, false>(g, blocks, s);
+    if (plan.tile == 128) return lin_launch<GemmTile<PL, F16, 128, 128, 2, 2>, DT, false>(g, blocks, s);
+    if (plan.split == 1) return lin_launch<GemmTile<PL, F16, 64, 64, 2, 2>, DT, false>(g, blocks, s);
+    const int rc = lin_launch<GemmTile<PL, F16, 64, 64, 2, 2>, DT, true>(g, blocks, s);
+    if (rc != 0) return rc;
+    const long long runs = (long long)g.m * ((g.n + 7) / 8);
+    linear_join_kernel<DT><<<(int)((runs + 255) / 256 < 4096 ? (runs + 255) / 256 : 4096), 256, 0, s>>>(g);
+    return (int)hipGetLastError();
+}
+
+template <int DT> bool lin_direct(const void* p, long long ld, int k) {
+    return DT == ODAMD_DTYPE_BF16 && ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && k % 8 == 0;
+}
+int lin_tiles(LinJobs& t, int unit_rows) {   // blocks of a launch over the jobs: 64 x 64 tiles, or groups of rows
+    long long at = 0;
+    for (int i = 0; i < t.n; ++i) {
+        t.j[i].tile0 = (int)at;
+        at += unit_rows ? (t.j[i].m + unit_rows - 1) / unit_rows : (((long long)t.j[i].m + 63) / 64) * ((t.j[i].n + 63) / 64);
+    }
+    return at > 0x7fffffffLL ? -1 : (int)at;
+}
+
+constexpr int LIN_ROWS = 8;   // up to this many rows the layer is read once for all of them, without matrix instructions
+
+template <int DT>
+int lin_forward_rows(const odamd_linear_desc& d, const LinEnd& end, hipStream_t s) {
+    constexpr int V = DT == ODAMD_DTYPE_F32 ? 4 : 8;
+    const bool wide = (((uintptr_t)d.x | (uintptr_t)d.w) & 15) == 0 && d.x_ld % V == 0 && d.w_ld % V == 0 && d.k % V == 0;
+    const LinRow p = {d.x, d.w, d.x_ld, d.w_ld, d.m, d.k, d.n, end};
+    const int blocks = (d.n + 3) / 4;
+#define ODAMD_ROWS(MR) (wide ? linear_rows_kernel<DT, MR, true><<<blocks, 256, 0, s>>>(p) : linear_rows_kernel<DT, MR, false><<<blocks, 256, 0, s>>>(p))
+    if (d.m == 1) ODAMD_ROWS(1);
+    else if (d.m == 2) ODAMD_ROWS(2);
+    else if (d.m <= 4) ODAMD_ROWS(4);
+    else ODAMD_ROWS(8);
+#undef ODAMD_ROWS
+    return (int)hipGetLastError();
+}
+
+// go = false: measures the workspace only
+template <int DT>
+int lin_forward(const odamd_linear_desc& d, LinSpace& ws, bool go, hipStream_t s) {
+    const LinEnd end = {d.bias, d.residual, d.y, d.z, d.r_ld, d.y_ld, d.z_ld, d.act};
+    if (d.m <= LIN_ROWS) return go ? lin_forward_rows<DT>(d, end, s) : 0;
+    constexpr int SIZE = DT == ODAMD_DTYPE_F32 ? 4 : 2;
+    LinGemm g = {};
+    g.end = end;
+    g.m = d.m;
+    g.n = d.n;
+    g.k_len = d.k;
+    LinJobs jobs = {};
+    const long long kp = lin_up(d.k, lin_chunk<DT>());
+    const auto operand = [&](const void* p, long long ld, int rows, GemmOperand& o, const unsigned*& max) {
+        // where the caller's rows can be read as they are, no workspace is used; measuring, the pointers are not known to be
+        if (go && lin_direct<DT>(p, ld, d.k)) {
+            o = {(const char*)p, ld * SIZE, rows};
+            return;
+        }
+        LinJob& j = jobs.j[jobs.n++];
+        j.src = p;
+        j.ld = ld;
+        j.m = rows;
+        j.n = d.k;
+        j.rows = ws.take(rows * kp * SIZE);
+        j.row_max = DT == ODAMD_DTYPE_F32 ? (unsigned*)ws.take(rows * 4LL) : nullptr;
+        max = j.row_max;
+        o = {j.rows, kp * SIZE, rows};
+    };
+    operand(d.x, d.x_ld, d.m, g.a, g.a_max);
+    operand(d.w, d.w_ld, d.n, g.b, g.b_max);
+    // a laid out operand is padded to whole chunks, one read in place is not: the tail is then read as zeros for both
+    if (go && jobs.n) {
+        const int blocks = lin_tiles(jobs, 4);
+        linear_lay_rows_kernel<DT><<<blocks, 256, 0, s>>>(jobs);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return (int)e;
+    }
+    if (DT == ODAMD_DTYPE_BF16) g.k_len = (int)lin_up(d.k, 8);
+    return lin_product<DT>(g, ws, go, s);
+}
+
+template <int DT>
+int lin_backward(const odamd_linear_grad_desc& d, LinSpace& ws, bool go, hipStream_t s) {
+    constexpr int SIZE = DT == ODAMD_DTYPE_F32 ? 4 : 2;
+    constexpr bool F32 = DT == ODAMD_DTYPE_F32;
+    const bool act = d.act != ODAMD_ACT_NONE;
+    const long long mp = lin_up(d.m, lin_chunk<DT>()), np = lin_up(d.n, lin_chunk<DT>());
+    LinJobs jobs = {};
+    LinJob* z = nullptr;
+    LinGemm gx = {}, gw = {};
+    // the largest magnitudes of all operands lie side by side: one launch clears them
+    unsigned* maxes = nullptr;
+    const long long n_max = F32 ? (long long)d.m + d.n + 2LL * d.k : 0;
+    if (F32) maxes = (unsigned*)ws.take(n_max * 4);
+    unsigned *z_row = maxes, *z_col = F32 ? maxes + d.m : nullptr, *w_col = F32 ? z_col + d.n : nullptr, *x_col = F32 ? w_col + d.k : nullptr;
+
+    z = &jobs.j[jobs.n++];
+    z->src = d.dy;
+    z->ld = d.dy_ld;
+    z->z = act ? d.z : nullptr;
+    z->z_ld = d.z_ld;
+    z->act = d.act;
+    z->m = d.m;
+    z->n = d.n;
+    if (d.dx) {
+        if (go && !act && lin_direct<DT>(d.dy, d.dy_ld, d.n)) {
+            gx.a = {(const char*)d.dy, d.dy_ld * SIZE, d.m};
+        } else {
+            z->rows = ws.take(d.m * np * SIZE);
+            z->row_max = z_row;
+            gx.a = {z->rows, np * SIZE, d.m};
+        }
+        LinJob& w = jobs.j[jobs.n++];
+        w.src = d.w;
+        w.ld = d.w_ld;
+        w.m = d.n;
+        w.n = d.k;
+        w.cols = ws.take(d.k * np * SIZE);
+        w.col_max = w_col;
+        gx.b = {w.cols, np * SIZE, d.k};
+        gx.a_max = z_row;
+        gx.b_max = w_col;
+        gx.m = d.m;
+        gx.n = d.k;
+        gx.k_len = (int)(F32 ? d.n : lin_up(d.n, 8));
+        gx.end.y = d.dx;
+        gx.end.y_ld = d.dx_ld;
+    }
+    if (d.dw) {
+        z->cols = ws.take(d.n * mp * SIZE);
+        z->col_max = z_col;
+        LinJob& x = jobs.j[jobs.n++];
+        x.src = d.x;
+        x.ld = d.x_ld;
+        x.m = d.m;
+        x.n = d.k;
+        x.cols = ws.take(d.k * mp * SIZE);
+        x.col_max = x_col;
+        gw.a = {z->cols, mp * SIZE, d.n};
+        gw.b = {x.cols, mp * SIZE, d.k};
+        gw.a_max = z_col;
+        gw.b_max = x_col;
+        gw.m = d.n;
+        gw.n = d.k;
+        gw.k_len = (int)mp;
+        gw.end.y = d.dw;
+        gw.end.y_ld = d.dw_ld;
+    }
+    const int row_blocks = (d.m + 63) / 64;
+    if (d.db) z->sums = (float*)ws.take((long long)row_blocks * d.n * 4);
+    if (go) {
+        const int blocks = lin_tiles(jobs, 0);
+        if (blocks < 0) return ODAMD_E_LIMIT;
+        if (F32) {
+            linear_clear_kernel<<<(int)((n_max + 255) / 256 < 1024 ? (n_max + 255) / 256 : 1024), 256, 0, s>>>(maxes, n_max);
+            linear_max_kernel<<<blocks, 256, 0, s>>>(jobs);
+        }
+        linear_lay_kernel<DT><<<blocks, 256, 0, s>>>(jobs);
+        if (d.db) linear_bias_grad_kernel<DT><<<(d.n + 63) / 64, 256, 0, s>>>(z->sums, row_blocks, d.n, d.db);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return (int)e;
+    }
+    int rc = 0;
+    const long long mark = ws.at;
+    long long most = ws.at;
+    if (d.dx) rc = lin_product<DT>(gx, ws, go, s);
+    most = ws.at > most ? ws.at : most;
+    ws.at = mark;                               // both products may use the same room for their parts: they follow one another
+    if (rc == 0 && d.dw) rc = lin_product<DT>(gw, ws, go, s);
+    ws.at = ws.at > most ? ws.at : most;
+    return rc;
+}
+
+constexpr long long LIN_MAX = 0x7fffffffLL - 1024;
+bool lin_sizes_ok(int m, int k, int n, int act, int dtype) {
+    return m >= 1 && k >= 1 && n >= 1 && m <= LIN_MAX && k <= LIN_MAX && n <= LIN_MAX && act >= ODAMD_ACT_NONE && act <= ODAMD_ACT_RELU
+           && (dtype == ODAMD_DTYPE_F32 || dtype == ODAMD_DTYPE_BF16);
+}
+bool lin_aligned(const void* p, int dtype) { return ((uintptr_t)p & (dtype == ODAMD_DTYPE_F32 ? 3 : 1)) == 0; }
+
+}  // namespace
+
+extern "C" {
+
+size_t odamd_linear_workspace_bytes(const odamd_linear_desc* d) {
+    if (!d || !lin_sizes_ok(d->m, d->k, d->n, d->act, d->dtype)) return 0;
+    LinSpace ws = {nullptr};
+    if (d->dtype == ODAMD_DTYPE_F32) lin_forward<ODAMD_DTYPE_F32>(*d, ws, false, nullptr);
+    else lin_forward<ODAMD_DTYPE_BF16>(*d, ws, false, nullptr);
+    return (size_t)ws.at;
+}
+
+int odamd_linear_forward(const odamd_linear_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!d || !d->x || !d->w || !d->y || !lin_sizes_ok(d->m, d->k, d->n, d->act, d->dtype)) return ODAMD_E_ARG;
+    if (d->x_ld < d->k || d->w_ld < d->k || d->y_ld < d->n || (d->residual && d->r_ld < d->n) || (d->z && d->z_ld < d->n)) return ODAMD_E_SHAPE;
+    if (!lin_aligned(d->x, d->dtype) || !lin_aligned(d->w, d->dtype) || !lin_aligned(d->y, d->dtype) || !lin_aligned(d->bias, d->dtype)
+        || !lin_aligned(d->residual, d->dtype) || !lin_aligned(d->z, d->dtype) || ((uintptr_t)workspace & 255)) return ODAMD_E_ALIGN;
+    const size_t need = odamd_linear_workspace_bytes(d);
+    if (need && !workspace) return ODAMD_E_ARG;
+    if (workspace_bytes < need) return ODAMD_E_WORKSPACE;
+    LinSpace ws = {(char*)workspace};
+    return d->dtype == ODAMD_DTYPE_F32 ? lin_forward<ODAMD_DTYPE_F32>(*d, ws, true, (hipStream_t)stream)
+                                       : lin_forward<ODAMD_DTYPE_BF16>(*d, ws, true, (hipStream_t)stream);
+}
+
+size_t odamd_linear_backward_workspace_bytes(const odamd_linear_grad_desc* d) {
+    if (!d || !lin_sizes_ok(d->m, d->k, d->n, d->act, d->dtype)) return 0;
+    LinSpace ws = {nullptr};
+    if (d->dtype == ODAMD_DTYPE_F32) lin_backward<ODAMD_DTYPE_F32>(*d, ws, false, nullptr);
+    else lin_backward<ODAMD_DTYPE_BF16>(*d, ws, false, nullptr);
+    return (size_t)ws.at;
+}
+
+int odamd_linear_backward(const odamd_linear_grad_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!d || !d->dy || !workspace || !lin_sizes_ok(d->m, d->k, d->n, d->act, d->dtype)) return ODAMD_E_ARG;
+    if (!d->dx && !d->dw && !d->db) return ODAMD_E_ARG;
+    if ((d->act != ODAMD_ACT_NONE && !d->z) || (d->dx && !d->w) || (d->dw && !d->x)) return ODAMD_E_ARG;
+    if (d->dy_ld < d->n || (d->act != ODAMD_ACT_NONE && d->z_ld < d->n) || (d->dx && (d->w_ld < d->k || d->dx_ld < d->k))
+        || (d->dw && (d->x_ld < d->k || d->dw_ld < d->k))) return ODAMD_E_SHAPE;
+    if (!lin_aligned(d->dy, d->dtype) || !lin_aligned(d->z, d->dtype) || !lin_aligned(d->x, d->dtype) || !lin_aligned(d->w, d->dtype)
+        || !lin_aligned(d->dx, d->dtype) || !lin_aligned(d->dw, d->dtype) || !lin_aligned(d->db, d->dtype) || ((uintptr_t)workspace & 255)) return ODAMD_E_ALIGN;
+    if (workspace_bytes < odamd_linear_backward_workspace_bytes(d)) return ODAMD_E_WORKSPACE;
+    LinSpace ws = {(char*)workspace};
+    return d->dtype == ODAMD_DTYPE_F32 ? lin_backward<ODAMD_DTYPE_F32>(*d, ws, true, (hipStream_t)stream)
+                                       : lin_backward<ODAMD_DTYPE_BF16>(*d, ws, true, (hipStream_t)stream);
+}
+
+}  // extern "C"

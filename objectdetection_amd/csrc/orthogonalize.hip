@@ -1,0 +1,465 @@
+// Orthogonalisation of matrices by Newton-Schulz products, and the optimizer step built on it.
+//
+//   X_0 = G / (|G|_F + eps), transposed where G has more rows than columns (X is m x n, m <= n);
+//   per step   A = X X^T,   P = a I + b A + c A A,   X <- P X.
+// The odd polynomial a s + b s^3 + c s^5 acts on every singular value s of X and leaves the singular vectors: with
+// (a, b, c) = (3.4445, -4.7750, 2.0315) five steps take singular values from 0.003 up to between 0.68 and 1.21 -- the values
+// never pass 1.21, so every entry of X and A stays under 1.5 and of P under 3.5.
+//
+// All products run on fp16 pairs (gemm.h, PL = 2) scaled by 2^12: the largest entry becomes 14 300, the smallest step
+// 2^-36.  Rounding to pairs costs 2^-22 of an entry; small singular values are multiplied by up to 3.4445 a step, so anything
+// coarser shows: bf16 products would leave a few percent in the result.
+// X is kept twice, by rows (X X^T reduces along n) and by columns (P X reduces along m): both products then read their
+// operands along the reduction.  A and P are symmetric: the tiles on and over the diagonal are computed, the rest mirrored.
+#include "common.h"
+#include "odamd.h"
+
+#include <math.h>
+
+namespace {
+
+#include "gemm.h"
+
+constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
+constexpr float NS_SCALE = 4096.0f, NS_UNSCALE2 = 1.0f / (4096.0f * 4096.0f);
+constexpr int NS_GROUPS = 112;        // groups of one launch: their table travels in the kernel's arguments (4 KiB at most)
+constexpr int NS_PARTS = 256;         // partial sums of squares per matrix, at most
+
+enum { ST_NORM, ST_SPLIT, ST_A, ST_P, ST_X, ST_OUT };
+
+// `count` matrices of one shape, one after the other
+struct NsGroup {
+    long long src;       // first element of the first matrix in the caller's buffers
+    unsigned ws;         // start of the first one's workspace, in 256-byte units
+    int m, n;            // m <= n
+    int count;
+    int tile0;           // tiles of the groups before this one
+    int tall;            // the caller's matrix is n x m
+};
+struct NsTable {
+    NsGroup g[NS_GROUPS];
+    int n, tiles;
+    char* ws;
+};
+static_assert(sizeof(NsTable) <= 3800, "kernel arguments are limited to 4 KiB");
+
+__host__ __device__ inline long long ns_up(long long v, int to) { return (v + to - 1) / to * to; }
+// Byte offsets within a matrix's workspace; end is its size.
+struct NsLayout { long long sums, x, xt0, xt1, a, p, end; };
+__host__ __device__ inline NsLayout ns_layout(int m, int n) {
+    NsLayout l;
+    const long long mp = ns_up(m, 32), np = ns_up(n, 32);
+    l.sums = 0;
+    l.x = NS_PARTS * 8;
+    l.xt0 = l.x + ns_up(m * np * 4, 256);
+    l.xt1 = l.xt0 + ns_up(n * mp * 4, 256);
+    l.a = l.xt1 + ns_up(n * mp * 4, 256);
+    l.p = l.a + ns_up(m * mp * 4, 256);
+    l.end = l.p + ns_up(m * mp * 4, 256);
+    return l;
+}
+// Elements one workgroup of the norm pass takes: a multiple of four that keeps the partial sums within NS_PARTS.
+__host__ __device__ inline long long ns_share(int m, int n) {
+    const long long total = (long long)m * n, least = (total + NS_PARTS - 1) / NS_PARTS;
+    return least < 4096 ? 4096 : ns_up(least, 1024);
+}
+__host__ __device__ inline int ns_parts(int m, int n) { return (int)(((long long)m * n + ns_share(m, n) - 1) / ns_share(m, n)); }
+__host__ __device__ inline int ns_tiles(int stage, int tile, int m, int n) {
+    const int mt = (m + tile - 1) / tile, nt = (n + tile - 1) / tile;
+    return stage == ST_NORM ? ns_parts(m, n) : stage == ST_A || stage == ST_P ? mt * (mt + 1) / 2 : mt * nt;
+}
+
+// What the optimizer step works on (orthogonalisation alone: in and out)
+struct NsIo {
+    const void* in;      // caller's matrices (the gradient, for the optimizer step)
+    void* out;
+    float* param;
+    float* momentum;
+    float* ema;
+    float mu, grad_scale, decay, lr02, ema_keep, ema_take;   // decay: 1 - lr weight_decay, lr02: 0.2 lr
+    int nesterov;
+    double eps;
+};
+
+struct NsPlace { int m, n, tall, tile; long long src; char* ws; };
+
+// Which matrix a tile belongs to
+__device__ __forceinline__ NsPlace ns_find(const NsTable& t, int tile, int stage, int tile_size) {
+    int lo = 0, hi = t.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t.g[mid].tile0 <= tile) lo = mid; else hi = mid - 1;
+    }
+    const NsGroup& g = t.g[lo];
+    const int each = ns_tiles(stage, tile_size, g.m, g.n), at = tile - g.tile0, which = at / each;
+    return {g.m, g.n, g.tall, at - which * each, g.src + (long long)which * g.m * g.n,
+            t.ws + (long long)g.ws * 256 + which * ns_layout(g.m, g.n).end};
+}
+
+// The optimizer's direction from the updated momentum
+__device__ __forceinline__ float ns_direction(const NsIo& io, float g, float m) {
+    return io.nesterov ? g * io.grad_scale + io.mu * m : m;
+}
+
+__device__ __forceinline__ double ns_block_sum(double v, double* shared) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) shared[wave] = v;
+    __syncthreads();
+    double s = 0.0;
+    for (int i = 0; i < (int)(blockDim.x >> 6); ++i) s += shared[i];
+    return s;
+}
+
+// Sums of squares in double (gradients of 1e-20 and of 1e20 have a norm too), a fixed share of a matrix per workgroup and
+// summed in a fixed order: the result does not change from run to run.  The optimizer step's momentum update happens here.
+template <bool MUON, int DT>
+__global__ void __launch_bounds__(256) ns_norm_kernel(NsTable t, NsIo io) {
+    __shared__ double part[4];
+    const NsPlace p = ns_find(t, blockIdx.x, ST_NORM, 0);
+    const long long total = (long long)p.m * p.n, share = ns_share(p.m, p.n), from = p.tile * share;
+    const long long to = from + share < total ? from + share : total;
+    double s = 0.0;
+    auto one = [&](long long i) {
+        float v;
+        if constexpr (MUON) {
+            const float g = ((const float*)io.in)[p.src + i];
+            const float m = io.mu * io.momentum[p.src + i] + g * io.grad_scale;
+            io.momentum[p.src + i] = m;
+            v = ns_direction(io, g, m);
+        } else if constexpr (DT == ODAMD_DTYPE_BF16) {
+            v = bf16_to_f32(((const uint16_t*)io.in)[p.src + i]);
+        } else {
+            v = ((const float*)io.in)[p.src + i];
+        }
+        s += (double)v * v;
+    };
+    for (long long i = from + threadIdx.x; i < to; i += 256) one(i);
+    s = ns_block_sum(s, part);
+    if (threadIdx.x == 0) ((double*)p.ws)[p.tile] = s;
+}
+
+// X by rows and by columns as fp16 pairs, 64 x 64 elements per workgroup
+template <bool MUON, int DT>
+__global__ void __launch_bounds__(256) ns_split_kernel(NsTable t, NsIo io) {
+    __shared__ double part[4];
+    __shared__ float tile[64][65];
+    const NsPlace p = ns_find(t, blockIdx.x, ST_SPLIT, 64);
+    const NsLayout l = ns_layout(p.m, p.n);
+    const int parts = ns_parts(p.m, p.n);
+    const double sum = ns_block_sum((int)threadIdx.x < parts ? ((const double*)p.ws)[threadIdx.x] : 0.0, part);
+    const float inv = (float)(1.0 / (sqrt(sum) + io.eps));
+    const int nt = (p.n + 63) / 64, i0 = p.tile / nt * 64, j0 = p.tile % nt * 64;
+    const int lane = threadIdx.x & 63, row = threadIdx.x >> 6;
+    // along the caller's rows
+    for (int q = row; q < 64; q += 4) {
+        const int i = p.tall ? i0 + lane : i0 + q, j = p.tall ? j0 + q : j0 + lane;
+        float v = 0.0f;
+        if (i < p.m && j < p.n) {
+            const long long at = p.src + (p.tall ? (long long)j * p.m + i : (long long)i * p.n + j);
+            if constexpr (MUON) v = ns_direction(io, ((const float*)io.in)[at], io.momentum[at]);
+            else if constexpr (DT == ODAMD_DTYPE_BF16) v = bf16_to_f32(((const uint16_t*)io.in)[at]);
+            else v = ((const float*)io.in)[at];
+            v *= inv;
+        }
+        if (p.tall) tile[lane][q] = v; else tile[q][lane] = v;
+    }
+    __syncthreads();
+    const int mp = (int)ns_up(p.m, 32), np = (int)ns_up(p.n, 32);
+    for (int q = threadIdx.x; q < 512; q += 256) {
+        float v[8];
+        const int r = q >> 3, c = (q & 7) * 8;
+        if (i0 + r < p.m && j0 + c < np) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = tile[r][c + e];
+            store_split8(p.ws + l.x + (long long)(i0 + r) * np * 4 + split_at(j0 + c), v, NS_SCALE);
+        }
+        if (j0 + r < p.n && i0 + c < mp) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = tile[c + e][r];
+            store_split8(p.ws + l.xt0 + (long long)(j0 + r) * mp * 4 + split_at(i0 + c), v, NS_SCALE);
+        }
+    }
+}
+
+// Results for the caller: eight values from element `at` on, the first `cnt` of them exist.
+template <bool MUON, int DT>
+__device__ __forceinline__ void ns_emit8(const NsIo& io, float step, long long at, int cnt, const float v[8]) {
+    if (cnt <= 0) return;
+    const int n = cnt < 8 ? cnt : 8;
+    if constexpr (MUON) {
+        f32x4_t* pp = (f32x4_t*)(io.param + at);
+        f32x4_t* ep = (f32x4_t*)(io.ema + at);
+        if (n == 8 && (((uintptr_t)pp | (io.ema ? (uintptr_t)ep : 0)) & 15) == 0) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                f32x4_t w = pp[q];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = w[e] * io.decay - step * v[4 * q + e];
+                pp[q] = w;
+                if (io.ema) {
+                    f32x4_t u = ep[q];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) u[e] = io.ema_keep * u[e] + io.ema_take * w[e];
+                    ep[q] = u;
+                }
+            }
+        } else {
+            for (int e = 0; e < n; ++e) {
+                const float w = io.param[at + e] * io.decay - step * v[e];
+                io.param[at + e] = w;
+                if (io.ema) io.ema[at + e] = io.ema_keep * io.ema[at + e] + io.ema_take * w;
+            }
+        }
+    } else if constexpr (DT == ODAMD_DTYPE_BF16) {
+        uint16_t* o = (uint16_t*)io.out + at;
+        if (n == 8 && ((uintptr_t)o & 15) == 0)
+            *(u32x4*)o = u32x4{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]), f32x2_to_bf16x2(v[4], v[5]), f32x2_to_bf16x2(v[6], v[7])};
+        else
+            for (int e = 0; e < n; ++e) o[e] = f32_to_bf16(v[e]);
+    } else {
+        float* o = (float*)io.out + at;
+        if (n == 8 && ((uintptr_t)o & 15) == 0) {
+            *(f32x4_t*)o = f32x4_t{v[0], v[1], v[2], v[3]};
+            *(f32x4_t*)(o + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+        } else {
+            for (int e = 0; e < n; ++e) o[e] = v[e];
+        }
+    }
+}
+
+// One product of the iteration for every matrix of the table
+template <typename TILE, int STAGE, bool MUON, int DT>
+__global__ void __launch_bounds__(TILE::THREADS) ns_product_kernel(NsTable t, NsIo io, int turn) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const NsPlace p = ns_find(t, gemm_xcd_remap(blockIdx.x, t.tiles), STAGE, TILE::TM);
+    const NsLayout l = ns_layout(p.m, p.n);
+    const int mp = (int)ns_up(p.m, 32), np = (int)ns_up(p.n, 32);
+    int ti, tj;
+    if (STAGE == ST_A || STAGE == ST_P) gemm_triangle_at(p.tile, ti, tj);
+    else gemm_tile_at(p.tile, (p.m + TILE::TM - 1) / TILE::TM, (p.n + TILE::TN - 1) / TILE::TN, ti, tj);
+    const int i0 = ti * TILE::TM, j0 = tj * TILE::TN;
+    TILE tile;
+    if constexpr (STAGE == ST_A) {
+        const GemmOperand x = {p.ws + l.x, (long long)np * 4, p.m};
+        tile.run(x, x, i0, j0, 0, np / 32, np, lds);
+    } else if constexpr (STAGE == ST_P) {
+        const GemmOperand a = {p.ws + l.a, (long long)mp * 4, p.m};
+        tile.run(a, a, i0, j0, 0, mp / 32, mp, lds);
+    } else {
+        const GemmOperand a = {p.ws + l.p, (long long)mp * 4, p.m}, b = {p.ws + (turn & 1 ? l.xt1 : l.xt0), (long long)mp * 4, p.n};
+        tile.run(a, b, i0, j0, 0, mp / 32, mp, lds);
+    }
+
+    if constexpr (STAGE == ST_A || STAGE == ST_P) {
+        char* out = p.ws + (STAGE == ST_A ? l.a : l.p);
+        // row i, columns j .. j+7
+        auto put = [&](int i, int j, float v[8]) {
+            if (i >= p.m || j >= mp) return;
+            const long long at = (long long)i * mp * 4 + split_at(j);
+            if constexpr (STAGE == ST_P) {
+                const f16x8_t hi = *(const f16x8_t*)(p.ws + l.a + at), lo = *(const f16x8_t*)(p.ws + l.a + at + 64);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    v[e] = (NS_C * NS_UNSCALE2) * v[e] + (NS_B / NS_SCALE) * ((float)hi[e] + (float)lo[e]) + (i == j + e ? NS_A : 0.0f);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] *= NS_UNSCALE2;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = j + e < p.m ? v[e] : 0.0f;
+            store_split8(out + at, v, NS_SCALE);
+        };
+        auto rows = [&](int i, int j, float v[8]) { put(i0 + i, j0 + j, v); };
+        auto cols = [&](int i, int j, float v[8]) { put(j0 + j, i0 + i, v); };
+        if (ti == tj) tile.template hand_out<true, false>(lds, rows, cols);
+        else tile.template hand_out<true, true>(lds, rows, cols);
+    } else if constexpr (STAGE == ST_X) {
+        char* xt = p.ws + (turn & 1 ? l.xt0 : l.xt1);
+        tile.template hand_out<true, true>(lds,
+            [&](int i, int j, float v[8]) {
+                i += i0; j += j0;
+                if (i >= p.m || j >= np) return;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = j + e < p.n ? v[e] * NS_UNSCALE2 : 0.0f;
+                store_split8(p.ws + l.x + (long long)i * np * 4 + split_at(j), v, NS_SCALE);
+            },
+            [&](int i, int j, float v[8]) {
+                i += i0; j += j0;
+                if (j >= p.n || i >= mp) return;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = i + e < p.m ? v[e] * NS_UNSCALE2 : 0.0f;
+                store_split8(xt + (long long)j * mp * 4 + split_at(i), v, NS_SCALE);
+            });
+    } else {
+        const float step = MUON ? io.lr02 * sqrtf((float)p.n) : 0.0f;
+        auto rows = [&](int i, int j, float v[8]) {
+            i += i0; j += j0;
+            if (i >= p.m) return;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= NS_UNSCALE2;
+            ns_emit8<MUON, DT>(io, step, p.src + (long long)i * p.n + j, p.n - j, v);
+        };
+        auto cols = [&](int i, int j, float v[8]) {
+            i += i0; j += j0;
+            if (j >= p.n) return;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= NS_UNSCALE2;
+            ns_emit8<MUON, DT>(io, step, p.src + (long long)j * p.m + i, p.m - i, v);
+        };
+        if (p.tall) tile.template hand_out<false, true>(lds, rows, cols);
+        else tile.template hand_out<true, false>(lds, rows, cols);
+    }
+}
+
+using NsTile256 = GemmTile<2, true, 256, 256, 2, 4>;
+using NsTile128 = GemmTile<2, true, 128, 128, 2, 2>;
+using NsTile64 = GemmTile<2, true, 64, 64, 2, 2>;
+
+// Tiles of a stage over the whole table
+int ns_count(NsTable& t, int stage, int tile) {
+    long long at = 0;
+    for (int i = 0; i < t.n; ++i) {
+        t.g[i].tile0 = (int)at;
+        at += (long long)ns_tiles(stage, tile, t.g[i].m, t.g[i].n) * t.g[i].count;
+    }
+    t.tiles = (int)at;
+    return at > 0x7fffffff ? -1 : (int)at;
+}
+
+template <typename TILE, int STAGE, bool MUON, int DT>
+int ns_launch_tile(const NsTable& t, const NsIo& io, int turn, hipStream_t s) {
+    const auto kernel = ns_product_kernel<TILE, STAGE, MUON, DT>;
+    const hipError_t e = odamd_ensure_lds((const void*)kernel, TILE::LDS);
+    if (e != hipSuccess) return (int)e;
+    kernel<<<t.tiles, TILE::THREADS, TILE::LDS, s>>>(t, io, turn);
+    return (int)hipGetLastError();
+}
+
+// The largest tile that still gives every compute unit one: a larger tile reads less per product, fewer tiles than compute
+// units leave some of those idle.
+template <int STAGE, bool MUON, int DT>
+int ns_product(NsTable& t, const NsIo& io, int turn, hipStream_t s) {
+    if (ns_count(t, STAGE, 256) >= 256) return ns_launch_tile<NsTile256, STAGE, MUON, DT>(t, io, turn, s);
+    if (ns_count(t, STAGE, 128) >= 256) return ns_launch_tile<NsTile128, STAGE, MUON, DT>(t, io, turn, s);
+    if (ns_count(t, STAGE, 64) < 0) return ODAMD_E_LIMIT;
+    return ns_launch_tile<NsTile64, STAGE, MUON, DT>(t, io, turn, s);
+}
+
+template <bool MUON, int DT>
+int ns_run(NsTable& t, const NsIo& io, int steps, hipStream_t s) {
+    if (ns_count(t, ST_NORM, 0) < 0) return ODAMD_E_LIMIT;
+    ns_norm_kernel<MUON, DT><<<t.tiles, 256, 0, s>>>(t, io);
+    if (ns_count(t, ST_SPLIT, 64) < 0) return ODAMD_E_LIMIT;
+    ns_split_kernel<MUON, DT><<<t.tiles, 256, 0, s>>>(t, io);
+    int rc = (int)hipGetLastError();
+    for (int k = 0; k < steps && rc == 0; ++k) {
+        rc = ns_product<ST_A, false, ODAMD_DTYPE_F32>(t, io, k, s);
+        if (rc == 0) rc = ns_product<ST_P, false, ODAMD_DTYPE_F32>(t, io, k, s);
+        if (rc == 0) rc = k + 1 < steps ? ns_product<ST_X, false, ODAMD_DTYPE_F32>(t, io, k, s) : ns_product<ST_OUT, MUON, DT>(t, io, k, s);
+    }
+    return rc;
+}
+
+bool ns_shape_ok(long long rows, long long cols) { return rows >= 1 && cols >= 1 && rows * cols <= 0x7fffffffLL; }
+
+void ns_orient(NsGroup& g, int rows, int cols) {
+    g.tall = rows > cols;
+    g.m = g.tall ? cols : rows;
+    g.n = g.tall ? rows : cols;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t odamd_orthogonalize_workspace_bytes(int batch, int rows, int cols) {
+    if (batch < 1 || !ns_shape_ok(rows, cols)) return 0;
+    NsGroup g;
+    ns_orient(g, rows, cols);
+    return (size_t)batch * ns_layout(g.m, g.n).end;
+}
+
+int odamd_orthogonalize(const void* x, void* out, int batch, int rows, int cols, int steps, double eps, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+    if (!x || !out || !workspace || batch < 1 || !ns_shape_ok(rows, cols) || steps < 1 || steps > 32 || !(eps >= 0.0)) return ODAMD_E_ARG;
+    if (dtype != ODAMD_DTYPE_F32 && dtype != ODAMD_DTYPE_BF16) return ODAMD_E_ARG;
+    if (((uintptr_t)x | (uintptr_t)out) & (dtype == ODAMD_DTYPE_F32 ? 3 : 1)) return ODAMD_E_ALIGN;
+    if ((uintptr_t)workspace & 255) return ODAMD_E_ALIGN;
+    if (workspace_bytes < odamd_orthogonalize_workspace_bytes(batch, rows, cols)) return ODAMD_E_WORKSPACE;
+    NsTable t;
+    t.n = 1;
+    t.ws = (char*)workspace;
+    ns_orient(t.g[0], rows, cols);
+    t.g[0].src = 0;
+    t.g[0].ws = 0;
+    t.g[0].count = batch;
+    NsIo io = {};
+    io.in = x;
+    io.out = out;
+    io.eps = eps;
+    return dtype == ODAMD_DTYPE_F32 ? ns_run<false, ODAMD_DTYPE_F32>(t, io, steps, (hipStream_t)stream)
+                                    : ns_run<false, ODAMD_DTYPE_BF16>(t, io, steps, (hipStream_t)stream);
+}
+
+size_t odamd_muon_workspace_bytes(const odamd_matrix* matrices_host, int n_matrices) {
+    if (!matrices_host || n_matrices < 1) return 0;
+    size_t most = 0;
+    for (int i = 0; i < n_matrices; i += NS_GROUPS) {
+        size_t at = 0;
+        for (int k = i; k < n_matrices && k < i + NS_GROUPS; ++k) {
+            if (!ns_shape_ok(matrices_host[k].rows, matrices_host[k].cols)) return 0;
+            NsGroup g;
+            ns_orient(g, matrices_host[k].rows, matrices_host[k].cols);
+            at += (size_t)ns_layout(g.m, g.n).end;
+        }
+        most = at > most ? at : most;
+    }
+    return most;
+}
+
+int odamd_muon_ema_step(float* param, const float* grad, float* momentum, float* ema, const odamd_matrix* matrices_host,
+                        int n_matrices, double lr, double momentum_decay, int nesterov, double weight_decay, int steps, double eps,
+                        double ema_decay, double grad_scale, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!param || !grad || !momentum || !matrices_host || !workspace || n_matrices < 1 || steps < 1 || steps > 32 || !(eps >= 0.0)) return ODAMD_E_ARG;
+    for (int k = 0; k < n_matrices; ++k)
+        if (matrices_host[k].offset < 0 || !ns_shape_ok(matrices_host[k].rows, matrices_host[k].cols)) return ODAMD_E_ARG;
+    if (((uintptr_t)param | (uintptr_t)grad | (uintptr_t)momentum | (uintptr_t)ema) & 3) return ODAMD_E_ALIGN;
+    if ((uintptr_t)workspace & 255) return ODAMD_E_ALIGN;
+    const size_t need = odamd_muon_workspace_bytes(matrices_host, n_matrices);
+    if (workspace_bytes < need) return ODAMD_E_WORKSPACE;
+    if (need / 256 > 0xffffffffULL) return ODAMD_E_LIMIT;
+    NsIo io = {};
+    io.in = grad;
+    io.param = param;
+    io.momentum = momentum;
+    io.ema = ema;
+    io.mu = (float)momentum_decay;
+    io.grad_scale = (float)grad_scale;
+    io.decay = (float)(1.0 - lr * weight_decay);
+    io.lr02 = (float)(0.2 * lr);
+    io.ema_keep = (float)ema_decay;
+    io.ema_take = (float)(1.0 - ema_decay);
+    io.nesterov = nesterov != 0;
+    io.eps = eps;
+    for (int i = 0; i < n_matrices; i += NS_GROUPS) {
+        NsTable t;
+        t.n = 0;
+        t.ws = (char*)workspace;
+        long long at = 0;
+        for (int k = i; k < n_matrices && k < i + NS_GROUPS; ++k) {
+            NsGroup& g = t.g[t.n++];
+            ns_orient(g, matrices_host[k].rows, matrices_host[k].cols);
+            g.src = matrices_host[k].offset;
+            g.count = 1;
+            g.ws = (unsigned)(at / 256);
+            at += ns_layout(g.m, g.n).end;
+        }
+        const int rc = ns_run<true, ODAMD_DTYPE_F32>(t, io, steps, (hipStream_t)stream);
+        if (rc != 0) return rc;
+    }
+    return ODAMD_OK;
+}
+
+}  // extern "C"

@@ -1259,23 +1259,44 @@ __global__ void __launch_bounds__(256) loss_finalize_kernel(LossP p, int nconf, 
 // ------------------------------------------------------------------------------------------
 // Adam (coupled L2, train_class.py:161-162) + EMA (train_class.py:485-493) over flat buffers.
 // ------------------------------------------------------------------------------------------
+struct AdamConst { float step_size, om_beta1, beta2, om_beta2, bc2_sqrt, eps, wd, ema_decay, om_ema_decay, grad_scale; };
+__device__ __forceinline__ void adam_ema_one(float* p, const float* g, float* m, float* v, float* ema, size_t i, const AdamConst& c) {
+    float w = p[i];
+    const float gr = g[i] * c.grad_scale + c.wd * w;
+    float mm = m[i];
+    mm = mm + c.om_beta1 * (gr - mm);                                 // exp_avg.lerp_(grad, 1 - beta1)
+    const float vv = c.beta2 * v[i] + c.om_beta2 * (gr * gr);
+    const float denom = sqrtf(vv) / c.bc2_sqrt + c.eps;
+    w = w - c.step_size * (mm / denom);
+    m[i] = mm;
+    v[i] = vv;
+    p[i] = w;
+    if (ema) ema[i] = c.ema_decay * ema[i] + c.om_ema_decay * w;
+}
 __global__ void __launch_bounds__(256)
 adam_ema_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v,
-                float* __restrict__ ema, size_t n, float step_size, float om_beta1, float beta2, float om_beta2,
-                float bc2_sqrt, float eps, float wd, float ema_decay, float om_ema_decay, float grad_scale) {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        float w = p[i];
-        const float gr = g[i] * grad_scale + wd * w;
-        float mm = m[i];
-        mm = mm + om_beta1 * (gr - mm);                                 // exp_avg.lerp_(grad, 1 - beta1)
-        const float vv = beta2 * v[i] + om_beta2 * (gr * gr);
-        const float denom = sqrtf(vv) / bc2_sqrt + eps;
-        w = w - step_size * (mm / denom);
-        m[i] = mm;
-        v[i] = vv;
-        p[i] = w;
-        if (ema) ema[i] = ema_decay * ema[i] + om_ema_decay * w;
+                float* __restrict__ ema, size_t n, AdamConst c) {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256)
+        adam_ema_one(p, g, m, v, ema, i, c);
+}
+
+// The same step over some ranges of the buffers only (what lies between the matrices of odamd_muon_ema_step): a
+// workgroup takes 1024 elements of one range; the table travels in the kernel's arguments.
+constexpr int ADAM_RANGES = 200;
+struct AdamRange { long long from; int len, block0; };
+struct AdamRanges { AdamRange r[ADAM_RANGES]; int n; };
+static_assert(sizeof(AdamRanges) <= 3600, "kernel arguments are limited to 4 KiB");
+__global__ void __launch_bounds__(256)
+adam_ema_ranges_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v,
+                       float* __restrict__ ema, AdamRanges t, AdamConst c) {
+    int lo = 0, hi = t.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t.r[mid].block0 <= (int)blockIdx.x) lo = mid; else hi = mid - 1;
     }
+    const int from = ((int)blockIdx.x - t.r[lo].block0) * 1024;
+    const int to = min(from + 1024, t.r[lo].len);
+    for (int i = from + threadIdx.x; i < to; i += 256) adam_ema_one(p, g, m, v, ema, (size_t)(t.r[lo].from + i), c);
 }
 
 __global__ void __launch_bounds__(256) ema_only_kernel(float* __restrict__ ema, const float* __restrict__ src, size_t n, float d, float omd) {
@@ -1393,6 +1414,11 @@ int ew_rows_grid(size_t npix, int rows) {
     return (int)(g > 4096 ? 4096 : (g < 1 ? 1 : g));
 }
 
+AdamConst adam_const(double lr, double beta1, double beta2, double eps, double weight_decay, int step, double ema_decay, double grad_scale) {
+    const double bc1 = 1.0 - pow(beta1, (double)step), bc2 = 1.0 - pow(beta2, (double)step);
+    return {(float)(lr / bc1), (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)sqrt(bc2), (float)eps,
+            (float)weight_decay, (float)ema_decay, (float)(1.0 - ema_decay), (float)grad_scale};
+}
 int ew_grid(size_t n) {
     size_t g = (n + 255) / 256;
     return (int)(g > 4096 ? 4096 : (g < 1 ? 1 : g));
@@ -1789,10 +1815,31 @@ int odamd_adam_ema_step(float* param, const float* grad, float* exp_avg, float* 
                         double beta1, double beta2, double eps, double weight_decay, int step, double ema_decay,
                         double grad_scale, void* stream) {
     if (!param || !grad || !exp_avg || !exp_avg_sq || n < 1 || step < 1) return ODAMD_E_ARG;
-    const double bc1 = 1.0 - pow(beta1, (double)step);
-    const double bc2 = 1.0 - pow(beta2, (double)step);
-    adam_ema_kernel<<<ew_grid(n), 256, 0, (hipStream_t)stream>>>(param, grad, exp_avg, exp_avg_sq, ema, n, (float)(lr / bc1), (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)sqrt(bc2), (float)eps, (float)weight_decay, (float)ema_decay, (float)(1.0 - ema_decay), (float)grad_scale);
+    const AdamConst c = adam_const(lr, beta1, beta2, eps, weight_decay, step, ema_decay, grad_scale);
+    adam_ema_kernel<<<ew_grid(n), 256, 0, (hipStream_t)stream>>>(param, grad, exp_avg, exp_avg_sq, ema, n, c);
     return (int)hipGetLastError();
+}
+
+int odamd_adam_ema_ranges_step(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, float* ema,
+                               const odamd_range* ranges_host, int n_ranges, double lr, double beta1, double beta2, double eps,
+                               double weight_decay, int step, double ema_decay, double grad_scale, void* stream) {
+    if (!param || !grad || !exp_avg || !exp_avg_sq || !ranges_host || n_ranges < 1 || step < 1) return ODAMD_E_ARG;
+    for (int k = 0; k < n_ranges; ++k)
+        if (ranges_host[k].offset < 0 || ranges_host[k].len < 1 || ranges_host[k].len > 0x7fffffffLL - 1024) return ODAMD_E_ARG;
+    const AdamConst c = adam_const(lr, beta1, beta2, eps, weight_decay, step, ema_decay, grad_scale);
+    for (int i = 0; i < n_ranges; ) {
+        AdamRanges t;
+        t.n = 0;
+        long long blocks = 0;
+        for (; i < n_ranges && t.n < ADAM_RANGES && blocks < 0x400000; ++i) {
+            t.r[t.n++] = {ranges_host[i].offset, (int)ranges_host[i].len, (int)blocks};
+            blocks += (ranges_host[i].len + 1023) / 1024;
+        }
+        adam_ema_ranges_kernel<<<(int)blocks, 256, 0, (hipStream_t)stream>>>(param, grad, exp_avg, exp_avg_sq, ema, t, c);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return (int)e;
+    }
+    return ODAMD_OK;
 }
 
 int odamd_ema_update(float* ema, const float* src, size_t n, double decay, void* stream) {

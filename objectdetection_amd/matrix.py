@@ -1,0 +1,242 @@
+"""Matrix operators beside the convolutions: the dense layer with its epilogue in one product (`linear`, differentiable),
+the orthogonalisation of matrices by Newton-Schulz products (`orthogonalize`) and the optimizer step built on it
+(`muon_step`, what `train_class.FusedMuon` runs).
+
+Tensors are float32 or bfloat16 on one GPU; every call enqueues its work on the current stream of the tensors' device
+and takes its workspace from torch's allocator, so it can be captured into a graph.
+"""
+import ctypes as C
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import lib, check
+
+ACTIVATIONS = {None: 0, 'silu': 1, 'gelu': 2, 'relu': 3}
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+MATRIX_DTYPE = np.dtype([('offset', '<i8'), ('rows', '<i4'), ('cols', '<i4')])      # odamd_matrix
+RANGE_DTYPE = np.dtype([('offset', '<i8'), ('len', '<i8')])                         # odamd_range
+
+
+def _stream():
+    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _workspace(size, device):
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
+def _check_tensor(name, t, dtype=None, device=None):
+    if not torch.is_tensor(t) or not t.is_cuda:
+        raise ValueError(f'{name} must be a CUDA tensor')
+    if t.dtype not in _DTYPES:
+        raise ValueError(f'{name} must be float32 or bfloat16, not {t.dtype}')
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f'{name} is {t.dtype}, the input {dtype}: one type for all')
+    if device is not None and t.device != device:
+        raise ValueError(f'{name} is on {t.device}, the input on {device}')
+
+
+def _rows(t):
+    """(..., c) -> (rows, c) with contiguous rows that do not overlap: a view where the strides allow one."""
+    c = t.shape[-1]
+    t = t.reshape(-1, c)
+    if (c > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < c):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t):
+    return max(t.stride(0), t.shape[1])
+
+
+# ---------------------------------------------------------------------------------------------
+# dense layer
+# ---------------------------------------------------------------------------------------------
+def _linear_forward(x, weight, bias, residual, act, keep_z):
+    """2-D operands as `_rows` leaves them -> (y, z or None)."""
+    m, k = x.shape
+    n = weight.shape[0]
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    z = torch.empty_like(y) if keep_z else None
+    d = _lib.LinearDesc(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(z), _ld(x),
+                        _ld(weight), 0 if residual is None else _ld(residual), n, n, m, k, n, act, _DTYPES[x.dtype])
+    with torch.cuda.device(x.device):
+        ws = _workspace(lib.odamd_linear_workspace_bytes(C.byref(d)), x.device)
+        check(lib.odamd_linear_forward(C.byref(d), _ptr(ws), 0 if ws is None else ws.numel(), _stream()), 'linear_forward')
+    return y, z
+
+
+def _linear_backward(dy, z, x, weight, act, want_dx, want_dw, want_db):
+    """Gradients of `_linear_forward` from 2-D operands; x and weight may be None where they are not needed."""
+    m, n = dy.shape
+    k = (weight if weight is not None else x).shape[1] if (want_dx or want_dw) else 1
+    dx = torch.empty((m, k), dtype=dy.dtype, device=dy.device) if want_dx else None
+    dw = torch.empty((n, k), dtype=dy.dtype, device=dy.device) if want_dw else None
+    db = torch.empty(n, dtype=dy.dtype, device=dy.device) if want_db else None
+    d = _lib.LinearGradDesc(dy.data_ptr(), _ptr(z), _ptr(x) if want_dw else None, _ptr(weight) if want_dx else None, _ptr(dx),
+                            _ptr(dw), _ptr(db), _ld(dy), 0 if z is None else _ld(z), _ld(x) if want_dw else 0,
+                            _ld(weight) if want_dx else 0, k, k, m, k, n, act, _DTYPES[dy.dtype])
+    with torch.cuda.device(dy.device):
+        ws = _workspace(lib.odamd_linear_backward_workspace_bytes(C.byref(d)), dy.device)
+        check(lib.odamd_linear_backward(C.byref(d), _ptr(ws), ws.numel(), _stream()), 'linear_backward')
+    return dx, dw, db
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        x2, w2 = _rows(x), _rows(weight)
+        keep_z = act != 0 and any(ctx.needs_input_grad[:3])
+        y, z = _linear_forward(x2, w2, bias if bias is None else bias.contiguous(),
+                               None if residual is None else _rows(residual), act, keep_z)
+        ctx.act, ctx.x_shape, ctx.y_shape = act, x.shape, x.shape[:-1] + (weight.shape[0],)
+        ctx.save_for_backward(x2 if ctx.needs_input_grad[1] else None, w2 if ctx.needs_input_grad[0] else None, z)
+        return y.view(ctx.y_shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if any(need[:3]):
+            dx, dw, db = _linear_backward(_rows(dy), z, x, weight, ctx.act, *need[:3])
+            dx = dx if dx is None else dx.view(ctx.x_shape)
+        return dx, dw, db, dy if need[3] else None, None
+
+
+def linear(x, weight, bias=None, activation=None, residual=None):
+    """act(x W^T + bias) + residual in one product.  x: (..., k); weight: (n, k); bias: (n,); residual: (..., n); all of one
+    type, float32 or bfloat16.  activation: None, 'silu', 'gelu' (the erf form) or 'relu'.  Rows may be strided (a slice of a
+    wider, concatenated buffer is read in place).  Differentiable once in all four tensors; in bfloat16 the pre-activation
+    that the backward pass keeps, and the gradient at it, are bfloat16.  float32 products carry 22 bits per value, counted
+    from the largest magnitude of its row; a float32 row with an infinity gives NaN or infinity."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f'activation {activation!r}: one of {list(ACTIVATIONS)}')
+    _check_tensor('x', x)
+    _check_tensor('weight', weight, x.dtype, x.device)
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or min(weight.shape) < 1:
+        raise ValueError(f'x (..., k) and weight (n, k) do not fit: {tuple(x.shape)} and {tuple(weight.shape)}')
+    n = weight.shape[0]
+    if bias is not None:
+        _check_tensor('bias', bias, x.dtype, x.device)
+        if tuple(bias.shape) != (n,):
+            raise ValueError(f'bias must have shape ({n},), not {tuple(bias.shape)}')
+    if residual is not None:
+        _check_tensor('residual', residual, x.dtype, x.device)
+        if residual.shape != x.shape[:-1] + (n,):
+            raise ValueError(f'residual must have shape {tuple(x.shape[:-1]) + (n,)}, not {tuple(residual.shape)}')
+    act = ACTIVATIONS[activation]
+    if x.numel() == 0:
+        # no rows: nothing to launch; the empty result stays connected to its inputs
+        y = x.new_empty(x.shape[:-1] + (n,))
+        if torch.is_grad_enabled():
+            y = y + 0 * x.sum() + 0 * weight.sum()
+            y = y if bias is None else y + 0 * bias.sum()
+            y = y if residual is None else y + residual
+        return y
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return _Linear.apply(x, weight, bias, residual, act)
+    y, _ = _linear_forward(_rows(x), _rows(weight), bias if bias is None else bias.contiguous(),
+                           None if residual is None else _rows(residual), act, False)
+    return y.view(x.shape[:-1] + (n,))
+
+
+# ---------------------------------------------------------------------------------------------
+# orthogonalisation and the optimizer step
+# ---------------------------------------------------------------------------------------------
+def orthogonalize(x, steps=5, eps=1e-7, out=None):
+    """Brings the singular values of every matrix of x (..., rows, cols) near one and keeps its singular vectors: `steps`
+    Newton-Schulz products with the coefficients (3.4445, -4.7750, 2.0315) from x / (|x|_F + eps) on.  Five steps take
+    singular values from 0.003 of the norm up to between 0.68 and 1.21.  float32 or bfloat16; the products carry 22 bits
+    either way, the result is rounded once.  `out` may be x itself.  A matrix with a NaN or an infinity gives NaN."""
+    _check_tensor('x', x)
+    if x.dim() < 2:
+        raise ValueError(f'x must have rows and columns, not shape {tuple(x.shape)}')
+    if not 1 <= int(steps) <= 32 or not eps >= 0:
+        raise ValueError('steps must be 1 to 32, eps must not be negative')
+    rows, cols = x.shape[-2:]
+    if rows * cols >= 2 ** 31:
+        raise ValueError('a matrix must have fewer than 2^31 elements')
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        _check_tensor('out', out, x.dtype, x.device)
+        if out.shape != x.shape or not out.is_contiguous():
+            raise ValueError('out must be contiguous and have the shape of x')
+    if x.numel() == 0:
+        return out
+    src = x.detach().contiguous()
+    batch = src.numel() // (rows * cols)
+    with torch.cuda.device(x.device):
+        ws = _workspace(lib.odamd_orthogonalize_workspace_bytes(batch, rows, cols), x.device)
+        check(lib.odamd_orthogonalize(src.data_ptr(), out.data_ptr(), batch, rows, cols, int(steps), float(eps),
+                                      _DTYPES[x.dtype], ws.data_ptr(), ws.numel(), _stream()), 'orthogonalize')
+    return out
+
+
+class MatrixTable:
+    """The matrices of a flat buffer, [(offset, rows, cols)], checked once: in the buffer, not overlapping."""
+
+    def __init__(self, matrices):
+        a = np.asarray(list(matrices), dtype=np.int64).reshape(-1, 3)
+        size = a[:, 1] * a[:, 2]
+        if len(a) == 0 or (a[:, 0] < 0).any() or (a[:, 1:] < 1).any() or (a[:, 1:] >= 2 ** 31).any() or (size >= 2 ** 31).any():
+            raise ValueError('matrices: at least one (offset, rows, cols), offsets from 0, sizes from 1, under 2^31 elements each')
+        order = np.argsort(a[:, 0], kind='stable')
+        ends = (a[:, 0] + size)[order]
+        if (a[order, 0][1:] < ends[:-1]).any():
+            raise ValueError('matrices overlap')
+        self.end = int(ends[-1])
+        self.table = np.zeros(len(a), MATRIX_DTYPE)
+        for i, name in enumerate(('offset', 'rows', 'cols')):
+            self.table[name] = a[:, i]
+        self.workspace_bytes = int(lib.odamd_muon_workspace_bytes(self.table.ctypes.data, len(a)))
+
+    def __len__(self):
+        return len(self.table)
+
+    def gaps(self, numel):
+        """What lies between the matrices of a buffer of `numel` elements, as (offset, length)."""
+        found, at = [], 0
+        for e in np.sort(self.table, order='offset'):
+            if e['offset'] > at:
+                found.append((at, int(e['offset']) - at))
+            at = int(e['offset']) + int(e['rows']) * int(e['cols'])
+        if numel > at:
+            found.append((at, numel - at))
+        return found
+
+
+def muon_step(param, grad, momentum, matrices, lr, momentum_decay=0.95, nesterov=True, weight_decay=0.0, ema=None,
+              ema_decay=0.0, grad_scale=1.0, steps=5, eps=1e-7):
+    """One optimizer step with orthogonalised momentum over the matrices of flat float32 buffers, in place:
+
+        m = momentum_decay m + grad_scale g;  u = grad_scale g + momentum_decay m  (nesterov; else m)
+        p = p (1 - lr weight_decay) - lr 0.2 sqrt(max(rows, cols)) orthogonalize(u)
+        ema = ema_decay ema + (1 - ema_decay) p
+
+    `matrices`: [(offset, rows, cols)] or a MatrixTable of them.  What lies between the matrices is not touched."""
+    table = matrices if isinstance(matrices, MatrixTable) else MatrixTable(matrices)
+    for name, t in (('param', param), ('grad', grad), ('momentum', momentum), ('ema', ema)):
+        if t is None and name == 'ema':
+            continue
+        _check_tensor(name, t, device=param.device)
+        if t.dtype != torch.float32 or t.dim() != 1 or not t.is_contiguous() or t.numel() != param.numel():
+            raise ValueError(f'{name} must be a flat contiguous float32 buffer of the length of param')
+    if table.end > param.numel():
+        raise ValueError(f'matrices end at {table.end}, the buffers at {param.numel()}')
+    if not 1 <= int(steps) <= 32 or not eps >= 0:
+        raise ValueError('steps must be 1 to 32, eps must not be negative')
+    with torch.cuda.device(param.device):
+        ws = _workspace(table.workspace_bytes, param.device)
+        check(lib.odamd_muon_ema_step(param.data_ptr(), grad.data_ptr(), momentum.data_ptr(), _ptr(ema),
+                                      table.table.ctypes.data, len(table), lr, momentum_decay, int(nesterov), weight_decay,
+                                      int(steps), eps, ema_decay, grad_scale, ws.data_ptr(), ws.numel(), _stream()),
+              'muon_ema_step')

@@ -11,6 +11,7 @@ sppcspc :178-223, head :226-236, decode :263-293, deploy :296-305.
 import torch
 
 from .. import engine
+from .. import matrix
 from .. import postprocess as _post
 
 
@@ -53,6 +54,26 @@ class cbs(_Block):
 
     def _emit(self, pb, x, out=None, pool=False):
         return pb.conv(self, x, out, pool)
+
+
+class linear(torch.nn.Module):
+    """Dense layer over the last axis with its epilogue in one product: act(x W^T + b) + residual.  act: None, 'silu', 'gelu'
+    or 'relu'.  Parameters follow the input's type (float32 or bfloat16)."""
+
+    def __init__(self, in_, out_, act=None, bias=True):
+        super().__init__()
+        if act not in matrix.ACTIVATIONS:
+            raise ValueError(f'activation {act!r}: one of {list(matrix.ACTIVATIONS)}')
+        self.act = act
+        self.weight = torch.nn.Parameter(torch.empty(out_, in_))
+        self.bias = torch.nn.Parameter(torch.empty(out_)) if bias else None
+        bound = in_ ** -0.5
+        for p in self.parameters():
+            torch.nn.init.uniform_(p, -bound, bound)
+
+    def forward(self, x, residual=None):
+        return matrix.linear(x, self.weight.to(x.dtype), None if self.bias is None else self.bias.to(x.dtype), self.act,
+                             residual)
 
 
 class concat(_Block):

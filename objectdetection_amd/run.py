@@ -46,6 +46,8 @@ def build_parser():
     p.add_argument('--local_rank', '--local-rank', default=int(os.environ.get('LOCAL_RANK', 0)), type=int)
     p.add_argument('--label_smooth', default=0.01, type=float)
     p.add_argument('--synthetic_images', default=512, type=int)
+    p.add_argument('--optimizer', default='adam', choices=('adam', 'muon'),
+                   help='muon: orthogonalised momentum for the convolutions, Adam for the rest')
     # flags of the reference kept for command-line compatibility
     p.add_argument('--amp', default=False, type=_bool, help='mixed precision: the bf16 training step (run.py:47)')
     p.add_argument('--latch', default=True, type=_bool)

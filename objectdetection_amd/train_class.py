@@ -19,6 +19,7 @@ import os
 import numpy as np
 import torch
 
+from . import matrix
 from . import postprocess as _post
 from . import train_engine as te
 from ._lib import lib, check
@@ -109,6 +110,8 @@ class FusedAdam:
     def load_state_dict(self, d):
         """Takes this class's own state_dict, or torch.optim.Adam's (what a reference checkpoint holds,
         train_class.py:166-167: per-parameter entries in model.parameters() order)."""
+        if d.get('kind', 'adam') != 'adam':
+            raise ValueError(f"optimizer state of kind {d['kind']!r} does not fit Adam: its moments mean something else")
         s = self.state
         if 'state' in d:
             step = 0
@@ -122,6 +125,44 @@ class FusedAdam:
                 step = max(step, int(e['step']))
             s.step = step
             return
+        s.step = d['step']
+        s.exp_avg.copy_(d['exp_avg'])
+        s.exp_avg_sq.copy_(d['exp_avg_sq'])
+
+
+class FusedMuon:
+    """Orthogonalised momentum for the weights with rows and columns, Adam for everything else (normalisation, biases, heads),
+    fused with the EMA update, over the model's flat buffers; the interface of FusedAdam.  The update has the root mean
+    square of an Adam step, so learning rate and weight decay carry over (the decay is decoupled for the matrices)."""
+
+    def __init__(self, model, lr, betas=(0.937, 0.999), weight_decay=0.0, eps=1e-8, momentum=0.95, nesterov=True):
+        self.state = model.train_state()
+        self.params = list(model.parameters())
+        self.param_groups = [{'lr': lr, 'betas': betas, 'weight_decay': weight_decay, 'eps': eps, 'momentum': momentum,
+                              'nesterov': nesterov}]
+        self.grad_scale = 1.0
+        self.ema = False
+        self.table = matrix.MatrixTable(te.muon_matrices(model, self.state))
+        self.rest = np.array(self.table.gaps(self.state.n), dtype=matrix.RANGE_DTYPE)
+
+    def step(self):
+        g = self.param_groups[0]
+        te.muon_optimizer_step(self.state, self.table, self.rest, g['lr'], g['weight_decay'], g['momentum'], g['nesterov'],
+                               g['betas'], g['eps'], self.grad_scale, self.ema)
+
+    def zero_grad(self):
+        self.state.grad.zero_()
+
+    def state_dict(self):
+        s = self.state
+        return {'kind': 'muon', 'step': s.step, 'exp_avg': s.exp_avg.clone(), 'exp_avg_sq': s.exp_avg_sq.clone(),
+                'param_groups': [dict(g) for g in self.param_groups]}
+
+    def load_state_dict(self, d):
+        """Takes this class's own state_dict only."""
+        if d.get('kind') != 'muon':
+            raise ValueError('not a state of this optimizer: the moments of another one mean something else')
+        s = self.state
         s.step = d['step']
         s.exp_avg.copy_(d['exp_avg'])
         s.exp_avg_sq.copy_(d['exp_avg_sq'])
@@ -147,7 +188,7 @@ class model_ema:
         self.state.ema_updates = v
 
     def update(self, model=None):
-        """No-op: the EMA is applied by FusedAdam.step() in the same launch as the parameters."""
+        """No-op: the EMA is applied by the optimizer's step() in the same launch as the parameters."""
 
     @property
     def ema_model(self):
@@ -391,7 +432,10 @@ class train_class:
     def optimizer_load(self):
         args = self.args
         wd = args.r_value if args.regularization == 'L2' else 0.0
-        opt = FusedAdam(self.model, args.lr_start, (0.937, 0.999), wd)
+        name = getattr(args, 'optimizer', 'adam')
+        if name not in ('adam', 'muon'):
+            raise ValueError(f"optimizer {name!r}: 'adam' or 'muon'")
+        opt = (FusedMuon if name == 'muon' else FusedAdam)(self.model, args.lr_start, (0.937, 0.999), wd)
         if self.model_dict['optimizer_state_dict'] is not None:
             opt.load_state_dict(self.model_dict['optimizer_state_dict'])
         step_epoch = max(len(self.train_dataloader), 1)

@@ -16,7 +16,7 @@ import weakref
 
 import torch
 
-from . import _lib, engine, postprocess as _post
+from . import _lib, engine, matrix, postprocess as _post
 from ._lib import lib, check
 from .engine import F32, BF16, Act, PlanBuilder, _round_up, CH_ALIGN
 
@@ -990,20 +990,50 @@ def ema_decay(update_total, decay=0.9999, tau=2000):
     return decay * (1 - math.exp(-update_total / tau))
 
 
+def _begin_step(state, ema):
+    """Counts a step; the decay and the buffer of the parameters' EMA (None without one)."""
+    state.step += 1
+    engine.touch_weights()                   # parameters are about to be written through raw pointers
+    if not ema or state.ema_param is None:
+        return 0.0, None
+    state.ema_updates += 1
+    return ema_decay(state.ema_updates), state.ema_param.data_ptr()
+
+
 def optimizer_step(state, lr, weight_decay=0.0005, betas=(0.937, 0.999), eps=1e-8, grad_scale=1.0, ema=True):
     """Adam with coupled L2 over the flat buffers, fused with the EMA of the parameters; the EMA
     of the BN running buffers follows in a second launch (train_class.py:211-213)."""
-    state.step += 1
-    engine.touch_weights()                   # parameters are about to be written through raw pointers
-    d = 0.0
-    ema_ptr = None
-    if ema and state.ema_param is not None:
-        state.ema_updates += 1
-        d = ema_decay(state.ema_updates)
-        ema_ptr = state.ema_param.data_ptr()
+    d, ema_ptr = _begin_step(state, ema)
     check(lib.odamd_adam_ema_step(state.param.data_ptr(), state.grad.data_ptr(), state.exp_avg.data_ptr(),
                                   state.exp_avg_sq.data_ptr(), ema_ptr, state.n, lr, betas[0], betas[1], eps,
                                   weight_decay, state.step, d, grad_scale, _stream()), 'adam_ema_step')
+    if ema_ptr is not None and state.nb:
+        check(lib.odamd_ema_update(state.ema_buffers.data_ptr(), state.buffers.data_ptr(), state.nb, d, _stream()),
+              'ema_update')
+
+
+def muon_matrices(model, state):
+    """(offset, rows, cols) in the flat buffers of every weight that the orthogonalised update serves: parameters with
+    rows and columns, convolutions as output channels x (input channels * taps).  The weights of the heads keep Adam:
+    their rows are box, confidence and class logits, whose scales differ by design."""
+    from .model import layer
+    heads = {id(p) for m in model.modules() if isinstance(m, layer.head) for p in m.parameters()}
+    return [(state.offsets[id(p)], p.shape[0], p.numel() // p.shape[0]) for p in model.parameters()
+            if p.dim() >= 2 and id(p) not in heads]
+
+
+def muon_optimizer_step(state, table, rest, lr, weight_decay=0.0005, momentum=0.95, nesterov=True, betas=(0.937, 0.999), eps=1e-8,
+                        grad_scale=1.0, ema=True):
+    """Orthogonalised momentum over the matrices of `table` (their momentum is the `exp_avg` buffer), Adam with coupled L2
+    over `rest` (an array of odamd_range: everything between them), the EMA of parameters and BN buffers with both."""
+    d, ema_ptr = _begin_step(state, ema)
+    matrix.muon_step(state.param, state.grad, state.exp_avg, table, lr, momentum, nesterov, weight_decay,
+                     state.ema_param if ema_ptr is not None else None, d, grad_scale)
+    if len(rest):
+        check(lib.odamd_adam_ema_ranges_step(state.param.data_ptr(), state.grad.data_ptr(), state.exp_avg.data_ptr(),
+                                             state.exp_avg_sq.data_ptr(), ema_ptr, rest.ctypes.data, len(rest), lr, betas[0],
+                                             betas[1], eps, weight_decay, state.step, d, grad_scale, _stream()),
+              'adam_ema_ranges_step')
     if ema_ptr is not None and state.nb:
         check(lib.odamd_ema_update(state.ema_buffers.data_ptr(), state.buffers.data_ptr(), state.nb, d, _stream()),
               'ema_update')

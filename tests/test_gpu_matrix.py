@@ -1,0 +1,522 @@
+"""GPU parity of the matrix operators against plain 64-bit arithmetic: dense layer forward and backward, orthogonalisation,
+optimizer step, and a training run of them together.
+
+Tolerances are worst-case bounds of the arithmetic, element by element.  float32 products use pairs of fp16 numbers: each
+factor is off by at most 2^-22 of itself (two half steps of 2^-11) and the product of the two low parts, another 2^-22, is
+left out; bfloat16 products are exact.  A float32 sum of K products is off by at most K 2^-24 of the sum of magnitudes.
+Results are rounded by half a step, torch.finfo(t).eps / 2."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+NS = (3.4445, -4.7750, 2.0315)
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+PAIR = {torch.float32: 3 * 2.0 ** -22, torch.bfloat16: 0.0}
+
+
+@pytest.fixture(scope='module')
+def mx():
+    from objectdetection_amd import matrix
+    return matrix
+
+
+def randn(*shape, seed=0, dtype=torch.float32, scale=1.0):
+    g = torch.Generator(device='cuda').manual_seed(1000 + seed)
+    return (torch.randn(*shape, generator=g, device='cuda') * scale).to(dtype)
+
+
+def act64(z, act):
+    f = torch.nn.functional
+    return {None: lambda t: t, 'silu': f.silu, 'gelu': f.gelu, 'relu': f.relu}[act](z)
+
+
+def slope64(z, act):
+    z = z.clone().requires_grad_()
+    return torch.autograd.grad(act64(z, act).sum(), z)[0] if act else torch.ones_like(z)
+
+
+def product_bound(a, b, dtype):
+    """|error| of a b^T: a (m, k), b (n, k) in 64 bits."""
+    k = a.shape[1]
+    return (PAIR[dtype] + (k + 8) * 2.0 ** -24) * (a.abs() @ b.abs().t())
+
+
+def close(got, ref, bound, dtype):
+    got = got.double()
+    assert got.shape == ref.shape
+    err, allowed = (got - ref).abs(), bound + HALF[dtype] * ref.abs() + 1e-30
+    assert bool(torch.isfinite(got).all())
+    worst = float((err / allowed).max()) if err.numel() else 0.0
+    assert worst <= 1.0, f'{worst:.3g} of the allowed error'
+
+
+def forward_reference(x, w, b, act, r):
+    x, w = x.double(), w.double()
+    z = x @ w.t() + (b.double() if b is not None else 0)
+    y = act64(z, act) + (r.double() if r is not None else 0)
+    return z, y
+
+
+def forward_bound(x, w, b, act, r, z, dtype):
+    e = product_bound(x.double(), w.double(), dtype) + 2.0 ** -23 * z.abs()
+    # no activation is steeper than 1.13; the float32 activation and the sum with r are off by a few steps
+    return 1.13 * e + 16 * 2.0 ** -24 * (z.abs() + 1) + (2.0 ** -23 * r.double().abs() if r is not None else 0)
+
+
+def check_linear(mx, x, w, b, act, r, backward=True):
+    dtype = x.dtype
+    leaves = [None if t is None else t.detach().requires_grad_() for t in (x, w, b, r)]
+    x, w, b, r = leaves
+    z, y64 = forward_reference(x.detach(), w.detach(), None if b is None else b.detach(), act, None if r is None else r.detach())
+    fb = forward_bound(x.detach(), w.detach(), b, act, None if r is None else r.detach(), z, dtype)
+    with torch.no_grad():
+        close(mx.linear(x, w, b, act, r), y64, fb, dtype)
+    if not backward:
+        return
+    y = mx.linear(x, w, b, act, r)
+    close(y.detach(), y64, fb, dtype)
+    dy = randn(*y.shape, seed=77, dtype=dtype)
+    wanted = [t for t in leaves if t is not None]
+    grads = dict(zip([n for n, t in zip('xwbr', leaves) if t is not None], torch.autograd.grad(y, wanted, dy)))
+    x64, w64, d64 = x.detach().double(), w.detach().double(), dy.double()
+    dz = d64 * slope64(z, act)
+    ez = product_bound(x64, w64, dtype) + (2.0 ** -23 + HALF[dtype]) * z.abs() + 2.0 ** -23
+    # slopes change by at most 0.8 per unit of z (silu 0.5, gelu 0.8); relu's jumps where z may have either sign
+    edz = d64.abs() * (0.8 * ez + 16 * 2.0 ** -24 * (1 + z.abs())) if act else torch.zeros_like(dz)
+    if act == 'relu':
+        edz = d64.abs() * (z.abs() <= ez)
+    db_bound = edz.sum(0) + (dz.shape[0] + 8) * 2.0 ** -24 * dz.abs().sum(0)
+    if dtype == torch.bfloat16 and act:
+        edz = edz + HALF[dtype] * (dz.abs() + edz)
+    close(grads['x'], dz @ w64, product_bound(dz.abs() + edz, w64.t().contiguous(), dtype) + edz @ w64.abs(), dtype)
+    close(grads['w'], dz.t().contiguous() @ x64,
+          product_bound((dz.abs() + edz).t().contiguous(), x64.t().contiguous(), dtype) + edz.t().contiguous() @ x64.abs(), dtype)
+    if b is not None:
+        close(grads['b'], dz.sum(0), db_bound, dtype)
+    if r is not None:
+        assert torch.equal(grads['r'], dy)
+
+
+SIZES = [(1, 1, 1), (1, 64, 40), (2, 7, 3), (3, 130, 65), (7, 129, 9), (8, 256, 130), (9, 64, 64), (17, 33, 31), (33, 8, 200),
+         (64, 64, 64), (65, 200, 63), (129, 72, 257), (300, 1000, 20), (1000, 24, 300)]
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('m, k, n', SIZES)
+def test_linear_against_64_bits(mx, m, k, n, dtype):
+    acts = [None, 'silu', 'gelu', 'relu']
+    act = acts[(m + k + n) % 4]
+    x, w = randn(m, k, dtype=dtype), randn(n, k, seed=1, dtype=dtype, scale=k ** -0.5)
+    check_linear(mx, x, w, randn(n, seed=2, dtype=dtype), act, randn(m, n, seed=3, dtype=dtype))
+    check_linear(mx, x, w, None, acts[(m + k + n + 1) % 4], None)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('act', [None, 'silu', 'gelu', 'relu'])
+def test_linear_activations(mx, act, dtype):
+    for m in (5, 70):
+        x, w = randn(m, 96, dtype=dtype, scale=3.0), randn(80, 96, seed=1, dtype=dtype, scale=0.2)
+        check_linear(mx, x, w, randn(80, seed=2, dtype=dtype), act, randn(m, 80, seed=3, dtype=dtype))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('m, k, n', [(2100, 264, 2050), (4000, 96, 4100), (50, 4000, 72)])
+def test_linear_tiles_and_split(mx, m, k, n, dtype):
+    """Sizes that reach the 128 and 256 wide tiles and the split reduction, ragged in every direction."""
+    x, w = randn(m, k, dtype=dtype), randn(n, k, seed=1, dtype=dtype, scale=k ** -0.5)
+    check_linear(mx, x, w, randn(n, seed=2, dtype=dtype), 'silu', randn(m, n, seed=3, dtype=dtype))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('m', [4, 40])
+def test_linear_strides_and_offsets(mx, m, dtype):
+    """Slices of wider buffers, unaligned starts, transposed and expanded views."""
+    k, n = 72, 48
+    wide = randn(m, k + 24, dtype=dtype)
+    w = randn(n, k, seed=1, dtype=dtype, scale=0.1)
+    for x in (wide[:, :k], wide[:, 8:8 + k], wide[:, 3:3 + k], randn(k, m, seed=5, dtype=dtype).t(),
+              randn(1, k, seed=6, dtype=dtype).expand(m, k), randn(2 * m, k, seed=7, dtype=dtype)[::2]):
+        check_linear(mx, x, w, None, 'silu', None)
+    check_linear(mx, wide[:, :k], randn(k, n, seed=8, dtype=dtype, scale=0.1).t(), randn(2 * n, seed=9, dtype=dtype)[::2],
+                 'gelu', randn(n, m, seed=10, dtype=dtype).t())
+    flat = randn(m * k + 1, seed=11, dtype=dtype)[1:].view(m, k)
+    check_linear(mx, flat, w, randn(n + 1, seed=12, dtype=dtype)[1:], 'relu', randn(m * n + 1, seed=13, dtype=dtype)[1:].view(m, n))
+    # a gradient without memory of its own (a sum's), and one in another order
+    x = wide[:, :k].detach().requires_grad_()
+    mx.linear(x, w, None, 'silu').sum().backward()
+    z = x.detach().double() @ w.double().t()
+    ref = slope64(z, 'silu') @ w.double()
+    assert float((x.grad.double() - ref).norm() / ref.norm()) < 4 * HALF[dtype] + 1e-5
+
+
+def test_linear_shapes_of_more_axes(mx):
+    x, w, b = randn(2, 3, 5, 40), randn(24, 40, seed=1), randn(24, seed=2)
+    y = mx.linear(x, w, b, 'silu')
+    assert y.shape == (2, 3, 5, 24)
+    assert torch.equal(y.view(-1, 24), mx.linear(x.view(-1, 40), w, b, 'silu'))
+    one = mx.linear(x[0, 0, 0], w, b, 'silu')
+    assert one.shape == (24,)
+    z = x[0, 0, 0].double() @ w.double().t() + b.double()
+    close(one, act64(z, 'silu'), forward_bound(x[0, 0, :1], w, b, 'silu', None, z[None], torch.float32)[0], torch.float32)
+    for lead in ((0,), (2, 0)):
+        x0 = torch.zeros(*lead, 40, device='cuda', requires_grad=True)
+        w0 = w.clone().requires_grad_()
+        y0 = mx.linear(x0, w0, b, 'silu')
+        assert y0.shape == lead + (24,)
+        y0.sum().backward()
+        assert x0.grad.shape == x0.shape and float(w0.grad.abs().max()) == 0.0
+
+
+@pytest.mark.parametrize('m', [3, 30])
+def test_linear_float32_keeps_the_range(mx, m):
+    """Rows of very different magnitude, the smallest and the largest: every row keeps its 22 bits."""
+    k, n = 200, 50
+    scale = torch.logspace(-36, 17, m, device='cuda', dtype=torch.float64)
+    x = (randn(m, k).double() * scale[:, None]).float()
+    w = (randn(n, k, seed=1).double() * torch.logspace(-3, 18, n, device='cuda', dtype=torch.float64)[:, None]).float()
+    ref = x.double() @ w.double().t()
+    close(mx.linear(x, w), ref, product_bound(x.double(), w.double(), torch.float32) + 2.0 ** -149, torch.float32)
+    x[m // 2] = 0
+    assert float(mx.linear(x, w)[m // 2].abs().max()) == 0.0
+    # what is no number stays in its row
+    x[1, 5] = float('nan')
+    x[2, 7] = float('inf')
+    y = mx.linear(x, w)
+    assert bool(torch.isnan(y[1]).all()) and not bool(torch.isfinite(y[2]).any())
+    keep = [i for i in range(m) if i not in (1, 2)]
+    assert bool(torch.isfinite(y[keep]).all())
+
+
+def test_linear_only_wanted_gradients(mx):
+    x, w, b = randn(20, 40), randn(24, 40, seed=1), randn(24, seed=2)
+    dy = randn(20, 24, seed=3)
+    full = torch.autograd.grad(mx.linear(*(t.requires_grad_() for t in (x, w, b)), 'silu'), (x, w, b), dy)
+    for i in range(3):
+        leaves = [t.detach().requires_grad_(i == q) for q, t in enumerate((x, w, b))]
+        got, = torch.autograd.grad(mx.linear(*leaves, 'silu'), leaves[i], dy)
+        assert torch.equal(got, full[i])
+
+
+def test_linear_gradient_against_differences(mx):
+    """float32, central differences of the 64-bit layer along random directions."""
+    x, w, b = randn(33, 20), randn(17, 20, seed=1), randn(17, seed=2)
+    for act in ('silu', 'gelu'):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        dy = randn(33, 17, seed=4)
+        grads = torch.autograd.grad(mx.linear(*leaves, act), leaves, dy)
+        for q in range(3):
+            d = randn(*leaves[q].shape, seed=20 + q).double()
+            h = 1e-4
+            vals = []
+            for s in (h, -h):
+                a = [t.detach().double() for t in leaves]
+                a[q] = a[q] + s * d
+                vals.append(float((act64(a[0] @ a[1].t() + a[2], act) * dy.double()).sum()))
+            slope, got = (vals[0] - vals[1]) / (2 * h), float((grads[q].double() * d).sum())
+            size = float((grads[q].double().abs() * d.abs()).sum())
+            # truncation: h^2 / 6 of a third derivative of order one per element; arithmetic: 2^-20 of the magnitudes
+            assert abs(slope - got) <= (2.0 ** -20 + 100 * h * h) * size
+
+
+def test_linear_refuses(mx):
+    x, w = randn(4, 8), randn(6, 8, seed=1)
+    for bad in (dict(x=x.half()), dict(weight=w.bfloat16()), dict(weight=w[0]), dict(weight=randn(6, 9)), dict(bias=randn(5)),
+                dict(bias=randn(6).bfloat16()), dict(residual=randn(4, 5)), dict(residual=randn(1, 6)), dict(weight=w.cpu()),
+                dict(activation='swish'), dict(weight=w[:, :0], x=x[:, :0])):
+        with pytest.raises(ValueError):
+            mx.linear(**dict(dict(x=x, weight=w), **bad))
+
+
+# ---------------------------------------------------------------------------------------------
+# orthogonalisation
+# ---------------------------------------------------------------------------------------------
+def orth64(g, steps=5, eps=1e-7):
+    a, b, c = NS
+    x = g.double()
+    x = x / (x.norm() + eps)
+    tall = x.shape[0] > x.shape[1]
+    x = x.t() if tall else x
+    for _ in range(steps):
+        s = x @ x.t()
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return x.t() if tall else x
+
+
+# A step multiplies a small singular value by 3.4445: five of them multiply the half step of float32 by 485
+ORTH_TOL = {torch.float32: 3.4445 ** 5 * 2.0 ** -24, torch.bfloat16: 3.4445 ** 5 * 2.0 ** -24 + 2.0 ** -8}
+
+
+def check_orth(got, g, **kw):
+    for i in range(g.shape[0]):
+        ref = orth64(g[i], **kw)
+        assert float((got[i].double() - ref).norm()) <= ORTH_TOL[g.dtype] * float(ref.norm())
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('batch, rows, cols', [(1, 1, 1), (3, 1, 7), (3, 7, 1), (1, 16, 27), (1, 27, 16), (2, 33, 31), (2, 64, 64), (1, 65, 130),
+                                               (3, 130, 65), (1, 128, 1152), (1, 255, 257), (5, 300, 40), (1, 1000, 333), (140, 20, 50)])
+def test_orthogonalize_against_64_bits(mx, batch, rows, cols, dtype):
+    g = randn(batch, rows, cols, dtype=dtype, scale=1e-3)
+    check_orth(mx.orthogonalize(g), g)
+
+
+def test_orthogonalize_large_tiles(mx):
+    for batch, rows, cols in ((1, 2100, 2300), (6, 1050, 1100)):
+        g = randn(batch, rows, cols)
+        check_orth(mx.orthogonalize(g), g)
+
+
+def test_orthogonalize_brings_singular_values_near_one(mx):
+    g = randn(1, 96, 300)
+    s = torch.linalg.svdvals(mx.orthogonalize(g)[0].cpu().double())
+    assert float(s.min()) > 0.6 and float(s.max()) < 1.25
+
+
+def test_orthogonalize_forms(mx):
+    g = randn(4, 40, 24)
+    whole = mx.orthogonalize(g)
+    assert torch.equal(mx.orthogonalize(g.view(2, 2, 40, 24)).view(4, 40, 24), whole)
+    assert torch.equal(mx.orthogonalize(g[2]), whole[2])
+    assert torch.equal(mx.orthogonalize(g), whole)                                  # the same bits every time
+    assert torch.equal(mx.orthogonalize(g.transpose(1, 2).contiguous().transpose(1, 2)), whole)
+    twin = g.clone()
+    assert mx.orthogonalize(twin, out=twin) is twin and torch.equal(twin, whole)    # in place
+    off = torch.empty(4 * 40 * 24 + 1, device='cuda')[1:].view(4, 40, 24)           # unaligned source and result
+    off.copy_(g)
+    assert torch.equal(mx.orthogonalize(off, out=off), whole)
+    check_orth(mx.orthogonalize(g, steps=1), g, steps=1)
+    check_orth(mx.orthogonalize(g, steps=3, eps=0.5), g, steps=3, eps=0.5)
+    # scale does not matter, also where squares leave float32's range
+    for s in (1e-18, 1e25):
+        assert float((mx.orthogonalize(g * s, eps=0.0) - mx.orthogonalize(g, eps=0.0)).norm() / whole.norm()) < 2 * ORTH_TOL[torch.float32]
+    assert mx.orthogonalize(g[:0]).shape == (0, 40, 24)
+    for bad in (g[0, 0], g.half(), g.cpu()):
+        with pytest.raises(ValueError):
+            mx.orthogonalize(bad)
+    for kw in (dict(steps=0), dict(steps=40), dict(eps=-1.0), dict(out=whole[:2]), dict(out=whole.transpose(1, 2)), dict(out=whole.bfloat16())):
+        with pytest.raises(ValueError):
+            mx.orthogonalize(g, **kw)
+
+
+def test_orthogonalize_zero_and_no_numbers(mx):
+    g = randn(5, 40, 70)
+    g[1] = 0
+    g[2, 3, 4] = float('nan')
+    g[3, 39, 69] = float('inf')
+    y = mx.orthogonalize(g)
+    assert float(y[1].abs().max()) == 0.0
+    assert bool(torch.isnan(y[2]).all()) and bool(torch.isnan(y[3]).all())
+    check_orth(y[[0, 4]], g[[0, 4]])
+
+
+# ---------------------------------------------------------------------------------------------
+# optimizer step
+# ---------------------------------------------------------------------------------------------
+def muon64(p, g, m, e, matrices, lr, mu, nesterov, wd, d, gs):
+    p, g, m = p.double(), g.double() * gs, m.double()
+    e = None if e is None else e.double()
+    for o, r, c in matrices:
+        s = slice(o, o + r * c)
+        m[s] = mu * m[s] + g[s]
+        u = g[s] + mu * m[s] if nesterov else m[s]
+        p[s] = p[s] * (1 - lr * wd) - lr * 0.2 * math.sqrt(max(r, c)) * orth64(u.view(r, c)).reshape(-1)
+        if e is not None:
+            e[s] = d * e[s] + (1 - d) * p[s]
+    return p, m, e
+
+
+@pytest.mark.parametrize('ema, nesterov', [(True, True), (False, False)])
+def test_muon_step_against_64_bits(mx, ema, nesterov):
+    shapes = [(16, 27), (32, 64), (1, 5), (5, 1), (33, 7), (64, 576), (130, 129), (3, 3)]
+    matrices, at = [], 4
+    for i, (r, c) in enumerate(shapes):
+        matrices.append((at, r, c))
+        at += r * c + (i % 3) * 5                       # odd offsets too, and gaps
+    p, g, m = randn(at + 9, scale=0.03), randn(at + 9, seed=1, scale=1e-3), randn(at + 9, seed=2, scale=1e-3)
+    e = randn(at + 9, seed=3, scale=0.03) if ema else None
+    args = (0.01, 0.9, nesterov, 0.1, 0.7, 0.5)
+    rp, rm, re = muon64(p, g, m, e, matrices, *args)
+    p1, g1, m1, e1 = p.clone(), g.clone(), m.clone(), None if e is None else e.clone()
+    mx.muon_step(p1, g1, m1, matrices, lr=0.01, momentum_decay=0.9, nesterov=nesterov, weight_decay=0.1, ema=e1, ema_decay=0.7,
+                 grad_scale=0.5)
+    assert torch.equal(g1, g)
+    assert float((m1.double() - rm).abs().max()) <= 4 * 2.0 ** -24 * float(rm.abs().max())
+    covered = torch.zeros_like(p, dtype=torch.bool)
+    for o, r, c in matrices:
+        s = slice(o, o + r * c)
+        covered[s] = True
+        step = 0.01 * 0.2 * math.sqrt(max(r, c)) * math.sqrt(min(r, c)) * 1.25     # Frobenius norm of the update, at most
+        allowed = ORTH_TOL[torch.float32] * step + 4 * 2.0 ** -24 * float(rp[s].norm())
+        assert float((p1[s].double() - rp[s]).norm()) <= allowed
+        if ema:
+            assert float((e1[s].double() - re[s]).norm()) <= allowed + 4 * 2.0 ** -24 * float(re[s].norm())
+    for new, old in ((p1, p), (m1, m)) + (((e1, e),) if ema else ()):
+        assert torch.equal(new[~covered], old[~covered])                         # what lies between stays
+    # the same bits again
+    p2, m2 = p.clone(), m.clone()
+    mx.muon_step(p2, g, m2, mx.MatrixTable(matrices), lr=0.01, momentum_decay=0.9, nesterov=nesterov, weight_decay=0.1, grad_scale=0.5)
+    assert torch.equal(p2, p1) and torch.equal(m2, m1)
+
+
+def test_muon_step_many_matrices(mx):
+    """More matrices than one launch's table holds."""
+    matrices = [(i * 64, 8, 8) for i in range(300)]
+    p, g, m = randn(300 * 64), randn(300 * 64, seed=1), torch.zeros(300 * 64, device='cuda')
+    rp, rm, _ = muon64(p, g, m, None, matrices, 0.1, 0.95, True, 0.0, 0.0, 1.0)
+    mx.muon_step(p, g, m, matrices, lr=0.1)
+    assert float((p.double() - rp).norm() / rp.norm()) < 1e-6 and float((m.double() - rm).abs().max()) == 0.0
+
+
+def test_muon_step_refuses(mx):
+    p = randn(100)
+    for bad in (dict(grad=randn(99)), dict(momentum=randn(100).bfloat16()), dict(ema=randn(100, 1)), dict(matrices=[(90, 3, 4)]),
+                dict(matrices=[(0, 5, 5), (24, 2, 2)]), dict(matrices=[]), dict(steps=0), dict(eps=-1.0), dict(grad=randn(200)[::2])):
+        kw = dict(dict(param=p, grad=randn(100, seed=1), momentum=randn(100, seed=2), matrices=[(0, 8, 8)], lr=0.1), **bad)
+        with pytest.raises(ValueError):
+            mx.muon_step(**kw)
+
+
+def test_adam_over_ranges_equals_adam():
+    from objectdetection_amd import matrix
+    from objectdetection_amd._lib import lib, check
+    n = 9000
+    bufs = [randn(n, seed=i, scale=0.1).abs() for i in range(5)]
+    whole = [b.clone() for b in bufs]
+    part = [b.clone() for b in bufs]
+    ranges = [(0, 1), (3, 2500), (2600, 1024), (3700, 5300)] + [(3624 + i, 1) for i in range(0, 60, 2)]
+    a = np.array(ranges, dtype=matrix.RANGE_DTYPE)
+    st = torch.cuda.current_stream().cuda_stream
+    args = (0.01, 0.937, 0.999, 1e-8, 5e-4, 3, 0.9, 0.5, st)
+    check(lib.odamd_adam_ema_step(*(b.data_ptr() for b in whole), n, *args))
+    check(lib.odamd_adam_ema_ranges_step(*(b.data_ptr() for b in part), a.ctypes.data, len(a), *args))
+    inside = torch.zeros(n, dtype=torch.bool, device='cuda')
+    for o, k in ranges:
+        inside[o:o + k] = True
+    for w, p, b in zip(whole, part, bufs):
+        assert torch.equal(p[inside], w[inside]) and torch.equal(p[~inside], b[~inside])
+
+
+# ---------------------------------------------------------------------------------------------
+# in use: streams, graphs, a training run
+# ---------------------------------------------------------------------------------------------
+def test_calls_on_two_streams_at_once(mx):
+    xs = [randn(40, 300, seed=i) for i in range(4)]
+    w = randn(70, 300, seed=9)
+    ref = [(mx.linear(x, w, None, 'silu'), mx.orthogonalize(x)) for x in xs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i, x in enumerate(xs):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append((mx.linear(x, w, None, 'silu'), mx.orthogonalize(x)))
+    torch.cuda.synchronize()
+    for (a, b), (c, d) in zip(ref, got):
+        assert torch.equal(a, c) and torch.equal(b, d)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+def test_captured_and_replayed(mx, dtype):
+    """Forward, backward, orthogonalisation and optimizer step in one graph; other inputs between the replays, eager work too."""
+    x, w, b, r = randn(30, 96, dtype=dtype), randn(64, 96, seed=1, dtype=dtype), randn(64, seed=2, dtype=dtype), randn(30, 64, seed=3, dtype=dtype)
+    dy = randn(30, 64, seed=4, dtype=dtype)
+    p, g, m = randn(2000), randn(2000, seed=5), torch.zeros(2000, device='cuda')
+    table = mx.MatrixTable([(0, 16, 27), (500, 30, 50)])
+
+    def work(x, p, m):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        y = mx.linear(*leaves[:3], 'silu', leaves[3])
+        grads = torch.autograd.grad(y, leaves, dy)
+        mx.muon_step(p, g, m, table, lr=0.01)
+        return (y.detach(), *grads, mx.orthogonalize(grads[1]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work(x.clone(), p.clone(), m.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    xs, ps, ms = x.clone(), p.clone(), m.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work(xs, ps, ms)
+    pe, me = p.clone(), m.clone()
+    for turn in range(4):
+        xs.copy_(randn(30, 96, seed=50 + turn, dtype=dtype))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref = work(xs.clone(), pe, me)
+        for a, c in zip(out, ref):
+            assert torch.equal(a, c)
+        assert torch.equal(ps, pe) and torch.equal(ms, me)
+
+
+def test_layer_trains_in_both_types(mx):
+    from objectdetection_amd.model import layer
+    torch.manual_seed(3)
+    net = torch.nn.ModuleList([layer.linear(40, 96, 'silu'), layer.linear(96, 40)]).cuda()
+    for dtype in (torch.float32, torch.bfloat16):
+        x = randn(50, 40, dtype=dtype)
+        net.zero_grad()
+        out = net[1](net[0](x), residual=x)
+        out.float().square().mean().backward()
+        leaf = [p.detach().to(dtype).double().requires_grad_() for p in net.parameters()]
+        z = torch.nn.functional.silu(x.double() @ leaf[0].t() + leaf[1]) @ leaf[2].t() + leaf[3] + x.double()
+        ref = torch.autograd.grad(z.square().mean(), leaf)
+        for p, q in zip(net.parameters(), ref):
+            # five roundings to the type between the input and a gradient
+            assert p.grad.dtype == torch.float32
+            assert float((p.grad.double() - q).norm() / q.norm()) < 5 * HALF[dtype] + 1e-5
+
+
+def test_detector_trains_with_muon():
+    """train_class with --optimizer muon: one step equals the 64-bit step on the gradients the backward pass left, Adam on
+    what lies between; a second trainer resumed from the saved state continues with the same bits."""
+    from objectdetection_amd.train_class import train_class, synthetic_dataset, FusedMuon
+    from oracle import patterns, training as otrain
+    a = patterns.default_args(input_size=64, output_class=3)
+    a.__dict__.update(device='cuda', batch=2, epoch=1, lr_start=0.001, lr_end_ratio=0.1, lr_end_epoch=10, warmup_ratio=0.01,
+                      regularization='L2', r_value=0.0005, ema=True, distributed=False, local_rank=0, weight_path='',
+                      weight_again=True, print_info=False, synthetic_images=8, save_path=None, amp=False, optimizer='muon')
+    ds = synthetic_dataset(a, 4, seed=5)
+    batch = ds.collate_fn([ds[0], ds[1]])
+    torch.manual_seed(1)
+    tc = train_class(a, dataloader=[batch] * 4, val_dataloader=[])
+    assert isinstance(tc.optimizer, FusedMuon)
+    tc.model.train()
+    st = tc.model.train_state()
+    image, screen, expend = batch[0].cuda(), batch[1], batch[2]
+    tc.train_step(image, screen, expend)                    # the state has moved once: momentum is not zero
+    p0, m0, v0, e0 = st.param.clone(), st.exp_avg.clone(), st.exp_avg_sq.clone(), st.ema_param.clone()
+    lr, updates = tc.optimizer.param_groups[0]['lr'], st.ema_updates
+    tc.train_step(image, screen, expend)
+    torch.cuda.synchronize()
+    matrices = [tuple(int(v) for v in e) for e in tc.optimizer.table.table.tolist()]
+    d = otrain.ema_decay(updates + 1)
+    rp, rm, re = muon64(p0, st.grad, m0, e0, matrices, lr, 0.95, True, 0.0005, d, 1.0)
+    for o, r, c in matrices:
+        s = slice(o, o + r * c)
+        step = lr * 0.2 * math.sqrt(r * c) * 1.25
+        allowed = ORTH_TOL[torch.float32] * step + 8 * 2.0 ** -24 * float(rp[s].norm())
+        assert float((st.param[s].double() - rp[s]).norm()) <= allowed
+        assert float((st.ema_param[s].double() - re[s]).norm()) <= allowed + 8 * 2.0 ** -24 * float(re[s].norm())
+    for o, n in tc.optimizer.rest.tolist():
+        s = slice(o, o + n)
+        p, m, v = p0[s].cpu().clone(), m0[s].cpu().clone(), v0[s].cpu().clone()
+        otrain.adam_step(p, st.grad[s].cpu(), m, v, 2, lr, weight_decay=0.0005)
+        np.testing.assert_allclose(st.param[s].cpu().numpy(), p.numpy(), rtol=1e-5, atol=0.01 * lr)
+    saved = {k: v.clone() if torch.is_tensor(v) else v for k, v in tc.optimizer.state_dict().items()}
+    twin = train_class(a, dataloader=[batch] * 4, val_dataloader=[])
+    ts = twin.model.train_state()
+    for n in ('param', 'buffers', 'counters', 'ema_param', 'ema_buffers'):
+        getattr(ts, n).copy_(getattr(st, n))
+    ts.ema_updates = st.ema_updates
+    twin.optimizer.load_state_dict(saved)
+    for g, h in zip(twin.optimizer.param_groups, tc.optimizer.param_groups):
+        g['lr'] = h['lr']
+    twin.model.train()
+    tc.train_step(image, screen, expend)
+    twin.train_step(image, screen, expend)
+    assert torch.equal(st.param, ts.param) and torch.equal(st.exp_avg, ts.exp_avg)
