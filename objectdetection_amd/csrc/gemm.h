@@ -12,7 +12,9 @@
 //
 // A workgroup holds a TM x TN tile of C in registers (WGM x WGN waves) and walks K in chunks of 128 bytes per row (64
 // bf16 values, or 32 pairs).  A chunk of A and B goes global -> LDS without passing registers
-// (global_load_lds_dwordx4), into the buffer that the chunk before the last one left; one barrier per chunk.  An LDS row is
+// (global_load_lds_dwordx4), NBUF - 1 rounds ahead; one barrier per round.  A round is one chunk, or KG of them, one for each
+// of KG groups of WGM x WGN waves whose sums are added at the end: where there are few tiles, a tile's chunks are a chain of
+// latencies (barrier, LDS reads, matrix instructions on one accumulator), and more waves on it hide them.  An LDS row is
 // eight 16-byte pieces; piece p of row r lies in slot p ^ (r & 7), so the eight lanes that read the same piece of eight
 // consecutive rows touch eight different slots.  The DMA writes LDS in lane order: the exchange of the slots is in the global
 // address each lane reads.
@@ -34,6 +36,12 @@ __device__ __forceinline__ void gemm_dma16(const char* g, char* l) {
 __device__ __forceinline__ int gemm_xcd_remap(int bid, int n) {
     const int q = n >> 3, r = n & 7, xcd = bid & 7, slot = bid >> 3;
     return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + slot;
+}
+
+// The same in stretches of 128 tiles, 16 per XCD: where tiles differ in length, every XCD gets its share of the long ones.
+__device__ __forceinline__ int gemm_xcd_stretch(int bid, int n) {
+    const int from = bid & ~127, len = min(128, n - from);
+    return from + gemm_xcd_remap(bid - from, len);
 }
 
 // Tile `t` of an mt x nt grid, walked in bands of 8 tile rows: the tiles in flight share 8 row blocks of A and few of B.
@@ -59,7 +67,7 @@ struct GemmOperand {
     int rows;          // rows past the last one are read as the last one; their results are not stored
 };
 
-template <int PL, bool F16>
+template <bool F16>
 __device__ __forceinline__ f32x16_t gemm_mma(u32x4 a, u32x4 b, f32x16_t c) {
     if constexpr (F16)
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
@@ -67,19 +75,22 @@ __device__ __forceinline__ f32x16_t gemm_mma(u32x4 a, u32x4 b, f32x16_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16v8_t, a), __builtin_bit_cast(bf16v8_t, b), c, 0, 0, 0);
 }
 
-template <int PL_, bool F16_, int TM_, int TN_, int WGM_, int WGN_>
+template <int PL_, bool F16_, int TM_, int TN_, int WGM_, int WGN_, int KG_, int NBUF_>
 struct GemmTile {
-    static constexpr int PL = PL_, TM = TM_, TN = TN_, WGM = WGM_, WGN = WGN_;
+    static constexpr int PL = PL_, TM = TM_, TN = TN_, WGM = WGM_, WGN = WGN_, KG = KG_, NBUF = NBUF_;
     static constexpr bool F16 = F16_;
-    static constexpr int NW = WGM * WGN, THREADS = 64 * NW;
+    static constexpr int NW = WGM * WGN, THREADS = 64 * NW * KG;
     static constexpr int WTM = TM / WGM, WTN = TN / WGN, FM = WTM / 32, FN = WTN / 32;
     static constexpr int BK = PL == 1 ? 64 : 32;                    // values of K per chunk
     static constexpr int BUF = (TM + TN) * 128;                     // bytes of one LDS buffer
     static constexpr int SLAB_LD = WTN + 4;                         // floats per row of a wave's epilogue slab
     static constexpr int SLAB = 32 * SLAB_LD * 4;
-    static constexpr int LDS = 2 * BUF > NW * SLAB ? 2 * BUF : NW * SLAB;
+    static constexpr int RING = NBUF * KG * BUF;                    // buffer of round i, group g: (i % NBUF) * KG + g
+    static constexpr int LDS = RING > NW * SLAB ? RING : NW * SLAB;
     static constexpr int NI = (TM + TN) / 8 / NW;                   // DMA instructions per wave and chunk
     static_assert((TM + TN) % (8 * NW) == 0 && TM % 8 == 0, "whole DMA instructions");
+    static_assert((KG - 1) * NW * FM * FN * 4096 <= RING, "the other groups' sums pass through the ring");
+    static_assert(NBUF >= 2 && NBUF <= 4 && LDS <= 160 * 1024, "LDS of a compute unit");
 
     f32x16_t acc[FM][FN];
 
@@ -87,7 +98,7 @@ struct GemmTile {
     // the rows are padded to whole chunks).
     __device__ __forceinline__ void run(const GemmOperand& a, const GemmOperand& b, int m0, int n0, int c0, int c1, int k_len,
                                         char* lds) {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int lane = threadIdx.x & 63, any = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = any / NW, wave = any % NW;
         const int wm = wave / WGN, wn = wave % WGN, r = lane & 31, h = lane >> 5;
 #pragma unroll
         for (int i = 0; i < FM; ++i)
@@ -106,26 +117,35 @@ struct GemmTile {
             const GemmOperand& o = is_a ? a : b;
             src[j] = o.p + (long long)min(row, o.rows - 1) * o.ld + piece * 16;
         }
-        auto issue = [&](int c, char* buf) {
+        // Round i of this group: chunk c0 + i KG + group; past the last chunk zeros, so that the groups stay in step
+        auto issue = [&](int i) {
+            const int c = c0 + i * KG + group;
+            char* buf = lds + (i % NBUF * KG + group) * BUF;
             const long long at = (long long)c * 128;
-            if (PL == 2 || (c + 1) * BK <= k_len) {
+            if ((KG == 1 || c < c1) && (PL == 2 || (c + 1) * BK <= k_len)) {
 #pragma unroll
                 for (int j = 0; j < NI; ++j) gemm_dma16(src[j] + at, buf + (wave + j * NW) * 1024);
             } else {
-                const bool in = c * BK + piece * 8 < k_len;
+                const bool in = (KG == 1 || c < c1) && (PL == 2 || c * BK + piece * 8 < k_len);
 #pragma unroll
                 for (int j = 0; j < NI; ++j) gemm_dma16(in ? src[j] + at : (const char*)g_gemm_zero, buf + (wave + j * NW) * 1024);
             }
         };
-        if (c0 >= c1) return;
-        issue(c0, lds);
+        const int rounds = (c1 - c0 + KG - 1) / KG;
+#pragma unroll
+        for (int q = 0; q < NBUF - 1; ++q)
+            if (q < rounds) issue(q);
         const int a_off = (wm * WTM + r) * 128, b_off = TM * 128 + (wn * WTN + r) * 128, sw = r & 7;
-        for (int c = c0; c < c1; ++c) {
-            char* buf = lds + ((c - c0) & 1) * BUF;
-            // every wave's pieces of chunk c are in LDS, every read of the other buffer has returned
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        for (int i = 0; i < rounds; ++i) {
+            // this wave's pieces of round i have landed (those of up to NBUF - 2 later rounds may still be on their way)
+            // and its reads of round i - 1 have returned; behind the barrier that holds for every wave
+            const int ahead = min(NBUF - 2, rounds - 1 - i);
+            if (NBUF > 3 && ahead == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NBUF > 3 ? 2 * NI : 0) : "memory");
+            else if (NBUF > 2 && ahead == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NBUF > 2 ? NI : 0) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
-            if (c + 1 < c1) issue(c + 1, lds + ((c - c0 + 1) & 1) * BUF);
+            const char* buf = lds + (i % NBUF * KG + group) * BUF;
+            if (i + NBUF - 1 < rounds) issue(i + NBUF - 1);
 #pragma unroll
             for (int s = 0; s < BK / 16; ++s) {
                 u32x4 fa[PL][FM], fb[PL][FN];
@@ -133,19 +153,51 @@ struct GemmTile {
                 for (int q = 0; q < PL; ++q) {
                     const int slot = ((4 * q + 2 * s + h) ^ sw) * 16;
 #pragma unroll
-                    for (int i = 0; i < FM; ++i) fa[q][i] = *(const u32x4*)(buf + a_off + i * 4096 + slot);
+                    for (int x = 0; x < FM; ++x) fa[q][x] = *(const u32x4*)(buf + a_off + x * 4096 + slot);
 #pragma unroll
-                    for (int j = 0; j < FN; ++j) fb[q][j] = *(const u32x4*)(buf + b_off + j * 4096 + slot);
+                    for (int y = 0; y < FN; ++y) fb[q][y] = *(const u32x4*)(buf + b_off + y * 4096 + slot);
                 }
                 // B is the instruction's row operand: a lane then holds one row m of C and runs of four columns n
 #pragma unroll
                 for (int q = 0; q < (PL == 1 ? 1 : 3); ++q)
 #pragma unroll
-                    for (int i = 0; i < FM; ++i)
+                    for (int x = 0; x < FM; ++x)
 #pragma unroll
-                        for (int j = 0; j < FN; ++j)
-                            acc[i][j] = gemm_mma<PL, F16>(fb[q == 1 ? PL - 1 : 0][j], fa[q == 2 ? PL - 1 : 0][i], acc[i][j]);
+                        for (int y = 0; y < FN; ++y)
+                            acc[x][y] = gemm_mma<F16>(fb[q == 1 ? PL - 1 : 0][y], fa[q == 2 ? PL - 1 : 0][x], acc[x][y]);
             }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();                               // every wave has read its last fragments: the ring is free
+        if constexpr (KG > 1) {
+            // the other groups leave their sums in LDS, the first adds them in order
+            const auto place = [&](int g, int x, int y, int q) {
+                return (f32x4_t*)(lds + ((((g - 1) * NW + wave) * FM * FN + x * FN + y) * 4 + q) * 1024 + lane * 16);
+            };
+            if (group > 0)
+#pragma unroll
+                for (int x = 0; x < FM; ++x)
+#pragma unroll
+                    for (int y = 0; y < FN; ++y)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            *place(group, x, y, q) = f32x4_t{acc[x][y][4 * q], acc[x][y][4 * q + 1], acc[x][y][4 * q + 2], acc[x][y][4 * q + 3]};
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            if (group == 0)
+#pragma unroll
+                for (int g = 1; g < KG; ++g)
+#pragma unroll
+                    for (int x = 0; x < FM; ++x)
+#pragma unroll
+                        for (int y = 0; y < FN; ++y)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const f32x4_t u = *place(g, x, y, q);
+                                acc[x][y][4 * q] += u[0]; acc[x][y][4 * q + 1] += u[1]; acc[x][y][4 * q + 2] += u[2]; acc[x][y][4 * q + 3] += u[3];
+                            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();                           // read before the slabs take the place
         }
     }
 
@@ -154,9 +206,8 @@ struct GemmTile {
     template <bool ROWS, bool COLS, typename FR, typename FC>
     __device__ __forceinline__ void hand_out(char* lds, FR&& rows, FC&& cols) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (KG > 1 && wave >= NW) return;                           // the first group holds the sums
         const int wm = wave / WGN, wn = wave % WGN, r = lane & 31, h = lane >> 5;
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();                               // every wave has read its last fragments
         float* slab = (float*)(lds + wave * SLAB);
         constexpr int LPR = WTN / 8, RPP = 64 / LPR;                // lanes per row, rows per pass
 #pragma unroll
@@ -212,6 +263,26 @@ __device__ __forceinline__ void store_split8(char* hi_at, const float v[8], floa
     }
     *(f16x8_t*)hi_at = hi;
     *(f16x8_t*)(hi_at + 64) = lo;
+}
+
+// ---- host: which tile ------------------------------------------------------------------------------------------------
+// Measured with pairs at 4096^3, 2048 x 1024 x 2048 and below: time of a chunk of one tile alone on a compute unit (0.69 us for
+// 128 x 128, 0.3 us for 64 x 64 with two wave groups), and its share of a unit's time where several tiles run there (0.87 and
+// 0.24 us; 2.75 us for 256 x 256, which fills a unit by itself).  The larger tile wins per product, the smaller one
+// spreads a small product over all 256 units: 4096 x 4096 x 4096 353 / 445 / 512 us in 256 / 128 / 64, 2048 x 1024 x 2048
+// - / 45 / 33 us.  bf16 chunks take two thirds of the time for every tile: the choice is the same.
+struct GemmLoad { double tiles = 0, chunks = 0, longest = 0; int kinds = 0; };   // chunks: summed over all tiles
+inline void gemm_load_add(GemmLoad& l, double tiles, double chunks) {
+    l.tiles += tiles;
+    l.chunks += tiles * chunks;
+    l.longest = chunks > l.longest ? chunks : l.longest;
+    ++l.kinds;
+}
+inline double gemm_time_us(int tile, const GemmLoad& l) {
+    const double alone = tile == 256 ? 2.75 : tile == 128 ? 0.69 : 0.3, share = tile == 256 ? 2.75 : tile == 128 ? 0.87 : 0.24;
+    // tiles of one length run in whole rounds
+    const double rounds = l.kinds == 1 ? (double)(((long long)l.tiles + 255) / 256) : l.chunks / (256.0 * l.longest);
+    return l.longest * (alone > share * rounds ? alone : share * rounds);
 }
 
 #endif

@@ -431,10 +431,10 @@ int lin_product(LinGemm g, LinSpace& ws, bool go, hipStream_t s) {
     if (plan.split > 1) g.part = (float*)ws.take((long long)plan.split * g.m * g.n * 4);
     if (!go) return 0;
     const long long blocks = (((long long)g.m + plan.tile - 1) / plan.tile) * ((g.n + plan.tile - 1) / plan.tile) * plan.split;
-    if (plan.tile == 256) return lin_launch<GemmTile<PL, F16, 256, 256, 2, 4>, DT, false>(g, blocks, s);
-    if (plan.tile == 128) return lin_launch<GemmTile<PL, F16, 128, 128, 2, 2>, DT, false>(g, blocks, s);
-    if (plan.split == 1) return lin_launch<GemmTile<PL, F16, 64, 64, 2, 2>, DT, false>(g, blocks, s);
-    const int rc = lin_launch<GemmTile<PL, F16, 64, 64, 2, 2>, DT, true>(g, blocks, s);
+    if (plan.tile == 256) return lin_launch<GemmTile<PL, F16, 256, 256, 4, 2, 1, 2>, DT, false>(g, blocks, s);
+    if (plan.tile == 128) return lin_launch<GemmTile<PL, F16, 128, 128, 2, 4, 1, 2>, DT, false>(g, blocks, s);
+    if (plan.split == 1) return lin_launch<GemmTile<PL, F16, 64, 64, 2, 2, 1, 2>, DT, false>(g, blocks, s);
+    const int rc = lin_launch<GemmTile<PL, F16, 64, 64, 2, 2, 1, 2>, DT, true>(g, blocks, s);
     if (rc != 0) return rc;
     const long long runs = (long long)g.m * ((g.n + 7) / 8);
     linear_join_kernel<DT><<<(int)((runs + 255) / 256 < 4096 ? (runs + 255) / 256 : 4096), 256, 0, s>>>(g);

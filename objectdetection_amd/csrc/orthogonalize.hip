@@ -6,11 +6,22 @@
 // (a, b, c) = (3.4445, -4.7750, 2.0315) five steps take singular values from 0.003 up to between 0.68 and 1.21 -- the values
 // never pass 1.21, so every entry of X and A stays under 1.5 and of P under 3.5.
 //
-// All products run on fp16 pairs (gemm.h, PL = 2) scaled by 2^12: the largest entry becomes 14 300, the smallest step
-// 2^-36.  Rounding to pairs costs 2^-22 of an entry; small singular values are multiplied by up to 3.4445 a step, so anything
-// coarser shows: bf16 products would leave a few percent in the result.
-// X is kept twice, by rows (X X^T reduces along n) and by columns (P X reduces along m): both products then read their
-// operands along the reduction.  A and P are symmetric: the tiles on and over the diagonal are computed, the rest mirrored.
+// Everything that happens to X is a polynomial in A_0 = X_0 X_0^T, so steps can also run on m x m matrices alone:
+//   X_t = Q X_0,   Q = P_t ... P_1,   A_(k+1) = P_k A_k P_k
+// with one product by X at the end of a phase of t steps: 1.5 m^2 n + (2 t - 1.5) m^3 multiply-adds for it (symmetric products
+// counted half) against t (1.5 m^2 n + 0.5 m^3).  What it costs is accuracy in the directions of small singular values: a
+// rounding of A grows by 3.4445^2 per step there, where a rounding of X grows by 3.4445.  Phases of two steps keep float32's
+// accuracy (error against 64 bits of 256 x 2304 noise with strong directions: 1.6e-6, one step a phase 1.9e-6) and serve
+// float32 results of matrices with n >= 2 m; squarer ones take one step a phase, which costs no more there.  Phases of
+// five serve bfloat16 results and the optimizer step: 3e-6 to 8e-5 on such matrices, under 8e-4 (3.4445^8 2^-24 = 1.2e-3)
+// where the singular values fall like 1 / i^2 or vanish; a bfloat16 result is rounded by 2e-3 and the step multiplies by the
+// learning rate.
+//
+// All products run on fp16 pairs (gemm.h, PL = 2) scaled by 2^12 (Q, which grows to 3.4445^k, by less): the largest entry
+// becomes 14 300, the smallest step 2^-36.  bf16 products would leave a few percent in the result.
+// X is kept twice, by rows (X X^T reduces along n) and by columns (Q X reduces along m): both products then read their
+// operands along the reduction.  The m x m matrices are symmetric: tiles on and over the diagonal are computed, the rest
+// mirrored.  All matrices of a call share every launch.
 #include "common.h"
 #include "odamd.h"
 
@@ -21,11 +32,14 @@ namespace {
 #include "gemm.h"
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
-constexpr float NS_SCALE = 4096.0f, NS_UNSCALE2 = 1.0f / (4096.0f * 4096.0f);
+constexpr float NS_SCALE = 4096.0f;
 constexpr int NS_GROUPS = 112;        // groups of one launch: their table travels in the kernel's arguments (4 KiB at most)
-constexpr int NS_PARTS = 256;         // partial sums of squares per matrix, at most
+constexpr int NS_PARTS = 512;         // partial sums of squares per matrix, at most
 
-enum { ST_NORM, ST_SPLIT, ST_A, ST_P, ST_X, ST_OUT };
+// stages: sums of squares, laying out, X X^T, P from A, products of square matrices, Q X, Q X to the caller
+enum { ST_NORM, ST_SPLIT, ST_A, ST_P, ST_Q, ST_X, ST_OUT };
+// square matrices: A, a product on the way to the next A, and three that P and Q take in turn
+enum { SQ_A, SQ_T, SQ_B, SQ_COUNT = 5 };
 
 // `count` matrices of one shape, one after the other
 struct NsGroup {
@@ -41,11 +55,17 @@ struct NsTable {
     int n, tiles;
     char* ws;
 };
-static_assert(sizeof(NsTable) <= 3800, "kernel arguments are limited to 4 KiB");
+// Up to two products of a stage: out = left right, squares by index, `scale` from the sum to the stored pair
+struct NsJobs {
+    int n, turn;         // turn: which of the two column copies of X is the current one
+    int left[2], right[2], out[2];
+    float scale[2];
+};
+static_assert(sizeof(NsTable) <= 3700, "kernel arguments are limited to 4 KiB");
 
 __host__ __device__ inline long long ns_up(long long v, int to) { return (v + to - 1) / to * to; }
 // Byte offsets within a matrix's workspace; end is its size.
-struct NsLayout { long long sums, x, xt0, xt1, a, p, end; };
+struct NsLayout { long long sums, x, xt0, xt1, sq, sq_size, end; };
 __host__ __device__ inline NsLayout ns_layout(int m, int n) {
     NsLayout l;
     const long long mp = ns_up(m, 32), np = ns_up(n, 32);
@@ -53,20 +73,20 @@ __host__ __device__ inline NsLayout ns_layout(int m, int n) {
     l.x = NS_PARTS * 8;
     l.xt0 = l.x + ns_up(m * np * 4, 256);
     l.xt1 = l.xt0 + ns_up(n * mp * 4, 256);
-    l.a = l.xt1 + ns_up(n * mp * 4, 256);
-    l.p = l.a + ns_up(m * mp * 4, 256);
-    l.end = l.p + ns_up(m * mp * 4, 256);
+    l.sq = l.xt1 + ns_up(n * mp * 4, 256);
+    l.sq_size = ns_up(m * mp * 4, 256);
+    l.end = l.sq + SQ_COUNT * l.sq_size;
     return l;
 }
-// Elements one workgroup of the norm pass takes: a multiple of four that keeps the partial sums within NS_PARTS.
+// Elements one workgroup of the norm pass takes: a multiple of eight that keeps the partial sums within NS_PARTS.
 __host__ __device__ inline long long ns_share(int m, int n) {
     const long long total = (long long)m * n, least = (total + NS_PARTS - 1) / NS_PARTS;
-    return least < 4096 ? 4096 : ns_up(least, 1024);
+    return least < 8192 ? 8192 : ns_up(least, 2048);
 }
 __host__ __device__ inline int ns_parts(int m, int n) { return (int)(((long long)m * n + ns_share(m, n) - 1) / ns_share(m, n)); }
 __host__ __device__ inline int ns_tiles(int stage, int tile, int m, int n) {
     const int mt = (m + tile - 1) / tile, nt = (n + tile - 1) / tile;
-    return stage == ST_NORM ? ns_parts(m, n) : stage == ST_A || stage == ST_P ? mt * (mt + 1) / 2 : mt * nt;
+    return stage == ST_NORM ? ns_parts(m, n) : stage == ST_A || stage == ST_P || stage == ST_Q ? mt * (mt + 1) / 2 : mt * nt;
 }
 
 // What the optimizer step works on (orthogonalisation alone: in and out)
@@ -121,21 +141,55 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(NsTable t, NsIo io) {
     const long long total = (long long)p.m * p.n, share = ns_share(p.m, p.n), from = p.tile * share;
     const long long to = from + share < total ? from + share : total;
     double s = 0.0;
-    auto one = [&](long long i) {
-        float v;
-        if constexpr (MUON) {
-            const float g = ((const float*)io.in)[p.src + i];
-            const float m = io.mu * io.momentum[p.src + i] + g * io.grad_scale;
-            io.momentum[p.src + i] = m;
-            v = ns_direction(io, g, m);
-        } else if constexpr (DT == ODAMD_DTYPE_BF16) {
-            v = bf16_to_f32(((const uint16_t*)io.in)[p.src + i]);
+    // eight elements a thread where all of them exist and their addresses allow 16-byte accesses
+    using T = typename std::conditional<DT == ODAMD_DTYPE_BF16, uint16_t, float>::type;
+    const T* in = (const T*)io.in + p.src;
+    float* mom = MUON ? io.momentum + p.src : nullptr;
+    const bool wide = (((uintptr_t)in | (uintptr_t)mom) & 15) == 0;
+    for (long long i = from + threadIdx.x * 8; i < to; i += 2048) {
+        const int cnt = to - i < 8 ? (int)(to - i) : 8;
+        float g[8], m[8];
+        if (wide && cnt == 8) {
+            if constexpr (DT == ODAMD_DTYPE_BF16) {
+                const u32x4 u = *(const u32x4*)(in + i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { g[2 * e] = __uint_as_float(u[e] << 16); g[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u); }
+            } else {
+                const f32x4_t u = *(const f32x4_t*)(in + i), v = *(const f32x4_t*)(in + i + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { g[e] = u[e]; g[e + 4] = v[e]; }
+            }
+            if constexpr (MUON) {
+                const f32x4_t u = *(const f32x4_t*)(mom + i), v = *(const f32x4_t*)(mom + i + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { m[e] = u[e]; m[e + 4] = v[e]; }
+            }
         } else {
-            v = ((const float*)io.in)[p.src + i];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (DT == ODAMD_DTYPE_BF16) g[e] = e < cnt ? bf16_to_f32(in[i + e]) : 0.0f;
+                else g[e] = e < cnt ? in[i + e] : 0.0f;
+                if constexpr (MUON) m[e] = e < cnt ? mom[i + e] : 0.0f;
+            }
         }
-        s += (double)v * v;
-    };
-    for (long long i = from + threadIdx.x; i < to; i += 256) one(i);
+        if constexpr (MUON) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                m[e] = io.mu * m[e] + g[e] * io.grad_scale;
+                g[e] = ns_direction(io, g[e], m[e]);
+            }
+            if (wide && cnt == 8) {
+                *(f32x4_t*)(mom + i) = f32x4_t{m[0], m[1], m[2], m[3]};
+                *(f32x4_t*)(mom + i + 4) = f32x4_t{m[4], m[5], m[6], m[7]};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e < cnt) mom[i + e] = m[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += (double)g[e] * g[e];
+    }
     s = ns_block_sum(s, part);
     if (threadIdx.x == 0) ((double*)p.ws)[p.tile] = s;
 }
@@ -148,7 +202,9 @@ __global__ void __launch_bounds__(256) ns_split_kernel(NsTable t, NsIo io) {
     const NsPlace p = ns_find(t, blockIdx.x, ST_SPLIT, 64);
     const NsLayout l = ns_layout(p.m, p.n);
     const int parts = ns_parts(p.m, p.n);
-    const double sum = ns_block_sum((int)threadIdx.x < parts ? ((const double*)p.ws)[threadIdx.x] : 0.0, part);
+    double mine = 0.0;
+    for (int i = threadIdx.x; i < parts; i += 256) mine += ((const double*)p.ws)[i];
+    const double sum = ns_block_sum(mine, part);
     const float inv = (float)(1.0 / (sqrt(sum) + io.eps));
     const int nt = (p.n + 63) / 64, i0 = p.tile / nt * 64, j0 = p.tile % nt * 64;
     const int lane = threadIdx.x & 63, row = threadIdx.x >> 6;
@@ -231,66 +287,69 @@ __device__ __forceinline__ void ns_emit8(const NsIo& io, float step, long long a
 
 // One product of the iteration for every matrix of the table
 template <typename TILE, int STAGE, bool MUON, int DT>
-__global__ void __launch_bounds__(TILE::THREADS) ns_product_kernel(NsTable t, NsIo io, int turn) {
+__global__ void __launch_bounds__(TILE::THREADS) ns_product_kernel(NsTable t, NsIo io, NsJobs jobs) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const NsPlace p = ns_find(t, gemm_xcd_remap(blockIdx.x, t.tiles), STAGE, TILE::TM);
+    const int block = (int)blockIdx.x, job = STAGE == ST_Q && block >= t.tiles ? 1 : 0, at = block - job * t.tiles;
+    const NsPlace p = ns_find(t, t.n == 1 ? gemm_xcd_remap(at, t.tiles) : gemm_xcd_stretch(at, t.tiles), STAGE, TILE::TM);
     const NsLayout l = ns_layout(p.m, p.n);
     const int mp = (int)ns_up(p.m, 32), np = (int)ns_up(p.n, 32);
+    const auto square = [&](int i) { return p.ws + l.sq + i * l.sq_size; };
     int ti, tj;
-    if (STAGE == ST_A || STAGE == ST_P) gemm_triangle_at(p.tile, ti, tj);
+    if (STAGE == ST_A || STAGE == ST_P || STAGE == ST_Q) gemm_triangle_at(p.tile, ti, tj);
     else gemm_tile_at(p.tile, (p.m + TILE::TM - 1) / TILE::TM, (p.n + TILE::TN - 1) / TILE::TN, ti, tj);
     const int i0 = ti * TILE::TM, j0 = tj * TILE::TN;
+    const int left = job ? jobs.left[1] : jobs.left[0], right = job ? jobs.right[1] : jobs.right[0], to = job ? jobs.out[1] : jobs.out[0];
+    const float scale = job ? jobs.scale[1] : jobs.scale[0];
     TILE tile;
     if constexpr (STAGE == ST_A) {
         const GemmOperand x = {p.ws + l.x, (long long)np * 4, p.m};
         tile.run(x, x, i0, j0, 0, np / 32, np, lds);
-    } else if constexpr (STAGE == ST_P) {
-        const GemmOperand a = {p.ws + l.a, (long long)mp * 4, p.m};
-        tile.run(a, a, i0, j0, 0, mp / 32, mp, lds);
     } else {
-        const GemmOperand a = {p.ws + l.p, (long long)mp * 4, p.m}, b = {p.ws + (turn & 1 ? l.xt1 : l.xt0), (long long)mp * 4, p.n};
+        const GemmOperand a = {square(left), (long long)mp * 4, p.m};
+        const GemmOperand b = STAGE == ST_P || STAGE == ST_Q ? GemmOperand{square(right), (long long)mp * 4, p.m}
+                                                             : GemmOperand{p.ws + (jobs.turn ? l.xt1 : l.xt0), (long long)mp * 4, p.n};
         tile.run(a, b, i0, j0, 0, mp / 32, mp, lds);
     }
 
-    if constexpr (STAGE == ST_A || STAGE == ST_P) {
-        char* out = p.ws + (STAGE == ST_A ? l.a : l.p);
+    if constexpr (STAGE == ST_A || STAGE == ST_P || STAGE == ST_Q) {
+        char* out = square(to);
         // row i, columns j .. j+7
         auto put = [&](int i, int j, float v[8]) {
             if (i >= p.m || j >= mp) return;
             const long long at = (long long)i * mp * 4 + split_at(j);
             if constexpr (STAGE == ST_P) {
-                const f16x8_t hi = *(const f16x8_t*)(p.ws + l.a + at), lo = *(const f16x8_t*)(p.ws + l.a + at + 64);
+                const f16x8_t hi = *(const f16x8_t*)(square(SQ_A) + at), lo = *(const f16x8_t*)(square(SQ_A) + at + 64);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    v[e] = (NS_C * NS_UNSCALE2) * v[e] + (NS_B / NS_SCALE) * ((float)hi[e] + (float)lo[e]) + (i == j + e ? NS_A : 0.0f);
+                    v[e] = (NS_C / NS_SCALE) * v[e] + NS_B * ((float)hi[e] + (float)lo[e]) + (i == j + e ? NS_A * NS_SCALE : 0.0f);
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] *= NS_UNSCALE2;
+                for (int e = 0; e < 8; ++e) v[e] *= scale;
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = j + e < p.m ? v[e] : 0.0f;
-            store_split8(out + at, v, NS_SCALE);
+            store_split8(out + at, v, 1.0f);
         };
         auto rows = [&](int i, int j, float v[8]) { put(i0 + i, j0 + j, v); };
         auto cols = [&](int i, int j, float v[8]) { put(j0 + j, i0 + i, v); };
         if (ti == tj) tile.template hand_out<true, false>(lds, rows, cols);
         else tile.template hand_out<true, true>(lds, rows, cols);
     } else if constexpr (STAGE == ST_X) {
-        char* xt = p.ws + (turn & 1 ? l.xt0 : l.xt1);
+        char* xt = p.ws + (jobs.turn ? l.xt0 : l.xt1);
         tile.template hand_out<true, true>(lds,
             [&](int i, int j, float v[8]) {
                 i += i0; j += j0;
                 if (i >= p.m || j >= np) return;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = j + e < p.n ? v[e] * NS_UNSCALE2 : 0.0f;
-                store_split8(p.ws + l.x + (long long)i * np * 4 + split_at(j), v, NS_SCALE);
+                for (int e = 0; e < 8; ++e) v[e] = j + e < p.n ? v[e] * scale : 0.0f;
+                store_split8(p.ws + l.x + (long long)i * np * 4 + split_at(j), v, 1.0f);
             },
             [&](int i, int j, float v[8]) {
                 i += i0; j += j0;
                 if (j >= p.n || i >= mp) return;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = i + e < p.m ? v[e] * NS_UNSCALE2 : 0.0f;
-                store_split8(xt + (long long)j * mp * 4 + split_at(i), v, NS_SCALE);
+                for (int e = 0; e < 8; ++e) v[e] = i + e < p.m ? v[e] * scale : 0.0f;
+                store_split8(xt + (long long)j * mp * 4 + split_at(i), v, 1.0f);
             });
     } else {
         const float step = MUON ? io.lr02 * sqrtf((float)p.n) : 0.0f;
@@ -298,14 +357,14 @@ __global__ void __launch_bounds__(TILE::THREADS) ns_product_kernel(NsTable t, Ns
             i += i0; j += j0;
             if (i >= p.m) return;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= NS_UNSCALE2;
+            for (int e = 0; e < 8; ++e) v[e] *= scale;
             ns_emit8<MUON, DT>(io, step, p.src + (long long)i * p.n + j, p.n - j, v);
         };
         auto cols = [&](int i, int j, float v[8]) {
             i += i0; j += j0;
             if (j >= p.n) return;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= NS_UNSCALE2;
+            for (int e = 0; e < 8; ++e) v[e] *= scale;
             ns_emit8<MUON, DT>(io, step, p.src + (long long)j * p.m + i, p.m - i, v);
         };
         if (p.tall) tile.template hand_out<false, true>(lds, rows, cols);
@@ -313,51 +372,113 @@ __global__ void __launch_bounds__(TILE::THREADS) ns_product_kernel(NsTable t, Ns
     }
 }
 
-using NsTile256 = GemmTile<2, true, 256, 256, 2, 4>;
-using NsTile128 = GemmTile<2, true, 128, 128, 2, 2>;
-using NsTile64 = GemmTile<2, true, 64, 64, 2, 2>;
+using NsTile256 = GemmTile<2, true, 256, 256, 4, 2, 1, 2>;
+using NsTile128 = GemmTile<2, true, 128, 128, 2, 4, 1, 2>;
+using NsTile64 = GemmTile<2, true, 64, 64, 2, 2, 1, 2>;
+using NsTile64Few = GemmTile<2, true, 64, 64, 2, 2, 2, 3>;   // two wave groups: one tile, or less, for a compute unit
 
-// Tiles of a stage over the whole table
+// Tiles of a stage over the whole table; -1: more than a launch takes
 int ns_count(NsTable& t, int stage, int tile) {
     long long at = 0;
     for (int i = 0; i < t.n; ++i) {
-        t.g[i].tile0 = (int)at;
+        t.g[i].tile0 = at > 0x7fffffff ? 0x7fffffff : (int)at;
         at += (long long)ns_tiles(stage, tile, t.g[i].m, t.g[i].n) * t.g[i].count;
     }
     t.tiles = (int)at;
-    return at > 0x7fffffff ? -1 : (int)at;
+    return at > 0x3fffffff ? -1 : (int)at;
 }
 
 template <typename TILE, int STAGE, bool MUON, int DT>
-int ns_launch_tile(const NsTable& t, const NsIo& io, int turn, hipStream_t s) {
+int ns_launch_tile(NsTable& t, const NsIo& io, const NsJobs& jobs, hipStream_t s) {
+    if (ns_count(t, STAGE, TILE::TM) < 0) return ODAMD_E_LIMIT;
     const auto kernel = ns_product_kernel<TILE, STAGE, MUON, DT>;
     const hipError_t e = odamd_ensure_lds((const void*)kernel, TILE::LDS);
     if (e != hipSuccess) return (int)e;
-    kernel<<<t.tiles, TILE::THREADS, TILE::LDS, s>>>(t, io, turn);
+    kernel<<<t.tiles * jobs.n, TILE::THREADS, TILE::LDS, s>>>(t, io, jobs);
     return (int)hipGetLastError();
 }
 
-// The largest tile that still gives every compute unit one: a larger tile reads less per product, fewer tiles than compute
-// units leave some of those idle.
 template <int STAGE, bool MUON, int DT>
-int ns_product(NsTable& t, const NsIo& io, int turn, hipStream_t s) {
-    if (ns_count(t, STAGE, 256) >= 256) return ns_launch_tile<NsTile256, STAGE, MUON, DT>(t, io, turn, s);
-    if (ns_count(t, STAGE, 128) >= 256) return ns_launch_tile<NsTile128, STAGE, MUON, DT>(t, io, turn, s);
-    if (ns_count(t, STAGE, 64) < 0) return ODAMD_E_LIMIT;
-    return ns_launch_tile<NsTile64, STAGE, MUON, DT>(t, io, turn, s);
+int ns_product(NsTable& t, const NsIo& io, const NsJobs& jobs, hipStream_t s) {
+    int best = 64;
+    double least = 0.0, tiles64 = 0.0;
+    for (int tile : {64, 128, 256}) {
+        GemmLoad load;
+        for (int i = 0; i < t.n; ++i)
+            gemm_load_add(load, (double)ns_tiles(STAGE, tile, t.g[i].m, t.g[i].n) * t.g[i].count * jobs.n,
+                          (double)(ns_up(STAGE == ST_A ? t.g[i].n : t.g[i].m, 32) / 32));
+        const double us = gemm_time_us(tile, load);
+        if (tile == 64) tiles64 = load.tiles;
+        if (tile == 64 || us < least) {
+            best = tile;
+            least = us;
+        }
+    }
+    if (best == 256) return ns_launch_tile<NsTile256, STAGE, MUON, DT>(t, io, jobs, s);
+    if (best == 128) return ns_launch_tile<NsTile128, STAGE, MUON, DT>(t, io, jobs, s);
+    if (tiles64 > 256.0) return ns_launch_tile<NsTile64, STAGE, MUON, DT>(t, io, jobs, s);
+    return ns_launch_tile<NsTile64Few, STAGE, MUON, DT>(t, io, jobs, s);
+}
+
+// Exponent that keeps a product of k P's (entries up to 3.4445^k) within fp16, an eighth of a bit to spare for rounding
+int ns_q_exponent(int k) {
+    const int e = (int)floor(log2(65504.0 / (1.1 * pow((double)NS_A, k))));
+    return e < 12 ? e : 12;
 }
 
 template <bool MUON, int DT>
 int ns_run(NsTable& t, const NsIo& io, int steps, hipStream_t s) {
+    constexpr bool LOOSE = MUON || DT == ODAMD_DTYPE_BF16;
+    int phase = LOOSE ? 5 : 2;
+    for (int i = 0; i < t.n; ++i)
+        if (!LOOSE && t.g[i].n < 2 * (long long)t.g[i].m) phase = 1;
     if (ns_count(t, ST_NORM, 0) < 0) return ODAMD_E_LIMIT;
     ns_norm_kernel<MUON, DT><<<t.tiles, 256, 0, s>>>(t, io);
     if (ns_count(t, ST_SPLIT, 64) < 0) return ODAMD_E_LIMIT;
     ns_split_kernel<MUON, DT><<<t.tiles, 256, 0, s>>>(t, io);
     int rc = (int)hipGetLastError();
-    for (int k = 0; k < steps && rc == 0; ++k) {
-        rc = ns_product<ST_A, false, ODAMD_DTYPE_F32>(t, io, k, s);
-        if (rc == 0) rc = ns_product<ST_P, false, ODAMD_DTYPE_F32>(t, io, k, s);
-        if (rc == 0) rc = k + 1 < steps ? ns_product<ST_X, false, ODAMD_DTYPE_F32>(t, io, k, s) : ns_product<ST_OUT, MUON, DT>(t, io, k, s);
+    NsJobs jobs = {};
+    const auto clear = [&] { jobs.n = 0; };
+    const auto add = [&](int left, int right, int out, int shift) {
+        jobs.left[jobs.n] = left;
+        jobs.right[jobs.n] = right;
+        jobs.out[jobs.n] = out;
+        jobs.scale[jobs.n++] = (float)ldexp(1.0, shift);
+    };
+    for (int done = 0; done < steps && rc == 0;) {
+        const int len = steps - done < phase ? steps - done : phase;
+        clear();
+        add(0, 0, SQ_A, -12);
+        rc = ns_product<ST_A, false, ODAMD_DTYPE_F32>(t, io, jobs, s);
+        int q = -1, eq = 0;
+        for (int k = 1; k <= len && rc == 0; ++k) {
+            const int p = q == SQ_B ? SQ_B + 1 : SQ_B, spare = 3 * SQ_B + 3 - p - (q < 0 ? SQ_B + 1 : q);
+            clear();
+            add(SQ_A, SQ_A, p, 0);
+            rc = ns_product<ST_P, false, ODAMD_DTYPE_F32>(t, io, jobs, s);
+            clear();
+            if (k < len) add(p, SQ_A, SQ_T, -12);
+            if (k > 1) {
+                const int e = ns_q_exponent(k);
+                add(q, p, spare, e - eq - 12);
+                q = spare;
+                eq = e;
+            } else {
+                q = p;
+                eq = 12;
+            }
+            if (jobs.n && rc == 0) rc = ns_product<ST_Q, false, ODAMD_DTYPE_F32>(t, io, jobs, s);
+            if (k < len && rc == 0) {
+                clear();
+                add(SQ_T, p, SQ_A, -12);
+                rc = ns_product<ST_Q, false, ODAMD_DTYPE_F32>(t, io, jobs, s);
+            }
+        }
+        done += len;
+        clear();
+        add(q, 0, 0, done < steps ? -eq : -eq - 12);
+        if (rc == 0) rc = done < steps ? ns_product<ST_X, false, ODAMD_DTYPE_F32>(t, io, jobs, s) : ns_product<ST_OUT, MUON, DT>(t, io, jobs, s);
+        jobs.turn ^= 1;
     }
     return rc;
 }
@@ -449,12 +570,16 @@ int odamd_muon_ema_step(float* param, const float* grad, float* momentum, float*
         t.ws = (char*)workspace;
         long long at = 0;
         for (int k = i; k < n_matrices && k < i + NS_GROUPS; ++k) {
-            NsGroup& g = t.g[t.n++];
+            NsGroup g;
             ns_orient(g, matrices_host[k].rows, matrices_host[k].cols);
             g.src = matrices_host[k].offset;
             g.count = 1;
             g.ws = (unsigned)(at / 256);
             at += ns_layout(g.m, g.n).end;
+            // the longest tiles first: short ones fill the end of a launch
+            int to = t.n++;
+            for (; to > 0 && (t.g[to - 1].m < g.m || (t.g[to - 1].m == g.m && t.g[to - 1].n < g.n)); --to) t.g[to] = t.g[to - 1];
+            t.g[to] = g;
         }
         const int rc = ns_run<true, ODAMD_DTYPE_F32>(t, io, steps, (hipStream_t)stream);
         if (rc != 0) return rc;

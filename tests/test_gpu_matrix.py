@@ -246,8 +246,11 @@ def orth64(g, steps=5, eps=1e-7):
     return x.t() if tall else x
 
 
-# A step multiplies a small singular value by 3.4445: five of them multiply the half step of float32 by 485
-ORTH_TOL = {torch.float32: 3.4445 ** 5 * 2.0 ** -24, torch.bfloat16: 3.4445 ** 5 * 2.0 ** -24 + 2.0 ** -8}
+# A step multiplies a small singular value by 3.4445: five of them multiply the half step of float32 by 485.  Where five steps
+# run on A = X X^T (bfloat16 results, the optimizer step), a half step of A is multiplied by 3.4445^2 in four of them and
+# enters P / a = 1 - (4.7750 / 3.4445) A + ... of the last.
+LOOSE = 4.7750 / 3.4445 * 3.4445 ** 8 * 2.0 ** -24
+ORTH_TOL = {torch.float32: 3.4445 ** 5 * 2.0 ** -24, torch.bfloat16: LOOSE + 2.0 ** -8}
 
 
 def check_orth(got, g, **kw):
@@ -349,8 +352,8 @@ def test_muon_step_against_64_bits(mx, ema, nesterov):
     for o, r, c in matrices:
         s = slice(o, o + r * c)
         covered[s] = True
-        step = 0.01 * 0.2 * math.sqrt(max(r, c)) * math.sqrt(min(r, c)) * 1.25     # Frobenius norm of the update, at most
-        allowed = ORTH_TOL[torch.float32] * step + 4 * 2.0 ** -24 * float(rp[s].norm())
+        step = 0.01 * 0.2 * math.sqrt(r * c) * 1.25     # Frobenius norm of the update, at most: singular values under 1.25
+        allowed = LOOSE * step + 4 * 2.0 ** -24 * float(rp[s].norm())
         assert float((p1[s].double() - rp[s]).norm()) <= allowed
         if ema:
             assert float((e1[s].double() - re[s]).norm()) <= allowed + 4 * 2.0 ** -24 * float(re[s].norm())
@@ -368,7 +371,9 @@ def test_muon_step_many_matrices(mx):
     p, g, m = randn(300 * 64), randn(300 * 64, seed=1), torch.zeros(300 * 64, device='cuda')
     rp, rm, _ = muon64(p, g, m, None, matrices, 0.1, 0.95, True, 0.0, 0.0, 1.0)
     mx.muon_step(p, g, m, matrices, lr=0.1)
-    assert float((p.double() - rp).norm() / rp.norm()) < 1e-6 and float((m.double() - rm).abs().max()) == 0.0
+    # 300 updates of norm 0.1 * 0.2 * sqrt(8 * 8) * 1.25 at most, each off by LOOSE of itself, and the roundings of p
+    assert float((p.double() - rp).norm()) <= LOOSE * 0.1 * 0.2 * 8 * 1.25 * math.sqrt(300) + 4 * 2.0 ** -24 * float(rp.norm())
+    assert float((m.double() - rm).abs().max()) == 0.0
 
 
 def test_muon_step_refuses(mx):
@@ -499,7 +504,7 @@ def test_detector_trains_with_muon():
     for o, r, c in matrices:
         s = slice(o, o + r * c)
         step = lr * 0.2 * math.sqrt(r * c) * 1.25
-        allowed = ORTH_TOL[torch.float32] * step + 8 * 2.0 ** -24 * float(rp[s].norm())
+        allowed = LOOSE * step + 8 * 2.0 ** -24 * float(rp[s].norm())
         assert float((st.param[s].double() - rp[s]).norm()) <= allowed
         assert float((st.ema_param[s].double() - re[s]).norm()) <= allowed + 8 * 2.0 ** -24 * float(re[s].norm())
     for o, n in tc.optimizer.rest.tolist():
