@@ -61,6 +61,10 @@ __device__ __forceinline__ void gemm_triangle_at(int t, int& ti, int& tj) {
     ti = t - j * (j + 1) / 2;
 }
 
+// 16-byte accesses at addresses that are only aligned to the element (global memory takes them)
+typedef f32x4_t f32x4_any __attribute__((aligned(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
 struct GemmOperand {
     const char* p;     // row 0 of the operand
     long long ld;      // bytes per row, a multiple of 16
@@ -268,7 +272,7 @@ __device__ __forceinline__ void store_split8(char* hi_at, const float v[8], floa
 // ---- host: which tile ------------------------------------------------------------------------------------------------
 // Measured with pairs at 4096^3, 2048 x 1024 x 2048 and below: time of a chunk of one tile alone on a compute unit (0.69 us for
 // 128 x 128, 0.3 us for 64 x 64 with two wave groups), and its share of a unit's time where several tiles run there (0.87 and
-// 0.24 us; 2.75 us for 256 x 256, which fills a unit by itself).  The larger tile wins per product, the smaller one
+// 0.27 us; 2.75 us for 256 x 256, which fills a unit by itself).  The larger tile wins per product, the smaller one
 // spreads a small product over all 256 units: 4096 x 4096 x 4096 353 / 445 / 512 us in 256 / 128 / 64, 2048 x 1024 x 2048
 // - / 45 / 33 us.  bf16 chunks take two thirds of the time for every tile: the choice is the same.
 struct GemmLoad { double tiles = 0, chunks = 0, longest = 0; int kinds = 0; };   // chunks: summed over all tiles
@@ -279,10 +283,12 @@ inline void gemm_load_add(GemmLoad& l, double tiles, double chunks) {
     ++l.kinds;
 }
 inline double gemm_time_us(int tile, const GemmLoad& l) {
-    const double alone = tile == 256 ? 2.75 : tile == 128 ? 0.69 : 0.3, share = tile == 256 ? 2.75 : tile == 128 ? 0.87 : 0.24;
+    const double alone = tile == 256 ? 2.75 : tile == 128 ? 0.69 : 0.3, share = tile == 256 ? 2.75 : tile == 128 ? 0.87 : 0.27;
     // tiles of one length run in whole rounds
     const double rounds = l.kinds == 1 ? (double)(((long long)l.tiles + 255) / 256) : l.chunks / (256.0 * l.longest);
-    return l.longest * (alone > share * rounds ? alone : share * rounds);
+    const double us = l.longest * (alone > share * rounds ? alone : share * rounds);
+    // of several lengths they pack as they come: half of the longest is left over at the end
+    return l.kinds == 1 ? us : us + 0.5 * l.longest * share;
 }
 
 #endif

@@ -5,8 +5,6 @@ the orthogonalisation of matrices by Newton-Schulz products (`orthogonalize`) an
 Tensors are float32 or bfloat16 on one GPU; every call enqueues its work on the current stream of the tensors' device
 and takes its workspace from torch's allocator, so it can be captured into a graph.
 """
-import ctypes as C
-
 import numpy as np
 import torch
 
@@ -19,8 +17,21 @@ MATRIX_DTYPE = np.dtype([('offset', '<i8'), ('rows', '<i4'), ('cols', '<i4')])  
 RANGE_DTYPE = np.dtype([('offset', '<i8'), ('len', '<i8')])                         # odamd_range
 
 
-def _stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)     # the handle alone, without a Stream object
+
+
+def _stream(device):
+    if _raw_stream is not None:
+        return _raw_stream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _call(device, fn, *args):
+    """fn(*args, current stream of `device`) with that device as the current one; its return code."""
+    if torch.cuda.current_device() == device.index:
+        return fn(*args, _stream(device))
+    with torch.cuda.device(device):
+        return fn(*args, _stream(device))
 
 
 def _ptr(t):
@@ -45,7 +56,8 @@ def _check_tensor(name, t, dtype=None, device=None):
 def _rows(t):
     """(..., c) -> (rows, c) with contiguous rows that do not overlap: a view where the strides allow one."""
     c = t.shape[-1]
-    t = t.reshape(-1, c)
+    if t.dim() != 2:
+        t = t.reshape(-1, c)
     if (c > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < c):
         t = t.contiguous()
     return t
@@ -66,9 +78,9 @@ def _linear_forward(x, weight, bias, residual, act, keep_z):
     z = torch.empty_like(y) if keep_z else None
     d = _lib.LinearDesc(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(z), _ld(x),
                         _ld(weight), 0 if residual is None else _ld(residual), n, n, m, k, n, act, _DTYPES[x.dtype])
-    with torch.cuda.device(x.device):
-        ws = _workspace(lib.odamd_linear_workspace_bytes(C.byref(d)), x.device)
-        check(lib.odamd_linear_forward(C.byref(d), _ptr(ws), 0 if ws is None else ws.numel(), _stream()), 'linear_forward')
+    size = lib.odamd_linear_workspace_bytes(d)
+    ws = _workspace(size, x.device)
+    check(_call(x.device, lib.odamd_linear_forward, d, _ptr(ws), size), 'linear_forward')
     return y, z
 
 
@@ -82,9 +94,9 @@ def _linear_backward(dy, z, x, weight, act, want_dx, want_dw, want_db):
     d = _lib.LinearGradDesc(dy.data_ptr(), _ptr(z), _ptr(x) if want_dw else None, _ptr(weight) if want_dx else None, _ptr(dx),
                             _ptr(dw), _ptr(db), _ld(dy), 0 if z is None else _ld(z), _ld(x) if want_dw else 0,
                             _ld(weight) if want_dx else 0, k, k, m, k, n, act, _DTYPES[dy.dtype])
-    with torch.cuda.device(dy.device):
-        ws = _workspace(lib.odamd_linear_backward_workspace_bytes(C.byref(d)), dy.device)
-        check(lib.odamd_linear_backward(C.byref(d), _ptr(ws), ws.numel(), _stream()), 'linear_backward')
+    size = lib.odamd_linear_backward_workspace_bytes(d)
+    ws = _workspace(size, dy.device)
+    check(_call(dy.device, lib.odamd_linear_backward, d, ws.data_ptr(), size), 'linear_backward')
     return dx, dw, db
 
 
@@ -174,10 +186,10 @@ def orthogonalize(x, steps=5, eps=1e-7, out=None):
         return out
     src = x.detach().contiguous()
     batch = src.numel() // (rows * cols)
-    with torch.cuda.device(x.device):
-        ws = _workspace(lib.odamd_orthogonalize_workspace_bytes(batch, rows, cols), x.device)
-        check(lib.odamd_orthogonalize(src.data_ptr(), out.data_ptr(), batch, rows, cols, int(steps), float(eps),
-                                      _DTYPES[x.dtype], ws.data_ptr(), ws.numel(), _stream()), 'orthogonalize')
+    size = lib.odamd_orthogonalize_workspace_bytes(batch, rows, cols)
+    ws = _workspace(size, x.device)
+    check(_call(x.device, lib.odamd_orthogonalize, src.data_ptr(), out.data_ptr(), batch, rows, cols, int(steps), float(eps),
+                _DTYPES[x.dtype], ws.data_ptr(), size), 'orthogonalize')
     return out
 
 
@@ -234,9 +246,7 @@ def muon_step(param, grad, momentum, matrices, lr, momentum_decay=0.95, nesterov
         raise ValueError(f'matrices end at {table.end}, the buffers at {param.numel()}')
     if not 1 <= int(steps) <= 32 or not eps >= 0:
         raise ValueError('steps must be 1 to 32, eps must not be negative')
-    with torch.cuda.device(param.device):
-        ws = _workspace(table.workspace_bytes, param.device)
-        check(lib.odamd_muon_ema_step(param.data_ptr(), grad.data_ptr(), momentum.data_ptr(), _ptr(ema),
-                                      table.table.ctypes.data, len(table), lr, momentum_decay, int(nesterov), weight_decay,
-                                      int(steps), eps, ema_decay, grad_scale, ws.data_ptr(), ws.numel(), _stream()),
-              'muon_ema_step')
+    ws = _workspace(table.workspace_bytes, param.device)
+    check(_call(param.device, lib.odamd_muon_ema_step, param.data_ptr(), grad.data_ptr(), momentum.data_ptr(), _ptr(ema),
+                table.table.ctypes.data, len(table), lr, momentum_decay, int(nesterov), weight_decay, int(steps), eps,
+                ema_decay, grad_scale, ws.data_ptr(), table.workspace_bytes), 'muon_ema_step')
