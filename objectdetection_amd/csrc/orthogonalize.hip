@@ -34,10 +34,13 @@ namespace {
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float NS_SCALE = 4096.0f;
 constexpr int NS_GROUPS = 112;        // groups of one launch: their table travels in the kernel's arguments (4 KiB at most)
+// m m n up to which one workgroup takes a matrix as a whole (m <= 64).  Whole / in launches, us: 16 x 27 12 / 73, 32 x 576 71 / 98,
+// 64 x 128 56 / 90, 64 x 256 94 / 94; 300 of 64 x 128 75 / 124, of 64 x 256 199 / 143.
+constexpr long long NS_WHOLE = 5 << 17;
 constexpr int NS_PARTS = 512;         // partial sums of squares per matrix, at most
 
-// stages: sums of squares, laying out, X X^T, P from A, products of square matrices, Q X, Q X to the caller
-enum { ST_NORM, ST_SPLIT, ST_A, ST_P, ST_Q, ST_X, ST_OUT };
+// stages: sums of squares, laying out, X X^T, P from A, products of square matrices, Q X, Q X to the caller; a matrix as a whole
+enum { ST_NORM, ST_SPLIT, ST_A, ST_P, ST_Q, ST_X, ST_OUT, ST_WHOLE };
 // square matrices: A, a product on the way to the next A, and three that P and Q take in turn
 enum { SQ_A, SQ_T, SQ_B, SQ_COUNT = 5 };
 
@@ -86,7 +89,7 @@ __host__ __device__ inline long long ns_share(int m, int n) {
 __host__ __device__ inline int ns_parts(int m, int n) { return (int)(((long long)m * n + ns_share(m, n) - 1) / ns_share(m, n)); }
 __host__ __device__ inline int ns_tiles(int stage, int tile, int m, int n) {
     const int mt = (m + tile - 1) / tile, nt = (n + tile - 1) / tile;
-    return stage == ST_NORM ? ns_parts(m, n) : stage == ST_A || stage == ST_P || stage == ST_Q ? mt * (mt + 1) / 2 : mt * nt;
+    return stage == ST_WHOLE ? 1 : stage == ST_NORM ? ns_parts(m, n) : stage == ST_A || stage == ST_P || stage == ST_Q ? mt * (mt + 1) / 2 : mt * nt;
 }
 
 // What the optimizer step works on (orthogonalisation alone: in and out)
@@ -141,26 +144,25 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(NsTable t, NsIo io) {
     const long long total = (long long)p.m * p.n, share = ns_share(p.m, p.n), from = p.tile * share;
     const long long to = from + share < total ? from + share : total;
     double s = 0.0;
-    // eight elements a thread where all of them exist and their addresses allow 16-byte accesses
+    // eight elements a thread
     using T = typename std::conditional<DT == ODAMD_DTYPE_BF16, uint16_t, float>::type;
     const T* in = (const T*)io.in + p.src;
     float* mom = MUON ? io.momentum + p.src : nullptr;
-    const bool wide = (((uintptr_t)in | (uintptr_t)mom) & 15) == 0;
     for (long long i = from + threadIdx.x * 8; i < to; i += 2048) {
         const int cnt = to - i < 8 ? (int)(to - i) : 8;
         float g[8], m[8];
-        if (wide && cnt == 8) {
+        if (cnt == 8) {
             if constexpr (DT == ODAMD_DTYPE_BF16) {
-                const u32x4 u = *(const u32x4*)(in + i);
+                const u32x4 u = *(const u32x4_any*)(in + i);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) { g[2 * e] = __uint_as_float(u[e] << 16); g[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u); }
             } else {
-                const f32x4_t u = *(const f32x4_t*)(in + i), v = *(const f32x4_t*)(in + i + 4);
+                const f32x4_t u = *(const f32x4_any*)(in + i), v = *(const f32x4_any*)(in + i + 4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) { g[e] = u[e]; g[e + 4] = v[e]; }
             }
             if constexpr (MUON) {
-                const f32x4_t u = *(const f32x4_t*)(mom + i), v = *(const f32x4_t*)(mom + i + 4);
+                const f32x4_t u = *(const f32x4_any*)(mom + i), v = *(const f32x4_any*)(mom + i + 4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) { m[e] = u[e]; m[e + 4] = v[e]; }
             }
@@ -178,9 +180,9 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(NsTable t, NsIo io) {
                 m[e] = io.mu * m[e] + g[e] * io.grad_scale;
                 g[e] = ns_direction(io, g[e], m[e]);
             }
-            if (wide && cnt == 8) {
-                *(f32x4_t*)(mom + i) = f32x4_t{m[0], m[1], m[2], m[3]};
-                *(f32x4_t*)(mom + i + 4) = f32x4_t{m[4], m[5], m[6], m[7]};
+            if (cnt == 8) {
+                *(f32x4_any*)(mom + i) = f32x4_t{m[0], m[1], m[2], m[3]};
+                *(f32x4_any*)(mom + i + 4) = f32x4_t{m[4], m[5], m[6], m[7]};
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
@@ -239,15 +241,130 @@ __global__ void __launch_bounds__(256) ns_split_kernel(NsTable t, NsIo io) {
     }
 }
 
+// A small matrix from the caller's buffers to the caller's buffers in one workgroup: X, A and P stay in LDS as float32, the products
+// run on v_mfma_f32_16x16x4_f32 (a sixteenth of the half-precision rate, but no pairs, no columns copy and no launches
+// between the steps).  16 x 27 takes 12 us this way and 73 us in eighteen launches.  T: m in 16-row tiles.  Rows of X lie ld
+// floats apart, ld = 4 modulo 32: sixteen rows at four consecutive k touch 64 different banks.
+__host__ __device__ inline int ns_small_ld(int n) { return (int)ns_up(ns_up(n, 16) - 4, 32) + 4; }
+__host__ __device__ inline long long ns_small_lds(int t, int n) { return 4LL * 16 * t * (ns_small_ld(n) + 2 * ns_small_ld(16 * t)); }
+
+template <int T, bool MUON, int DT>
+__global__ void __launch_bounds__(256) ns_whole_kernel(NsTable t, NsIo io, int steps) {
+    extern __shared__ __attribute__((aligned(16))) float space[];
+    __shared__ double part[4];
+    const NsPlace p = ns_find(t, blockIdx.x, ST_WHOLE, 0);
+    const int ld = ns_small_ld(p.n), lda = ns_small_ld(16 * T);
+    float *x = space, *a = x + 16 * T * ld, *pm = a + 16 * T * lda;
+    const int total = p.m * p.n, cols = p.tall ? p.m : p.n;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, h = lane >> 4;
+    const auto place = [&](int i) {                       // element i of the caller's matrix in X
+        const int row = i / cols, col = i - row * cols;
+        return p.tall ? col * ld + row : row * ld + col;
+    };
+    for (int i = threadIdx.x; i < 16 * T * ld; i += 256) x[i] = 0.0f;
+    __syncthreads();
+    double s = 0.0;
+    for (int i = threadIdx.x; i < total; i += 256) {
+        float v;
+        if constexpr (MUON) {
+            const float g = ((const float*)io.in)[p.src + i], m = io.mu * io.momentum[p.src + i] + g * io.grad_scale;
+            io.momentum[p.src + i] = m;
+            v = ns_direction(io, g, m);
+        } else if constexpr (DT == ODAMD_DTYPE_BF16) {
+            v = bf16_to_f32(((const uint16_t*)io.in)[p.src + i]);
+        } else {
+            v = ((const float*)io.in)[p.src + i];
+        }
+        x[place(i)] = v;
+        s += (double)v * v;
+    }
+    s = ns_block_sum(s, part);                            // its barrier also closes the writes of X
+    const float inv = (float)(1.0 / (sqrt(s) + io.eps));
+    for (int i = threadIdx.x; i < 16 * T * ld; i += 256) x[i] *= inv;
+    __syncthreads();
+    // out tile (ti, tj) of l r^T over k values, both of them rows `stride` apart
+    const auto product = [&](const float* l, const float* rr, int stride, int ti, int tj, int k) {
+        f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float *la = l + (ti * 16 + r) * stride + h, *lb = rr + (tj * 16 + r) * stride + h;
+#pragma unroll 4
+        for (int q = 0; q < k; q += 4) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(la[q], lb[q], acc, 0, 0, 0);
+        return acc;
+    };
+    constexpr int TRI = T * (T + 1) / 2;
+    for (int step = 0; step < steps; ++step) {
+        for (int tile = wave; tile < TRI; tile += 4) {
+            int ti, tj;
+            gemm_triangle_at(tile, ti, tj);
+            const f32x4_t v = product(x, x, ld, ti, tj, (int)ns_up(p.n, 4));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = ti * 16 + 4 * h + e, j = tj * 16 + r;
+                a[i * lda + j] = v[e];
+                a[j * lda + i] = v[e];
+            }
+        }
+        __syncthreads();
+        for (int tile = wave; tile < TRI; tile += 4) {
+            int ti, tj;
+            gemm_triangle_at(tile, ti, tj);
+            const f32x4_t v = product(a, a, lda, ti, tj, 16 * T);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = ti * 16 + 4 * h + e, j = tj * 16 + r;
+                // without a I: the float32 sum a X + (P - a I) X keeps the last bits of X
+                const float u = NS_B * a[i * lda + j] + NS_C * v[e];
+                pm[i * lda + j] = u;
+                pm[j * lda + i] = u;
+            }
+        }
+        __syncthreads();
+        // a wave owns sixteen columns of X: it has read them when it writes them
+        for (int j0 = wave * 16; j0 < p.n; j0 += 64) {
+            float col[4 * T];
+#pragma unroll
+            for (int q = 0; q < 4 * T; ++q) col[q] = x[(4 * q + h) * ld + j0 + r];
+            f32x4_t acc[T];
+#pragma unroll
+            for (int ti = 0; ti < T; ++ti)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[ti][e] = NS_A * x[(ti * 16 + 4 * h + e) * ld + j0 + r];
+#pragma unroll
+            for (int q = 0; q < 4 * T; ++q)
+#pragma unroll
+                for (int ti = 0; ti < T; ++ti)
+                    acc[ti] = __builtin_amdgcn_mfma_f32_16x16x4f32(pm[(ti * 16 + r) * lda + 4 * q + h], col[q], acc[ti], 0, 0, 0);
+#pragma unroll
+            for (int ti = 0; ti < T; ++ti)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[(ti * 16 + 4 * h + e) * ld + j0 + r] = acc[ti][e];
+        }
+        __syncthreads();
+    }
+    const float step = MUON ? io.lr02 * sqrtf((float)p.n) : 0.0f;
+    for (int i = threadIdx.x; i < total; i += 256) {
+        const float v = x[place(i)];
+        const long long at = p.src + i;
+        if constexpr (MUON) {
+            const float w = io.param[at] * io.decay - step * v;
+            io.param[at] = w;
+            if (io.ema) io.ema[at] = io.ema_keep * io.ema[at] + io.ema_take * w;
+        } else if constexpr (DT == ODAMD_DTYPE_BF16) {
+            ((uint16_t*)io.out)[at] = f32_to_bf16(v);
+        } else {
+            ((float*)io.out)[at] = v;
+        }
+    }
+}
+
 // Results for the caller: eight values from element `at` on, the first `cnt` of them exist.
 template <bool MUON, int DT>
 __device__ __forceinline__ void ns_emit8(const NsIo& io, float step, long long at, int cnt, const float v[8]) {
     if (cnt <= 0) return;
     const int n = cnt < 8 ? cnt : 8;
     if constexpr (MUON) {
-        f32x4_t* pp = (f32x4_t*)(io.param + at);
-        f32x4_t* ep = (f32x4_t*)(io.ema + at);
-        if (n == 8 && (((uintptr_t)pp | (io.ema ? (uintptr_t)ep : 0)) & 15) == 0) {
+        f32x4_any* pp = (f32x4_any*)(io.param + at);
+        f32x4_any* ep = (f32x4_any*)(io.ema + at);
+        if (n == 8) {
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 f32x4_t w = pp[q];
@@ -270,15 +387,15 @@ __device__ __forceinline__ void ns_emit8(const NsIo& io, float step, long long a
         }
     } else if constexpr (DT == ODAMD_DTYPE_BF16) {
         uint16_t* o = (uint16_t*)io.out + at;
-        if (n == 8 && ((uintptr_t)o & 15) == 0)
-            *(u32x4*)o = u32x4{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]), f32x2_to_bf16x2(v[4], v[5]), f32x2_to_bf16x2(v[6], v[7])};
+        if (n == 8)
+            *(u32x4_any*)o = u32x4{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]), f32x2_to_bf16x2(v[4], v[5]), f32x2_to_bf16x2(v[6], v[7])};
         else
             for (int e = 0; e < n; ++e) o[e] = f32_to_bf16(v[e]);
     } else {
         float* o = (float*)io.out + at;
-        if (n == 8 && ((uintptr_t)o & 15) == 0) {
-            *(f32x4_t*)o = f32x4_t{v[0], v[1], v[2], v[3]};
-            *(f32x4_t*)(o + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+        if (n == 8) {
+            *(f32x4_any*)o = f32x4_t{v[0], v[1], v[2], v[3]};
+            *(f32x4_any*)(o + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
         } else {
             for (int e = 0; e < n; ++e) o[e] = v[e];
         }
@@ -426,8 +543,31 @@ int ns_q_exponent(int k) {
     return e < 12 ? e : 12;
 }
 
+template <int T, bool MUON, int DT>
+int ns_whole(NsTable& t, const NsIo& io, int steps, long long lds, hipStream_t s) {
+    if (ns_count(t, ST_WHOLE, 0) < 0) return ODAMD_E_LIMIT;
+    const auto kernel = ns_whole_kernel<T, MUON, DT>;
+    const hipError_t e = odamd_ensure_lds((const void*)kernel, (size_t)lds);
+    if (e != hipSuccess) return (int)e;
+    kernel<<<t.tiles, 256, (size_t)lds, s>>>(t, io, steps);
+    return (int)hipGetLastError();
+}
+
 template <bool MUON, int DT>
 int ns_run(NsTable& t, const NsIo& io, int steps, hipStream_t s) {
+    int tallest = 0;
+    long long lds = 0, work = 0;
+    for (int i = 0; i < t.n; ++i) {
+        const int rows = (t.g[i].m + 15) / 16;
+        tallest = rows > tallest ? rows : tallest;
+        work = (long long)t.g[i].m * t.g[i].m * t.g[i].n > work ? (long long)t.g[i].m * t.g[i].m * t.g[i].n : work;
+    }
+    if (tallest <= 4 && work <= NS_WHOLE) {
+        for (int i = 0; i < t.n; ++i) lds = ns_small_lds(tallest, t.g[i].n) > lds ? ns_small_lds(tallest, t.g[i].n) : lds;
+        if (lds <= 128 * 1024)
+            return tallest == 1 ? ns_whole<1, MUON, DT>(t, io, steps, lds, s) : tallest == 2 ? ns_whole<2, MUON, DT>(t, io, steps, lds, s)
+                 : tallest == 3 ? ns_whole<3, MUON, DT>(t, io, steps, lds, s) : ns_whole<4, MUON, DT>(t, io, steps, lds, s);
+    }
     constexpr bool LOOSE = MUON || DT == ODAMD_DTYPE_BF16;
     int phase = LOOSE ? 5 : 2;
     for (int i = 0; i < t.n; ++i)

@@ -104,12 +104,13 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
         x2, w2 = _rows(x), _rows(weight)
-        keep_z = act != 0 and any(ctx.needs_input_grad[:3])
+        need = ctx.needs_input_grad
+        keep_z = act != 0 and (need[0] or need[1] or need[2])
         y, z = _linear_forward(x2, w2, bias if bias is None else bias.contiguous(),
                                None if residual is None else _rows(residual), act, keep_z)
-        ctx.act, ctx.x_shape, ctx.y_shape = act, x.shape, x.shape[:-1] + (weight.shape[0],)
-        ctx.save_for_backward(x2 if ctx.needs_input_grad[1] else None, w2 if ctx.needs_input_grad[0] else None, z)
-        return y.view(ctx.y_shape)
+        ctx.act, ctx.x_shape = act, x.shape
+        ctx.save_for_backward(x2 if need[1] else None, w2 if need[0] else None, z)
+        return y if x.dim() == 2 else y.view(x.shape[:-1] + (weight.shape[0],))
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -117,9 +118,10 @@ class _Linear(torch.autograd.Function):
         x, weight, z = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = db = None
-        if any(need[:3]):
+        if need[0] or need[1] or need[2]:
             dx, dw, db = _linear_backward(_rows(dy), z, x, weight, ctx.act, *need[:3])
-            dx = dx if dx is None else dx.view(ctx.x_shape)
+            if dx is not None and len(ctx.x_shape) != 2:
+                dx = dx.view(ctx.x_shape)
         return dx, dw, db, dy if need[3] else None, None
 
 
