@@ -205,17 +205,42 @@ struct GemmTile {
         }
     }
 
-    // Hands the tile out in runs of eight: rows(m, n, v[8]) for C[m][n .. n+7], cols(m, n, v[8]) for C[m .. m+7][n]
-    // (m, n relative to the tile).  Every wave passes 32 rows at a time through a slab of LDS of its own.
-    template <bool ROWS, bool COLS, typename FR, typename FC>
-    __device__ __forceinline__ void hand_out(char* lds, FR&& rows, FC&& cols) {
+    // First of the eight columns this lane hands out by rows
+    __device__ __forceinline__ int row_column() const {
+        return (threadIdx.x >> 6) % NW % WGN * WTN + (threadIdx.x & 63) % (WTN / 8) * 8;
+    }
+
+    // Hands the tile out in runs of eight, m and n relative to the tile: rows(m, n, v[8], x) for C[m][n .. n+7] and
+    // cols(m, n, v[8], x) for C[m .. m+7][n], x = what load(m, n) of that kind gave before.  Every wave passes 32 rows at a time
+    // through a slab of LDS of its own; BATCH of its loads are under way together, the first of them while the slab is
+    // written (a load that waits for the store before it costs the epilogue a memory latency for every run).
+    template <bool ROWS, bool COLS, int BATCH, typename LR, typename FR, typename LC, typename FC>
+    __device__ __forceinline__ void hand_out(char* lds, LR&& load_row, FR&& rows, LC&& load_col, FC&& cols) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         if (KG > 1 && wave >= NW) return;                           // the first group holds the sums
-        const int wm = wave / WGN, wn = wave % WGN, r = lane & 31, h = lane >> 5;
+        const int wm = wave / WGN * WTM, wn = wave % WGN * WTN, r = lane & 31, h = lane >> 5;
         float* slab = (float*)(lds + wave * SLAB);
         constexpr int LPR = WTN / 8, RPP = 64 / LPR;                // lanes per row, rows per pass
+        constexpr int PASSES = WTN / 16, B = BATCH < PASSES ? BATCH : PASSES;
+        static_assert(PASSES % B == 0, "whole batches");
+        const auto row_at = [&](int i, int p) { return wm + i * 32 + p * RPP + lane / LPR; };
+        const int row_n = wn + lane % LPR * 8;
+        const auto col_m = [&](int i, int p) { return wm + i * 32 + (p * 64 + lane) / WTN * 8; };
+        const auto col_n = [&](int p) { return wn + (p * 64 + lane) % WTN; };
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
+            decltype(load_row(0, 0)) xr[B];
+            decltype(load_col(0, 0)) xc[B];
+            const auto fetch_rows = [&](int p) {
+#pragma unroll
+                for (int q = 0; q < B; ++q) xr[q] = load_row(row_at(i, p + q), row_n);
+            };
+            const auto fetch_cols = [&](int p) {
+#pragma unroll
+                for (int q = 0; q < B; ++q) xc[q] = load_col(col_m(i, p + q), col_n(p + q));
+            };
+            if constexpr (ROWS) fetch_rows(0);
+            else fetch_cols(0);
 #pragma unroll
             for (int j = 0; j < FN; ++j)
 #pragma unroll
@@ -225,27 +250,31 @@ struct GemmTile {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if constexpr (ROWS) {
 #pragma unroll
-                for (int p = 0; p < 32 / RPP; ++p) {
-                    const int row = p * RPP + lane / LPR, col = (lane % LPR) * 8;
-                    const f32x4_t u = *(const f32x4_t*)(slab + row * SLAB_LD + col), w = *(const f32x4_t*)(slab + row * SLAB_LD + col + 4);
+                for (int p = 0; p < PASSES; ++p) {
+                    if (p % B == 0 && p > 0) fetch_rows(p);
+                    const float* at = slab + (p * RPP + lane / LPR) * SLAB_LD + lane % LPR * 8;
+                    const f32x4_t u = *(const f32x4_t*)at, w = *(const f32x4_t*)(at + 4);
                     float v[8] = {u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]};
-                    rows(wm * WTM + i * 32 + row, wn * WTN + col, v);
+                    rows(row_at(i, p), row_n, v, xr[p % B]);
                 }
+                if constexpr (COLS) fetch_cols(0);
             }
             if constexpr (COLS) {
 #pragma unroll
-                for (int p = 0; p < 4 * WTN / 64; ++p) {
+                for (int p = 0; p < PASSES; ++p) {
+                    if (p % B == 0 && p > 0) fetch_cols(p);
                     const int n = (p * 64 + lane) % WTN, g = (p * 64 + lane) / WTN;
                     float v[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] = slab[(g * 8 + e) * SLAB_LD + n];
-                    cols(wm * WTM + i * 32 + g * 8, wn * WTN + n, v);
+                    cols(col_m(i, p), col_n(p), v, xc[p % B]);
                 }
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
     }
 };
+struct GemmNothing {};
 
 // v (already scaled) as a pair of fp16 numbers.  A value that is no number, or beyond fp16, keeps that in hi alone.
 __device__ __forceinline__ void split_f16(float v, _Float16& hi, _Float16& lo) {

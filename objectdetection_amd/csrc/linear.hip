@@ -128,25 +128,70 @@ __device__ __forceinline__ void lin_store8(void* base, long long at, int cnt, co
             if (e < cnt) d[e] = LinType<DT>::put(v[e]);
     }
 }
-// Row i, columns j .. j + cnt - 1 (cnt <= 8)
-template <int DT, int ACT>
-__device__ __forceinline__ void lin_finish8(const LinEnd& p, long long i, int j, int cnt, float v[8]) {
-    if (p.bias) {
-        float b[8];
-        lin_load8<DT>(p.bias, j, cnt, b);
+// Eight values of the caller's type, as loaded
+template <int DT> struct LinRaw { f32x4_t a, b; };
+template <> struct LinRaw<ODAMD_DTYPE_BF16> { u32x4 a; };
+template <int DT>
+__device__ __forceinline__ LinRaw<DT> lin_raw8(const void* base, long long at, int cnt) {
+    LinRaw<DT> r = {};
+    const typename LinType<DT>::T* s = (const typename LinType<DT>::T*)base + at;
+    if (cnt == 8) {
+        if constexpr (DT == ODAMD_DTYPE_F32) {
+            r.a = *(const f32x4_any*)s;
+            r.b = *(const f32x4_any*)(s + 4);
+        } else {
+            r.a = *(const u32x4_any*)s;
+        }
+    } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += b[e];
+        for (int e = 0; e < 8; ++e)
+            if (e < cnt) {
+                if constexpr (DT == ODAMD_DTYPE_F32) {
+                    if (e < 4) r.a[e & 3] = s[e];
+                    else r.b[e & 3] = s[e];
+                } else r.a[e >> 1] |= (uint32_t)s[e] << (16 * (e & 1));
+            }
     }
+    return r;
+}
+__device__ __forceinline__ void lin_values(const LinRaw<ODAMD_DTYPE_F32>& r, float v[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[e] = r.a[e]; v[e + 4] = r.b[e]; }
+}
+__device__ __forceinline__ void lin_values(const LinRaw<ODAMD_DTYPE_BF16>& r, float v[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[2 * e] = __uint_as_float(r.a[e] << 16); v[2 * e + 1] = __uint_as_float(r.a[e] & 0xffff0000u); }
+}
+// Row i, columns j .. j + cnt - 1 (cnt <= 8): bias[8] and the residual's values are there already
+template <int DT, int ACT>
+__device__ __forceinline__ void lin_finish8(const LinEnd& p, long long i, int j, int cnt, float v[8], const float bias[8], const LinRaw<DT>& residual) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += bias[e];
     if (p.z) lin_store8<DT>(p.z, i * p.z_ld + j, cnt, v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = lin_act<DT == ODAMD_DTYPE_BF16, ACT>(v[e]);
     if (p.residual) {
         float r[8];
-        lin_load8<DT>(p.residual, i * p.r_ld + j, cnt, r);
+        lin_values(residual, r);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += r[e];
     }
     lin_store8<DT>(p.y, i * p.y_ld + j, cnt, v);
+}
+template <int DT>
+__device__ __forceinline__ void lin_bias8(const LinEnd& p, int j, int cnt, float b[8]) {
+    if (p.bias && cnt > 0) {
+        lin_load8<DT>(p.bias, j, cnt, b);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = 0.0f;
+    }
+}
+template <int DT, int ACT>
+__device__ __forceinline__ void lin_finish8(const LinEnd& p, long long i, int j, int cnt, float v[8]) {
+    float bias[8];
+    lin_bias8<DT>(p, j, cnt, bias);
+    lin_finish8<DT, ACT>(p, i, j, cnt, v, bias, p.residual ? lin_raw8<DT>(p.residual, i * p.r_ld + j, cnt) : LinRaw<DT>{});
 }
 
 // ---- a few rows: one wave per output column, W read once from memory, no matrix instructions ------------------------
@@ -429,20 +474,36 @@ __global__ void __launch_bounds__(TILE::THREADS) linear_product_kernel(LinLaunch
     const int i0 = ti * TILE::TM, j0 = tj * TILE::TN;
     TILE tile;
     tile.run(p.a, p.b, i0, j0, part * p.per, min(p.chunks, (part + 1) * p.per), p.k_len, lds);
-    auto rows = [&](int i, int j, float v[8]) {
-        i += i0;
-        j += j0;
-        if (i >= p.m || j >= p.n) return;
-        const int cnt = min(8, p.n - j);
-        if constexpr (DT == ODAMD_DTYPE_F32) {
-            const int s = lin_shift(p.a_max[i]);
+    // a lane hands out the same eight columns in all its rows: bias and exponents are loaded once
+    const int col = j0 + tile.row_column(), cnt = max(0, min(8, p.n - col));
+    float bias[8];
+    int shift[8];
+    lin_bias8<DT>(p.end, col, cnt, bias);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], -(s + lin_shift(p.b_max[min(j + e, p.n - 1)])));
+    for (int e = 0; e < 8; ++e) shift[e] = DT == ODAMD_DTYPE_F32 && e < cnt ? lin_shift(p.b_max[col + e]) : 0;
+    struct Before { LinRaw<DT> residual; unsigned max; };
+    const auto before = [&](int i, int) {
+        Before x = {};
+        if (i0 + i < p.m && cnt > 0) {
+            if (!PART && p.end.residual) x.residual = lin_raw8<DT>(p.end.residual, (long long)(i0 + i) * p.end.r_ld + col, cnt);
+            if (DT == ODAMD_DTYPE_F32) x.max = p.a_max[i0 + i];
         }
-        if constexpr (PART) lin_store8<ODAMD_DTYPE_F32>(p.part, ((long long)part * p.m + i) * p.n + j, cnt, v);
-        else lin_finish8<DT, ACT>(p.end, i, j, cnt, v);
+        return x;
     };
-    tile.template hand_out<true, false>(lds, rows, rows);
+    const auto rows = [&](int i, int, float v[8], const Before& x) {
+        i += i0;
+        if (i >= p.m || cnt <= 0) return;
+        if constexpr (DT == ODAMD_DTYPE_F32) {
+            const int s = lin_shift(x.max);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], -(s + shift[e]));
+        }
+        if constexpr (PART) lin_store8<ODAMD_DTYPE_F32>(p.part, ((long long)part * p.m + i) * p.n + col, cnt, v);
+        else lin_finish8<DT, ACT>(p.end, i, col, cnt, v, bias, x.residual);
+    };
+    const auto none = [](int, int) { return GemmNothing{}; };
+    const auto never = [](int, int, float*, const GemmNothing&) {};
+    tile.template hand_out<true, false, 4>(lds, before, rows, none, never);
 }
 
 // Sums the parts of a split reduction in their order (up to two products, the second from run `first` on)

@@ -356,48 +356,71 @@ __global__ void __launch_bounds__(256) ns_whole_kernel(NsTable t, NsIo io, int s
     }
 }
 
-// Results for the caller: eight values from element `at` on, the first `cnt` of them exist.
-template <bool MUON, int DT>
-__device__ __forceinline__ void ns_emit8(const NsIo& io, float step, long long at, int cnt, const float v[8]) {
-    if (cnt <= 0) return;
-    const int n = cnt < 8 ? cnt : 8;
+// Eight values of param and ema before the step, from element `at` on; the first `cnt` of them exist.
+template <bool MUON> struct NsOld {};
+template <> struct NsOld<true> { f32x4_t w[2], e[2]; };
+template <bool MUON>
+__device__ __forceinline__ NsOld<MUON> ns_old8(const NsIo& io, long long at, int cnt) {
+    NsOld<MUON> x = {};
     if constexpr (MUON) {
-        f32x4_any* pp = (f32x4_any*)(io.param + at);
-        f32x4_any* ep = (f32x4_any*)(io.ema + at);
-        if (n == 8) {
+        if (cnt == 8) {
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                f32x4_t w = pp[q];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = w[e] * io.decay - step * v[4 * q + e];
-                pp[q] = w;
-                if (io.ema) {
-                    f32x4_t u = ep[q];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) u[e] = io.ema_keep * u[e] + io.ema_take * w[e];
-                    ep[q] = u;
-                }
+                x.w[q] = *(const f32x4_any*)(io.param + at + 4 * q);
+                if (io.ema) x.e[q] = *(const f32x4_any*)(io.ema + at + 4 * q);
             }
         } else {
-            for (int e = 0; e < n; ++e) {
-                const float w = io.param[at + e] * io.decay - step * v[e];
-                io.param[at + e] = w;
-                if (io.ema) io.ema[at + e] = io.ema_keep * io.ema[at + e] + io.ema_take * w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x.w[e >> 2][e & 3] = e < cnt ? io.param[at + e] : 0.0f;
+                x.e[e >> 2][e & 3] = e < cnt && io.ema ? io.ema[at + e] : 0.0f;
             }
+        }
+    }
+    return x;
+}
+// Results for the caller
+template <bool MUON, int DT>
+__device__ __forceinline__ void ns_emit8(const NsIo& io, float step, long long at, int cnt, const float v[8], const NsOld<MUON>& x) {
+    if (cnt <= 0) return;
+    if constexpr (MUON) {
+        f32x4_t w[2], u[2];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            w[e >> 2][e & 3] = x.w[e >> 2][e & 3] * io.decay - step * v[e];
+            u[e >> 2][e & 3] = io.ema_keep * x.e[e >> 2][e & 3] + io.ema_take * w[e >> 2][e & 3];
+        }
+        if (cnt == 8) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                *(f32x4_any*)(io.param + at + 4 * q) = w[q];
+                if (io.ema) *(f32x4_any*)(io.ema + at + 4 * q) = u[q];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < cnt) {
+                    io.param[at + e] = w[e >> 2][e & 3];
+                    if (io.ema) io.ema[at + e] = u[e >> 2][e & 3];
+                }
         }
     } else if constexpr (DT == ODAMD_DTYPE_BF16) {
         uint16_t* o = (uint16_t*)io.out + at;
-        if (n == 8)
+        if (cnt == 8)
             *(u32x4_any*)o = u32x4{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]), f32x2_to_bf16x2(v[4], v[5]), f32x2_to_bf16x2(v[6], v[7])};
         else
-            for (int e = 0; e < n; ++e) o[e] = f32_to_bf16(v[e]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < cnt) o[e] = f32_to_bf16(v[e]);
     } else {
         float* o = (float*)io.out + at;
-        if (n == 8) {
+        if (cnt == 8) {
             *(f32x4_any*)o = f32x4_t{v[0], v[1], v[2], v[3]};
             *(f32x4_any*)(o + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
         } else {
-            for (int e = 0; e < n; ++e) o[e] = v[e];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < cnt) o[e] = v[e];
         }
     }
 }
@@ -430,38 +453,50 @@ __global__ void __launch_bounds__(TILE::THREADS) ns_product_kernel(NsTable t, Ns
 
     if constexpr (STAGE == ST_A || STAGE == ST_P || STAGE == ST_Q) {
         char* out = square(to);
-        // row i, columns j .. j+7
-        auto put = [&](int i, int j, float v[8]) {
+        // row i, columns j .. j+7; P needs A's values of that place
+        struct Before { f16x8_t hi, lo; };
+        const auto get = [&](int i, int j) {
+            Before x = {};
+            if (STAGE == ST_P && i < p.m && j < mp) {
+                const char* at = square(SQ_A) + (long long)i * mp * 4 + split_at(j);
+                x.hi = *(const f16x8_t*)at;
+                x.lo = *(const f16x8_t*)(at + 64);
+            }
+            return x;
+        };
+        const auto put = [&](int i, int j, float v[8], const Before& x) {
             if (i >= p.m || j >= mp) return;
-            const long long at = (long long)i * mp * 4 + split_at(j);
             if constexpr (STAGE == ST_P) {
-                const f16x8_t hi = *(const f16x8_t*)(square(SQ_A) + at), lo = *(const f16x8_t*)(square(SQ_A) + at + 64);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    v[e] = (NS_C / NS_SCALE) * v[e] + NS_B * ((float)hi[e] + (float)lo[e]) + (i == j + e ? NS_A * NS_SCALE : 0.0f);
+                    v[e] = (NS_C / NS_SCALE) * v[e] + NS_B * ((float)x.hi[e] + (float)x.lo[e]) + (i == j + e ? NS_A * NS_SCALE : 0.0f);
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] *= scale;
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = j + e < p.m ? v[e] : 0.0f;
-            store_split8(out + at, v, 1.0f);
+            store_split8(out + (long long)i * mp * 4 + split_at(j), v, 1.0f);
         };
-        auto rows = [&](int i, int j, float v[8]) { put(i0 + i, j0 + j, v); };
-        auto cols = [&](int i, int j, float v[8]) { put(j0 + j, i0 + i, v); };
-        if (ti == tj) tile.template hand_out<true, false>(lds, rows, cols);
-        else tile.template hand_out<true, true>(lds, rows, cols);
+        const auto get_row = [&](int i, int j) { return get(i0 + i, j0 + j); };
+        const auto get_col = [&](int i, int j) { return get(j0 + j, i0 + i); };
+        const auto rows = [&](int i, int j, float v[8], const Before& x) { put(i0 + i, j0 + j, v, x); };
+        const auto cols = [&](int i, int j, float v[8], const Before& x) { put(j0 + j, i0 + i, v, x); };
+        if (ti == tj) tile.template hand_out<true, false, 4>(lds, get_row, rows, get_col, cols);
+        else tile.template hand_out<true, true, 4>(lds, get_row, rows, get_col, cols);
     } else if constexpr (STAGE == ST_X) {
         char* xt = p.ws + (jobs.turn ? l.xt0 : l.xt1);
-        tile.template hand_out<true, true>(lds,
-            [&](int i, int j, float v[8]) {
+        const auto none = [](int, int) { return GemmNothing{}; };
+        tile.template hand_out<true, true, 1>(lds, none,
+            [&](int i, int j, float v[8], const GemmNothing&) {
                 i += i0; j += j0;
                 if (i >= p.m || j >= np) return;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = j + e < p.n ? v[e] * scale : 0.0f;
                 store_split8(p.ws + l.x + (long long)i * np * 4 + split_at(j), v, 1.0f);
             },
-            [&](int i, int j, float v[8]) {
+            none,
+            [&](int i, int j, float v[8], const GemmNothing&) {
                 i += i0; j += j0;
                 if (j >= p.n || i >= mp) return;
 #pragma unroll
@@ -470,22 +505,22 @@ __global__ void __launch_bounds__(TILE::THREADS) ns_product_kernel(NsTable t, Ns
             });
     } else {
         const float step = MUON ? io.lr02 * sqrtf((float)p.n) : 0.0f;
-        auto rows = [&](int i, int j, float v[8]) {
-            i += i0; j += j0;
-            if (i >= p.m) return;
+        // X[i][j .. j+7] of a wide matrix, X[i .. i+7][j] of a tall one: eight neighbours in the caller's buffer either way
+        const auto at_row = [&](int i, int j) { return p.src + (long long)(i0 + i) * p.n + j0 + j; };
+        const auto at_col = [&](int i, int j) { return p.src + (long long)(j0 + j) * p.m + i0 + i; };
+        const auto count_row = [&](int i, int j) { return i0 + i < p.m ? min(8, p.n - j0 - j) : 0; };
+        const auto count_col = [&](int i, int j) { return j0 + j < p.n ? min(8, p.m - i0 - i) : 0; };
+        const auto emit = [&](long long at, int cnt, float v[8], const NsOld<MUON>& x) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] *= scale;
-            ns_emit8<MUON, DT>(io, step, p.src + (long long)i * p.n + j, p.n - j, v);
+            ns_emit8<MUON, DT>(io, step, at, cnt, v, x);
         };
-        auto cols = [&](int i, int j, float v[8]) {
-            i += i0; j += j0;
-            if (j >= p.n) return;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= scale;
-            ns_emit8<MUON, DT>(io, step, p.src + (long long)j * p.m + i, p.m - i, v);
-        };
-        if (p.tall) tile.template hand_out<false, true>(lds, rows, cols);
-        else tile.template hand_out<true, false>(lds, rows, cols);
+        const auto old_row = [&](int i, int j) { return ns_old8<MUON>(io, at_row(i, j), count_row(i, j)); };
+        const auto old_col = [&](int i, int j) { return ns_old8<MUON>(io, at_col(i, j), count_col(i, j)); };
+        const auto rows = [&](int i, int j, float v[8], const NsOld<MUON>& x) { emit(at_row(i, j), count_row(i, j), v, x); };
+        const auto cols = [&](int i, int j, float v[8], const NsOld<MUON>& x) { emit(at_col(i, j), count_col(i, j), v, x); };
+        if (p.tall) tile.template hand_out<false, true, 2>(lds, old_row, rows, old_col, cols);
+        else tile.template hand_out<true, false, 2>(lds, old_row, rows, old_col, cols);
     }
 }
 
