@@ -15,8 +15,9 @@
 // (global_load_lds_dwordx4), NBUF - 1 rounds ahead; one barrier per round.  A round is one chunk, or KG of them, one for each
 // of KG groups of WGM x WGN waves whose sums are added at the end: where there are few tiles, a tile's chunks are a chain of
 // latencies (barrier, LDS reads, matrix instructions on one accumulator), and more waves on it hide them.  An LDS row is
-// eight 16-byte pieces; piece p of row r lies in slot p ^ (r & 7), so the eight lanes that read the same piece of eight
-// consecutive rows touch eight different slots.  The DMA writes LDS in lane order: the exchange of the slots is in the global
+// eight 16-byte pieces; piece p of row r lies in slot p ^ (r / 2 & 7): sixteen lanes that read the same piece of sixteen
+// consecutive rows, two rows to a sweep of the 64 banks, touch every bank once (with p ^ (r & 7) half of the LDS cycles were
+// conflicts).  The DMA writes LDS in lane order: the exchange of the slots is in the global
 // address each lane reads.
 #ifndef ODAMD_GEMM_H
 #define ODAMD_GEMM_H
@@ -69,7 +70,21 @@ struct GemmOperand {
     const char* p;     // row 0 of the operand
     long long ld;      // bytes per row, a multiple of 16
     int rows;          // rows past the last one are read as the last one; their results are not stored
+    int cols = 0;      // reduction along the rows: values per row (rows past the last one are read as zeros, columns past
+                       // the last as the last eight; a row's memory holds a multiple of eight)
 };
+
+// Eight values of K, four rows each, of the column this lane's read returns
+typedef short gemm_s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x4 gemm_read_tr(const char* first, const char* second) {
+    typedef __attribute__((address_space(3))) gemm_s16x4* lds_ptr;
+    const gemm_s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)first);
+    const gemm_s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)second);
+    const uint2 u = __builtin_bit_cast(uint2, a), v = __builtin_bit_cast(uint2, b);
+    return u32x4{u.x, u.y, v.x, v.y};
+}
+// By how many 32-byte units row k of a chunk with rows of `width` values is turned
+template <int WIDTH> __device__ __forceinline__ int gemm_turn(int k) { return WIDTH >= 128 ? (k & 3) * 2 : (k >> 1 & 1) * 2; }
 
 template <bool F16>
 __device__ __forceinline__ f32x16_t gemm_mma(u32x4 a, u32x4 b, f32x16_t c) {
@@ -99,9 +114,11 @@ struct GemmTile {
     f32x16_t acc[FM][FN];
 
     // Chunks [c0, c1) of K into acc.  k_len: values of K (PL = 1: a multiple of 8, pieces past it are read as zeros; PL = 2:
-    // the rows are padded to whole chunks).
+    // the rows are padded to whole chunks).  TA, TB: A, B lie with the reduction along their rows.
+    template <bool TA = false, bool TB = false>
     __device__ __forceinline__ void run(const GemmOperand& a, const GemmOperand& b, int m0, int n0, int c0, int c1, int k_len,
                                         char* lds) {
+        static_assert(PL == 1 || (!TA && !TB), "pairs lie along the reduction");
         const int lane = threadIdx.x & 63, any = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = any / NW, wave = any % NW;
         const int wm = wave / WGN, wn = wave % WGN, r = lane & 31, h = lane >> 5;
 #pragma unroll
@@ -111,35 +128,66 @@ struct GemmTile {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 
+        // DMA instruction j of this wave brings 1 KiB of A (the first TM / 8 instructions) or of B
         const char* src[NI];
-        const int piece = (lane & 7) ^ (lane >> 3);
+        int row[NI];                                                // reduction along the rows: this lane's row within a chunk
+        // row t * 8 + lane / 8 of the chunk; t is even or odd as the wave is
+        static_assert(NW % 2 == 0 && TM % 16 == 0, "a wave's instructions are all even or all odd");
+        const int piece = (lane & 7) ^ ((wave & 1) * 4 + (lane >> 4));
+        const auto along = [&](const GemmOperand& o, int first, int t) {
+            return o.p + (long long)min(first + t * 8 + (lane >> 3), o.rows - 1) * o.ld + piece * 16;
+        };
+        const auto across = [&](auto width, const GemmOperand& o, int first, int t, int& k) {
+            constexpr int W = width.value, SLOTS = W / 8;           // 16-byte slots per row
+            k = t * (64 / SLOTS) + lane / SLOTS;
+            const int slot = lane % SLOTS, col = first + ((((slot >> 1) ^ gemm_turn<W>(k)) << 1) | (slot & 1)) * 8;
+            return o.p + (long long)k * o.ld + min(col, (o.cols - 1) & ~7) * 2;
+        };
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
-            const int row8 = (wave + j * NW) * 8;                   // wave uniform: A and B instructions do not mix
-            const bool is_a = row8 < TM;
-            const int row = is_a ? m0 + row8 + (lane >> 3) : n0 + row8 - TM + (lane >> 3);
-            const GemmOperand& o = is_a ? a : b;
-            src[j] = o.p + (long long)min(row, o.rows - 1) * o.ld + piece * 16;
+            const int t = wave + j * NW;                            // wave uniform
+            row[j] = 0;
+            if (t * 8 < TM) {
+                if constexpr (TA) src[j] = across(std::integral_constant<int, TM>{}, a, m0, t, row[j]);
+                else src[j] = along(a, m0, t);
+            } else {
+                if constexpr (TB) src[j] = across(std::integral_constant<int, TN>{}, b, n0, t - TM / 8, row[j]);
+                else src[j] = along(b, n0, t - TM / 8);
+            }
         }
         // Round i of this group: chunk c0 + i KG + group; past the last chunk zeros, so that the groups stay in step
         auto issue = [&](int i) {
             const int c = c0 + i * KG + group;
             char* buf = lds + (i % NBUF * KG + group) * BUF;
             const long long at = (long long)c * 128;
-            if ((KG == 1 || c < c1) && (PL == 2 || (c + 1) * BK <= k_len)) {
+            const long long at_a = TA ? c * 64LL * a.ld : at, at_b = TB ? c * 64LL * b.ld : at;
+            const int rows_a = TA ? a.rows : 0x7fffffff, rows_b = TB ? b.rows : 0x7fffffff;
+            if ((KG == 1 || c < c1) && (PL == 2 || ((c + 1) * BK <= k_len && (c + 1) * BK <= rows_a && (c + 1) * BK <= rows_b))) {
 #pragma unroll
-                for (int j = 0; j < NI; ++j) gemm_dma16(src[j] + at, buf + (wave + j * NW) * 1024);
+                for (int j = 0; j < NI; ++j)
+                    gemm_dma16(src[j] + ((wave + j * NW) * 8 < TM ? at_a : at_b), buf + (wave + j * NW) * 1024);
             } else {
-                const bool in = (KG == 1 || c < c1) && (PL == 2 || c * BK + piece * 8 < k_len);
 #pragma unroll
-                for (int j = 0; j < NI; ++j) gemm_dma16(in ? src[j] + at : (const char*)g_gemm_zero, buf + (wave + j * NW) * 1024);
+                for (int j = 0; j < NI; ++j) {
+                    const bool is_a = (wave + j * NW) * 8 < TM, turned = is_a ? TA : TB;
+                    const bool in = (KG == 1 || c < c1) && (PL == 2 || (turned ? c * BK + row[j] < (is_a ? rows_a : rows_b) : c * BK + piece * 8 < k_len));
+                    gemm_dma16(in ? src[j] + (is_a ? at_a : at_b) : (const char*)g_gemm_zero, buf + (wave + j * NW) * 1024);
+                }
             }
         };
         const int rounds = (c1 - c0 + KG - 1) / KG;
 #pragma unroll
         for (int q = 0; q < NBUF - 1; ++q)
             if (q < rounds) issue(q);
-        const int a_off = (wm * WTM + r) * 128, b_off = TM * 128 + (wn * WTN + r) * 128, sw = r & 7;
+        const int a_off = (wm * WTM + r) * 128, b_off = TM * 128 + (wn * WTN + r) * 128, sw = r >> 1 & 7;
+        // transposing reads: lane i of sixteen addresses four columns of row i / 4; lanes 32 on take the next eight rows of K
+        const int tr_row = h * 8 + (lane >> 2 & 3), tr_unit = lane >> 4 & 1, tr_at = (lane & 3) * 8;
+        const auto turned = [&](auto width, const char* base, int col, int s) {
+            constexpr int W = width.value;
+            const int unit = (col / 16 + tr_unit) ^ gemm_turn<W>(tr_row);
+            const char* at = base + (s * 16 + tr_row) * (W * 2) + unit * 32 + tr_at;
+            return gemm_read_tr(at, at + 4 * W * 2);
+        };
         for (int i = 0; i < rounds; ++i) {
             // this wave's pieces of round i have landed (those of up to NBUF - 2 later rounds may still be on their way)
             // and its reads of round i - 1 have returned; behind the barrier that holds for every wave
@@ -157,9 +205,15 @@ struct GemmTile {
                 for (int q = 0; q < PL; ++q) {
                     const int slot = ((4 * q + 2 * s + h) ^ sw) * 16;
 #pragma unroll
-                    for (int x = 0; x < FM; ++x) fa[q][x] = *(const u32x4*)(buf + a_off + x * 4096 + slot);
+                    for (int x = 0; x < FM; ++x) {
+                        if constexpr (TA) fa[q][x] = turned(std::integral_constant<int, TM>{}, buf, wm * WTM + x * 32, s);
+                        else fa[q][x] = *(const u32x4*)(buf + a_off + x * 4096 + slot);
+                    }
 #pragma unroll
-                    for (int y = 0; y < FN; ++y) fb[q][y] = *(const u32x4*)(buf + b_off + y * 4096 + slot);
+                    for (int y = 0; y < FN; ++y) {
+                        if constexpr (TB) fb[q][y] = turned(std::integral_constant<int, TN>{}, buf + TM * 128, wn * WTN + y * 32, s);
+                        else fb[q][y] = *(const u32x4*)(buf + b_off + y * 4096 + slot);
+                    }
                 }
                 // B is the instruction's row operand: a lane then holds one row m of C and runs of four columns n
 #pragma unroll

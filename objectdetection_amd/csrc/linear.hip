@@ -4,8 +4,9 @@
 // bfloat16 operands run on bf16 matrix instructions as they are; float32 operands as fp16 pairs (gemm.h) with a power of
 // two per row of each operand, so that a row's largest value sits just under 2^15: 22 bits per value down to 2^-17 of the row's
 // largest, and the same absolute step below.  Sums are float32, z and dz are kept in the operands' type.
-// Every product reduces along the contiguous axis of both operands: the backward pass lays W, x and dz out by columns
-// first (one launch for all three), because dx reduces over the outputs and dW over the rows.
+// dx reduces over the outputs and dW over the rows: in bfloat16 the products read W, x and dz with the reduction along their
+// rows, out of the caller's tensors; float32 pairs need a power of two per column there, so that W, x and dz are laid out
+// by columns first (one launch for all three).
 #include "common.h"
 #include "odamd.h"
 
@@ -425,6 +426,7 @@ struct LinGemm {
     const unsigned* b_max;
     float* part;             // split reduction: [split][m][n]
     int m, n, k_len, chunks, per, split;   // chunks of K, chunks per split part
+    int a_turned;            // backward pass in bfloat16: B lies with the reduction along its rows, A too where this is set
     LinEnd end;
 };
 // The column sums of 64-row blocks that db is made of
@@ -455,7 +457,7 @@ __device__ __forceinline__ void lin_bias_grad(const LinSums& p, int block, doubl
     }
 }
 
-template <typename TILE, int DT, int ACT, bool PART>
+template <typename TILE, int DT, int ACT, bool PART, bool TURNED>
 __global__ void __launch_bounds__(TILE::THREADS) linear_product_kernel(LinLaunch t) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     int block = (int)blockIdx.x;
@@ -473,7 +475,13 @@ __global__ void __launch_bounds__(TILE::THREADS) linear_product_kernel(LinLaunch
     gemm_tile_at(PART ? id - part * mt * nt : id, mt, nt, ti, tj);
     const int i0 = ti * TILE::TM, j0 = tj * TILE::TN;
     TILE tile;
-    tile.run(p.a, p.b, i0, j0, part * p.per, min(p.chunks, (part + 1) * p.per), p.k_len, lds);
+    const int c0 = part * p.per, c1 = min(p.chunks, (part + 1) * p.per);
+    if constexpr (TURNED) {
+        if (p.a_turned) tile.template run<true, true>(p.a, p.b, i0, j0, c0, c1, p.k_len, lds);
+        else tile.template run<false, true>(p.a, p.b, i0, j0, c0, c1, p.k_len, lds);
+    } else {
+        tile.run(p.a, p.b, i0, j0, c0, c1, p.k_len, lds);
+    }
     // a lane hands out the same eight columns in all its rows: bias and exponents are loaded once
     const int col = j0 + tile.row_column(), cnt = max(0, min(8, p.n - col));
     float bias[8];
@@ -503,7 +511,7 @@ __global__ void __launch_bounds__(TILE::THREADS) linear_product_kernel(LinLaunch
     };
     const auto none = [](int, int) { return GemmNothing{}; };
     const auto never = [](int, int, float*, const GemmNothing&) {};
-    tile.template hand_out<true, false, 4>(lds, before, rows, none, never);
+    tile.template hand_out<true, false, 8>(lds, before, rows, none, never);
 }
 
 // Sums the parts of a split reduction in their order (up to two products, the second from run `first` on)
@@ -541,7 +549,7 @@ struct LinSpace {
 struct LinPlan { int tile, split; };
 // Tile and number of parts the reductions are cut into, by the estimated time of the launch (`count` products).  A larger
 // tile wins per product; but a 256 x 256 tile fills its compute unit, nothing runs beside its epilogue, and all units reach
-// theirs together: (25600, 1024, 4096) with bias, SiLU and residual in bf16 takes 382 us in 256, 329 in 128 and 408 us in
+// theirs together: (25600, 1024, 4096) with bias, SiLU and residual in bf16 takes 290 us in 256, 300 in 128 and 383 us in
 // 64.  Where even 64 x 64 tiles leave units idle, parts of four chunks or more fill them, for the price of a second
 // launch that adds them up (4 us, and their bytes once out and once in).
 template <int DT>
@@ -565,7 +573,7 @@ LinPlan lin_plan(const LinGemm* g, int count) {
             if (!fits) break;
             const double rounds = ceil(load.tiles / 256.0), bytes = (double)tile * tile * (DT == ODAMD_DTYPE_F32 ? 8.0 : 4.0);
             const double us = gemm_time_us(tile, load) * (DT == ODAMD_DTYPE_F32 ? 1.0 : 2.0 / 3.0)
-                              + rounds * bytes / 20.0e3 * (tile == 256 ? 1.0 : 0.4) + extra;
+                              + rounds * bytes / 20.0e3 * (tile == 256 ? 0.9 : 0.8) + extra;
             if (least < 0.0 || us < least) {
                 best = {tile, split};
                 least = us;
@@ -574,7 +582,7 @@ LinPlan lin_plan(const LinGemm* g, int count) {
     return best;
 }
 
-template <typename TILE, int DT, int ACT, bool PART>
+template <typename TILE, int DT, int ACT, bool PART, bool TURNED>
 int lin_launch(LinLaunch& t, int count, hipStream_t s) {
     long long at = 0;
     for (int q = 0; q < 2; ++q) {
@@ -584,26 +592,26 @@ int lin_launch(LinLaunch& t, int count, hipStream_t s) {
     }
     t.block2 = (int)at;
     at += t.sums.db ? (t.sums.n + 63) / 64 : 0;
-    const auto kernel = linear_product_kernel<TILE, DT, ACT, PART>;
+    const auto kernel = linear_product_kernel<TILE, DT, ACT, PART, TURNED>;
     const hipError_t e = odamd_ensure_lds((const void*)kernel, TILE::LDS);
     if (e != hipSuccess) return (int)e;
     kernel<<<(int)at, TILE::THREADS, TILE::LDS, s>>>(t);
     return (int)hipGetLastError();
 }
-template <int DT, int ACT, bool PART>
+template <int DT, int ACT, bool PART, bool TURNED>
 int lin_launch_tile(LinLaunch& t, int count, int tile, hipStream_t s) {
     constexpr int PL = LinType<DT>::PL;
     constexpr bool F16 = DT == ODAMD_DTYPE_F32;
     if constexpr (!PART)
-        if (tile == 256) return lin_launch<GemmTile<PL, F16, 256, 256, 4, 2, 1, 2>, DT, ACT, false>(t, count, s);
-    if (tile == 128) return lin_launch<GemmTile<PL, F16, 128, 128, 2, 4, 1, 2>, DT, ACT, PART>(t, count, s);
+        if (tile == 256) return lin_launch<GemmTile<PL, F16, 256, 256, 4, 2, 1, 2>, DT, ACT, false, TURNED>(t, count, s);
+    if (tile == 128) return lin_launch<GemmTile<PL, F16, 128, 128, 2, 4, 1, 2>, DT, ACT, PART, TURNED>(t, count, s);
     long long tiles = 0;
     for (int q = 0; q < count; ++q) tiles += (((long long)t.g[q].m + 63) / 64) * (((long long)t.g[q].n + 63) / 64) * t.g[q].split;
-    if (tiles > 256) return lin_launch<GemmTile<PL, F16, 64, 64, 2, 2, 1, 2>, DT, ACT, PART>(t, count, s);
-    return lin_launch<GemmTile<PL, F16, 64, 64, 2, 2, 2, 3>, DT, ACT, PART>(t, count, s);
+    if (tiles > 256) return lin_launch<GemmTile<PL, F16, 64, 64, 2, 2, 1, 2>, DT, ACT, PART, TURNED>(t, count, s);
+    return lin_launch<GemmTile<PL, F16, 64, 64, 2, 2, 2, 3>, DT, ACT, PART, TURNED>(t, count, s);
 }
 // `count` products (0: db alone), measuring their workspace or running them
-template <int DT>
+template <int DT, bool BACKWARD>
 int lin_products(LinLaunch& t, int count, LinSpace& ws, bool go, hipStream_t s) {
     const LinPlan plan = lin_plan<DT>(t.g, count);
     bool split = false;
@@ -616,12 +624,14 @@ int lin_products(LinLaunch& t, int count, LinSpace& ws, bool go, hipStream_t s) 
         if (plan.split > 1) g.part = (float*)ws.take((long long)g.split * g.m * g.n * 4);
     }
     if (!go) return 0;
+    constexpr bool TURNED = BACKWARD && DT == ODAMD_DTYPE_BF16;
     int rc = 0;
     if (!split) {
-        lin_with_act(t.g[0].end.act, [&](auto act) { rc = lin_launch_tile<DT, act.value, false>(t, count, plan.tile, s); });
+        if constexpr (BACKWARD) rc = lin_launch_tile<DT, ODAMD_ACT_NONE, false, TURNED>(t, count, plan.tile, s);
+        else lin_with_act(t.g[0].end.act, [&](auto act) { rc = lin_launch_tile<DT, act.value, false, false>(t, count, plan.tile, s); });
         return rc;
     }
-    rc = lin_launch_tile<DT, ODAMD_ACT_NONE, true>(t, count, plan.tile, s);
+    rc = lin_launch_tile<DT, ODAMD_ACT_NONE, true, TURNED>(t, count, plan.tile, s);
     if (rc != 0) return rc;
     const long long first = (long long)t.g[0].m * ((t.g[0].n + 7) / 8);
     const long long total = first + (count > 1 ? (long long)t.g[1].m * ((t.g[1].n + 7) / 8) : 0), blocks = (total + 255) / 256;
@@ -698,94 +708,142 @@ int lin_forward(const odamd_linear_desc& d, LinSpace& ws, bool go, hipStream_t s
         if (e != hipSuccess) return (int)e;
     }
     if (DT == ODAMD_DTYPE_BF16) g.k_len = (int)lin_up(d.k, 8);
-    return lin_products<DT>(launch, 1, ws, go, s);
+    return lin_products<DT, false>(launch, 1, ws, go, s);
 }
 
-template <int DT>
-int lin_backward(const odamd_linear_grad_desc& d, LinSpace& ws, bool go, hipStream_t s) {
-    constexpr int SIZE = DT == ODAMD_DTYPE_F32 ? 4 : 2;
-    constexpr bool F32 = DT == ODAMD_DTYPE_F32;
-    const bool act = d.act != ODAMD_ACT_NONE;
-    const long long mp = lin_up(d.m, lin_chunk<DT>()), np = lin_up(d.n, lin_chunk<DT>());
+// What both forms of the backward pass share: the job that makes dz, the two products' sizes and results, db
+struct LinBackward {
     LinJobs jobs = {};
-    LinJob* z = nullptr;
     LinLaunch launch = {};
-    LinGemm &gx = launch.g[0], &gw = launch.g[d.dx ? 1 : 0];
-    // the largest magnitudes of all operands lie side by side: one launch clears them
-    unsigned* maxes = nullptr;
-    const long long n_max = F32 ? (long long)d.m + d.n + 2LL * d.k : 0;
-    if (F32) maxes = (unsigned*)ws.take(n_max * 4);
-    unsigned *z_row = maxes, *z_col = F32 ? maxes + d.m : nullptr, *w_col = F32 ? z_col + d.n : nullptr, *x_col = F32 ? w_col + d.k : nullptr;
+    int count = 0;
+    LinGemm *gx = nullptr, *gw = nullptr;
+    LinJob& dz() { return jobs.j[0]; }
 
-    z = &jobs.j[jobs.n++];
-    z->src = d.dy;
-    z->ld = d.dy_ld;
-    z->z = act ? d.z : nullptr;
-    z->z_ld = d.z_ld;
-    z->act = d.act;
-    z->m = d.m;
-    z->n = d.n;
-    if (d.dx) {
-        if (go && !act && lin_direct<DT>(d.dy, d.dy_ld, d.n)) {
-            gx.a = {(const char*)d.dy, d.dy_ld * SIZE, d.m};
-        } else {
-            z->rows = ws.take(d.m * np * SIZE);
-            z->row_max = z_row;
-            gx.a = {z->rows, np * SIZE, d.m};
+    LinBackward(const odamd_linear_grad_desc& d, LinSpace& ws) {
+        jobs.n = 1;
+        dz().src = d.dy;
+        dz().ld = d.dy_ld;
+        dz().z = d.act != ODAMD_ACT_NONE ? d.z : nullptr;
+        dz().z_ld = d.z_ld;
+        dz().act = d.act;
+        dz().m = d.m;
+        dz().n = d.n;
+        if (d.dx) {
+            gx = &launch.g[count++];
+            gx->m = d.m;
+            gx->n = d.k;
+            gx->end.y = d.dx;
+            gx->end.y_ld = d.dx_ld;
         }
-        LinJob& w = jobs.j[jobs.n++];
-        w.src = d.w;
-        w.ld = d.w_ld;
-        w.m = d.n;
-        w.n = d.k;
-        w.cols = ws.take(d.k * np * SIZE);
-        w.col_max = w_col;
-        gx.b = {w.cols, np * SIZE, d.k};
-        gx.a_max = z_row;
-        gx.b_max = w_col;
-        gx.m = d.m;
-        gx.n = d.k;
-        gx.k_len = (int)(F32 ? d.n : lin_up(d.n, 8));
-        gx.end.y = d.dx;
-        gx.end.y_ld = d.dx_ld;
+        if (d.dw) {
+            gw = &launch.g[count++];
+            gw->m = d.n;
+            gw->n = d.k;
+            gw->end.y = d.dw;
+            gw->end.y_ld = d.dw_ld;
+        }
+        if (d.db) {
+            const int blocks = (d.m + 63) / 64;
+            dz().sums = (float*)ws.take((long long)blocks * d.n * 4);
+            launch.sums = {dz().sums, d.db, blocks, d.n};
+        }
+    }
+    LinJob& add(const void* src, long long ld, int m, int n) {
+        LinJob& j = jobs.j[jobs.n++];
+        j.src = src;
+        j.ld = ld;
+        j.m = m;
+        j.n = n;
+        return j;
+    }
+};
+
+int lin_backward_bf16(const odamd_linear_grad_desc& d, LinSpace& ws, bool go, hipStream_t s) {
+    constexpr int DT = ODAMD_DTYPE_BF16;
+    LinBackward t(d, ws);
+    const long long np = lin_up(d.n, 64), kp = lin_up(d.k, 64);
+    // dz by rows serves both products; dy itself where there is no activation and its rows can be read as they are
+    GemmOperand dz = {};
+    const bool direct = go && d.act == ODAMD_ACT_NONE && lin_direct<DT>(d.dy, d.dy_ld, d.n);
+    if (t.count) {
+        if (!direct) t.dz().rows = ws.take(d.m * np * 2);
+        dz = direct ? GemmOperand{(const char*)d.dy, d.dy_ld * 2, d.m, d.n} : GemmOperand{t.dz().rows, np * 2, d.m, d.n};
+    }
+    const auto across = [&](const void* p, long long ld, int rows) {
+        if (go && lin_direct<DT>(p, ld, d.k)) return GemmOperand{(const char*)p, ld * 2, rows, d.k};
+        LinJob& j = t.add(p, ld, rows, d.k);
+        j.rows = ws.take(rows * kp * 2);
+        return GemmOperand{j.rows, kp * 2, rows, d.k};
+    };
+    if (d.dx) {
+        t.gx->a = dz;
+        t.gx->b = across(d.w, d.w_ld, d.n);
+        t.gx->k_len = (int)lin_up(d.n, 8);
     }
     if (d.dw) {
-        z->cols = ws.take(d.n * mp * SIZE);
-        z->col_max = z_col;
-        LinJob& x = jobs.j[jobs.n++];
-        x.src = d.x;
-        x.ld = d.x_ld;
-        x.m = d.m;
-        x.n = d.k;
-        x.cols = ws.take(d.k * mp * SIZE);
-        x.col_max = x_col;
-        gw.a = {z->cols, mp * SIZE, d.n};
-        gw.b = {x.cols, mp * SIZE, d.k};
-        gw.a_max = z_col;
-        gw.b_max = x_col;
-        gw.m = d.n;
-        gw.n = d.k;
-        gw.k_len = (int)mp;
-        gw.end.y = d.dw;
-        gw.end.y_ld = d.dw_ld;
+        t.gw->a = dz;
+        t.gw->a_turned = 1;
+        t.gw->b = across(d.x, d.x_ld, d.m);
+        t.gw->k_len = (int)lin_up(d.m, 8);
     }
-    const int row_blocks = (d.m + 63) / 64;
-    if (d.db) {
-        z->sums = (float*)ws.take((long long)row_blocks * d.n * 4);
-        launch.sums = {z->sums, d.db, row_blocks, d.n};
-    }
-    if (go) {
-        const int blocks = lin_tiles(jobs, 0);
+    if (go && (t.dz().rows || t.dz().sums || t.jobs.n > 1)) {
+        const int blocks = lin_tiles(t.jobs, 0);
         if (blocks < 0) return ODAMD_E_LIMIT;
-        if (F32) {
-            linear_clear_kernel<<<(int)((n_max + 255) / 256 < 1024 ? (n_max + 255) / 256 : 1024), 256, 0, s>>>(maxes, n_max);
-            linear_max_kernel<<<blocks, 256, 0, s>>>(jobs);
-        }
-        linear_lay_kernel<DT><<<blocks, 256, 0, s>>>(jobs);
+        linear_lay_kernel<DT><<<blocks, 256, 0, s>>>(t.jobs);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return (int)e;
     }
-    return lin_products<DT>(launch, (d.dx ? 1 : 0) + (d.dw ? 1 : 0), ws, go, s);
+    return lin_products<DT, true>(t.launch, t.count, ws, go, s);
+}
+
+int lin_backward_f32(const odamd_linear_grad_desc& d, LinSpace& ws, bool go, hipStream_t s) {
+    constexpr int DT = ODAMD_DTYPE_F32;
+    LinBackward t(d, ws);
+    const long long mp = lin_up(d.m, 32), np = lin_up(d.n, 32);
+    // the largest magnitudes of all operands lie side by side: one launch clears them
+    const long long n_max = (long long)d.m + d.n + 2LL * d.k;
+    unsigned* maxes = (unsigned*)ws.take(n_max * 4);
+    unsigned *z_row = maxes, *z_col = maxes + d.m, *w_col = z_col + d.n, *x_col = w_col + d.k;
+    if (d.dx) {
+        t.dz().rows = ws.take(d.m * np * 4);
+        t.dz().row_max = z_row;
+        LinJob& w = t.add(d.w, d.w_ld, d.n, d.k);
+        w.cols = ws.take(d.k * np * 4);
+        w.col_max = w_col;
+        t.gx->a = {t.dz().rows, np * 4, d.m};
+        t.gx->b = {w.cols, np * 4, d.k};
+        t.gx->a_max = z_row;
+        t.gx->b_max = w_col;
+        t.gx->k_len = d.n;
+    }
+    if (d.dw) {
+        t.dz().cols = ws.take(d.n * mp * 4);
+        t.dz().col_max = z_col;
+        LinJob& x = t.add(d.x, d.x_ld, d.m, d.k);
+        x.cols = ws.take(d.k * mp * 4);
+        x.col_max = x_col;
+        t.gw->a = {t.dz().cols, mp * 4, d.n};
+        t.gw->b = {x.cols, mp * 4, d.k};
+        t.gw->a_max = z_col;
+        t.gw->b_max = x_col;
+        t.gw->k_len = d.m;
+    }
+    if (go) {
+        const int blocks = lin_tiles(t.jobs, 0);
+        if (blocks < 0) return ODAMD_E_LIMIT;
+        if (t.count) {
+            linear_clear_kernel<<<(int)((n_max + 255) / 256 < 1024 ? (n_max + 255) / 256 : 1024), 256, 0, s>>>(maxes, n_max);
+            linear_max_kernel<<<blocks, 256, 0, s>>>(t.jobs);
+        }
+        linear_lay_kernel<DT><<<blocks, 256, 0, s>>>(t.jobs);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return (int)e;
+    }
+    return lin_products<DT, true>(t.launch, t.count, ws, go, s);
+}
+
+int lin_backward(const odamd_linear_grad_desc& d, LinSpace& ws, bool go, hipStream_t s) {
+    return d.dtype == ODAMD_DTYPE_F32 ? lin_backward_f32(d, ws, go, s) : lin_backward_bf16(d, ws, go, s);
 }
 
 constexpr long long LIN_MAX = 0x7fffffffLL - 1024;
@@ -823,23 +881,23 @@ int odamd_linear_forward(const odamd_linear_desc* d, void* workspace, size_t wor
 size_t odamd_linear_backward_workspace_bytes(const odamd_linear_grad_desc* d) {
     if (!d || !lin_sizes_ok(d->m, d->k, d->n, d->act, d->dtype)) return 0;
     LinSpace ws = {nullptr};
-    if (d->dtype == ODAMD_DTYPE_F32) lin_backward<ODAMD_DTYPE_F32>(*d, ws, false, nullptr);
-    else lin_backward<ODAMD_DTYPE_BF16>(*d, ws, false, nullptr);
+    lin_backward(*d, ws, false, nullptr);
     return (size_t)ws.at;
 }
 
 int odamd_linear_backward(const odamd_linear_grad_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!d || !d->dy || !workspace || !lin_sizes_ok(d->m, d->k, d->n, d->act, d->dtype)) return ODAMD_E_ARG;
+    if (!d || !d->dy || !lin_sizes_ok(d->m, d->k, d->n, d->act, d->dtype)) return ODAMD_E_ARG;
     if (!d->dx && !d->dw && !d->db) return ODAMD_E_ARG;
     if ((d->act != ODAMD_ACT_NONE && !d->z) || (d->dx && !d->w) || (d->dw && !d->x)) return ODAMD_E_ARG;
     if (d->dy_ld < d->n || (d->act != ODAMD_ACT_NONE && d->z_ld < d->n) || (d->dx && (d->w_ld < d->k || d->dx_ld < d->k))
         || (d->dw && (d->x_ld < d->k || d->dw_ld < d->k))) return ODAMD_E_SHAPE;
     if (!lin_aligned(d->dy, d->dtype) || !lin_aligned(d->z, d->dtype) || !lin_aligned(d->x, d->dtype) || !lin_aligned(d->w, d->dtype)
         || !lin_aligned(d->dx, d->dtype) || !lin_aligned(d->dw, d->dtype) || !lin_aligned(d->db, d->dtype) || ((uintptr_t)workspace & 255)) return ODAMD_E_ALIGN;
-    if (workspace_bytes < odamd_linear_backward_workspace_bytes(d)) return ODAMD_E_WORKSPACE;
+    const size_t need = odamd_linear_backward_workspace_bytes(d);
+    if (need && !workspace) return ODAMD_E_ARG;
+    if (workspace_bytes < need) return ODAMD_E_WORKSPACE;
     LinSpace ws = {(char*)workspace};
-    return d->dtype == ODAMD_DTYPE_F32 ? lin_backward<ODAMD_DTYPE_F32>(*d, ws, true, (hipStream_t)stream)
-                                       : lin_backward<ODAMD_DTYPE_BF16>(*d, ws, true, (hipStream_t)stream);
+    return lin_backward(*d, ws, true, (hipStream_t)stream);
 }
 
 }  // extern "C"
