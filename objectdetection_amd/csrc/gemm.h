@@ -361,9 +361,9 @@ __device__ __forceinline__ void store_split8(char* hi_at, const float v[8], floa
 struct GemmLoad { double tiles = 0, chunks = 0, longest = 0; int kinds = 0; };   // chunks: summed over all tiles
 inline void gemm_load_add(GemmLoad& l, double tiles, double chunks) {
     l.tiles += tiles;
+    if (l.kinds == 0 || chunks != l.longest) ++l.kinds;
     l.chunks += tiles * chunks;
     l.longest = chunks > l.longest ? chunks : l.longest;
-    ++l.kinds;
 }
 inline double gemm_time_us(int tile, const GemmLoad& l) {
     const double alone = tile == 256 ? 2.75 : tile == 128 ? 0.69 : 0.3, share = tile == 256 ? 2.75 : tile == 128 ? 0.87 : 0.27;

@@ -470,6 +470,7 @@ __global__ void __launch_bounds__(TILE::THREADS) linear_product_kernel(LinLaunch
     block -= second ? t.block1 : 0;
     const int mt = (p.m + TILE::TM - 1) / TILE::TM, nt = (p.n + TILE::TN - 1) / TILE::TN;
     const int id = gemm_xcd_remap(block, (second ? t.block2 - t.block1 : t.block1));
+    // PART: a product of the launch may be cut
     const int part = PART ? id / (mt * nt) : 0;
     int ti, tj;
     gemm_tile_at(PART ? id - part * mt * nt : id, mt, nt, ti, tj);
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(TILE::THREADS) linear_product_kernel(LinLaunch
     const auto before = [&](int i, int) {
         Before x = {};
         if (i0 + i < p.m && cnt > 0) {
-            if (!PART && p.end.residual) x.residual = lin_raw8<DT>(p.end.residual, (long long)(i0 + i) * p.end.r_ld + col, cnt);
+            if ((!PART || p.split == 1) && p.end.residual) x.residual = lin_raw8<DT>(p.end.residual, (long long)(i0 + i) * p.end.r_ld + col, cnt);
             if (DT == ODAMD_DTYPE_F32) x.max = p.a_max[i0 + i];
         }
         return x;
@@ -506,7 +507,7 @@ __global__ void __launch_bounds__(TILE::THREADS) linear_product_kernel(LinLaunch
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], -(s + shift[e]));
         }
-        if constexpr (PART) lin_store8<ODAMD_DTYPE_F32>(p.part, ((long long)part * p.m + i) * p.n + col, cnt, v);
+        if (PART && p.split > 1) lin_store8<ODAMD_DTYPE_F32>(p.part, ((long long)part * p.m + i) * p.n + col, cnt, v);
         else lin_finish8<DT, ACT>(p.end, i, col, cnt, v, bias, x.residual);
     };
     const auto none = [](int, int) { return GemmNothing{}; };
@@ -514,14 +515,19 @@ __global__ void __launch_bounds__(TILE::THREADS) linear_product_kernel(LinLaunch
     tile.template hand_out<true, false, 8>(lds, before, rows, none, never);
 }
 
-// Sums the parts of a split reduction in their order (up to two products, the second from run `first` on)
+// Sums the parts of split reductions in their order
+struct LinJoin {
+    LinGemm g[2];
+    long long runs[2];   // runs of eight columns of each
+    int n;
+};
 template <int DT>
-__global__ void __launch_bounds__(256) linear_join_kernel(LinLaunch t, long long first, long long total) {
-    for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < total; q += (long long)gridDim.x * 256) {
-        const bool second = q >= first;
+__global__ void __launch_bounds__(256) linear_join_kernel(LinJoin t) {
+    for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < t.runs[0] + t.runs[1]; q += (long long)gridDim.x * 256) {
+        const bool second = q >= t.runs[0];
         const LinGemm& p = second ? t.g[1] : t.g[0];
         const int runs = (p.n + 7) / 8;
-        const long long at = second ? q - first : q, i = at / runs;
+        const long long at = second ? q - t.runs[0] : q, i = at / runs;
         const int j = (int)(at - i * runs) * 8, cnt = min(8, p.n - j);
         float v[8], u[8];
         lin_load8<ODAMD_DTYPE_F32>(p.part, i * p.n + j, cnt, v);
@@ -546,36 +552,37 @@ struct LinSpace {
     }
 };
 
-struct LinPlan { int tile, split; };
-// Tile and number of parts the reductions are cut into, by the estimated time of the launch (`count` products).  A larger
+struct LinPlan { int tile, longest; };   // longest: chunks a workgroup takes at most
+// Tile and length of the parts the reductions are cut into, by the estimated time of the launch (`count` products).  A larger
 // tile wins per product; but a 256 x 256 tile fills its compute unit, nothing runs beside its epilogue, and all units reach
 // theirs together: (25600, 1024, 4096) with bias, SiLU and residual in bf16 takes 290 us in 256, 300 in 128 and 383 us in
-// 64.  Where even 64 x 64 tiles leave units idle, parts of four chunks or more fill them, for the price of a second
-// launch that adds them up (4 us, and their bytes once out and once in).
+// 64.  Where tiles leave units idle, or two products of a launch differ in length, parts of four chunks or more fill them,
+// for the price of a second launch that adds them up (4 us, and their bytes once out and once in).
 template <int DT>
 LinPlan lin_plan(const LinGemm* g, int count) {
-    LinPlan best = {64, 1};
+    int all = 1;
+    for (int q = 0; q < count; ++q) {
+        const int chunks = (g[q].k_len + lin_chunk<DT>() - 1) / lin_chunk<DT>();
+        all = chunks > all ? chunks : all;
+    }
+    LinPlan best = {64, all};
     double least = -1.0;
     for (int tile : {64, 128, 256})
-        for (int split = 1; split <= 32; split *= 2) {
-            if (split > 1 && tile == 256) break;
+        for (int cut = 1; cut <= 32 && (cut == 1 || all / cut >= 4); cut *= 2) {
+            const int longest = (all + cut - 1) / cut;
             GemmLoad load;
-            double extra = split > 1 ? 4.0 : 0.0;
-            bool fits = true;
+            double extra = 0.0;
             for (int q = 0; q < count; ++q) {
-                const int chunks = (g[q].k_len + lin_chunk<DT>() - 1) / lin_chunk<DT>();
-                const int per = (chunks + split - 1) / split, parts = (chunks + per - 1) / per;
-                fits = fits && (split == 1 || per >= 4);
+                const int chunks = (g[q].k_len + lin_chunk<DT>() - 1) / lin_chunk<DT>(), parts = (chunks + longest - 1) / longest;
                 const double tiles = (double)((g[q].m + (long long)tile - 1) / tile) * ((g[q].n + (long long)tile - 1) / tile);
-                gemm_load_add(load, tiles * parts, per);
-                if (parts > 1) extra += parts * (double)g[q].m * g[q].n * 8.0 / 3.0e6;
+                gemm_load_add(load, tiles * parts, (chunks + parts - 1) / parts);
+                if (parts > 1) extra += 4.0 / count + parts * (double)g[q].m * g[q].n * 8.0 / 3.0e6;
             }
-            if (!fits) break;
             const double rounds = ceil(load.tiles / 256.0), bytes = (double)tile * tile * (DT == ODAMD_DTYPE_F32 ? 8.0 : 4.0);
             const double us = gemm_time_us(tile, load) * (DT == ODAMD_DTYPE_F32 ? 1.0 : 2.0 / 3.0)
                               + rounds * bytes / 20.0e3 * (tile == 256 ? 0.9 : 0.8) + extra;
             if (least < 0.0 || us < least) {
-                best = {tile, split};
+                best = {tile, longest};
                 least = us;
             }
         }
@@ -602,8 +609,7 @@ template <int DT, int ACT, bool PART, bool TURNED>
 int lin_launch_tile(LinLaunch& t, int count, int tile, hipStream_t s) {
     constexpr int PL = LinType<DT>::PL;
     constexpr bool F16 = DT == ODAMD_DTYPE_F32;
-    if constexpr (!PART)
-        if (tile == 256) return lin_launch<GemmTile<PL, F16, 256, 256, 4, 2, 1, 2>, DT, ACT, false, TURNED>(t, count, s);
+    if (tile == 256) return lin_launch<GemmTile<PL, F16, 256, 256, 4, 2, 1, 2>, DT, ACT, PART, TURNED>(t, count, s);
     if (tile == 128) return lin_launch<GemmTile<PL, F16, 128, 128, 2, 4, 1, 2>, DT, ACT, PART, TURNED>(t, count, s);
     long long tiles = 0;
     for (int q = 0; q < count; ++q) tiles += (((long long)t.g[q].m + 63) / 64) * (((long long)t.g[q].n + 63) / 64) * t.g[q].split;
@@ -614,28 +620,31 @@ int lin_launch_tile(LinLaunch& t, int count, int tile, hipStream_t s) {
 template <int DT, bool BACKWARD>
 int lin_products(LinLaunch& t, int count, LinSpace& ws, bool go, hipStream_t s) {
     const LinPlan plan = lin_plan<DT>(t.g, count);
-    bool split = false;
+    LinJoin join = {};
     for (int q = 0; q < count; ++q) {
         LinGemm& g = t.g[q];
         g.chunks = (g.k_len + lin_chunk<DT>() - 1) / lin_chunk<DT>();
-        g.per = (g.chunks + plan.split - 1) / plan.split;
+        g.split = (g.chunks + plan.longest - 1) / plan.longest;
+        g.per = (g.chunks + g.split - 1) / g.split;
         g.split = (g.chunks + g.per - 1) / g.per;
-        split = split || plan.split > 1;
-        if (plan.split > 1) g.part = (float*)ws.take((long long)g.split * g.m * g.n * 4);
+        if (g.split > 1) {
+            g.part = (float*)ws.take((long long)g.split * g.m * g.n * 4);
+            join.g[join.n] = g;
+            join.runs[join.n++] = (long long)g.m * ((g.n + 7) / 8);
+        }
     }
     if (!go) return 0;
     constexpr bool TURNED = BACKWARD && DT == ODAMD_DTYPE_BF16;
     int rc = 0;
-    if (!split) {
+    if (join.n == 0) {
         if constexpr (BACKWARD) rc = lin_launch_tile<DT, ODAMD_ACT_NONE, false, TURNED>(t, count, plan.tile, s);
         else lin_with_act(t.g[0].end.act, [&](auto act) { rc = lin_launch_tile<DT, act.value, false, false>(t, count, plan.tile, s); });
         return rc;
     }
     rc = lin_launch_tile<DT, ODAMD_ACT_NONE, true, TURNED>(t, count, plan.tile, s);
     if (rc != 0) return rc;
-    const long long first = (long long)t.g[0].m * ((t.g[0].n + 7) / 8);
-    const long long total = first + (count > 1 ? (long long)t.g[1].m * ((t.g[1].n + 7) / 8) : 0), blocks = (total + 255) / 256;
-    linear_join_kernel<DT><<<(int)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(t, first, total);
+    const long long blocks = (join.runs[0] + join.runs[1] + 255) / 256;
+    linear_join_kernel<DT><<<(int)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(join);
     return (int)hipGetLastError();
 }
 
