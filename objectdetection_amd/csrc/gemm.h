@@ -106,6 +106,10 @@ struct GemmTile {
     static constexpr int SLAB = 32 * SLAB_LD * 4;
     static constexpr int RING = NBUF * KG * BUF;                    // buffer of round i, group g: (i % NBUF) * KG + g
     static constexpr int LDS = RING > NW * SLAB ? RING : NW * SLAB;
+    // Pairs work long enough on a fragment to hide the next one's read from registers; bf16 products gain nothing from it
+    // (25600 x 4096 x 1024 in 256 x 256: 243 us without, 252 with; pairs, 8192 x 1024 x 2304 in 128 x 128: 105 and 91 us), and a
+    // 256 x 256 tile has no registers for it (it spills, and the optimizer step's last product takes 1059 instead of 940 us).
+    static constexpr bool PIPE = PL == 2 && KG == 1 && NBUF == 2 && FM * FN <= 4;
     static constexpr int NI = (TM + TN) / 8 / NW;                   // DMA instructions per wave and chunk
     static_assert((TM + TN) % (8 * NW) == 0 && TM % 8 == 0, "whole DMA instructions");
     static_assert((KG - 1) * NW * FM * FN * 4096 <= RING, "the other groups' sums pass through the ring");
@@ -176,9 +180,6 @@ struct GemmTile {
             }
         };
         const int rounds = (c1 - c0 + KG - 1) / KG;
-#pragma unroll
-        for (int q = 0; q < NBUF - 1; ++q)
-            if (q < rounds) issue(q);
         const int a_off = (wm * WTM + r) * 128, b_off = TM * 128 + (wn * WTN + r) * 128, sw = r >> 1 & 7;
         // transposing reads: lane i of sixteen addresses four columns of row i / 4; lanes 32 on take the next eight rows of K
         const int tr_row = h * 8 + (lane >> 2 & 3), tr_unit = lane >> 4 & 1, tr_at = (lane & 3) * 8;
@@ -188,41 +189,82 @@ struct GemmTile {
             const char* at = base + (s * 16 + tr_row) * (W * 2) + unit * 32 + tr_at;
             return gemm_read_tr(at, at + 4 * W * 2);
         };
-        for (int i = 0; i < rounds; ++i) {
-            // this wave's pieces of round i have landed (those of up to NBUF - 2 later rounds may still be on their way)
-            // and its reads of round i - 1 have returned; behind the barrier that holds for every wave
-            const int ahead = min(NBUF - 2, rounds - 1 - i);
-            if (NBUF > 3 && ahead == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NBUF > 3 ? 2 * NI : 0) : "memory");
-            else if (NBUF > 2 && ahead == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NBUF > 2 ? NI : 0) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            const char* buf = lds + (i % NBUF * KG + group) * BUF;
-            if (i + NBUF - 1 < rounds) issue(i + NBUF - 1);
+        constexpr int STEPS = BK / 16, SUMS = PL == 1 ? 1 : 3;      // steps of a chunk, matrix instructions per product
+        u32x4 fa[PIPE ? 2 : 1][PL][FM], fb[PIPE ? 2 : 1][PL][FN];
+        const auto read = [&](const char* buf, int s, int to) {     // the fragments of step s
 #pragma unroll
-            for (int s = 0; s < BK / 16; ++s) {
-                u32x4 fa[PL][FM], fb[PL][FN];
+            for (int q = 0; q < PL; ++q) {
+                const int slot = ((4 * q + 2 * s + h) ^ sw) * 16;
 #pragma unroll
-                for (int q = 0; q < PL; ++q) {
-                    const int slot = ((4 * q + 2 * s + h) ^ sw) * 16;
-#pragma unroll
-                    for (int x = 0; x < FM; ++x) {
-                        if constexpr (TA) fa[q][x] = turned(std::integral_constant<int, TM>{}, buf, wm * WTM + x * 32, s);
-                        else fa[q][x] = *(const u32x4*)(buf + a_off + x * 4096 + slot);
-                    }
-#pragma unroll
-                    for (int y = 0; y < FN; ++y) {
-                        if constexpr (TB) fb[q][y] = turned(std::integral_constant<int, TN>{}, buf + TM * 128, wn * WTN + y * 32, s);
-                        else fb[q][y] = *(const u32x4*)(buf + b_off + y * 4096 + slot);
-                    }
+                for (int x = 0; x < FM; ++x) {
+                    if constexpr (TA) fa[to][q][x] = turned(std::integral_constant<int, TM>{}, buf, wm * WTM + x * 32, s);
+                    else fa[to][q][x] = *(const u32x4*)(buf + a_off + x * 4096 + slot);
                 }
-                // B is the instruction's row operand: a lane then holds one row m of C and runs of four columns n
 #pragma unroll
-                for (int q = 0; q < (PL == 1 ? 1 : 3); ++q)
+                for (int y = 0; y < FN; ++y) {
+                    if constexpr (TB) fb[to][q][y] = turned(std::integral_constant<int, TN>{}, buf + TM * 128, wn * WTN + y * 32, s);
+                    else fb[to][q][y] = *(const u32x4*)(buf + b_off + y * 4096 + slot);
+                }
+            }
+        };
+        // B is the instruction's row operand: a lane then holds one row m of C and runs of four columns n
+        const auto multiply = [&](int f) {
 #pragma unroll
-                    for (int x = 0; x < FM; ++x)
+            for (int q = 0; q < SUMS; ++q)
 #pragma unroll
-                        for (int y = 0; y < FN; ++y)
-                            acc[x][y] = gemm_mma<F16>(fb[q == 1 ? PL - 1 : 0][y], fa[q == 2 ? PL - 1 : 0][x], acc[x][y]);
+                for (int x = 0; x < FM; ++x)
+#pragma unroll
+                    for (int y = 0; y < FN; ++y)
+                        acc[x][y] = gemm_mma<F16>(fb[f][q == 1 ? PL - 1 : 0][y], fa[f][q == 2 ? PL - 1 : 0][x], acc[x][y]);
+        };
+        if constexpr (PIPE) {
+            // The fragments of the next step are read while the matrix cores work on this one's, over the end of a chunk too:
+            // in a chunk's last step this wave's fragments of it are in registers and its pieces of the next chunk in LDS; behind
+            // the barrier that holds for every wave, and the chunk's buffer may take the one after the next.
+            issue(0);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            if (rounds > 1) issue(1);
+            read(lds, 0, 0);
+            for (int i = 0; i < rounds; ++i) {
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    if (s + 1 < STEPS) {
+                        read(lds + (i & 1) * BUF, s + 1, (s + 1) & 1);
+                    } else {
+                        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                        __builtin_amdgcn_s_barrier();
+                        read(lds + (~i & 1) * BUF, 0, (s + 1) & 1); // behind the last chunk: of no use, but within LDS
+                        if (i + 2 < rounds) issue(i + 2);
+                    }
+                    multiply(s & 1);
+                    constexpr int READS = PL * (FM + FN);
+#pragma unroll
+                    for (int q = 0; q < READS; ++q) {               // one LDS read, then its share of the matrix instructions
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x008, SUMS * FM * FN / READS, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < NBUF - 1; ++q)
+                if (q < rounds) issue(q);
+            for (int i = 0; i < rounds; ++i) {
+                // this wave's pieces of round i have landed (those of up to NBUF - 2 later rounds may still be on their way)
+                // and its reads of round i - 1 have returned; behind the barrier that holds for every wave
+                const int ahead = min(NBUF - 2, rounds - 1 - i);
+                if (NBUF > 3 && ahead == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NBUF > 3 ? 2 * NI : 0) : "memory");
+                else if (NBUF > 2 && ahead == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NBUF > 2 ? NI : 0) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                if (i + NBUF - 1 < rounds) issue(i + NBUF - 1);
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    read(lds + (i % NBUF * KG + group) * BUF, s, 0);
+                    multiply(0);
+                }
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -353,11 +395,11 @@ __device__ __forceinline__ void store_split8(char* hi_at, const float v[8], floa
 }
 
 // ---- host: which tile ------------------------------------------------------------------------------------------------
-// Measured with pairs at 4096^3, 2048 x 1024 x 2048 and below: time of a chunk of one tile alone on a compute unit (0.69 us for
-// 128 x 128, 0.3 us for 64 x 64 with two wave groups), and its share of a unit's time where several tiles run there (0.87 and
-// 0.27 us; 2.75 us for 256 x 256, which fills a unit by itself).  The larger tile wins per product, the smaller one
-// spreads a small product over all 256 units: 4096 x 4096 x 4096 353 / 445 / 512 us in 256 / 128 / 64, 2048 x 1024 x 2048
-// - / 45 / 33 us.  bf16 chunks take two thirds of the time for every tile: the choice is the same.
+// Measured with pairs at 4096^3, 8192 x 1024 x 2304 and below: time of a 128-byte chunk, in us, of tiles that have a compute unit
+// to themselves (64 x 64: 0.3 with two wave groups, 0.49 with one, which two tiles of a unit run beside each other), and
+// the share of a unit's time a tile's chunk takes where more of them run there.  The larger tile wins per product, the
+// smaller one spreads a small product over all 256 units: 4096 x 4096 x 4096 takes 353 / 367 / 512 us in 256 / 128 / 64,
+// 2048 x 1024 x 2048 - / 44 / 34 us.  bf16 chunks take two thirds of the time.
 struct GemmLoad { double tiles = 0, chunks = 0, longest = 0; int kinds = 0; };   // chunks: summed over all tiles
 inline void gemm_load_add(GemmLoad& l, double tiles, double chunks) {
     l.tiles += tiles;
@@ -365,13 +407,14 @@ inline void gemm_load_add(GemmLoad& l, double tiles, double chunks) {
     l.chunks += tiles * chunks;
     l.longest = chunks > l.longest ? chunks : l.longest;
 }
-inline double gemm_time_us(int tile, const GemmLoad& l) {
-    const double alone = tile == 256 ? 2.75 : tile == 128 ? 0.69 : 0.3, share = tile == 256 ? 2.75 : tile == 128 ? 0.87 : 0.27;
+inline double gemm_time_us(int tile, const GemmLoad& l, bool pairs) {
     // tiles of one length run in whole rounds
     const double rounds = l.kinds == 1 ? (double)(((long long)l.tiles + 255) / 256) : l.chunks / (256.0 * l.longest);
+    const double share = tile == 256 ? 2.75 : tile == 128 ? (pairs ? 0.75 : 0.87) : 0.24;
+    const double alone = tile == 256 ? 2.75 : tile == 128 ? 0.75 : l.tiles <= 256.0 ? 0.3 : 0.49;
     const double us = l.longest * (alone > share * rounds ? alone : share * rounds);
-    // of several lengths they pack as they come: half of the longest is left over at the end
-    return l.kinds == 1 ? us : us + 0.5 * l.longest * share;
+    // of several lengths they pack as they come: a quarter of the longest is left over at the end
+    return (l.kinds == 1 ? us : us + 0.25 * l.longest * share) * (pairs ? 1.0 : 2.0 / 3.0);
 }
 
 #endif

@@ -579,7 +579,7 @@ LinPlan lin_plan(const LinGemm* g, int count) {
                 if (parts > 1) extra += 4.0 / count + parts * (double)g[q].m * g[q].n * 8.0 / 3.0e6;
             }
             const double rounds = ceil(load.tiles / 256.0), bytes = (double)tile * tile * (DT == ODAMD_DTYPE_F32 ? 8.0 : 4.0);
-            const double us = gemm_time_us(tile, load) * (DT == ODAMD_DTYPE_F32 ? 1.0 : 2.0 / 3.0)
+            const double us = gemm_time_us(tile, load, DT == ODAMD_DTYPE_F32)
                               + rounds * bytes / 20.0e3 * (tile == 256 ? 0.9 : 0.8) + extra;
             if (least < 0.0 || us < least) {
                 best = {tile, longest};
@@ -610,7 +610,7 @@ int lin_launch_tile(LinLaunch& t, int count, int tile, hipStream_t s) {
     constexpr int PL = LinType<DT>::PL;
     constexpr bool F16 = DT == ODAMD_DTYPE_F32;
     if (tile == 256) return lin_launch<GemmTile<PL, F16, 256, 256, 4, 2, 1, 2>, DT, ACT, PART, TURNED>(t, count, s);
-    if (tile == 128) return lin_launch<GemmTile<PL, F16, 128, 128, 2, 4, 1, 2>, DT, ACT, PART, TURNED>(t, count, s);
+    if (tile == 128) return lin_launch<GemmTile<PL, F16, 128, 128, 2, PL == 2 ? 2 : 4, 1, 2>, DT, ACT, PART, TURNED>(t, count, s);
     long long tiles = 0;
     for (int q = 0; q < count; ++q) tiles += (((long long)t.g[q].m + 63) / 64) * (((long long)t.g[q].n + 63) / 64) * t.g[q].split;
     if (tiles > 256) return lin_launch<GemmTile<PL, F16, 64, 64, 2, 2, 1, 2>, DT, ACT, PART, TURNED>(t, count, s);

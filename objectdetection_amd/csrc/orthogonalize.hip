@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(TILE::THREADS) ns_product_kernel(NsTable t, Ns
 }
 
 using NsTile256 = GemmTile<2, true, 256, 256, 4, 2, 1, 2>;
-using NsTile128 = GemmTile<2, true, 128, 128, 2, 4, 1, 2>;
+using NsTile128 = GemmTile<2, true, 128, 128, 2, 2, 1, 2>;
 using NsTile64 = GemmTile<2, true, 64, 64, 2, 2, 1, 2>;
 using NsTile64Few = GemmTile<2, true, 64, 64, 2, 2, 2, 3>;   // two wave groups: one tile, or less, for a compute unit
 
@@ -559,7 +559,7 @@ int ns_product(NsTable& t, const NsIo& io, const NsJobs& jobs, hipStream_t s) {
         for (int i = 0; i < t.n; ++i)
             gemm_load_add(load, (double)ns_tiles(STAGE, tile, t.g[i].m, t.g[i].n) * t.g[i].count * jobs.n,
                           (double)(ns_up(STAGE == ST_A ? t.g[i].n : t.g[i].m, 32) / 32));
-        const double us = gemm_time_us(tile, load);
+        const double us = gemm_time_us(tile, load, true);
         if (tile == 64) tiles64 = load.tiles;
         if (tile == 64 || us < least) {
             best = tile;
