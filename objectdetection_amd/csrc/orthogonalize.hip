@@ -135,6 +135,32 @@ __device__ __forceinline__ double ns_block_sum(double v, double* shared) {
     return s;
 }
 
+// Eight of the caller's values; zeros for those past the first `cnt`
+template <int DT>
+__device__ __forceinline__ void ns_load8(const void* base, long long at, int cnt, float v[8]) {
+    if constexpr (DT == ODAMD_DTYPE_BF16) {
+        const uint16_t* s = (const uint16_t*)base + at;
+        if (cnt == 8) {
+            const u32x4 u = *(const u32x4_any*)s;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { v[2 * e] = __uint_as_float(u[e] << 16); v[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u); }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = e < cnt ? bf16_to_f32(s[e]) : 0.0f;
+        }
+    } else {
+        const float* s = (const float*)base + at;
+        if (cnt == 8) {
+            const f32x4_t u = *(const f32x4_any*)s, w = *(const f32x4_any*)(s + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { v[e] = u[e]; v[e + 4] = w[e]; }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = e < cnt ? s[e] : 0.0f;
+        }
+    }
+}
+
 // Sums of squares in double (gradients of 1e-20 and of 1e20 have a norm too), a fixed share of a matrix per workgroup and
 // summed in a fixed order: the result does not change from run to run.  The optimizer step's momentum update happens here.
 template <bool MUON, int DT>
@@ -145,35 +171,12 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(NsTable t, NsIo io) {
     const long long to = from + share < total ? from + share : total;
     double s = 0.0;
     // eight elements a thread
-    using T = typename std::conditional<DT == ODAMD_DTYPE_BF16, uint16_t, float>::type;
-    const T* in = (const T*)io.in + p.src;
     float* mom = MUON ? io.momentum + p.src : nullptr;
     for (long long i = from + threadIdx.x * 8; i < to; i += 2048) {
         const int cnt = to - i < 8 ? (int)(to - i) : 8;
         float g[8], m[8];
-        if (cnt == 8) {
-            if constexpr (DT == ODAMD_DTYPE_BF16) {
-                const u32x4 u = *(const u32x4_any*)(in + i);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) { g[2 * e] = __uint_as_float(u[e] << 16); g[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u); }
-            } else {
-                const f32x4_t u = *(const f32x4_any*)(in + i), v = *(const f32x4_any*)(in + i + 4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) { g[e] = u[e]; g[e + 4] = v[e]; }
-            }
-            if constexpr (MUON) {
-                const f32x4_t u = *(const f32x4_any*)(mom + i), v = *(const f32x4_any*)(mom + i + 4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) { m[e] = u[e]; m[e + 4] = v[e]; }
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if constexpr (DT == ODAMD_DTYPE_BF16) g[e] = e < cnt ? bf16_to_f32(in[i + e]) : 0.0f;
-                else g[e] = e < cnt ? in[i + e] : 0.0f;
-                if constexpr (MUON) m[e] = e < cnt ? mom[i + e] : 0.0f;
-            }
-        }
+        ns_load8<DT>(io.in, p.src + i, cnt, g);
+        if constexpr (MUON) ns_load8<ODAMD_DTYPE_F32>(mom, i, cnt, m);
         if constexpr (MUON) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -208,35 +211,39 @@ __global__ void __launch_bounds__(256) ns_split_kernel(NsTable t, NsIo io) {
     for (int i = threadIdx.x; i < parts; i += 256) mine += ((const double*)p.ws)[i];
     const double sum = ns_block_sum(mine, part);
     const float inv = (float)(1.0 / (sqrt(sum) + io.eps));
-    const int nt = (p.n + 63) / 64, i0 = p.tile / nt * 64, j0 = p.tile % nt * 64;
-    const int lane = threadIdx.x & 63, row = threadIdx.x >> 6;
-    // along the caller's rows
-    for (int q = row; q < 64; q += 4) {
-        const int i = p.tall ? i0 + lane : i0 + q, j = p.tall ? j0 + q : j0 + lane;
-        float v = 0.0f;
-        if (i < p.m && j < p.n) {
-            const long long at = p.src + (p.tall ? (long long)j * p.m + i : (long long)i * p.n + j);
-            if constexpr (MUON) v = ns_direction(io, ((const float*)io.in)[at], io.momentum[at]);
-            else if constexpr (DT == ODAMD_DTYPE_BF16) v = bf16_to_f32(((const uint16_t*)io.in)[at]);
-            else v = ((const float*)io.in)[at];
-            v *= inv;
+    // in the caller's rows and columns: what lies along its rows goes out as it comes, the other copy through LDS
+    const int rows = p.tall ? p.n : p.m, cols = p.tall ? p.m : p.n, ct = (cols + 63) / 64;
+    const int r0 = p.tile / ct * 64, c0 = p.tile % ct * 64, c = (threadIdx.x & 7) * 8;
+    const int rp = (int)ns_up(rows, 32), cp = (int)ns_up(cols, 32);
+    char* along = p.ws + (p.tall ? l.xt0 : l.x);
+    char* across = p.ws + (p.tall ? l.x : l.xt0);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int r = (threadIdx.x >> 3) + 32 * q, cnt = r0 + r < rows ? max(0, min(8, cols - c0 - c)) : 0;
+        const long long at = p.src + (long long)(r0 + r) * cols + c0 + c;
+        float v[8], m[8];
+        ns_load8<DT>(io.in, at, cnt, v);
+        if constexpr (MUON) {
+            ns_load8<ODAMD_DTYPE_F32>(io.momentum, at, cnt, m);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = ns_direction(io, v[e], m[e]);
         }
-        if (p.tall) tile[lane][q] = v; else tile[q][lane] = v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[e] = e < cnt ? v[e] * inv : 0.0f;
+            tile[r][c + e] = v[e];
+        }
+        if (r0 + r < rows && c0 + c < cp) store_split8(along + (long long)(r0 + r) * cp * 4 + split_at(c0 + c), v, NS_SCALE);
     }
     __syncthreads();
-    const int mp = (int)ns_up(p.m, 32), np = (int)ns_up(p.n, 32);
-    for (int q = threadIdx.x; q < 512; q += 256) {
-        float v[8];
-        const int r = q >> 3, c = (q & 7) * 8;
-        if (i0 + r < p.m && j0 + c < np) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = tile[r][c + e];
-            store_split8(p.ws + l.x + (long long)(i0 + r) * np * 4 + split_at(j0 + c), v, NS_SCALE);
-        }
-        if (j0 + r < p.n && i0 + c < mp) {
+    for (int q = 0; q < 2; ++q) {
+        const int r = (threadIdx.x >> 3) + 32 * q;
+        float v[8];
+        if (c0 + r < cols && r0 + c < rp) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = tile[c + e][r];
-            store_split8(p.ws + l.xt0 + (long long)(j0 + r) * mp * 4 + split_at(i0 + c), v, NS_SCALE);
+            store_split8(across + (long long)(c0 + r) * rp * 4 + split_at(r0 + c), v, NS_SCALE);
         }
     }
 }
