@@ -395,11 +395,20 @@ __device__ __forceinline__ void store_split8(char* hi_at, const float v[8], floa
 }
 
 // ---- host: which tile ------------------------------------------------------------------------------------------------
-// Measured with pairs at 4096^3, 8192 x 1024 x 2304 and below: time of a 128-byte chunk, in us, of tiles that have a compute unit
-// to themselves (64 x 64: 0.3 with two wave groups, 0.49 with one, which two tiles of a unit run beside each other), and
-// the share of a unit's time a tile's chunk takes where more of them run there.  The larger tile wins per product, the
-// smaller one spreads a small product over all 256 units: 4096 x 4096 x 4096 takes 353 / 367 / 512 us in 256 / 128 / 64,
-// 2048 x 1024 x 2048 - / 44 / 34 us.  bf16 chunks take two thirds of the time.
+// Time of a 128-byte chunk of all tiles of a compute unit, in us, by how many tiles a unit has to run (`rounds`; measured
+// with pairs at 4096^3, 8192 x 1024 x 2304 and below).  The larger tile wins per product, the smaller one spreads a small
+// product over all 256 units: 4096 x 4096 x 4096 takes 353 / 367 / 512 us in 256 / 128 / 64, 2048 x 1024 x 2048
+// - / 44 / 34 us.  bf16 chunks take two thirds of the time.
+inline double gemm_chunk_us(int tile, double rounds, bool pairs) {
+    if (tile == 256) return 2.75 * (rounds > 1.0 ? rounds : 1.0);
+    if (tile == 128) {
+        if (rounds <= 1.0) return 0.75;
+        if (!pairs) return 0.87 * rounds;
+        return rounds <= 2.0 ? 0.75 + 0.51 * (rounds - 1.0) : 0.75 * rounds;      // two tiles of a unit run beside each other
+    }
+    if (rounds <= 1.0) return 0.3;                                               // two wave groups on a tile
+    return 0.25 * rounds > 0.49 ? 0.25 * rounds : 0.49;                          // one: 0.49 alone, and up to two in that time
+}
 struct GemmLoad { double tiles = 0, chunks = 0, longest = 0; int kinds = 0; };   // chunks: summed over all tiles
 inline void gemm_load_add(GemmLoad& l, double tiles, double chunks) {
     l.tiles += tiles;
@@ -407,14 +416,22 @@ inline void gemm_load_add(GemmLoad& l, double tiles, double chunks) {
     l.chunks += tiles * chunks;
     l.longest = chunks > l.longest ? chunks : l.longest;
 }
-inline double gemm_time_us(int tile, const GemmLoad& l, bool pairs) {
-    // tiles of one length run in whole rounds
-    const double rounds = l.kinds == 1 ? (double)(((long long)l.tiles + 255) / 256) : l.chunks / (256.0 * l.longest);
-    const double share = tile == 256 ? 2.75 : tile == 128 ? (pairs ? 0.75 : 0.87) : 0.24;
-    const double alone = tile == 256 ? 2.75 : tile == 128 ? 0.75 : l.tiles <= 256.0 ? 0.3 : 0.49;
-    const double us = l.longest * (alone > share * rounds ? alone : share * rounds);
-    // of several lengths they pack as they come: a quarter of the longest is left over at the end
-    return (l.kinds == 1 ? us : us + 0.25 * l.longest * share) * (pairs ? 1.0 : 2.0 / 3.0);
+// `bytes`: what the epilogue moves per element of C.  A unit's share of the memory rate is 20 GB/s; some of it runs beside another
+// tile's products, a 256 x 256 tile's least.
+inline double gemm_time_us(int tile, const GemmLoad& l, bool pairs, double bytes) {
+    double rounds = l.chunks / (256.0 * l.longest), rest = 0.0;
+    if (l.kinds == 1) {
+        // tiles of one length run in whole rounds; where several share a unit, the last round is not quite one (528 tiles of
+        // 64 x 64 on 256 units: 2.7 rounds)
+        const double whole = (double)(((long long)l.tiles + 255) / 256);
+        rounds = tile < 256 && whole > 1.0 && whole - 0.35 > rounds ? whole - 0.35 : whole;
+    } else {
+        // of several lengths they pack as they come: a quarter of the longest is left over at the end
+        rest = 0.25 * l.longest * (tile == 256 ? 2.75 : tile == 128 ? 0.75 : 0.25);
+    }
+    const double each = l.tiles / 256.0 > 1.0 ? l.kinds == 1 ? rounds : l.tiles / 256.0 : 1.0;
+    return (l.longest * gemm_chunk_us(tile, rounds, pairs) + rest) * (pairs ? 1.0 : 2.0 / 3.0)
+           + each * tile * tile * bytes / 20.0e3 * (tile == 256 ? 0.9 : 0.8);
 }
 
 #endif

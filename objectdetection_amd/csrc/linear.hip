@@ -578,9 +578,7 @@ LinPlan lin_plan(const LinGemm* g, int count) {
                 gemm_load_add(load, tiles * parts, (chunks + parts - 1) / parts);
                 if (parts > 1) extra += 4.0 / count + parts * (double)g[q].m * g[q].n * 8.0 / 3.0e6;
             }
-            const double rounds = ceil(load.tiles / 256.0), bytes = (double)tile * tile * (DT == ODAMD_DTYPE_F32 ? 8.0 : 4.0);
-            const double us = gemm_time_us(tile, load, DT == ODAMD_DTYPE_F32)
-                              + rounds * bytes / 20.0e3 * (tile == 256 ? 0.9 : 0.8) + extra;
+            const double us = gemm_time_us(tile, load, DT == ODAMD_DTYPE_F32, DT == ODAMD_DTYPE_F32 ? 8.0 : 4.0) + extra;
             if (least < 0.0 || us < least) {
                 best = {tile, longest};
                 least = us;

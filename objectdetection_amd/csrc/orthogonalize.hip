@@ -39,9 +39,13 @@ constexpr int NS_GROUPS = 112;        // groups of one launch: their table trave
 constexpr long long NS_WHOLE = 5 << 17;
 constexpr int NS_PARTS = 512;         // partial sums of squares per matrix, at most
 
-// stages: sums of squares, laying out, X X^T, P from A, products of square matrices, Q X, Q X to the caller; a matrix as a whole
-enum { ST_NORM, ST_SPLIT, ST_A, ST_P, ST_Q, ST_X, ST_OUT, ST_WHOLE };
-// square matrices: A, a product on the way to the next A, and three that P and Q take in turn
+// stages: sums of squares, laying out, X X^T (whole, or a part of its reduction), P from A, products of square matrices, Q X,
+// Q X to the caller; a matrix as a whole
+enum { ST_NORM, ST_SPLIT, ST_A, ST_AP, ST_P, ST_Q, ST_X, ST_OUT, ST_WHOLE };
+__host__ __device__ constexpr bool ns_symmetric(int stage) { return stage == ST_A || stage == ST_AP || stage == ST_P || stage == ST_Q; }
+__host__ __device__ constexpr bool ns_along_n(int stage) { return stage == ST_A || stage == ST_AP; }   // reduces over n, the others over m
+// square matrices: A, a product on the way to the next A, and three that P and Q take in turn; X X^T leaves the sums of a cut
+// reduction in all but the first
 enum { SQ_A, SQ_T, SQ_B, SQ_COUNT = 5 };
 
 // `count` matrices of one shape, one after the other
@@ -58,7 +62,9 @@ struct NsTable {
     int n, tiles;
     char* ws;
 };
-// Up to two products of a stage: out = left right, squares by index, `scale` from the sum to the stored pair
+// Up to two products of a stage: out = left right, squares by index, `scale` from the sum to the stored pair.  ST_AP: n parts of
+// the reduction instead, at most NS_CUTS.
+constexpr int NS_CUTS = SQ_COUNT - SQ_T;   // a part's sums lie in the place of a square that is not in use yet
 struct NsJobs {
     int n, turn;         // turn: which of the two column copies of X is the current one
     int left[2], right[2], out[2];
@@ -89,8 +95,11 @@ __host__ __device__ inline long long ns_share(int m, int n) {
 __host__ __device__ inline int ns_parts(int m, int n) { return (int)(((long long)m * n + ns_share(m, n) - 1) / ns_share(m, n)); }
 __host__ __device__ inline int ns_tiles(int stage, int tile, int m, int n) {
     const int mt = (m + tile - 1) / tile, nt = (n + tile - 1) / tile;
-    return stage == ST_WHOLE ? 1 : stage == ST_NORM ? ns_parts(m, n) : stage == ST_A || stage == ST_P || stage == ST_Q ? mt * (mt + 1) / 2 : mt * nt;
+    return stage == ST_WHOLE ? 1 : stage == ST_NORM ? ns_parts(m, n) : ns_symmetric(stage) ? mt * (mt + 1) / 2 : mt * nt;
 }
+
+// Chunks of a part
+__host__ __device__ inline int ns_cut(int chunks, int cuts) { return (chunks + cuts - 1) / cuts; }
 
 // What the optimizer step works on (orthogonalisation alone: in and out)
 struct NsIo {
@@ -436,13 +445,14 @@ __device__ __forceinline__ void ns_emit8(const NsIo& io, float step, long long a
 template <typename TILE, int STAGE, bool MUON, int DT>
 __global__ void __launch_bounds__(TILE::THREADS) ns_product_kernel(NsTable t, NsIo io, NsJobs jobs) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int block = (int)blockIdx.x, job = STAGE == ST_Q && block >= t.tiles ? 1 : 0, at = block - job * t.tiles;
+    const int block = (int)blockIdx.x, job = STAGE == ST_AP ? block / t.tiles : STAGE == ST_Q && block >= t.tiles ? 1 : 0;
+    const int at = block - job * t.tiles;
     const NsPlace p = ns_find(t, t.n == 1 ? gemm_xcd_remap(at, t.tiles) : gemm_xcd_stretch(at, t.tiles), STAGE, TILE::TM);
     const NsLayout l = ns_layout(p.m, p.n);
     const int mp = (int)ns_up(p.m, 32), np = (int)ns_up(p.n, 32);
     const auto square = [&](int i) { return p.ws + l.sq + i * l.sq_size; };
     int ti, tj;
-    if (STAGE == ST_A || STAGE == ST_P || STAGE == ST_Q) gemm_triangle_at(p.tile, ti, tj);
+    if (ns_symmetric(STAGE)) gemm_triangle_at(p.tile, ti, tj);
     else gemm_tile_at(p.tile, (p.m + TILE::TM - 1) / TILE::TM, (p.n + TILE::TN - 1) / TILE::TN, ti, tj);
     const int i0 = ti * TILE::TM, j0 = tj * TILE::TN;
     const int left = job ? jobs.left[1] : jobs.left[0], right = job ? jobs.right[1] : jobs.right[0], to = job ? jobs.out[1] : jobs.out[0];
@@ -451,6 +461,22 @@ __global__ void __launch_bounds__(TILE::THREADS) ns_product_kernel(NsTable t, Ns
     if constexpr (STAGE == ST_A) {
         const GemmOperand x = {p.ws + l.x, (long long)np * 4, p.m};
         tile.run(x, x, i0, j0, 0, np / 32, np, lds);
+    } else if constexpr (STAGE == ST_AP) {
+        const GemmOperand x = {p.ws + l.x, (long long)np * 4, p.m};
+        const int per = ns_cut(np / 32, jobs.n), from = job * per;
+        if (from >= np / 32) return;                       // a short matrix has fewer parts
+        tile.run(x, x, i0, j0, from, min(np / 32, from + per), np, lds);
+        float* sums = (float*)square(SQ_T + job);
+        const auto none = [](int, int) { return GemmNothing{}; };
+        const auto rows = [&](int i, int j, float v[8], const GemmNothing&) {
+            i += i0; j += j0;
+            if (i >= p.m || j >= mp) return;
+            f32x4_t* at = (f32x4_t*)(sums + (long long)i * mp + j);
+            at[0] = f32x4_t{v[0], v[1], v[2], v[3]};
+            at[1] = f32x4_t{v[4], v[5], v[6], v[7]};
+        };
+        tile.template hand_out<true, false, 1>(lds, none, rows, none, rows);
+        return;
     } else {
         const GemmOperand a = {square(left), (long long)mp * 4, p.m};
         const GemmOperand b = STAGE == ST_P || STAGE == ST_Q ? GemmOperand{square(right), (long long)mp * 4, p.m}
@@ -458,7 +484,8 @@ __global__ void __launch_bounds__(TILE::THREADS) ns_product_kernel(NsTable t, Ns
         tile.run(a, b, i0, j0, 0, mp / 32, mp, lds);
     }
 
-    if constexpr (STAGE == ST_A || STAGE == ST_P || STAGE == ST_Q) {
+    if constexpr (STAGE == ST_AP) {
+    } else if constexpr (STAGE == ST_A || STAGE == ST_P || STAGE == ST_Q) {
         char* out = square(to);
         // row i, columns j .. j+7; P needs A's values of that place
         struct Before { f16x8_t hi, lo; };
@@ -531,6 +558,53 @@ __global__ void __launch_bounds__(TILE::THREADS) ns_product_kernel(NsTable t, Ns
     }
 }
 
+// A from the parts of a cut reduction, summed in their order: 64 x 64 elements per workgroup, mirrored like a product's tile
+__global__ void __launch_bounds__(256) ns_join_kernel(NsTable t, int cuts, float scale) {
+    __shared__ float tile[64][65];
+    const NsPlace p = ns_find(t, blockIdx.x, ST_AP, 64);
+    const NsLayout l = ns_layout(p.m, p.n);
+    const int mp = (int)ns_up(p.m, 32), chunks = (int)ns_up(p.n, 32) / 32, per = ns_cut(chunks, cuts), parts = (chunks + per - 1) / per;
+    int ti, tj;
+    gemm_triangle_at(p.tile, ti, tj);
+    const int i0 = ti * 64, j0 = tj * 64, c = (threadIdx.x & 7) * 8;
+    char* out = p.ws + l.sq + SQ_A * l.sq_size;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int r = (threadIdx.x >> 3) + 32 * q, i = i0 + r, j = j0 + c;
+        if (i >= p.m || j >= mp) continue;
+        f32x4_t u[NS_CUTS][2];
+#pragma unroll
+        for (int k = 0; k < NS_CUTS; ++k)
+            if (k < parts) {
+                const f32x4_t* at = (const f32x4_t*)((const float*)(p.ws + l.sq + (SQ_T + k) * l.sq_size) + (long long)i * mp + j);
+                u[k][0] = at[0];
+                u[k][1] = at[1];
+            }
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float s = u[0][e >> 2][e & 3];
+#pragma unroll
+            for (int k = 1; k < NS_CUTS; ++k)
+                if (k < parts) s += u[k][e >> 2][e & 3];
+            v[e] = j + e < p.m ? s * scale : 0.0f;
+            tile[r][c + e] = v[e];
+        }
+        store_split8(out + (long long)i * mp * 4 + split_at(j), v, 1.0f);
+    }
+    if (ti == tj) return;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int r = (threadIdx.x >> 3) + 32 * q;          // all rows of a tile over the diagonal exist
+        float v[8];
+        if (j0 + r >= p.m) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = tile[c + e][r];
+        store_split8(out + (long long)(j0 + r) * mp * 4 + split_at(i0 + c), v, 1.0f);
+    }
+}
+
 using NsTile256 = GemmTile<2, true, 256, 256, 4, 2, 1, 2>;
 using NsTile128 = GemmTile<2, true, 128, 128, 2, 2, 1, 2>;
 using NsTile64 = GemmTile<2, true, 64, 64, 2, 2, 1, 2>;
@@ -558,25 +632,49 @@ int ns_launch_tile(NsTable& t, const NsIo& io, const NsJobs& jobs, hipStream_t s
 }
 
 template <int STAGE, bool MUON, int DT>
+int ns_launch64(NsTable& t, const NsIo& io, const NsJobs& jobs, hipStream_t s) {
+    const int tiles = ns_count(t, STAGE, 64);
+    if (tiles < 0) return ODAMD_E_LIMIT;
+    return (long long)tiles * jobs.n > 256 ? ns_launch_tile<NsTile64, STAGE, MUON, DT>(t, io, jobs, s)
+                                           : ns_launch_tile<NsTile64Few, STAGE, MUON, DT>(t, io, jobs, s);
+}
+
+template <int STAGE, bool MUON, int DT>
 int ns_product(NsTable& t, const NsIo& io, const NsJobs& jobs, hipStream_t s) {
-    int best = 64;
-    double least = 0.0, tiles64 = 0.0;
-    for (int tile : {64, 128, 256}) {
-        GemmLoad load;
-        for (int i = 0; i < t.n; ++i)
-            gemm_load_add(load, (double)ns_tiles(STAGE, tile, t.g[i].m, t.g[i].n) * t.g[i].count * jobs.n,
-                          (double)(ns_up(STAGE == ST_A ? t.g[i].n : t.g[i].m, 32) / 32));
-        const double us = gemm_time_us(tile, load, true);
-        if (tile == 64) tiles64 = load.tiles;
-        if (tile == 64 || us < least) {
-            best = tile;
-            least = us;
+    constexpr double epilogue = STAGE == ST_OUT ? (MUON ? 16.0 : DT == ODAMD_DTYPE_BF16 ? 2.0 : 4.0) : STAGE == ST_P ? 12.0 : 8.0;
+    int best = 64, cuts = 1;
+    double least = -1.0;
+    for (int tile : {64, 128, 256})
+        for (int cut = 1; cut <= (STAGE == ST_A && tile < 256 ? NS_CUTS : 1); ++cut) {
+            GemmLoad load;
+            double bytes = 0.0;
+            for (int i = 0; i < t.n; ++i) {
+                const NsGroup& g = t.g[i];
+                const int chunks = (int)(ns_up(ns_along_n(STAGE) ? g.n : g.m, 32) / 32), per = ns_cut(chunks, cut);
+                gemm_load_add(load, (double)ns_tiles(STAGE, tile, g.m, g.n) * g.count * jobs.n * ((chunks + per - 1) / per), (double)per);
+                bytes += 4.0 * g.m * g.m * g.count;
+            }
+            // a cut reduction costs a second launch (5 us) and half a square per part, once out and once in
+            const double us = gemm_time_us(tile, load, true, epilogue) + (cut > 1 ? 5.0 + cut * bytes / 3.0e6 : 0.0);
+            if (least < 0.0 || us < least) {
+                best = tile;
+                cuts = cut;
+                least = us;
+            }
         }
-    }
+    if constexpr (STAGE == ST_A)
+        if (cuts > 1) {
+            NsJobs parts = jobs;
+            parts.n = cuts;
+            const int rc = best == 128 ? ns_launch_tile<NsTile128, ST_AP, MUON, DT>(t, io, parts, s) : ns_launch64<ST_AP, MUON, DT>(t, io, parts, s);
+            if (rc != 0) return rc;
+            if (ns_count(t, ST_AP, 64) < 0) return ODAMD_E_LIMIT;
+            ns_join_kernel<<<t.tiles, 256, 0, s>>>(t, cuts, jobs.scale[0]);
+            return (int)hipGetLastError();
+        }
     if (best == 256) return ns_launch_tile<NsTile256, STAGE, MUON, DT>(t, io, jobs, s);
     if (best == 128) return ns_launch_tile<NsTile128, STAGE, MUON, DT>(t, io, jobs, s);
-    if (tiles64 > 256.0) return ns_launch_tile<NsTile64, STAGE, MUON, DT>(t, io, jobs, s);
-    return ns_launch_tile<NsTile64Few, STAGE, MUON, DT>(t, io, jobs, s);
+    return ns_launch64<STAGE, MUON, DT>(t, io, jobs, s);
 }
 
 // Exponent that keeps a product of k P's (entries up to 3.4445^k) within fp16, an eighth of a bit to spare for rounding
