@@ -33,6 +33,13 @@ __device__ __forceinline__ void gemm_dma16(const char* g, char* l) {
                                      (__attribute__((address_space(3))) void*)l, 16, 0, 0);
 }
 
+// Accesses to LDS stay on their side of it, in the compiler's order too.
+__device__ __forceinline__ void gemm_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // Blocks that run on one XCD (block index modulo 8) take neighbouring tiles: they share operand rows in that XCD's L2.
 __device__ __forceinline__ int gemm_xcd_remap(int bid, int n) {
     const int q = n >> 3, r = n & 7, xcd = bid & 7, slot = bid >> 3;
@@ -223,7 +230,7 @@ struct GemmTile {
             // the barrier that holds for every wave, and the chunk's buffer may take the one after the next.
             issue(0);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
+            gemm_barrier();
             if (rounds > 1) issue(1);
             read(lds, 0, 0);
             for (int i = 0; i < rounds; ++i) {
@@ -233,7 +240,7 @@ struct GemmTile {
                         read(lds + (i & 1) * BUF, s + 1, (s + 1) & 1);
                     } else {
                         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                        __builtin_amdgcn_s_barrier();
+                        gemm_barrier();
                         read(lds + (~i & 1) * BUF, 0, (s + 1) & 1); // behind the last chunk: of no use, but within LDS
                         if (i + 2 < rounds) issue(i + 2);
                     }
@@ -258,7 +265,7 @@ struct GemmTile {
                 if (NBUF > 3 && ahead == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NBUF > 3 ? 2 * NI : 0) : "memory");
                 else if (NBUF > 2 && ahead == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NBUF > 2 ? NI : 0) : "memory");
                 else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                __builtin_amdgcn_s_barrier();
+                gemm_barrier();
                 if (i + NBUF - 1 < rounds) issue(i + NBUF - 1);
 #pragma unroll
                 for (int s = 0; s < STEPS; ++s) {
@@ -268,7 +275,7 @@ struct GemmTile {
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();                               // every wave has read its last fragments: the ring is free
+        gemm_barrier();                               // every wave has read its last fragments: the ring is free
         if constexpr (KG > 1) {
             // the other groups leave their sums in LDS, the first adds them in order
             const auto place = [&](int g, int x, int y, int q) {
@@ -283,7 +290,7 @@ struct GemmTile {
                         for (int q = 0; q < 4; ++q)
                             *place(group, x, y, q) = f32x4_t{acc[x][y][4 * q], acc[x][y][4 * q + 1], acc[x][y][4 * q + 2], acc[x][y][4 * q + 3]};
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
+            gemm_barrier();
             if (group == 0)
 #pragma unroll
                 for (int g = 1; g < KG; ++g)
@@ -297,7 +304,7 @@ struct GemmTile {
                                 acc[x][y][4 * q] += u[0]; acc[x][y][4 * q + 1] += u[1]; acc[x][y][4 * q + 2] += u[2]; acc[x][y][4 * q + 3] += u[3];
                             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();                           // read before the slabs take the place
+            gemm_barrier();                           // read before the slabs take the place
         }
     }
 
@@ -394,7 +401,11 @@ __device__ __forceinline__ void store_split8(char* hi_at, const float v[8], floa
     *(f16x8_t*)(hi_at + 64) = lo;
 }
 
-// ---- host: which tile ------------------------------------------------------------------------------------------------
+// ---- host ------------------------------------------------------------------------------------------------------------
+// A launch has fewer than 2^32 threads.
+inline bool gemm_grid_ok(long long blocks, int threads) { return blocks * threads <= 0xffffffffLL; }
+
+// ---- which tile ------------------------------------------------------------------------------------------------
 // Time of a 128-byte chunk of all tiles of a compute unit, in us, by how many tiles a unit has to run (`rounds`; measured
 // with pairs at 4096^3, 8192 x 1024 x 2304 and below).  The larger tile wins per product, the smaller one spreads a small
 // product over all 256 units: 4096 x 4096 x 4096 takes 353 / 367 / 512 us in 256 / 128 / 64, 2048 x 1024 x 2048

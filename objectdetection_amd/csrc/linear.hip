@@ -49,19 +49,20 @@ __device__ __forceinline__ float lin_act(float z) {
     if constexpr (ACT == ODAMD_ACT_RELU) return z < 0.0f ? 0.0f : z;
     return z;
 }
+// dy act'(z)
 template <bool FAST, int ACT>
-__device__ __forceinline__ float lin_slope(float z) {
+__device__ __forceinline__ float lin_grad(float dy, float z) {
     if constexpr (ACT == ODAMD_ACT_SILU) {
         const float p = FAST ? sigmoid_fast(z) : 1.0f / (1.0f + expf(-z));
-        return p * (1.0f + z * (1.0f - p));
+        return dy * (p * (1.0f + z * (1.0f - p)));
     }
     if constexpr (ACT == ODAMD_ACT_GELU) {
         const float e = FAST ? erf_fast(z * 0.70710678118654752f) : erff(z * 0.70710678118654752f);
         const float g = FAST ? __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f) : expf(-0.5f * z * z);
-        return 0.5f * (1.0f + e) + z * g * 0.39894228040143268f;
+        return dy * (0.5f * (1.0f + e) + z * g * 0.39894228040143268f);
     }
-    if constexpr (ACT == ODAMD_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-    return 1.0f;
+    if constexpr (ACT == ODAMD_ACT_RELU) return z <= 0.0f ? 0.0f : dy;   // also where dy is an infinity
+    return dy;
 }
 // Calls f with the activation as a compile-time constant
 template <typename F>
@@ -279,7 +280,7 @@ __device__ __forceinline__ void lin_values8(const LinJob& p, int i, int j, float
         lin_load8<DT>(p.z, i * p.z_ld + j, cnt, z);
         lin_with_act(p.act, [&](auto act) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= lin_slope<DT == ODAMD_DTYPE_BF16, act.value>(z[e]);
+            for (int e = 0; e < 8; ++e) v[e] = lin_grad<DT == ODAMD_DTYPE_BF16, act.value>(v[e], z[e]);
         });
     }
 }
@@ -566,6 +567,7 @@ LinPlan lin_plan(const LinGemm* g, int count) {
         all = chunks > all ? chunks : all;
     }
     LinPlan best = {64, all};
+    if (count == 0) return best;
     double least = -1.0;
     for (int tile : {64, 128, 256})
         for (int cut = 1; cut <= 32 && (cut == 1 || all / cut >= 4); cut *= 2) {
@@ -597,6 +599,7 @@ int lin_launch(LinLaunch& t, int count, hipStream_t s) {
     }
     t.block2 = (int)at;
     at += t.sums.db ? (t.sums.n + 63) / 64 : 0;
+    if (!gemm_grid_ok(at, TILE::THREADS)) return ODAMD_E_LIMIT;
     const auto kernel = linear_product_kernel<TILE, DT, ACT, PART, TURNED>;
     const hipError_t e = odamd_ensure_lds((const void*)kernel, TILE::LDS);
     if (e != hipSuccess) return (int)e;
@@ -649,13 +652,14 @@ int lin_products(LinLaunch& t, int count, LinSpace& ws, bool go, hipStream_t s) 
 template <int DT> bool lin_direct(const void* p, long long ld, int k) {
     return DT == ODAMD_DTYPE_BF16 && ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && k % 8 == 0;
 }
-int lin_tiles(LinJobs& t, int unit_rows) {   // blocks of a launch over the jobs: 64 x 64 tiles, or groups of rows
+// Blocks of a launch over the jobs: 64 x 64 tiles, or groups of rows; -1: more than a launch takes
+int lin_tiles(LinJobs& t, int unit_rows) {
     long long at = 0;
     for (int i = 0; i < t.n; ++i) {
         t.j[i].tile0 = (int)at;
         at += unit_rows ? (t.j[i].m + unit_rows - 1) / unit_rows : (((long long)t.j[i].m + 63) / 64) * ((t.j[i].n + 63) / 64);
     }
-    return at > 0x7fffffffLL ? -1 : (int)at;
+    return gemm_grid_ok(at, 256) ? (int)at : -1;
 }
 
 constexpr int LIN_ROWS = 8;   // up to this many rows the layer is read once for all of them, without matrix instructions
@@ -666,6 +670,7 @@ int lin_forward_rows(const odamd_linear_desc& d, const LinEnd& end, hipStream_t 
     const bool wide = (((uintptr_t)d.x | (uintptr_t)d.w) & 15) == 0 && d.x_ld % V == 0 && d.w_ld % V == 0 && d.k % V == 0;
     const LinRow p = {d.x, d.w, d.x_ld, d.w_ld, d.m, d.k, d.n, end};
     const int blocks = (d.n + 3) / 4;
+    if (!gemm_grid_ok(blocks, 256)) return ODAMD_E_LIMIT;
 #define ODAMD_ROWS(MR) (wide ? linear_rows_kernel<DT, MR, true><<<blocks, 256, 0, s>>>(p) : linear_rows_kernel<DT, MR, false><<<blocks, 256, 0, s>>>(p))
     if (d.m == 1) ODAMD_ROWS(1);
     else if (d.m == 2) ODAMD_ROWS(2);
@@ -710,6 +715,7 @@ int lin_forward(const odamd_linear_desc& d, LinSpace& ws, bool go, hipStream_t s
     // a laid out operand is padded to whole chunks, one read in place is not: the tail is then read as zeros for both
     if (go && jobs.n) {
         const int blocks = lin_tiles(jobs, 4);
+        if (blocks < 0) return ODAMD_E_LIMIT;
         linear_lay_rows_kernel<DT><<<blocks, 256, 0, s>>>(jobs);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return (int)e;

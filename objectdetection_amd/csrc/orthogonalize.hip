@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(256) ns_split_kernel(NsTable t, NsIo io) {
     double mine = 0.0;
     for (int i = threadIdx.x; i < parts; i += 256) mine += ((const double*)p.ws)[i];
     const double sum = ns_block_sum(mine, part);
-    const float inv = (float)(1.0 / (sqrt(sum) + io.eps));
+    const double inv = 1.0 / (sqrt(sum) + io.eps);         // in double: a float32 norm may lie at either end of float32's range
     // in the caller's rows and columns: what lies along its rows goes out as it comes, the other copy through LDS
     const int rows = p.tall ? p.n : p.m, cols = p.tall ? p.m : p.n, ct = (cols + 63) / 64;
     const int r0 = p.tile / ct * 64, c0 = p.tile % ct * 64, c = (threadIdx.x & 7) * 8;
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(256) ns_split_kernel(NsTable t, NsIo io) {
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            v[e] = e < cnt ? v[e] * inv : 0.0f;
+            v[e] = e < cnt ? (float)(v[e] * inv) : 0.0f;
             tile[r][c + e] = v[e];
         }
         if (r0 + r < rows && c0 + c < cp) store_split8(along + (long long)(r0 + r) * cp * 4 + split_at(c0 + c), v, NS_SCALE);
@@ -295,8 +295,8 @@ __global__ void __launch_bounds__(256) ns_whole_kernel(NsTable t, NsIo io, int s
         s += (double)v * v;
     }
     s = ns_block_sum(s, part);                            // its barrier also closes the writes of X
-    const float inv = (float)(1.0 / (sqrt(s) + io.eps));
-    for (int i = threadIdx.x; i < 16 * T * ld; i += 256) x[i] *= inv;
+    const double inv = 1.0 / (sqrt(s) + io.eps);
+    for (int i = threadIdx.x; i < 16 * T * ld; i += 256) x[i] = (float)(x[i] * inv);
     __syncthreads();
     // out tile (ti, tj) of l r^T over k values, both of them rows `stride` apart
     const auto product = [&](const float* l, const float* rr, int stride, int ti, int tj, int k) {
@@ -610,20 +610,20 @@ using NsTile128 = GemmTile<2, true, 128, 128, 2, 2, 1, 2>;
 using NsTile64 = GemmTile<2, true, 64, 64, 2, 2, 1, 2>;
 using NsTile64Few = GemmTile<2, true, 64, 64, 2, 2, 2, 3>;   // two wave groups: one tile, or less, for a compute unit
 
-// Tiles of a stage over the whole table; -1: more than a launch takes
-int ns_count(NsTable& t, int stage, int tile) {
+// Tiles of a stage over the whole table; -1: more than a launch of `threads` for each takes
+int ns_count(NsTable& t, int stage, int tile, int threads) {
     long long at = 0;
     for (int i = 0; i < t.n; ++i) {
         t.g[i].tile0 = at > 0x7fffffff ? 0x7fffffff : (int)at;
         at += (long long)ns_tiles(stage, tile, t.g[i].m, t.g[i].n) * t.g[i].count;
     }
     t.tiles = (int)at;
-    return at > 0x3fffffff ? -1 : (int)at;
+    return gemm_grid_ok(at, threads) ? (int)at : -1;
 }
 
 template <typename TILE, int STAGE, bool MUON, int DT>
 int ns_launch_tile(NsTable& t, const NsIo& io, const NsJobs& jobs, hipStream_t s) {
-    if (ns_count(t, STAGE, TILE::TM) < 0) return ODAMD_E_LIMIT;
+    if (ns_count(t, STAGE, TILE::TM, TILE::THREADS * jobs.n) < 0) return ODAMD_E_LIMIT;
     const auto kernel = ns_product_kernel<TILE, STAGE, MUON, DT>;
     const hipError_t e = odamd_ensure_lds((const void*)kernel, TILE::LDS);
     if (e != hipSuccess) return (int)e;
@@ -633,7 +633,7 @@ int ns_launch_tile(NsTable& t, const NsIo& io, const NsJobs& jobs, hipStream_t s
 
 template <int STAGE, bool MUON, int DT>
 int ns_launch64(NsTable& t, const NsIo& io, const NsJobs& jobs, hipStream_t s) {
-    const int tiles = ns_count(t, STAGE, 64);
+    const int tiles = ns_count(t, STAGE, 64, NsTile64::THREADS * jobs.n);
     if (tiles < 0) return ODAMD_E_LIMIT;
     return (long long)tiles * jobs.n > 256 ? ns_launch_tile<NsTile64, STAGE, MUON, DT>(t, io, jobs, s)
                                            : ns_launch_tile<NsTile64Few, STAGE, MUON, DT>(t, io, jobs, s);
@@ -668,7 +668,7 @@ int ns_product(NsTable& t, const NsIo& io, const NsJobs& jobs, hipStream_t s) {
             parts.n = cuts;
             const int rc = best == 128 ? ns_launch_tile<NsTile128, ST_AP, MUON, DT>(t, io, parts, s) : ns_launch64<ST_AP, MUON, DT>(t, io, parts, s);
             if (rc != 0) return rc;
-            if (ns_count(t, ST_AP, 64) < 0) return ODAMD_E_LIMIT;
+            if (ns_count(t, ST_AP, 64, 256) < 0) return ODAMD_E_LIMIT;
             ns_join_kernel<<<t.tiles, 256, 0, s>>>(t, cuts, jobs.scale[0]);
             return (int)hipGetLastError();
         }
@@ -685,7 +685,7 @@ int ns_q_exponent(int k) {
 
 template <int T, bool MUON, int DT>
 int ns_whole(NsTable& t, const NsIo& io, int steps, long long lds, hipStream_t s) {
-    if (ns_count(t, ST_WHOLE, 0) < 0) return ODAMD_E_LIMIT;
+    if (ns_count(t, ST_WHOLE, 0, 256) < 0) return ODAMD_E_LIMIT;
     const auto kernel = ns_whole_kernel<T, MUON, DT>;
     const hipError_t e = odamd_ensure_lds((const void*)kernel, (size_t)lds);
     if (e != hipSuccess) return (int)e;
@@ -712,9 +712,9 @@ int ns_run(NsTable& t, const NsIo& io, int steps, hipStream_t s) {
     int phase = LOOSE ? 5 : 2;
     for (int i = 0; i < t.n; ++i)
         if (!LOOSE && t.g[i].n < 2 * (long long)t.g[i].m) phase = 1;
-    if (ns_count(t, ST_NORM, 0) < 0) return ODAMD_E_LIMIT;
+    if (ns_count(t, ST_NORM, 0, 256) < 0) return ODAMD_E_LIMIT;
     ns_norm_kernel<MUON, DT><<<t.tiles, 256, 0, s>>>(t, io);
-    if (ns_count(t, ST_SPLIT, 64) < 0) return ODAMD_E_LIMIT;
+    if (ns_count(t, ST_SPLIT, 64, 256) < 0) return ODAMD_E_LIMIT;
     ns_split_kernel<MUON, DT><<<t.tiles, 256, 0, s>>>(t, io);
     int rc = (int)hipGetLastError();
     NsJobs jobs = {};

@@ -14,6 +14,7 @@ from ._lib import lib, check
 ACTIVATIONS = {None: 0, 'silu': 1, 'gelu': 2, 'relu': 3}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 MATRIX_DTYPE = np.dtype([('offset', '<i8'), ('rows', '<i4'), ('cols', '<i4')])      # odamd_matrix
+_MOST = 2 ** 31 - 1025                                                               # rows, columns, matrices of a call
 RANGE_DTYPE = np.dtype([('offset', '<i8'), ('len', '<i8')])                         # odamd_range
 
 
@@ -147,6 +148,8 @@ def linear(x, weight, bias=None, activation=None, residual=None):
         if residual.shape != x.shape[:-1] + (n,):
             raise ValueError(f'residual must have shape {tuple(x.shape[:-1]) + (n,)}, not {tuple(residual.shape)}')
     act = ACTIVATIONS[activation]
+    if max(x.numel() // x.shape[-1], *weight.shape) > _MOST:
+        raise ValueError(f'at most {_MOST} rows, inputs and outputs')
     if x.numel() == 0:
         # no rows: nothing to launch; the empty result stays connected to its inputs
         y = x.new_empty(x.shape[:-1] + (n,))
@@ -176,8 +179,8 @@ def orthogonalize(x, steps=5, eps=1e-7, out=None):
     if not 1 <= int(steps) <= 32 or not eps >= 0:
         raise ValueError('steps must be 1 to 32, eps must not be negative')
     rows, cols = x.shape[-2:]
-    if rows * cols >= 2 ** 31:
-        raise ValueError('a matrix must have fewer than 2^31 elements')
+    if rows * cols >= 2 ** 31 or x.shape[:-2].numel() > _MOST:
+        raise ValueError(f'a matrix must have fewer than 2^31 elements, a batch at most {_MOST} matrices')
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     else:

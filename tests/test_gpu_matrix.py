@@ -132,6 +132,16 @@ def test_linear_tiles_and_split(mx, m, k, n, dtype):
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('m, k, n', [(9000, 136, 520), (5001, 129, 131), (2100, 263, 2049), (70, 1500, 3001), (2500, 1030, 1033)])
+def test_linear_long_reductions_backward(mx, m, k, n, dtype):
+    """dW and db of many rows, dx of many outputs: one of the two products cut, or both, aligned and not."""
+    x, w = randn(m, k, dtype=dtype), randn(n, k, seed=1, dtype=dtype, scale=k ** -0.5)
+    b = randn(n, seed=2, dtype=dtype)
+    check_linear(mx, x, w, b, 'gelu', None)
+    check_linear(mx, x, w, b, None, randn(m, n, seed=3, dtype=dtype))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
 @pytest.mark.parametrize('m', [4, 40])
 def test_linear_strides_and_offsets(mx, m, dtype):
     """Slices of wider buffers, unaligned starts, transposed and expanded views."""
@@ -201,6 +211,21 @@ def test_linear_only_wanted_gradients(mx):
         assert torch.equal(got, full[i])
 
 
+def test_linear_relu_closes_the_gradient(mx):
+    """Where relu is closed nothing passes, an infinity neither; other rows and columns do not see it."""
+    for dtype in (torch.float32, torch.bfloat16):
+        x, w = randn(30, 40, dtype=dtype).abs(), randn(24, 40, seed=1, dtype=dtype).abs()
+        w[3] = -w[3]
+        leaves = [x.requires_grad_(), w.requires_grad_()]
+        dy = randn(30, 24, seed=2, dtype=dtype)
+        dy[:, 3] = float('inf')
+        dx, dw = torch.autograd.grad(mx.linear(*leaves, activation='relu'), leaves, dy)
+        clean = dy.clone()
+        clean[:, 3] = 0
+        rx, rw = torch.autograd.grad(mx.linear(*leaves, activation='relu'), leaves, clean)
+        assert torch.equal(dx, rx) and torch.equal(dw, rw) and float(dw[3].abs().max()) == 0.0
+
+
 def test_linear_gradient_against_differences(mx):
     """float32, central differences of the 64-bit layer along random directions."""
     x, w, b = randn(33, 20), randn(17, 20, seed=1), randn(17, seed=2)
@@ -226,7 +251,7 @@ def test_linear_refuses(mx):
     x, w = randn(4, 8), randn(6, 8, seed=1)
     for bad in (dict(x=x.half()), dict(weight=w.bfloat16()), dict(weight=w[0]), dict(weight=randn(6, 9)), dict(bias=randn(5)),
                 dict(bias=randn(6).bfloat16()), dict(residual=randn(4, 5)), dict(residual=randn(1, 6)), dict(weight=w.cpu()),
-                dict(activation='swish'), dict(weight=w[:, :0], x=x[:, :0])):
+                dict(activation='swish'), dict(weight=w[:, :0], x=x[:, :0]), dict(x=x[:1, :1].expand(2 ** 31, 1), weight=w[:, :1])):
         with pytest.raises(ValueError):
             mx.linear(**dict(dict(x=x, weight=w), **bad))
 
@@ -271,6 +296,42 @@ def test_orthogonalize_large_tiles(mx):
     for batch, rows, cols in ((1, 2100, 2300), (6, 1050, 1100)):
         g = randn(batch, rows, cols)
         check_orth(mx.orthogonalize(g), g)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('batch, rows, cols', [(1, 70, 4000), (1, 4001, 70), (3, 129, 2049), (8, 256, 1200), (1, 257, 9000), (1, 500, 20011), (2, 1025, 4100)])
+def test_orthogonalize_long_reductions(mx, batch, rows, cols, dtype):
+    """Few tiles of X X^T and a long reduction: it is cut into parts."""
+    g = randn(batch, rows, cols, dtype=dtype)
+    got = mx.orthogonalize(g)
+    check_orth(got, g)
+    assert torch.equal(mx.orthogonalize(g), got)
+
+
+@pytest.mark.parametrize('rows, cols', [(30, 50), (90, 100), (90, 400), (150, 2000)])
+def test_orthogonalize_more_steps(mx, rows, cols):
+    """Up to two phases of five steps and a rest; a step leaves an error of a product and multiplies what came before by 3.4445
+    at most, a geometric sum of 1 / (1 - 1 / 3.4445) = 1.41 times its last term."""
+    g = randn(1, rows, cols)
+    for steps in (1, 2, 3, 4, 6, 7, 12):
+        ref, size = orth64(g[0], steps=steps), orth64(g[0], steps=steps).norm()
+        grown = 3.4445 ** min(steps, 7)                 # the smallest singular values here pass one within seven steps
+        assert float((mx.orthogonalize(g, steps=steps)[0].double() - ref).norm()) <= 1.41 * grown * PAIR[torch.float32] * float(size) + 1e-30
+        low = g.bfloat16()
+        ref = orth64(low[0], steps=steps)
+        loose = LOOSE * 3.4445 ** max(0, min(steps, 7) - 5)
+        assert float((mx.orthogonalize(low, steps=steps)[0].double() - ref).norm()) <= (loose + 2.0 ** -8) * float(ref.norm())
+
+
+@pytest.mark.parametrize('rows, cols', [(20, 30), (100, 333)])
+def test_orthogonalize_ends_of_the_range(mx, rows, cols):
+    """Norms over and under float32's range, subnormal values: the norm is held in 64 bits."""
+    for scale in (2.0 ** 124, 2.0 ** -128, 2.0 ** -140):
+        g = randn(1, rows, cols)
+        g = (g / g.abs().max()).double().mul(scale).float()
+        check_orth(mx.orthogonalize(g, eps=0.0), g, eps=0.0)
+    g = randn(1, rows, cols, dtype=torch.bfloat16) * 2.0 ** 123
+    check_orth(mx.orthogonalize(g, eps=0.0), g, eps=0.0)
 
 
 def test_orthogonalize_brings_singular_values_near_one(mx):
@@ -376,6 +437,23 @@ def test_muon_step_many_matrices(mx):
     assert float((m.double() - rm).abs().max()) == 0.0
 
 
+def test_muon_step_long_and_short_reductions(mx):
+    """One table, reductions from one chunk to many: those of the short ones have fewer parts."""
+    shapes = [(96, 6000), (6000, 96), (80, 33), (33, 80), (128, 1152), (256, 256), (1, 9000), (9000, 1), (200, 2000)]
+    matrices, at = [], 0
+    for r, c in shapes:
+        matrices.append((at, r, c))
+        at += r * c + 3
+    p, g, m = randn(at, scale=0.03), randn(at, seed=1, scale=1e-3), randn(at, seed=2, scale=1e-3)
+    rp, rm, _ = muon64(p, g, m, None, matrices, 0.01, 0.95, True, 0.1, 0.0, 1.0)
+    mx.muon_step(p, g, m, matrices, lr=0.01, weight_decay=0.1)
+    for o, r, c in matrices:
+        s = slice(o, o + r * c)
+        step = 0.01 * 0.2 * math.sqrt(max(r, c)) * 1.25 * math.sqrt(min(r, c))
+        assert float((p[s].double() - rp[s]).norm()) <= LOOSE * step + 4 * 2.0 ** -24 * float(rp[s].norm())
+        assert float((m[s].double() - rm[s]).abs().max()) <= 4 * 2.0 ** -24 * float(rm[s].abs().max())
+
+
 def test_muon_step_refuses(mx):
     p = randn(100)
     for bad in (dict(grad=randn(99)), dict(momentum=randn(100).bfloat16()), dict(ema=randn(100, 1)), dict(matrices=[(90, 3, 4)]),
@@ -456,6 +534,28 @@ def test_captured_and_replayed(mx, dtype):
         for a, c in zip(out, ref):
             assert torch.equal(a, c)
         assert torch.equal(ps, pe) and torch.equal(ms, me)
+
+
+def test_two_graphs_at_once(mx):
+    """Two captured graphs replayed on two streams at the same time: neither uses the other's workspace."""
+    def work(x, w):
+        return mx.linear(x, w, None, 'silu'), mx.orthogonalize(x)
+    cases = [(randn(100, 700, seed=i), randn(60, 700, seed=10 + i)) for i in range(2)]
+    refs = [work(*c) for c in cases]
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in cases]
+    for c in cases:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(work(*c))
+    for _ in range(3):
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                for _ in range(5):
+                    g.replay()
+        torch.cuda.synchronize()
+        for out, ref in zip(outs, refs):
+            assert all(torch.equal(a, b) for a, b in zip(out, ref))
 
 
 def test_layer_trains_in_both_types(mx):

@@ -9,7 +9,7 @@ import torch
 from objectdetection_amd import _lib, matrix
 from objectdetection_amd._lib import lib
 
-E_ARG, E_ALIGN, E_WORKSPACE, E_SHAPE = -1, -2, -3, -4
+E_ARG, E_ALIGN, E_WORKSPACE, E_SHAPE, E_LIMIT = -1, -2, -3, -4, -5
 P = 1 << 20            # a well aligned address that is never followed
 
 
@@ -72,6 +72,19 @@ def test_orthogonalize_refuses():
     need = lib.odamd_orthogonalize_workspace_bytes(3, 8, 16)
     assert need > 0 and call(batch=3, size=need - 1) == E_WORKSPACE
     assert lib.odamd_orthogonalize_workspace_bytes(0, 8, 16) == 0
+
+
+def test_more_than_a_launch_takes_is_refused():
+    """A launch has fewer than 2^32 threads."""
+    huge = 1 << 62
+    row = _desc(m=1, k=1, n=1 << 30, x_ld=1, w_ld=1, y_ld=1 << 30)
+    assert lib.odamd_linear_forward(C.byref(row), P, huge, None) == E_LIMIT
+    many = _desc(m=1 << 30, k=1, n=1, x_ld=1, w_ld=1, y_ld=1, dtype=0)
+    assert lib.odamd_linear_forward(C.byref(many), P, huge, None) == E_LIMIT
+    grad = _grad_desc(m=1 << 30, k=1024, n=1024, dy_ld=1024, z_ld=1024, x_ld=1024, w_ld=1024, dx_ld=1024, dw_ld=1024)
+    assert lib.odamd_linear_backward(C.byref(grad), P, huge, None) == E_LIMIT
+    for rows, cols in ((1, 1), (128, 128)):
+        assert lib.odamd_orthogonalize(P, P, 1 << 25, rows, cols, 5, 0.0, 0, P, huge, None) == E_LIMIT
 
 
 def test_muon_and_ranges_refuse():
