@@ -18,7 +18,10 @@ _MOST = 2 ** 31 - 1025                                                          
 RANGE_DTYPE = np.dtype([('offset', '<i8'), ('len', '<i8')])                         # odamd_range
 
 
-_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)     # the handle alone, without a Stream object
+# the stream's handle and the device's number alone, without a Stream object or a check for lazy initialisation (a CUDA tensor
+# is at hand wherever they are asked): 0.1 us each instead of 2.8 and 0.25
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+_current_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)
 
 
 def _stream(device):
@@ -29,7 +32,7 @@ def _stream(device):
 
 def _call(device, fn, *args):
     """fn(*args, current stream of `device`) with that device as the current one; its return code."""
-    if torch.cuda.current_device() == device.index:
+    if _current_device() == device.index:
         return fn(*args, _stream(device))
     with torch.cuda.device(device):
         return fn(*args, _stream(device))
@@ -56,9 +59,11 @@ def _check_tensor(name, t, dtype=None, device=None):
 
 def _rows(t):
     """(..., c) -> (rows, c) with contiguous rows that do not overlap: a view where the strides allow one."""
-    c = t.shape[-1]
     if t.dim() != 2:
-        t = t.reshape(-1, c)
+        t = t.reshape(-1, t.shape[-1])
+    elif t.is_contiguous():
+        return t
+    c = t.shape[1]
     if (c > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < c):
         t = t.contiguous()
     return t
@@ -75,8 +80,8 @@ def _linear_forward(x, weight, bias, residual, act, keep_z):
     """2-D operands as `_rows` leaves them -> (y, z or None)."""
     m, k = x.shape
     n = weight.shape[0]
-    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    z = torch.empty_like(y) if keep_z else None
+    y = x.new_empty((m, n))
+    z = x.new_empty((m, n)) if keep_z else None
     d = _lib.LinearDesc(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(z), _ld(x),
                         _ld(weight), 0 if residual is None else _ld(residual), n, n, m, k, n, act, _DTYPES[x.dtype])
     size = lib.odamd_linear_workspace_bytes(d)
@@ -89,9 +94,9 @@ def _linear_backward(dy, z, x, weight, act, want_dx, want_dw, want_db):
     """Gradients of `_linear_forward` from 2-D operands; x and weight may be None where they are not needed."""
     m, n = dy.shape
     k = (weight if weight is not None else x).shape[1] if (want_dx or want_dw) else 1
-    dx = torch.empty((m, k), dtype=dy.dtype, device=dy.device) if want_dx else None
-    dw = torch.empty((n, k), dtype=dy.dtype, device=dy.device) if want_dw else None
-    db = torch.empty(n, dtype=dy.dtype, device=dy.device) if want_db else None
+    dx = dy.new_empty((m, k)) if want_dx else None
+    dw = dy.new_empty((n, k)) if want_dw else None
+    db = dy.new_empty((n,)) if want_db else None
     d = _lib.LinearGradDesc(dy.data_ptr(), _ptr(z), _ptr(x) if want_dw else None, _ptr(weight) if want_dx else None, _ptr(dx),
                             _ptr(dw), _ptr(db), _ld(dy), 0 if z is None else _ld(z), _ld(x) if want_dw else 0,
                             _ld(weight) if want_dx else 0, k, k, m, k, n, act, _DTYPES[dy.dtype])
@@ -114,8 +119,12 @@ class _Linear(torch.autograd.Function):
         return y if x.dim() == 2 else y.view(x.shape[:-1] + (weight.shape[0],))
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        # under create_graph the gradients have to refuse a second derivative; the wrapper that sees to it costs 5 us a call
+        return _Linear.gradients_once(ctx, dy) if torch.is_grad_enabled() else _Linear.gradients(ctx, dy)
+
+    @staticmethod
+    def gradients(ctx, dy):
         x, weight, z = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = db = None
@@ -124,6 +133,9 @@ class _Linear(torch.autograd.Function):
             if dx is not None and len(ctx.x_shape) != 2:
                 dx = dx.view(ctx.x_shape)
         return dx, dw, db, dy if need[3] else None, None
+
+
+_Linear.gradients_once = staticmethod(torch.autograd.function.once_differentiable(_Linear.gradients))
 
 
 def linear(x, weight, bias=None, activation=None, residual=None):
@@ -162,7 +174,7 @@ def linear(x, weight, bias=None, activation=None, residual=None):
         return _Linear.apply(x, weight, bias, residual, act)
     y, _ = _linear_forward(_rows(x), _rows(weight), bias if bias is None else bias.contiguous(),
                            None if residual is None else _rows(residual), act, False)
-    return y.view(x.shape[:-1] + (n,))
+    return y if x.dim() == 2 else y.view(x.shape[:-1] + (n,))
 
 
 # ---------------------------------------------------------------------------------------------

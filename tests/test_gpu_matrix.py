@@ -226,6 +226,15 @@ def test_linear_relu_closes_the_gradient(mx):
         assert torch.equal(dx, rx) and torch.equal(dw, rw) and float(dw[3].abs().max()) == 0.0
 
 
+def test_linear_differentiates_once(mx):
+    leaves = [t.requires_grad_() for t in (randn(20, 40), randn(24, 40, seed=1), randn(24, seed=2), randn(20, 24, seed=3))]
+    first = torch.autograd.grad(mx.linear(*leaves[:3], 'silu', leaves[3]).square().sum(), leaves)
+    second = torch.autograd.grad(mx.linear(*leaves[:3], 'silu', leaves[3]).square().sum(), leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        second[0].sum().backward()
+
+
 def test_linear_gradient_against_differences(mx):
     """float32, central differences of the 64-bit layer along random directions."""
     x, w, b = randn(33, 20), randn(17, 20, seed=1), randn(17, seed=2)
