@@ -385,7 +385,7 @@ int odamd_adam_ema_ranges_step(float* param, const float* grad, float* exp_avg, 
  *   out = X, transposed back.
  * Products carry 22 bits per factor and sum in float32, whatever dtype is; out is rounded once.  A matrix that holds a NaN
  * or an infinity gives NaN throughout, a zero matrix zeros.  Values of X under 2^-36 count as zero: a matrix whose norm lies
- * far under eps comes out as zero.  rows * cols < 2^31.  The workspace is 256-byte aligned. */
+ * far under eps comes out as zero.  rows * cols is at most 2^31 - 2^16.  The workspace is 256-byte aligned. */
 size_t odamd_orthogonalize_workspace_bytes(int batch, int rows, int cols);
 int odamd_orthogonalize(const void* x, void* out, int batch, int rows, int cols, int steps, double eps, int dtype,
                         void* workspace, size_t workspace_bytes, void* stream);
@@ -400,7 +400,7 @@ int odamd_orthogonalize(const void* x, void* out, int batch, int rows, int cols,
  * is 256-byte aligned. */
 typedef struct {
     long long offset; /* >= 0 */
-    int rows, cols;   /* rows * cols < 2^31 */
+    int rows, cols;   /* rows * cols at most 2^31 - 2^16 */
 } odamd_matrix;
 size_t odamd_muon_workspace_bytes(const odamd_matrix* matrices_host, int n_matrices);
 int odamd_muon_ema_step(float* param, const float* grad, float* momentum, float* ema, const odamd_matrix* matrices_host,

@@ -31,17 +31,15 @@ namespace {
 
 #include "gemm.h"
 
-constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
+constexpr double NS_A = 3.4445, NS_B = -4.7750, NS_C = 2.0315;
 constexpr float NS_SCALE = 4096.0f;
 constexpr int NS_GROUPS = 112;        // groups of one launch: their table travels in the kernel's arguments (4 KiB at most)
-// m m n up to which one workgroup takes a matrix as a whole (m <= 64).  Whole / in launches, us: 16 x 27 12 / 73, 32 x 576 71 / 98,
-// 64 x 128 56 / 90, 64 x 256 94 / 94; 300 of 64 x 128 75 / 124, of 64 x 256 199 / 143.
-constexpr long long NS_WHOLE = 5 << 17;
+constexpr int NS_FEW_STEPS = 10;      // steps that matrices of at most 64 rows run on A alone
 constexpr int NS_PARTS = 512;         // partial sums of squares per matrix, at most
 
 // stages: sums of squares, laying out, X X^T (whole, or a part of its reduction), P from A, products of square matrices, Q X,
-// Q X to the caller; a matrix as a whole
-enum { ST_NORM, ST_SPLIT, ST_A, ST_AP, ST_P, ST_Q, ST_X, ST_OUT, ST_WHOLE };
+// Q X to the caller; of matrices of few rows: all in one, G G^T, the steps, Q G
+enum { ST_NORM, ST_SPLIT, ST_A, ST_AP, ST_P, ST_Q, ST_X, ST_OUT, ST_WHOLE, ST_GRAM, ST_STEPS, ST_QG };
 __host__ __device__ constexpr bool ns_symmetric(int stage) { return stage == ST_A || stage == ST_AP || stage == ST_P || stage == ST_Q; }
 __host__ __device__ constexpr bool ns_along_n(int stage) { return stage == ST_A || stage == ST_AP; }   // reduces over n, the others over m
 // square matrices: A, a product on the way to the next A, and three that P and Q take in turn; X X^T leaves the sums of a cut
@@ -73,6 +71,16 @@ struct NsJobs {
 static_assert(sizeof(NsTable) <= 3700, "kernel arguments are limited to 4 KiB");
 
 __host__ __device__ inline long long ns_up(long long v, int to) { return (v + to - 1) / to * to; }
+// Columns of an m x n matrix with few rows that a workgroup takes (t: m in 16-row tiles): all of them, or at least what its
+// waves have under way at once, and at most 32 parts.  Parts cost two launches more; one workgroup / parts, us: 16 x 1000 15.0 /
+// 16.4, 16 x 2000 22 / 17, 32 x 1000 35 / 32, 48 x 256 35 / 38, 48 x 512 44 / 40, 64 x 256 59 / 61, 64 x 512 75 / 64.
+__host__ __device__ inline int ns_few_cols(int t, int n) {
+    return n <= 1024 / t ? (int)ns_up(n, 16) : (int)ns_up(ns_up(n, 32) / 32, t <= 2 ? 512 : 128);
+}
+// Workspace of a matrix then: Q and the partial sums of G G^T, in 64 bits
+__host__ __device__ inline long long ns_few_bytes(int t, int cols, int n) {
+    return ns_up(8LL * (256 * t * t + ((long long)n + cols - 1) / cols * 128 * t * (t + 1)), 256);
+}
 // Byte offsets within a matrix's workspace; end is its size.
 struct NsLayout { long long sums, x, xt0, xt1, sq, sq_size, end; };
 __host__ __device__ inline NsLayout ns_layout(int m, int n) {
@@ -85,6 +93,9 @@ __host__ __device__ inline NsLayout ns_layout(int m, int n) {
     l.sq = l.xt1 + ns_up(n * mp * 4, 256);
     l.sq_size = ns_up(m * mp * 4, 256);
     l.end = l.sq + SQ_COUNT * l.sq_size;
+    const int rows = (m + 15) / 16;
+    const long long few = rows <= 4 ? ns_few_bytes(rows, ns_few_cols(rows, n), n) : 0;
+    l.end = few > l.end ? few : l.end;
     return l;
 }
 // Elements one workgroup of the norm pass takes: a multiple of eight that keeps the partial sums within NS_PARTS.
@@ -94,8 +105,10 @@ __host__ __device__ inline long long ns_share(int m, int n) {
 }
 __host__ __device__ inline int ns_parts(int m, int n) { return (int)(((long long)m * n + ns_share(m, n) - 1) / ns_share(m, n)); }
 __host__ __device__ inline int ns_tiles(int stage, int tile, int m, int n) {
-    const int mt = (m + tile - 1) / tile, nt = (n + tile - 1) / tile;
-    return stage == ST_WHOLE ? 1 : stage == ST_NORM ? ns_parts(m, n) : ns_symmetric(stage) ? mt * (mt + 1) / 2 : mt * nt;
+    if (stage == ST_WHOLE || stage == ST_STEPS) return 1;
+    if (stage == ST_NORM) return ns_parts(m, n);
+    const int mt = (int)((m + (long long)tile - 1) / tile), nt = (int)((n + (long long)tile - 1) / tile);
+    return stage == ST_GRAM || stage == ST_QG ? nt : ns_symmetric(stage) ? mt * (mt + 1) / 2 : mt * nt;
 }
 
 // Chunks of a part
@@ -257,118 +270,328 @@ __global__ void __launch_bounds__(256) ns_split_kernel(NsTable t, NsIo io) {
     }
 }
 
-// A small matrix from the caller's buffers to the caller's buffers in one workgroup: X, A and P stay in LDS as float32, the products
-// run on v_mfma_f32_16x16x4_f32 (a sixteenth of the half-precision rate, but no pairs, no columns copy and no launches
-// between the steps).  16 x 27 takes 12 us this way and 73 us in eighteen launches.  T: m in 16-row tiles.  Rows of X lie ld
-// floats apart, ld = 4 modulo 32: sixteen rows at four consecutive k touch 64 different banks.
-__host__ __device__ inline int ns_small_ld(int n) { return (int)ns_up(ns_up(n, 16) - 4, 32) + 4; }
-__host__ __device__ inline long long ns_small_lds(int t, int n) { return 4LL * 16 * t * (ns_small_ld(n) + 2 * ns_small_ld(16 * t)); }
-
-template <int T, bool MUON, int DT>
-__global__ void __launch_bounds__(256) ns_whole_kernel(NsTable t, NsIo io, int steps) {
-    extern __shared__ __attribute__((aligned(16))) float space[];
-    __shared__ double part[4];
-    const NsPlace p = ns_find(t, blockIdx.x, ST_WHOLE, 0);
-    const int ld = ns_small_ld(p.n), lda = ns_small_ld(16 * T);
-    float *x = space, *a = x + 16 * T * ld, *pm = a + 16 * T * lda;
-    const int total = p.m * p.n, cols = p.tall ? p.m : p.n;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, h = lane >> 4;
-    const auto place = [&](int i) {                       // element i of the caller's matrix in X
-        const int row = i / cols, col = i - row * cols;
-        return p.tall ? col * ld + row : row * ld + col;
-    };
-    for (int i = threadIdx.x; i < 16 * T * ld; i += 256) x[i] = 0.0f;
-    __syncthreads();
-    double s = 0.0;
-    for (int i = threadIdx.x; i < total; i += 256) {
-        float v;
-        if constexpr (MUON) {
-            const float g = ((const float*)io.in)[p.src + i], m = io.mu * io.momentum[p.src + i] + g * io.grad_scale;
-            io.momentum[p.src + i] = m;
-            v = ns_direction(io, g, m);
-        } else if constexpr (DT == ODAMD_DTYPE_BF16) {
-            v = bf16_to_f32(((const uint16_t*)io.in)[p.src + i]);
-        } else {
-            v = ((const float*)io.in)[p.src + i];
+// ---- at most 64 rows -------------------------------------------------------------------------------------------------
+// All steps run on A = X X^T, in 64 bits (v_mfma_f64_16x16x4_f64, half the rate of the float32 instruction): a rounding of A, 2^-53,
+// grows to 2^-53 3.4445^18 = 5e-7 in ten steps, so the result has float32's accuracy, and the caller's matrix is read twice only,
+// for G G^T (whose trace is the norm) and for Q G.  What it costs is latency: 3 dependent products of m x m per step.
+// T: m in 16-row tiles.  Squares lie in LDS, rows LD doubles apart: sixteen rows at two neighbouring k touch all 64 banks.
+template <int T_> struct NsFew {
+    static constexpr int T = T_, N = 16 * T, LD = N + 2, SQ = N * LD, TRI = T * (T + 1) / 2;
+    static constexpr int WAVES = 8, THREADS = 64 * WAVES;
+    static constexpr int KEPT = T <= 2 ? WAVES : WAVES / 2;  // waves whose sums lie in LDS side by side
+    static constexpr int SUMS = TRI * 256;                   // G G^T: the tiles on and over the diagonal
+    static constexpr int LDS = 8 * (3 * SQ > KEPT * SUMS ? 3 * SQ : KEPT * SUMS);
+    static constexpr int AT_ONCE = T <= 2 ? 4 : 1;           // groups of sixteen columns a wave has under way
+};
+typedef double f64x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f64x4_t ns_mma64(double a, double b, f64x4_t c) {
+    return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0);
+}
+// Four values of the caller's, `stride` apart; zeros for those past the first cnt
+template <int DT>
+__device__ __forceinline__ void ns_load4(const void* base, long long at, long long stride, int cnt, float v[4]) {
+    if constexpr (DT == ODAMD_DTYPE_F32) {
+        const float* s = (const float*)base + at;
+        if (stride == 1 && cnt == 4) {
+            const f32x4_t u = *(const f32x4_any*)s;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = u[e];
+            return;
         }
-        x[place(i)] = v;
-        s += (double)v * v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = e < cnt ? s[e * stride] : 0.0f;
+    } else {
+        const uint16_t* s = (const uint16_t*)base + at;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = e < cnt ? bf16_to_f32(s[e * stride]) : 0.0f;
     }
-    s = ns_block_sum(s, part);                            // its barrier also closes the writes of X
-    const double inv = 1.0 / (sqrt(s) + io.eps);
-    for (int i = threadIdx.x; i < 16 * T * ld; i += 256) x[i] = (float)(x[i] * inv);
+}
+template <int DT>
+__device__ __forceinline__ void ns_store4(void* base, long long at, long long stride, int cnt, const float v[4]) {
+    if constexpr (DT == ODAMD_DTYPE_F32) {
+        float* d = (float*)base + at;
+        if (stride == 1 && cnt == 4) {
+            *(f32x4_any*)d = f32x4_t{v[0], v[1], v[2], v[3]};
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < cnt) d[e * stride] = v[e];
+    } else {
+        uint16_t* d = (uint16_t*)base + at;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < cnt) d[e * stride] = f32_to_bf16(v[e]);
+    }
+}
+
+// G G^T over columns [from, to): every wave's sums side by side in `sums`.  A lane loads four neighbouring columns of a row; that
+// instruction e takes column 4 h + e of each group of sixteen does not matter to a sum over them.  The optimizer step's momentum
+// update happens here.
+template <int T, bool MUON, int DT>
+__device__ __forceinline__ void ns_few_gram(const NsIo& io, const NsPlace& p, int from, int to, double* sums) {
+    using F = NsFew<T>;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, h = lane >> 4;
+    const long long sr = p.tall ? 1 : p.n, sc = p.tall ? p.m : 1;
+    f64x4_t acc[F::TRI] = {};
+    for (int c0 = from + wave * 16 * F::AT_ONCE; c0 < to; c0 += F::WAVES * 16 * F::AT_ONCE) {
+        float x[F::AT_ONCE][T][4], m[F::AT_ONCE][T][4];
+#pragma unroll
+        for (int g = 0; g < F::AT_ONCE; ++g)
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                const int row = 16 * t + r, c = c0 + 16 * g + 4 * h, cnt = row < p.m ? max(0, min(4, to - c)) : 0;
+                const long long at = p.src + row * sr + c * sc;
+                ns_load4<DT>(io.in, at, sc, cnt, x[g][t]);
+                if constexpr (MUON) ns_load4<DT>(io.momentum, at, sc, cnt, m[g][t]);
+            }
+#pragma unroll
+        for (int g = 0; g < F::AT_ONCE; ++g) {
+            if constexpr (MUON)
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    const int row = 16 * t + r, c = c0 + 16 * g + 4 * h, cnt = row < p.m ? max(0, min(4, to - c)) : 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        m[g][t][e] = io.mu * m[g][t][e] + x[g][t][e] * io.grad_scale;
+                        x[g][t][e] = e < cnt ? ns_direction(io, x[g][t][e], m[g][t][e]) : 0.0f;
+                    }
+                    ns_store4<DT>(io.momentum, p.src + row * sr + c * sc, sc, cnt, m[g][t]);
+                }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                int k = 0;
+#pragma unroll
+                for (int j = 0; j < T; ++j)
+#pragma unroll
+                    for (int i = 0; i <= j; ++i, ++k) acc[k] = ns_mma64((double)x[g][i][e], (double)x[g][j][e], acc[k]);
+            }
+        }
+    }
+    const auto at = [&](int w, int k, int e) -> double& { return sums[(w * F::TRI + k) * 256 + e * 64 + lane]; };
+    if constexpr (F::KEPT < F::WAVES) {
+        // the second half of the waves hands its sums to the first
+        if (wave >= F::KEPT)
+#pragma unroll
+            for (int k = 0; k < F::TRI; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) at(wave - F::KEPT, k, e) = acc[k][e];
+        __syncthreads();
+        if (wave < F::KEPT)
+#pragma unroll
+            for (int k = 0; k < F::TRI; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[k][e] += at(wave, k, e);
+    }
+    if (wave < F::KEPT)
+#pragma unroll
+        for (int k = 0; k < F::TRI; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) at(wave, k, e) = acc[k][e];
     __syncthreads();
-    // out tile (ti, tj) of l r^T over k values, both of them rows `stride` apart
-    const auto product = [&](const float* l, const float* rr, int stride, int ti, int tj, int k) {
-        f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        const float *la = l + (ti * 16 + r) * stride + h, *lb = rr + (tj * 16 + r) * stride + h;
-#pragma unroll 4
-        for (int q = 0; q < k; q += 4) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(la[q], lb[q], acc, 0, 0, 0);
+}
+// Value u of the sums of all waves, added in order
+template <int T>
+__device__ __forceinline__ double ns_few_sum(const double* sums, int u) {
+    double s = sums[u];
+#pragma unroll
+    for (int w = 1; w < NsFew<T>::KEPT; ++w) s += sums[w * NsFew<T>::SUMS + u];
+    return s;
+}
+
+// Q / (|G| + eps) from G G^T: value u of it is get(u).  Left in the third square of `lds`.
+template <int T, typename GET>
+__device__ __forceinline__ double* ns_few_steps(double* lds, int steps, double eps, GET&& get) {
+    using F = NsFew<T>;
+    constexpr int EACH = (F::SUMS + F::THREADS - 1) / F::THREADS, LD = F::LD;
+    double *a = lds, *p = lds + F::SQ, *q = lds + 2 * F::SQ;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, h = lane >> 4;
+    double v[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int u = i * F::THREADS + (int)threadIdx.x;
+        v[i] = u < F::SUMS ? get(u) : 0.0;
+    }
+    __syncthreads();                                          // the sums' place is the squares'
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int u = i * F::THREADS + (int)threadIdx.x;
+        if (u < F::SUMS) {
+            int ti, tj;
+            gemm_triangle_at(u >> 8, ti, tj);
+            const int row = ti * 16 + (u >> 6 & 3) * 4 + (u >> 4 & 3), col = tj * 16 + (u & 15);
+            a[row * LD + col] = v[i];
+            a[col * LD + row] = v[i];
+        }
+    }
+    __syncthreads();
+    double sum = lane < F::N ? a[lane * LD + lane] : 0.0;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    const double inv = 1.0 / (sqrt(sum) + eps);
+    __syncthreads();
+    for (int i = threadIdx.x; i < F::SQ; i += F::THREADS) a[i] = i % LD < F::N ? a[i] * inv * inv : 0.0;
+    __syncthreads();
+    // tile k (on or over the diagonal) of left right, both symmetric
+    const auto product = [&](const double* left, const double* right, int k) {
+        int ti, tj;
+        gemm_triangle_at(k, ti, tj);
+        const double *x = left + (ti * 16 + r) * LD + h, *y = right + (tj * 16 + r) * LD + h;
+        f64x4_t acc = {};
+#pragma unroll
+        for (int s = 0; s < F::N; s += 4) acc = ns_mma64(x[s], y[s], acc);
         return acc;
     };
-    constexpr int TRI = T * (T + 1) / 2;
+    const auto put = [&](double* to, int k, f64x4_t val, double scale) {
+        int ti, tj;
+        gemm_triangle_at(k, ti, tj);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = ti * 16 + 4 * e + h, col = tj * 16 + r;
+            to[row * LD + col] = val[e] * scale;
+            to[col * LD + row] = val[e] * scale;
+        }
+    };
+    constexpr int TURNS = (2 * F::TRI + F::WAVES - 1) / F::WAVES;
     for (int step = 0; step < steps; ++step) {
-        for (int tile = wave; tile < TRI; tile += 4) {
+        const bool last = step + 1 == steps;
+        for (int k = wave; k < F::TRI; k += F::WAVES) {
+            f64x4_t s = product(a, a, k);
             int ti, tj;
-            gemm_triangle_at(tile, ti, tj);
-            const f32x4_t v = product(x, x, ld, ti, tj, (int)ns_up(p.n, 4));
+            gemm_triangle_at(k, ti, tj);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int i = ti * 16 + 4 * h + e, j = tj * 16 + r;
-                a[i * lda + j] = v[e];
-                a[j * lda + i] = v[e];
+                const int row = ti * 16 + 4 * e + h, col = tj * 16 + r;
+                s[e] = (row == col ? NS_A : 0.0) + NS_B * a[row * LD + col] + NS_C * s[e];
             }
+            put(p, k, s, 1.0);
+            if (step == 0) put(q, k, s, last ? inv : 1.0);
         }
         __syncthreads();
-        for (int tile = wave; tile < TRI; tile += 4) {
-            int ti, tj;
-            gemm_triangle_at(tile, ti, tj);
-            const f32x4_t v = product(a, a, lda, ti, tj, 16 * T);
+        // Q <- Q P and A <- P A P, by way of registers: the results take their operands' place
+        f64x4_t next[TURNS];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = ti * 16 + 4 * h + e, j = tj * 16 + r;
-                // without a I: the float32 sum a X + (P - a I) X keeps the last bits of X
-                const float u = NS_B * a[i * lda + j] + NS_C * v[e];
-                pm[i * lda + j] = u;
-                pm[j * lda + i] = u;
-            }
+        for (int i = 0; i < TURNS; ++i) {
+            const int k = i * F::WAVES + wave;
+            if (k < F::TRI ? step > 0 : k < 2 * F::TRI && !last) next[i] = k < F::TRI ? product(q, p, k) : product(p, a, k - F::TRI);
         }
         __syncthreads();
-        // a wave owns sixteen columns of X: it has read them when it writes them
-        for (int j0 = wave * 16; j0 < p.n; j0 += 64) {
-            float col[4 * T];
 #pragma unroll
-            for (int q = 0; q < 4 * T; ++q) col[q] = x[(4 * q + h) * ld + j0 + r];
-            f32x4_t acc[T];
+        for (int i = 0; i < TURNS; ++i) {
+            const int k = i * F::WAVES + wave;
+            if (k < F::TRI ? step > 0 : k < 2 * F::TRI && !last) put(k < F::TRI ? q : a, k < F::TRI ? k : k - F::TRI, next[i], last ? inv : 1.0);
+        }
+        __syncthreads();
+        if (last) break;
 #pragma unroll
-            for (int ti = 0; ti < T; ++ti)
+        for (int i = 0; i < TURNS; ++i) {
+            const int k = i * F::WAVES + wave;
+            if (k < F::TRI) next[i] = product(p, a, k);
+        }
+        __syncthreads();
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[ti][e] = NS_A * x[(ti * 16 + 4 * h + e) * ld + j0 + r];
-#pragma unroll
-            for (int q = 0; q < 4 * T; ++q)
-#pragma unroll
-                for (int ti = 0; ti < T; ++ti)
-                    acc[ti] = __builtin_amdgcn_mfma_f32_16x16x4f32(pm[(ti * 16 + r) * lda + 4 * q + h], col[q], acc[ti], 0, 0, 0);
-#pragma unroll
-            for (int ti = 0; ti < T; ++ti)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[(ti * 16 + 4 * h + e) * ld + j0 + r] = acc[ti][e];
+        for (int i = 0; i < TURNS; ++i) {
+            const int k = i * F::WAVES + wave;
+            if (k < F::TRI) put(a, k, next[i], 1.0);
         }
         __syncthreads();
     }
+    return q;
+}
+
+// Columns [from, to) of Q G to the caller.  A lane holds rows 4 h + e of a tile and one column, of G and of the result: the product
+// takes Q's rows in the order that puts them there.
+template <int T, bool MUON, int DT>
+__device__ __forceinline__ void ns_few_out(const NsIo& io, const NsPlace& p, int from, int to, const double* q) {
+    using F = NsFew<T>;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, h = lane >> 4, qr = (r & 3) * 4 + (r >> 2);
+    const long long sr = p.tall ? 1 : p.n, sc = p.tall ? p.m : 1;
     const float step = MUON ? io.lr02 * sqrtf((float)p.n) : 0.0f;
-    for (int i = threadIdx.x; i < total; i += 256) {
-        const float v = x[place(i)];
-        const long long at = p.src + i;
-        if constexpr (MUON) {
-            const float w = io.param[at] * io.decay - step * v;
-            io.param[at] = w;
-            if (io.ema) io.ema[at] = io.ema_keep * io.ema[at] + io.ema_take * w;
-        } else if constexpr (DT == ODAMD_DTYPE_BF16) {
-            ((uint16_t*)io.out)[at] = f32_to_bf16(v);
-        } else {
-            ((float*)io.out)[at] = v;
+    for (int c0 = from + wave * 16 * F::AT_ONCE; c0 < to; c0 += F::WAVES * 16 * F::AT_ONCE) {
+        float x[F::AT_ONCE][T][4], m[F::AT_ONCE][T][4];
+        const auto place = [&](int g, int t, int& cnt) {
+            const int row = 16 * t + 4 * h, c = c0 + 16 * g + r;
+            cnt = c < to ? max(0, min(4, p.m - row)) : 0;
+            return p.src + row * sr + c * sc;
+        };
+#pragma unroll
+        for (int g = 0; g < F::AT_ONCE; ++g)
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                int cnt;
+                const long long at = place(g, t, cnt);
+                ns_load4<DT>(io.in, at, sr, cnt, x[g][t]);
+                if constexpr (MUON) ns_load4<DT>(io.momentum, at, sr, cnt, m[g][t]);
+            }
+#pragma unroll
+        for (int g = 0; g < F::AT_ONCE; ++g) {
+            f64x4_t acc[T] = {};
+            if constexpr (T > 2) asm volatile("" ::: "memory");   // Q comes from LDS anew: registers do not hold it beside the rest
+#pragma unroll
+            for (int k = 0; k < T; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const double b = MUON ? ns_direction(io, x[g][k][e], m[g][k][e]) : x[g][k][e];
+#pragma unroll
+                    for (int i = 0; i < T; ++i) acc[i] = ns_mma64(q[(16 * i + qr) * F::LD + 16 * k + 4 * h + e], b, acc[i]);
+                }
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                int cnt;
+                const long long at = place(g, t, cnt);
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (float)acc[t][e];
+                if constexpr (MUON) {
+                    float w[4], old[4];
+                    ns_load4<DT>(io.param, at, sr, cnt, w);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = w[e] * io.decay - step * v[e];
+                    ns_store4<DT>(io.param, at, sr, cnt, w);
+                    if (io.ema) {
+                        ns_load4<DT>(io.ema, at, sr, cnt, old);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) old[e] = io.ema_keep * old[e] + io.ema_take * w[e];
+                        ns_store4<DT>(io.ema, at, sr, cnt, old);
+                    }
+                } else {
+                    ns_store4<DT>(io.out, at, sr, cnt, v);
+                }
+            }
         }
+    }
+}
+
+// The three parts in one workgroup, or (`cols` columns a workgroup) as three launches: partial sums of G G^T; Q; Q G
+template <int T, int STAGE, bool MUON, int DT>
+__global__ void __launch_bounds__(NsFew<T>::THREADS) ns_few_kernel(NsTable t, NsIo io, int steps, int cols) {
+    using F = NsFew<T>;
+    extern __shared__ __attribute__((aligned(16))) char space[];
+    double* lds = (double*)space;
+    const NsPlace p = ns_find(t, blockIdx.x, STAGE, cols);
+    double* q_at = (double*)p.ws;                             // Q, then the partial sums
+    double* parts = q_at + F::N * F::N;
+    const int from = p.tile * cols, to = from + min(p.n - from, cols);
+    if constexpr (STAGE == ST_WHOLE) {
+        ns_few_gram<T, MUON, DT>(io, p, 0, p.n, lds);
+        const double* q = ns_few_steps<T>(lds, steps, io.eps, [&](int u) { return ns_few_sum<T>(lds, u); });
+        ns_few_out<T, MUON, DT>(io, p, 0, p.n, q);
+    } else if constexpr (STAGE == ST_GRAM) {
+        ns_few_gram<T, MUON, DT>(io, p, from, to, lds);
+        for (int u = threadIdx.x; u < F::SUMS; u += F::THREADS) parts[(long long)p.tile * F::SUMS + u] = ns_few_sum<T>(lds, u);
+    } else if constexpr (STAGE == ST_STEPS) {
+        const int n_parts = ns_tiles(ST_GRAM, cols, p.m, p.n);
+        const double* q = ns_few_steps<T>(lds, steps, io.eps, [&](int u) {
+            double s = parts[u];
+#pragma unroll 8
+            for (int k = 1; k < n_parts; ++k) s += parts[(long long)k * F::SUMS + u];
+            return s;
+        });
+        for (int i = threadIdx.x; i < F::N * F::N; i += F::THREADS) q_at[i] = q[i / F::N * F::LD + i % F::N];
+    } else {
+        for (int i = threadIdx.x; i < F::N * F::N; i += F::THREADS) lds[i / F::N * F::LD + i % F::N] = q_at[i];
+        __syncthreads();
+        ns_few_out<T, MUON, DT>(io, p, from, to, lds);
     }
 }
 
@@ -503,7 +726,7 @@ __global__ void __launch_bounds__(TILE::THREADS) ns_product_kernel(NsTable t, Ns
             if constexpr (STAGE == ST_P) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    v[e] = (NS_C / NS_SCALE) * v[e] + NS_B * ((float)x.hi[e] + (float)x.lo[e]) + (i == j + e ? NS_A * NS_SCALE : 0.0f);
+                    v[e] = (float)(NS_C / NS_SCALE) * v[e] + (float)NS_B * ((float)x.hi[e] + (float)x.lo[e]) + (i == j + e ? (float)(NS_A * NS_SCALE) : 0.0f);
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] *= scale;
@@ -679,35 +902,47 @@ int ns_product(NsTable& t, const NsIo& io, const NsJobs& jobs, hipStream_t s) {
 
 // Exponent that keeps a product of k P's (entries up to 3.4445^k) within fp16, an eighth of a bit to spare for rounding
 int ns_q_exponent(int k) {
-    const int e = (int)floor(log2(65504.0 / (1.1 * pow((double)NS_A, k))));
+    const int e = (int)floor(log2(65504.0 / (1.1 * pow(NS_A, k))));
     return e < 12 ? e : 12;
 }
 
-template <int T, bool MUON, int DT>
-int ns_whole(NsTable& t, const NsIo& io, int steps, long long lds, hipStream_t s) {
-    if (ns_count(t, ST_WHOLE, 0, 256) < 0) return ODAMD_E_LIMIT;
-    const auto kernel = ns_whole_kernel<T, MUON, DT>;
-    const hipError_t e = odamd_ensure_lds((const void*)kernel, (size_t)lds);
+int ns_few_rows(const NsTable& t) {   // rows of the tallest matrix, in 16-row tiles
+    int rows = 0;
+    for (int i = 0; i < t.n; ++i) rows = t.g[i].m > rows ? t.g[i].m : rows;
+    return (rows + 15) / 16;
+}
+int ns_longest(const NsTable& t) {
+    int n = 0;
+    for (int i = 0; i < t.n; ++i) n = t.g[i].n > n ? t.g[i].n : n;
+    return n;
+}
+
+// All matrices have at most 16 T rows, the longest `n` columns
+template <int T, int STAGE, bool MUON, int DT>
+int ns_few_launch(NsTable& t, const NsIo& io, int steps, int cols, hipStream_t s) {
+    using F = NsFew<T>;
+    if (ns_count(t, STAGE, cols, F::THREADS) < 0) return ODAMD_E_LIMIT;
+    const auto kernel = ns_few_kernel<T, STAGE, MUON, DT>;
+    const hipError_t e = odamd_ensure_lds((const void*)kernel, F::LDS);
     if (e != hipSuccess) return (int)e;
-    kernel<<<t.tiles, 256, (size_t)lds, s>>>(t, io, steps);
+    kernel<<<t.tiles, F::THREADS, F::LDS, s>>>(t, io, steps, cols);
     return (int)hipGetLastError();
+}
+template <int T, bool MUON, int DT>
+int ns_few(NsTable& t, const NsIo& io, int steps, int n, hipStream_t s) {
+    const int cols = ns_few_cols(T, n);
+    if (cols >= n) return ns_few_launch<T, ST_WHOLE, MUON, DT>(t, io, steps, cols, s);
+    int rc = ns_few_launch<T, ST_GRAM, MUON, DT>(t, io, steps, cols, s);
+    if (rc == 0) rc = ns_few_launch<T, ST_STEPS, false, ODAMD_DTYPE_F32>(t, io, steps, cols, s);
+    return rc == 0 ? ns_few_launch<T, ST_QG, MUON, DT>(t, io, steps, cols, s) : rc;
 }
 
 template <bool MUON, int DT>
 int ns_run(NsTable& t, const NsIo& io, int steps, hipStream_t s) {
-    int tallest = 0;
-    long long lds = 0, work = 0;
-    for (int i = 0; i < t.n; ++i) {
-        const int rows = (t.g[i].m + 15) / 16;
-        tallest = rows > tallest ? rows : tallest;
-        work = (long long)t.g[i].m * t.g[i].m * t.g[i].n > work ? (long long)t.g[i].m * t.g[i].m * t.g[i].n : work;
-    }
-    if (tallest <= 4 && work <= NS_WHOLE) {
-        for (int i = 0; i < t.n; ++i) lds = ns_small_lds(tallest, t.g[i].n) > lds ? ns_small_lds(tallest, t.g[i].n) : lds;
-        if (lds <= 128 * 1024)
-            return tallest == 1 ? ns_whole<1, MUON, DT>(t, io, steps, lds, s) : tallest == 2 ? ns_whole<2, MUON, DT>(t, io, steps, lds, s)
-                 : tallest == 3 ? ns_whole<3, MUON, DT>(t, io, steps, lds, s) : ns_whole<4, MUON, DT>(t, io, steps, lds, s);
-    }
+    const int rows = ns_few_rows(t), cols = ns_longest(t);
+    if (rows <= 4 && steps <= NS_FEW_STEPS)
+        return rows == 1 ? ns_few<1, MUON, DT>(t, io, steps, cols, s) : rows == 2 ? ns_few<2, MUON, DT>(t, io, steps, cols, s)
+             : rows == 3 ? ns_few<3, MUON, DT>(t, io, steps, cols, s) : ns_few<4, MUON, DT>(t, io, steps, cols, s);
     constexpr bool LOOSE = MUON || DT == ODAMD_DTYPE_BF16;
     int phase = LOOSE ? 5 : 2;
     for (int i = 0; i < t.n; ++i)
@@ -763,12 +998,38 @@ int ns_run(NsTable& t, const NsIo& io, int steps, hipStream_t s) {
     return rc;
 }
 
-bool ns_shape_ok(long long rows, long long cols) { return rows >= 1 && cols >= 1 && rows * cols <= 0x7fffffffLL; }
+// 2^31 less what a position passes the last column by
+bool ns_shape_ok(long long rows, long long cols) { return rows >= 1 && cols >= 1 && rows * cols <= 0x7fff0000LL; }
 
 void ns_orient(NsGroup& g, int rows, int cols) {
     g.tall = rows > cols;
     g.m = g.tall ? cols : rows;
     g.n = g.tall ? rows : cols;
+}
+
+// The table of matrices from number `from` on
+void ns_fill(NsTable& t, const odamd_matrix* matrices, int from, int count) {
+    t.n = 0;
+    for (int k = from; k < count && k < from + NS_GROUPS; ++k) {
+        NsGroup g = {};
+        ns_orient(g, matrices[k].rows, matrices[k].cols);
+        g.src = matrices[k].offset;
+        g.count = 1;
+        // the longest tiles first: short ones fill the end of a launch
+        int to = t.n++;
+        for (; to > 0 && (t.g[to - 1].m < g.m || (t.g[to - 1].m == g.m && t.g[to - 1].n < g.n)); --to) t.g[to] = t.g[to - 1];
+        t.g[to] = g;
+    }
+}
+// Places their workspaces one behind the other; the bytes of all of them
+long long ns_place(NsTable& t, int steps) {
+    const int rows = ns_few_rows(t), n = ns_longest(t);
+    long long at = 0;
+    for (int i = 0; i < t.n; ++i) {
+        t.g[i].ws = (unsigned)(at / 256);
+        at += rows <= 4 && steps <= NS_FEW_STEPS ? ns_few_bytes(rows, ns_few_cols(rows, n), t.g[i].n) : ns_layout(t.g[i].m, t.g[i].n).end;
+    }
+    return at;
 }
 
 }  // namespace
@@ -806,16 +1067,16 @@ int odamd_orthogonalize(const void* x, void* out, int batch, int rows, int cols,
 
 size_t odamd_muon_workspace_bytes(const odamd_matrix* matrices_host, int n_matrices) {
     if (!matrices_host || n_matrices < 1) return 0;
+    for (int k = 0; k < n_matrices; ++k)
+        if (!ns_shape_ok(matrices_host[k].rows, matrices_host[k].cols)) return 0;
     size_t most = 0;
     for (int i = 0; i < n_matrices; i += NS_GROUPS) {
-        size_t at = 0;
-        for (int k = i; k < n_matrices && k < i + NS_GROUPS; ++k) {
-            if (!ns_shape_ok(matrices_host[k].rows, matrices_host[k].cols)) return 0;
-            NsGroup g;
-            ns_orient(g, matrices_host[k].rows, matrices_host[k].cols);
-            at += (size_t)ns_layout(g.m, g.n).end;
+        NsTable t;
+        ns_fill(t, matrices_host, i, n_matrices);
+        for (int steps : {1, NS_FEW_STEPS + 1}) {
+            const size_t need = (size_t)ns_place(t, steps);
+            most = need > most ? need : most;
         }
-        most = at > most ? at : most;
     }
     return most;
 }
@@ -846,21 +1107,9 @@ int odamd_muon_ema_step(float* param, const float* grad, float* momentum, float*
     io.eps = eps;
     for (int i = 0; i < n_matrices; i += NS_GROUPS) {
         NsTable t;
-        t.n = 0;
+        ns_fill(t, matrices_host, i, n_matrices);
+        ns_place(t, steps);
         t.ws = (char*)workspace;
-        long long at = 0;
-        for (int k = i; k < n_matrices && k < i + NS_GROUPS; ++k) {
-            NsGroup g;
-            ns_orient(g, matrices_host[k].rows, matrices_host[k].cols);
-            g.src = matrices_host[k].offset;
-            g.count = 1;
-            g.ws = (unsigned)(at / 256);
-            at += ns_layout(g.m, g.n).end;
-            // the longest tiles first: short ones fill the end of a launch
-            int to = t.n++;
-            for (; to > 0 && (t.g[to - 1].m < g.m || (t.g[to - 1].m == g.m && t.g[to - 1].n < g.n)); --to) t.g[to] = t.g[to - 1];
-            t.g[to] = g;
-        }
         const int rc = ns_run<true, ODAMD_DTYPE_F32>(t, io, steps, (hipStream_t)stream);
         if (rc != 0) return rc;
     }

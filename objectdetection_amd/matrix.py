@@ -15,6 +15,7 @@ ACTIVATIONS = {None: 0, 'silu': 1, 'gelu': 2, 'relu': 3}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 MATRIX_DTYPE = np.dtype([('offset', '<i8'), ('rows', '<i4'), ('cols', '<i4')])      # odamd_matrix
 _MOST = 2 ** 31 - 1025                                                               # rows, columns, matrices of a call
+_ELEMENTS = 2 ** 31 - 2 ** 16                                                        # elements of a matrix
 RANGE_DTYPE = np.dtype([('offset', '<i8'), ('len', '<i8')])                         # odamd_range
 
 
@@ -191,17 +192,17 @@ def orthogonalize(x, steps=5, eps=1e-7, out=None):
     if not 1 <= int(steps) <= 32 or not eps >= 0:
         raise ValueError('steps must be 1 to 32, eps must not be negative')
     rows, cols = x.shape[-2:]
-    if rows * cols >= 2 ** 31 or x.shape[:-2].numel() > _MOST:
-        raise ValueError(f'a matrix must have fewer than 2^31 elements, a batch at most {_MOST} matrices')
+    if rows * cols > _ELEMENTS or x.shape[:-2].numel() > _MOST:
+        raise ValueError(f'a matrix has at most {_ELEMENTS} elements, a batch at most {_MOST} matrices')
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(x.shape)
     else:
         _check_tensor('out', out, x.dtype, x.device)
         if out.shape != x.shape or not out.is_contiguous():
             raise ValueError('out must be contiguous and have the shape of x')
     if x.numel() == 0:
         return out
-    src = x.detach().contiguous()
+    src = x if x.is_contiguous() else x.detach().contiguous()
     batch = src.numel() // (rows * cols)
     size = lib.odamd_orthogonalize_workspace_bytes(batch, rows, cols)
     ws = _workspace(size, x.device)
@@ -216,8 +217,8 @@ class MatrixTable:
     def __init__(self, matrices):
         a = np.asarray(list(matrices), dtype=np.int64).reshape(-1, 3)
         size = a[:, 1] * a[:, 2]
-        if len(a) == 0 or (a[:, 0] < 0).any() or (a[:, 1:] < 1).any() or (a[:, 1:] >= 2 ** 31).any() or (size >= 2 ** 31).any():
-            raise ValueError('matrices: at least one (offset, rows, cols), offsets from 0, sizes from 1, under 2^31 elements each')
+        if len(a) == 0 or (a[:, 0] < 0).any() or (a[:, 1:] < 1).any() or (a[:, 1:] >= 2 ** 31).any() or (size > _ELEMENTS).any():
+            raise ValueError(f'matrices: at least one (offset, rows, cols), offsets from 0, sizes from 1, at most {_ELEMENTS} elements each')
         order = np.argsort(a[:, 0], kind='stable')
         ends = (a[:, 0] + size)[order]
         if (a[order, 0][1:] < ends[:-1]).any():

@@ -317,6 +317,37 @@ def test_orthogonalize_long_reductions(mx, batch, rows, cols, dtype):
     assert torch.equal(mx.orthogonalize(g), got)
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('batch, rows, cols', [
+    (3, 1, 1023), (2, 1, 1025), (1, 1, 70001), (2, 1500, 2), (40, 5, 1024), (2, 5, 4264), (1, 16, 16), (1, 16, 40000), (3, 17, 512),
+    (2, 33000, 31), (2, 32, 513), (1, 32, 1030), (3, 33, 341), (2, 342, 33), (1, 48, 343), (2, 45, 9000), (5, 49, 63), (2, 64, 256),
+    (300, 64, 70), (2, 257, 64), (3, 61, 1001), (1, 20000, 64)])
+def test_orthogonalize_few_rows(mx, batch, rows, cols, dtype):
+    """Up to 64 rows: 64-bit arithmetic, in one workgroup or in parts.  Five steps multiply a rounding by 3e4 at most, 2^-53 to
+    4e-12: what is left is the rounding of the result."""
+    g = randn(batch, rows, cols, dtype=dtype, scale=1e-3)
+    got = mx.orthogonalize(g)
+    for i in {0, batch // 2, batch - 1}:
+        ref = orth64(g[i])
+        assert float((got[i].double() - ref).norm()) <= (HALF[dtype] + 1e-10) * float(ref.norm())
+    assert torch.equal(mx.orthogonalize(g), got)
+
+
+def test_orthogonalize_few_rows_of_no_rank(mx):
+    """Equal and zero rows, ten steps: directions without a singular value stay at zero (a rounding of A, 2^-53, grows by
+    3.4445^2 a step and is seen under a root)."""
+    g = randn(2, 40, 300)
+    g[0, 7:] = g[0, 3]
+    g[1, :, 50:] = 0
+    g[1, 10:20] = 0
+    for steps in (1, 5, 10):
+        got = mx.orthogonalize(g, steps=steps)
+        for i in range(2):
+            ref = orth64(g[i], steps=steps)
+            assert float((got[i].double() - ref).norm()) <= (2.0 ** -24 + 3.4445 ** (2 * steps) * 2.0 ** -53 * 40) * float(ref.norm())
+    assert float(mx.orthogonalize(g)[1, 10:20].abs().max()) == 0.0
+
+
 @pytest.mark.parametrize('rows, cols', [(30, 50), (90, 100), (90, 400), (150, 2000)])
 def test_orthogonalize_more_steps(mx, rows, cols):
     """Up to two phases of five steps and a rest; a step leaves an error of a product and multiplies what came before by 3.4445
@@ -461,6 +492,34 @@ def test_muon_step_long_and_short_reductions(mx):
         step = 0.01 * 0.2 * math.sqrt(max(r, c)) * 1.25 * math.sqrt(min(r, c))
         assert float((p[s].double() - rp[s]).norm()) <= LOOSE * step + 4 * 2.0 ** -24 * float(rp[s].norm())
         assert float((m[s].double() - rm[s]).abs().max()) <= 4 * 2.0 ** -24 * float(rm[s].abs().max())
+
+
+@pytest.mark.parametrize('top', [16, 32, 48, 64])
+@pytest.mark.parametrize('long', [200, 5000])
+def test_muon_step_few_rows(mx, top, long):
+    """Tables of matrices of few rows, of different sizes, in one workgroup each and in parts; buffers between guard values."""
+    shapes = [(top, top), (3, long), (long, top), (top - 3, 77), (1, 1), (9, 5), (5, 9), (long - 1, 2)]
+    matrices, at = [], 1
+    for r, c in shapes:
+        matrices.append((at, r, c))
+        at += r * c + 2
+    p, g, m, e = (randn(at, seed=i, scale=s) for i, s in enumerate((0.03, 1e-3, 1e-3, 0.03)))
+    for ema, nesterov in ((e, True), (None, False)):
+        rp, rm, re = muon64(p, g, m, ema, matrices, 0.01, 0.95, nesterov, 0.1, 0.7, 0.5)
+        p1, m1, e1 = p.clone(), m.clone(), None if ema is None else ema.clone()
+        mx.muon_step(p1, g, m1, matrices, lr=0.01, nesterov=nesterov, weight_decay=0.1, ema=e1, ema_decay=0.7, grad_scale=0.5)
+        inside = torch.zeros_like(p, dtype=torch.bool)
+        for o, r, c in matrices:
+            s = slice(o, o + r * c)
+            inside[s] = True
+            step = 0.01 * 0.2 * math.sqrt(r * c) * 1.25
+            allowed = LOOSE * step + 4 * 2.0 ** -24 * float(rp[s].norm())
+            assert float((p1[s].double() - rp[s]).norm()) <= allowed
+            assert float((m1[s].double() - rm[s]).abs().max()) <= 4 * 2.0 ** -24 * float(rm[s].abs().max())
+            if ema is not None:
+                assert float((e1[s].double() - re[s]).norm()) <= allowed + 4 * 2.0 ** -24 * float(re[s].norm())
+        for new, old in ((p1, p), (m1, m)) + (((e1, e),) if ema is not None else ()):
+            assert torch.equal(new[~inside], old[~inside])
 
 
 def test_muon_step_refuses(mx):
