@@ -383,9 +383,12 @@ int odamd_adam_ema_ranges_step(float* param, const float* grad, float* exp_avg, 
  *   X = G / (|G|_F + eps), transposed while rows > cols;
  *   `steps` times (1 .. 32):  A = X X^T,  X = a X + (b A + c A A) X,  (a, b, c) = (3.4445, -4.7750, 2.0315);
  *   out = X, transposed back.
- * Products carry 22 bits per factor and sum in float32, whatever dtype is; out is rounded once.  A matrix that holds a NaN
- * or an infinity gives NaN throughout, a zero matrix zeros.  Values of X under 2^-36 count as zero: a matrix whose norm lies
- * far under eps comes out as zero.  rows * cols is at most 2^31 - 2^16.  The workspace is 256-byte aligned. */
+ * Matrices whose shorter side is at most 64 are computed in 64 bits and rounded once (steps over 10: as the others).  The
+ * others' products carry 22 bits per factor and sum in float32; out is rounded once.  With a float32 result a rounding grows by
+ * 3.4445 per step in directions of small singular values, as in any float32 arithmetic of these formulas; with a bfloat16
+ * result steps run in groups of five on A alone, which costs up to 1e-3 of the result's norm there, half a bfloat16 step.
+ * A matrix that holds a NaN or an infinity gives NaN throughout, a zero matrix zeros (eps = 0: NaN).  The norm is held in 64
+ * bits.  Over 64 rows values of X under 2^-36 count as zero: a matrix whose norm lies far under eps comes out as zero.  rows * cols is at most 2^31 - 2^16.  The workspace is 256-byte aligned. */
 size_t odamd_orthogonalize_workspace_bytes(int batch, int rows, int cols);
 int odamd_orthogonalize(const void* x, void* out, int batch, int rows, int cols, int steps, double eps, int dtype,
                         void* workspace, size_t workspace_bytes, void* stream);
@@ -395,7 +398,8 @@ int odamd_orthogonalize(const void* x, void* out, int batch, int rows, int cols,
  *   m = momentum_decay m + grad_scale g;   u = nesterov ? grad_scale g + momentum_decay m : m;
  *   p = p (1 - lr weight_decay) - lr 0.2 sqrt(max(rows, cols)) O,   O = u orthogonalised as above;
  *   ema = ema_decay ema + (1 - ema_decay) p   where ema != NULL.
- * 0.2 sqrt(max(rows, cols)) gives the update the root mean square of an Adam step, so that one learning rate and one weight
+ * O is accurate to 1e-3 of its norm at least (the groups of five above; 64 bits where all matrices of up to 112 in a row have
+ * a side of at most 64).  0.2 sqrt(max(rows, cols)) gives the update the root mean square of an Adam step, so that one learning rate and one weight
  * decay serve both.  Elements outside the matrices are neither read nor written; matrices must not overlap.  The workspace
  * is 256-byte aligned. */
 typedef struct {

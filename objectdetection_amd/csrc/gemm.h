@@ -3,9 +3,9 @@
 //
 // Two operand forms, one data path:
 //   PL = 1: bf16 values, one v_mfma_f32_32x32x16_bf16 per 32 x 32 x 16 block;
-//   PL = 2: every value as a pair of fp16 numbers, v = (hi + lo) 2^-s; 32 hi and then their 32 lo lie side by side.  hi holds the upper 11 bits of v, lo the
-//           next 11, so hi_a hi_b + hi_a lo_b + lo_a hi_b (three v_mfma_f32_32x32x16_f16) carries a product to 2^-22, the
-//           dropped lo_a lo_b.  Float32 operands run at a third of the half-precision matrix rate this way, which is five
+//   PL = 2: every value as a pair of fp16 numbers, v = (hi + lo) 2^-s; 32 hi and then their 32 lo lie side by side.  hi holds
+//           the upper 11 bits of v, lo the next 11, so hi_a hi_b + hi_a lo_b + lo_a hi_b (three v_mfma_f32_32x32x16_f16)
+//           carries a product to 2^-22, the dropped lo_a lo_b.  Float32 operands run at a third of the half-precision matrix rate this way, which is five
 //           times the rate of the float32 matrix instructions; 2^s is a power of two, so it costs no rounding.  fp16
 //           has no more exponents than its scale gives it: the caller's scale keeps the largest value under 65504, and the
 //           smallest step, 2^-24, lies 2^-39 or less under it.

@@ -7,6 +7,9 @@
 // dx reduces over the outputs and dW over the rows: in bfloat16 the products read W, x and dz with the reduction along their
 // rows, out of the caller's tensors; float32 pairs need a power of two per column there, so that W, x and dz are laid out
 // by columns first (one launch for all three).
+// Times: (25600, 1024, 4096) bf16 with bias, SiLU and residual 285 us, 243 of them the product (a library product of that size
+// takes 206 us), the rest the epilogue's 420 MB; forward and backward of (8192, 1024, 4096) bf16 304 us; (4097, 1155, 1001)
+// float32 with GELU 66 us.  Few rows go without matrix instructions: (1, 1024, 1024) bf16 takes 3 us, a call of it 13 on the host.
 #include "common.h"
 #include "odamd.h"
 
@@ -196,7 +199,7 @@ __device__ __forceinline__ void lin_finish8(const LinEnd& p, long long i, int j,
     lin_finish8<DT, ACT>(p, i, j, cnt, v, bias, p.residual ? lin_raw8<DT>(p.residual, i * p.r_ld + j, cnt) : LinRaw<DT>{});
 }
 
-// ---- a few rows: one wave per output column, W read once from memory, no matrix instructions ------------------------
+// ---- a few rows: W read once from memory, no matrix instructions -----------------------------------------------------
 struct LinRow {
     const void* x;
     const void* w;
@@ -204,42 +207,67 @@ struct LinRow {
     int m, k, n;
     LinEnd end;
 };
+// A workgroup takes four output columns of up to eight rows.  One row: a wave per column.  More rows: COLS columns a wave, which
+// share the x it loads, and COLS waves share a column's reduction, so that as many waves read W.  What bounds it: reading W
+// (1 x 4096 x 4096 bf16 7.5 us, 4.5 TB/s; 8 x 8192 x 8192 26 us, 5.1 TB/s), with many rows the x and W that come out of the
+// caches again.  8 x 4096 x 4096 bf16 with 1 / 2 / 4 columns a wave: 15.7 / 11.0 / 10.6 us, in float32 30 / 22 / 18 us.
 template <int DT, int MR, bool WIDE>
 __global__ void __launch_bounds__(256) linear_rows_kernel(LinRow p) {
     using T = typename LinType<DT>::T;
-    constexpr int V = WIDE ? 16 / (int)sizeof(T) : 1;
-    const int lane = threadIdx.x & 63, col = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (col >= p.n) return;
-    const T* w = (const T*)p.w + col * p.w_ld;
-    const T* x = (const T*)p.x;
-    float acc[MR];
+    constexpr int V = WIDE ? 16 / (int)sizeof(T) : 1, COLS = MR < 4 ? MR : 4, N = MR * COLS;
+    __shared__ float part[4][N];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col0 = blockIdx.x * 4 + wave / COLS * COLS, row0 = blockIdx.y * MR;
+    // rows and columns past the last one are computed like the last one and not stored: all loads of a step go out together
+    const T *x[MR], *w[COLS];
 #pragma unroll
-    for (int i = 0; i < MR; ++i) acc[i] = 0.0f;
-    for (int k = lane * V; k < p.k; k += 64 * V) {
-        T wv[V];
-        if constexpr (WIDE) *(u32x4*)wv = *(const u32x4*)(w + k);
-        else wv[0] = w[k];
+    for (int i = 0; i < MR; ++i) x[i] = (const T*)p.x + min(row0 + i, p.m - 1) * p.x_ld;
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) w[c] = (const T*)p.w + min(col0 + c, p.n - 1) * p.w_ld;
+    float acc[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+    for (int k = (wave % COLS * 64 + lane) * V; k < p.k; k += 64 * V * COLS) {
+        T wv[COLS][V], xv[MR][V];
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+            if constexpr (WIDE) *(u32x4*)wv[c] = *(const u32x4*)(w[c] + k);
+            else wv[c][0] = w[c][k];
+        }
 #pragma unroll
         for (int i = 0; i < MR; ++i) {
-            if (i >= p.m) break;
-            T xv[V];
-            if constexpr (WIDE) *(u32x4*)xv = *(const u32x4*)(x + i * p.x_ld + k);
-            else xv[0] = x[i * p.x_ld + k];
-#pragma unroll
-            for (int e = 0; e < V; ++e) acc[i] = fmaf(LinType<DT>::get(xv[e]), LinType<DT>::get(wv[e]), acc[i]);
+            if constexpr (WIDE) *(u32x4*)xv[i] = *(const u32x4*)(x[i] + k);
+            else xv[i][0] = x[i][k];
         }
-    }
-    float mine = 0.0f;
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < MR; ++i) {
-        float s = acc[i];
+        for (int i = 0; i < MR; ++i)
 #pragma unroll
-        for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
-        mine = lane == i ? s : mine;
+            for (int c = 0; c < COLS; ++c)
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[c * MR + i] = fmaf(LinType<DT>::get(xv[i][e]), LinType<DT>::get(wv[c][e]), acc[c * MR + i]);
     }
-    if (lane < p.m) {
-        float v[8] = {mine};
-        lin_with_act(p.end.act, [&](auto act) { lin_finish8<DT, act.value>(p.end, lane, col, 1, v); });
+    // sums over the lanes: while there are several values, a lane hands half of them on and keeps the other half
+    int at = 0, o = 32;
+#pragma unroll
+    for (int half = N / 2; half >= 1; half /= 2, o >>= 1) {
+        const bool upper = lane & o;
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+            const float first = acc[i], second = acc[i + half];
+            acc[i] = (upper ? second : first) + __shfl_xor(upper ? first : second, o);
+        }
+        at = at * 2 + upper;
+    }
+    for (; o; o >>= 1) acc[0] += __shfl_xor(acc[0], o);
+    part[wave][at] = acc[0];                                // lanes of one value hold the same sum
+    __syncthreads();
+    const int c = threadIdx.x / MR, i = threadIdx.x % MR, col = blockIdx.x * 4 + c;
+    if (c < 4 && row0 + i < p.m && col < p.n) {
+        float v[8] = {};
+#pragma unroll
+        for (int s = 0; s < COLS; ++s) v[0] += part[c / COLS * COLS + s][c % COLS * MR + i];
+        lin_with_act(p.end.act, [&](auto act) { lin_finish8<DT, act.value>(p.end, row0 + i, col, 1, v); });
     }
 }
 
@@ -556,7 +584,7 @@ struct LinSpace {
 struct LinPlan { int tile, longest; };   // longest: chunks a workgroup takes at most
 // Tile and length of the parts the reductions are cut into, by the estimated time of the launch (`count` products).  A larger
 // tile wins per product; but a 256 x 256 tile fills its compute unit, nothing runs beside its epilogue, and all units reach
-// theirs together: (25600, 1024, 4096) with bias, SiLU and residual in bf16 takes 290 us in 256, 300 in 128 and 383 us in
+// theirs together: (25600, 1024, 4096) with bias, SiLU and residual in bf16 takes 285 us in 256, 300 in 128 and 383 us in
 // 64.  Where tiles leave units idle, or two products of a launch differ in length, parts of four chunks or more fill them,
 // for the price of a second launch that adds them up (4 us, and their bytes once out and once in).
 template <int DT>
@@ -662,15 +690,25 @@ int lin_tiles(LinJobs& t, int unit_rows) {
     return gemm_grid_ok(at, 256) ? (int)at : -1;
 }
 
-constexpr int LIN_ROWS = 8;   // up to this many rows the layer is read once for all of them, without matrix instructions
+// Whether a layer goes without matrix instructions: up to eight rows always (8 x 4096 x 4096 bf16 10.6 us, in products 13.7), more
+// where its workgroups are few.  Products cost a launch or two for laying operands out, the rows a step per eight of them;
+// rows / products, us: float32 512 x 256 x 256 (4096 workgroups) 9.2 / 10.6, 1024 x 256 x 256 15.7 / 11.3, 128 x 1024 x 1024
+// 13.5 / 18.1, 256 x 1024 x 1024 22.5 / 19.9, 32 x 4096 x 4096 46 / 55; bfloat16 read in place 128 x 256 x 256 (1024) 4.2 / 4.5,
+// 256 x 256 x 256 6.8 / 4.5, 64 x 1024 x 1024 8.3 / 7.8; bfloat16 laid out 64 x 513 x 1024 (2048) 7.0 / 8.9, 128 x 513 x 1024
+// 11.0 / 9.0.
+template <int DT>
+bool lin_by_rows(int m, int n, bool direct) {
+    const long long blocks = ((m + 7LL) / 8) * ((n + 3LL) / 4);
+    return m <= 8 || blocks <= (DT == ODAMD_DTYPE_F32 ? 4096 : direct ? 1024 : 2048);
+}
 
 template <int DT>
 int lin_forward_rows(const odamd_linear_desc& d, const LinEnd& end, hipStream_t s) {
     constexpr int V = DT == ODAMD_DTYPE_F32 ? 4 : 8;
     const bool wide = (((uintptr_t)d.x | (uintptr_t)d.w) & 15) == 0 && d.x_ld % V == 0 && d.w_ld % V == 0 && d.k % V == 0;
     const LinRow p = {d.x, d.w, d.x_ld, d.w_ld, d.m, d.k, d.n, end};
-    const int blocks = (d.n + 3) / 4;
-    if (!gemm_grid_ok(blocks, 256)) return ODAMD_E_LIMIT;
+    const dim3 blocks((d.n + 3) / 4, (d.m + 7) / 8);
+    if (!gemm_grid_ok(blocks.x, 256)) return ODAMD_E_LIMIT;
 #define ODAMD_ROWS(MR) (wide ? linear_rows_kernel<DT, MR, true><<<blocks, 256, 0, s>>>(p) : linear_rows_kernel<DT, MR, false><<<blocks, 256, 0, s>>>(p))
     if (d.m == 1) ODAMD_ROWS(1);
     else if (d.m == 2) ODAMD_ROWS(2);
@@ -684,7 +722,9 @@ int lin_forward_rows(const odamd_linear_desc& d, const LinEnd& end, hipStream_t 
 template <int DT>
 int lin_forward(const odamd_linear_desc& d, LinSpace& ws, bool go, hipStream_t s) {
     const LinEnd end = {d.bias, d.residual, d.y, d.z, d.r_ld, d.y_ld, d.z_ld, d.act};
-    if (d.m <= LIN_ROWS) return go ? lin_forward_rows<DT>(d, end, s) : 0;
+    // measuring, the pointers are not known: the workspace of products serves where only they may say
+    const bool direct = !go || (lin_direct<DT>(d.x, d.x_ld, d.k) && lin_direct<DT>(d.w, d.w_ld, d.k));
+    if (lin_by_rows<DT>(d.m, d.n, direct)) return go ? lin_forward_rows<DT>(d, end, s) : 0;
     constexpr int SIZE = DT == ODAMD_DTYPE_F32 ? 4 : 2;
     LinLaunch launch = {};
     LinGemm& g = launch.g[0];

@@ -10,18 +10,25 @@
 //   X_t = Q X_0,   Q = P_t ... P_1,   A_(k+1) = P_k A_k P_k
 // with one product by X at the end of a phase of t steps: 1.5 m^2 n + (2 t - 1.5) m^3 multiply-adds for it (symmetric products
 // counted half) against t (1.5 m^2 n + 0.5 m^3).  What it costs is accuracy in the directions of small singular values: a
-// rounding of A grows by 3.4445^2 per step there, where a rounding of X grows by 3.4445.  Phases of two steps keep float32's
-// accuracy (error against 64 bits of 256 x 2304 noise with strong directions: 1.6e-6, one step a phase 1.9e-6) and serve
-// float32 results of matrices with n >= 2 m; squarer ones take one step a phase, which costs no more there.  Phases of
-// five serve bfloat16 results and the optimizer step: 3e-6 to 8e-5 on such matrices, under 8e-4 (3.4445^8 2^-24 = 1.2e-3)
-// where the singular values fall like 1 / i^2 or vanish; a bfloat16 result is rounded by 2e-3 and the step multiplies by the
-// learning rate.
+// rounding of A grows by 3.4445^2 per step there, where a rounding of X grows by 3.4445.
+//   - At most 64 rows: A and all that follows in 64 bits, up to ten steps in one phase (further down: "at most 64 rows").
+//   - More rows, float32 results: phases of two steps, which keep float32's accuracy (error against 64 bits of 256 x 2304 noise
+//     with strong directions: 1.6e-6, one step a phase 1.9e-6), where n >= 2 m; one step a phase on squarer ones, which costs no
+//     more there.
+//   - More rows, bfloat16 results and the optimizer step: phases of five.  3e-6 to 8e-5 on such matrices, under 8e-4
+//     (3.4445^8 2^-24 = 1.2e-3) where the singular values fall like 1 / i^2 or vanish; a bfloat16 result is rounded by 2e-3,
+//     and the step multiplies by the learning rate.
 //
-// All products run on fp16 pairs (gemm.h, PL = 2) scaled by 2^12 (Q, which grows to 3.4445^k, by less): the largest entry
-// becomes 14 300, the smallest step 2^-36.  bf16 products would leave a few percent in the result.
+// The products of more rows run on fp16 pairs (gemm.h, PL = 2) scaled by 2^12 (Q, which grows to 3.4445^k, by less): the largest
+// entry becomes 14 300, the smallest step 2^-36.  bf16 products would leave a few percent in the result.
 // X is kept twice, by rows (X X^T reduces along n) and by columns (Q X reduces along m): both products then read their
 // operands along the reduction.  The m x m matrices are symmetric: tiles on and over the diagonal are computed, the rest
 // mirrored.  All matrices of a call share every launch.
+//
+// Eight 256 x 2304 in float32 take 195 us: 20 launches of 5 to 20 us, each a chain of a few latencies.  A step over the 94
+// matrices of the detector's largest preset takes 4.6 ms: 3.8 ms of products at 55 % of the matrix rate of a large library
+// product (tiles on the diagonal compute both halves; 128 x 128 tiles are bound by LDS reads and matrix instructions alike) and
+// 0.73 ms of norm and layout at the rate of a copy.
 #include "common.h"
 #include "odamd.h"
 

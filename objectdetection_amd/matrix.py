@@ -143,7 +143,8 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     """act(x W^T + bias) + residual in one product.  x: (..., k); weight: (n, k); bias: (n,); residual: (..., n); all of one
     type, float32 or bfloat16.  activation: None, 'silu', 'gelu' (the erf form) or 'relu'.  Rows may be strided (a slice of a
     wider, concatenated buffer is read in place).  Differentiable once in all four tensors; in bfloat16 the pre-activation
-    that the backward pass keeps, and the gradient at it, are bfloat16.  float32 products carry 22 bits per value, counted
+    that the backward pass keeps, and the gradient at it, are bfloat16.  As with every differentiable torch operation, a backward
+    pass is captured into a graph on leaves that no eager graph holds any more (detached copies of them will do).  float32 products carry 22 bits per value, counted
     from the largest magnitude of its row; a float32 row with an infinity gives NaN or infinity."""
     if activation not in ACTIVATIONS:
         raise ValueError(f'activation {activation!r}: one of {list(ACTIVATIONS)}')
@@ -184,8 +185,10 @@ def linear(x, weight, bias=None, activation=None, residual=None):
 def orthogonalize(x, steps=5, eps=1e-7, out=None):
     """Brings the singular values of every matrix of x (..., rows, cols) near one and keeps its singular vectors: `steps`
     Newton-Schulz products with the coefficients (3.4445, -4.7750, 2.0315) from x / (|x|_F + eps) on.  Five steps take
-    singular values from 0.003 of the norm up to between 0.68 and 1.21.  float32 or bfloat16; the products carry 22 bits
-    either way, the result is rounded once.  `out` may be x itself.  A matrix with a NaN or an infinity gives NaN."""
+    singular values from 0.003 of the norm up to between 0.68 and 1.21.  float32 or bfloat16, rounded once.  Matrices with a side
+    of at most 64 are computed in 64 bits, others with products of 22 bits; bfloat16 results of those are off by up to 1e-3 of
+    their norm in directions of small singular values (half a bfloat16 step).  `out` may be x itself.  Not differentiable: the
+    result belongs to no graph.  A matrix with a NaN or an infinity gives NaN."""
     _check_tensor('x', x)
     if x.dim() < 2:
         raise ValueError(f'x must have rows and columns, not shape {tuple(x.shape)}')

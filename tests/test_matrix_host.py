@@ -49,9 +49,10 @@ def test_workspaces_are_asked_for_and_checked():
     assert lib.odamd_linear_forward(None, None, 0, None) == E_ARG
     assert lib.odamd_linear_backward(None, None, 0, None) == E_ARG
     assert lib.odamd_linear_workspace_bytes(C.byref(_desc(m=1))) == 0              # read in place, no workspace
-    d = _desc(dtype=0, x_ld=64, w_ld=64)
+    assert lib.odamd_linear_workspace_bytes(C.byref(_desc(dtype=0))) == 0          # so are few workgroups
+    d = _desc(dtype=0, m=40000)
     need = lib.odamd_linear_workspace_bytes(C.byref(d))
-    assert need >= (16 + 32) * 64 * 4
+    assert need >= (40000 + 32) * 64 * 4
     assert lib.odamd_linear_forward(C.byref(d), P, need - 1, None) == E_WORKSPACE
     assert lib.odamd_linear_forward(C.byref(d), None, need, None) == E_ARG
     assert lib.odamd_linear_forward(C.byref(d), P + 64, need, None) == E_ALIGN
