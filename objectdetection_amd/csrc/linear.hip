@@ -899,7 +899,7 @@ int lin_backward(const odamd_linear_grad_desc& d, LinSpace& ws, bool go, hipStre
     return d.dtype == ODAMD_DTYPE_F32 ? lin_backward_f32(d, ws, go, s) : lin_backward_bf16(d, ws, go, s);
 }
 
-constexpr long long LIN_MAX = 0x7fffffffLL - 1024;
+constexpr long long LIN_MAX = 0x7fff0000LL;   // 2^31 less what an index passes its end by
 bool lin_sizes_ok(int m, int k, int n, int act, int dtype) {
     return m >= 1 && k >= 1 && n >= 1 && m <= LIN_MAX && k <= LIN_MAX && n <= LIN_MAX && act >= ODAMD_ACT_NONE && act <= ODAMD_ACT_RELU
            && (dtype == ODAMD_DTYPE_F32 || dtype == ODAMD_DTYPE_BF16);

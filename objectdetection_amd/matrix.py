@@ -14,8 +14,7 @@ from ._lib import lib, check
 ACTIVATIONS = {None: 0, 'silu': 1, 'gelu': 2, 'relu': 3}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 MATRIX_DTYPE = np.dtype([('offset', '<i8'), ('rows', '<i4'), ('cols', '<i4')])      # odamd_matrix
-_MOST = 2 ** 31 - 1025                                                               # rows, columns, matrices of a call
-_ELEMENTS = 2 ** 31 - 2 ** 16                                                        # elements of a matrix
+_MOST = 2 ** 31 - 2 ** 16                                       # rows, columns and matrices of a call, elements of a matrix
 RANGE_DTYPE = np.dtype([('offset', '<i8'), ('len', '<i8')])                         # odamd_range
 
 
@@ -195,8 +194,8 @@ def orthogonalize(x, steps=5, eps=1e-7, out=None):
     if not 1 <= int(steps) <= 32 or not eps >= 0:
         raise ValueError('steps must be 1 to 32, eps must not be negative')
     rows, cols = x.shape[-2:]
-    if rows * cols > _ELEMENTS or x.shape[:-2].numel() > _MOST:
-        raise ValueError(f'a matrix has at most {_ELEMENTS} elements, a batch at most {_MOST} matrices')
+    if rows * cols > _MOST or x.shape[:-2].numel() > _MOST:
+        raise ValueError(f'at most {_MOST} elements of a matrix and matrices')
     if out is None:
         out = x.new_empty(x.shape)
     else:
@@ -220,8 +219,8 @@ class MatrixTable:
     def __init__(self, matrices):
         a = np.asarray(list(matrices), dtype=np.int64).reshape(-1, 3)
         size = a[:, 1] * a[:, 2]
-        if len(a) == 0 or (a[:, 0] < 0).any() or (a[:, 1:] < 1).any() or (a[:, 1:] >= 2 ** 31).any() or (size > _ELEMENTS).any():
-            raise ValueError(f'matrices: at least one (offset, rows, cols), offsets from 0, sizes from 1, at most {_ELEMENTS} elements each')
+        if len(a) == 0 or (a[:, 0] < 0).any() or (a[:, 1:] < 1).any() or (a[:, 1:] >= 2 ** 31).any() or (size > _MOST).any():
+            raise ValueError(f'matrices: at least one (offset, rows, cols), offsets from 0, sizes from 1, at most {_MOST} elements each')
         order = np.argsort(a[:, 0], kind='stable')
         ends = (a[:, 0] + size)[order]
         if (a[order, 0][1:] < ends[:-1]).any():
@@ -257,6 +256,7 @@ def muon_step(param, grad, momentum, matrices, lr, momentum_decay=0.95, nesterov
 
     `matrices`: [(offset, rows, cols)] or a MatrixTable of them.  What lies between the matrices is not touched."""
     table = matrices if isinstance(matrices, MatrixTable) else MatrixTable(matrices)
+    _check_tensor('param', param)
     for name, t in (('param', param), ('grad', grad), ('momentum', momentum), ('ema', ema)):
         if t is None and name == 'ema':
             continue

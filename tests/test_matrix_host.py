@@ -29,7 +29,7 @@ def _grad_desc(**kw):
 
 @pytest.mark.parametrize('change, code', [
     (dict(x=None), E_ARG), (dict(w=None), E_ARG), (dict(y=None), E_ARG), (dict(m=0), E_ARG), (dict(k=0), E_ARG),
-    (dict(n=-1), E_ARG), (dict(act=4), E_ARG), (dict(act=-1), E_ARG), (dict(dtype=2), E_ARG), (dict(m=2 ** 31 - 1), E_ARG),
+    (dict(n=-1), E_ARG), (dict(act=4), E_ARG), (dict(act=-1), E_ARG), (dict(dtype=2), E_ARG), (dict(m=2 ** 31 - 1), E_ARG), (dict(k=2 ** 31 - 2 ** 15, x_ld=2 ** 31, w_ld=2 ** 31), E_ARG),
     (dict(x_ld=63), E_SHAPE), (dict(w_ld=63), E_SHAPE), (dict(y_ld=31), E_SHAPE), (dict(residual=P, r_ld=31), E_SHAPE),
     (dict(z=P, z_ld=31), E_SHAPE), (dict(x=P + 1), E_ALIGN), (dict(dtype=0, w=P + 2), E_ALIGN), (dict(bias=P + 1), E_ALIGN)])
 def test_linear_forward_refuses(change, code):
@@ -125,8 +125,9 @@ def test_python_refuses_what_does_not_fit():
         matrix.linear(x, w, activation='tanh')
     with pytest.raises(ValueError, match='CUDA'):
         matrix.orthogonalize(x)
-    with pytest.raises(ValueError, match='CUDA'):
-        matrix.muon_step(x, x, x, [(0, 4, 8)], 0.1)
+    for p in (x, None):
+        with pytest.raises(ValueError, match='CUDA'):
+            matrix.muon_step(p, x, x, [(0, 4, 8)], 0.1)
     from objectdetection_amd.model import layer
     with pytest.raises(ValueError, match='activation'):
         layer.linear(8, 6, act='tanh')
