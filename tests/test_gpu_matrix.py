@@ -126,7 +126,7 @@ def test_linear_activations(mx, act, dtype):
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
-@pytest.mark.parametrize('m, k, n', [(2100, 264, 2050), (4000, 96, 4100), (50, 4000, 72)])
+@pytest.mark.parametrize('m, k, n', [(2100, 264, 2050), (4000, 96, 4100), (50, 4000, 72), (4097, 300, 1001), (2056, 520, 2000)])
 def test_linear_tiles_and_split(mx, m, k, n, dtype):
     """Sizes that reach the 128 and 256 wide tiles and the split reduction, ragged in every direction."""
     x, w = randn(m, k, dtype=dtype), randn(n, k, seed=1, dtype=dtype, scale=k ** -0.5)
