@@ -412,9 +412,10 @@ int odamd_muon_ema_step(float* param, const float* grad, float* momentum, float*
                         double eps, double ema_decay, double grad_scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Dense layer with its epilogue in one product: y = act(x W^T + b) + r.  x: m rows of k values, x_ld elements apart; w: n rows
- * of k; bias: n values or NULL; residual, y, z: m rows of n.  All of them of `dtype`, rows contiguous, row strides in elements
- * and at least the row's length.  z != NULL also receives x W^T + b, which the backward pass of an activation needs.  r may be
- * y itself; no other operand may overlap an output.  Sums are float32 and y is rounded once; float32 products carry 22 bits
+ * of k; bias: n values or NULL; residual, y, z: m rows of n.  All of them but z of `dtype`, rows contiguous, row strides in
+ * elements and at least the row's length.  z != NULL also receives x W^T + b, which the backward pass of an activation needs: in
+ * float32, or where `dtype` is bfloat16 in float16 (past its range an infinity, and with ODAMD_ACT_RELU its smallest positive
+ * number for a smaller one).  r may be y itself; no other operand may overlap an output.  Sums are float32 and y is rounded once; float32 products carry 22 bits
  * of each value, counted from the largest magnitude of its row of x or w down to 2^-17 of it and with the same absolute
  * step below.  A float32 row that holds an infinity gives NaN or infinity.  m, k and n are at most 2^31 - 2^16.
  * The workspace (256-byte aligned) may be NULL where the query returns 0. */

@@ -3,7 +3,7 @@
 //   dz = dy act'(z),  z = x W^T + b;   dx = dz W,   dW = dz^T x,   db = column sums of dz   (dr = dy, the caller's own)
 // bfloat16 operands run on bf16 matrix instructions as they are; float32 operands as fp16 pairs (gemm.h) with a power of
 // two per row of each operand, so that a row's largest value sits just under 2^15: 22 bits per value down to 2^-17 of the row's
-// largest, and the same absolute step below.  Sums are float32, z and dz are kept in the operands' type.
+// largest, and the same absolute step below.  Sums are float32; dz is kept in the operands' type, z in float32 or, beside bfloat16, in float16.
 // dx reduces over the outputs and dW over the rows: in bfloat16 the products read W, x and dz with the reduction along their
 // rows, out of the caller's tensors; float32 pairs need a power of two per column there, so that W, x and dz are laid out
 // by columns first (one launch for all three).
@@ -167,12 +167,55 @@ __device__ __forceinline__ void lin_values(const LinRaw<ODAMD_DTYPE_BF16>& r, fl
 #pragma unroll
     for (int e = 0; e < 4; ++e) { v[2 * e] = __uint_as_float(r.a[e] << 16); v[2 * e + 1] = __uint_as_float(r.a[e] & 0xffff0000u); }
 }
+// The pre-activation for the backward pass.  Beside bfloat16 it is kept in float16: three bits more for the slope, at the same
+// size (with bfloat16 dW of 4197 rows is 1.45 times as far off as the rounding of its result alone, with float16 1.39: what dz's
+// rounding leaves); beyond float16's range every activation is straight, so the end of the range stands for an infinity, and a
+// positive value under it stays positive where relu asks for the sign.
+template <int DT, int ACT>
+__device__ __forceinline__ void lin_store_z8(void* base, long long at, int cnt, const float v[8]) {
+    if constexpr (DT == ODAMD_DTYPE_F32) {
+        lin_store8<DT>(base, at, cnt, v);
+    } else {
+        _Float16* d = (_Float16*)base + at;
+        f16x8_t u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = (_Float16)(ACT == ODAMD_ACT_RELU && v[e] > 0.0f ? fmaxf(v[e], 0x1p-24f) : v[e]);
+        if (cnt == 8) {
+            *(u32x4_any*)d = __builtin_bit_cast(u32x4, u);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < cnt) d[e] = u[e];
+        }
+    }
+}
+template <int DT>
+__device__ __forceinline__ void lin_load_z8(const void* base, long long at, int cnt, float v[8]) {
+    if constexpr (DT == ODAMD_DTYPE_F32) {
+        lin_load8<DT>(base, at, cnt, v);
+    } else {
+        const _Float16* s = (const _Float16*)base + at;
+        f16x8_t u = {};
+        if (cnt == 8) {
+            u = __builtin_bit_cast(f16x8_t, *(const u32x4_any*)s);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < cnt) u[e] = s[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float z = (float)u[e];
+            v[e] = fabsf(z) > 65504.0f ? copysignf(65504.0f, z) : z;
+        }
+    }
+}
 // Row i, columns j .. j + cnt - 1 (cnt <= 8): bias[8] and the residual's values are there already
 template <int DT, int ACT>
 __device__ __forceinline__ void lin_finish8(const LinEnd& p, long long i, int j, int cnt, float v[8], const float bias[8], const LinRaw<DT>& residual) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += bias[e];
-    if (p.z) lin_store8<DT>(p.z, i * p.z_ld + j, cnt, v);
+    if (p.z) lin_store_z8<DT, ACT>(p.z, i * p.z_ld + j, cnt, v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = lin_act<DT == ODAMD_DTYPE_BF16, ACT>(v[e]);
     if (p.residual) {
@@ -305,7 +348,7 @@ __device__ __forceinline__ void lin_values8(const LinJob& p, int i, int j, float
     lin_load8<DT>(p.src, i * p.ld + j, cnt, v);
     if (p.z) {
         float z[8];
-        lin_load8<DT>(p.z, i * p.z_ld + j, cnt, z);
+        lin_load_z8<DT>(p.z, i * p.z_ld + j, cnt, z);
         lin_with_act(p.act, [&](auto act) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = lin_grad<DT == ODAMD_DTYPE_BF16, act.value>(v[e], z[e]);

@@ -13,6 +13,7 @@ from ._lib import lib, check
 
 ACTIVATIONS = {None: 0, 'silu': 1, 'gelu': 2, 'relu': 3}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_Z_DTYPES = {torch.float32: torch.float32, torch.bfloat16: torch.float16}         # the pre-activation kept for the backward pass
 MATRIX_DTYPE = np.dtype([('offset', '<i8'), ('rows', '<i4'), ('cols', '<i4')])      # odamd_matrix
 _MOST = 2 ** 31 - 2 ** 16                                       # rows, columns and matrices of a call, elements of a matrix
 RANGE_DTYPE = np.dtype([('offset', '<i8'), ('len', '<i8')])                         # odamd_range
@@ -81,7 +82,7 @@ def _linear_forward(x, weight, bias, residual, act, keep_z):
     m, k = x.shape
     n = weight.shape[0]
     y = x.new_empty((m, n))
-    z = x.new_empty((m, n)) if keep_z else None
+    z = x.new_empty((m, n), dtype=_Z_DTYPES[x.dtype]) if keep_z else None
     d = _lib.LinearDesc(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(z), _ld(x),
                         _ld(weight), 0 if residual is None else _ld(residual), n, n, m, k, n, act, _DTYPES[x.dtype])
     size = lib.odamd_linear_workspace_bytes(d)
@@ -142,7 +143,7 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     """act(x W^T + bias) + residual in one product.  x: (..., k); weight: (n, k); bias: (n,); residual: (..., n); all of one
     type, float32 or bfloat16.  activation: None, 'silu', 'gelu' (the erf form) or 'relu'.  Rows may be strided (a slice of a
     wider, concatenated buffer is read in place).  Differentiable once in all four tensors; in bfloat16 the pre-activation
-    that the backward pass keeps, and the gradient at it, are bfloat16.  As with every differentiable torch operation, a backward
+    that the backward pass keeps is float16 and the gradient at it bfloat16.  As with every differentiable torch operation, a backward
     pass is captured into a graph on leaves that no eager graph holds any more (detached copies of them will do).  float32 products carry 22 bits per value, counted
     from the largest magnitude of its row; a float32 row with an infinity gives NaN or infinity."""
     if activation not in ACTIVATIONS:

@@ -213,6 +213,33 @@ def test_linear_only_wanted_gradients(mx):
         assert torch.equal(got, full[i])
 
 
+def test_linear_keeps_the_slope_of_large_values(mx):
+    """Pre-activations past float16's range: every activation is straight there, slopes are 0 and 1."""
+    for dtype in (torch.float32, torch.bfloat16):
+        x, w = randn(24, 8, dtype=dtype).abs() + 1, randn(40, 8, seed=1, dtype=dtype).abs() + 1
+        w[::2] = -w[::2]
+        x = (x * 2.0 ** 17).requires_grad_()
+        dy = randn(24, 40, seed=2, dtype=dtype)
+        for act in ('silu', 'gelu', 'relu'):
+            dx, = torch.autograd.grad(mx.linear(x, w, None, act), x, dy)
+            open_ = dy.clone()
+            open_[:, ::2] = 0
+            ref = open_.double() @ w.double()
+            close(dx, ref, product_bound(open_.double(), w.double().t().contiguous(), dtype), dtype)
+
+
+def test_linear_relu_at_any_scale(mx):
+    """relu asks for the sign of the smallest pre-activations too."""
+    for dtype in (torch.float32, torch.bfloat16):
+        for m in (6, 3000):
+            x, w, dy = randn(m, 24, dtype=dtype), randn(40, 24, seed=1, dtype=dtype), randn(m, 40, seed=2, dtype=dtype)
+            grads = []
+            for scale in (1.0, 2.0 ** -30):
+                leaf = (x * scale).requires_grad_()
+                grads.append(torch.autograd.grad(mx.linear(leaf, w * 2.0 ** -8, None, 'relu'), leaf, dy)[0])
+            assert torch.equal(*grads)
+
+
 def test_linear_relu_closes_the_gradient(mx):
     """Where relu is closed nothing passes, an infinity neither; other rows and columns do not see it."""
     for dtype in (torch.float32, torch.bfloat16):
