@@ -491,6 +491,125 @@ __global__ void __launch_bounds__(256) linear_lay_rows_kernel(LinJobs t) {
     }
 }
 
+// ---- the backward pass of a small layer in one launch, without matrix instructions ------------------------------------
+// Both gradients are sums of rows of V with coefficients out of dz: dx[i] = sum_r dz[i][r] W[r], dw[i] = sum_r dz[r][i] x[r].  A
+// workgroup takes eight rows of a result and 64 of its columns (a column a lane: four a lane leave too few workgroups, 64 x 64 x 64
+// 5.7 us instead of 4.2); its waves share the sum, 16 terms each at a time, and add up in LDS.  dz stays in float32 and is in nobody's
+// memory: every workgroup makes the eight rows or columns of it that it needs.  Bound by latency in the few workgroups of a small
+// layer, by the vector unit in more.  Eight waves for float32, sixteen for bfloat16, whose loads bring half as much (78 x 225 of
+// 40 rows: 5.7 us, with eight 7.8).
+struct LinSmall {
+    const void* dy;
+    const void* z;
+    const void* v[2];        // W, x
+    void* out[2];            // dx, dw
+    void* db;
+    long long dy_ld, z_ld, v_ld[2], out_ld[2];
+    int m, k, n;
+    int block1;              // blocks of dx
+};
+template <int DT> __host__ __device__ constexpr int lin_small_threads() { return DT == ODAMD_DTYPE_F32 ? 512 : 1024; }
+template <int DT> __host__ __device__ constexpr int lin_small_terms() { return lin_small_threads<DT>() / 4; }
+
+template <int DT, int ACT>
+__global__ void __launch_bounds__(lin_small_threads<DT>()) linear_small_backward_kernel(LinSmall p) {
+    using T = typename LinType<DT>::T;
+    constexpr int THREADS = lin_small_threads<DT>(), TERMS = lin_small_terms<DT>(), WAVES = THREADS / 64, SHARE = TERMS / WAVES;
+    __shared__ __attribute__((aligned(16))) float coef[2][TERMS][8];
+    __shared__ float joined[4][8][64];
+    __shared__ double bias[WAVES][8];
+    const int which = (int)blockIdx.x >= p.block1, block = blockIdx.x - (which ? p.block1 : 0);
+    const int rows = which ? p.n : p.m, terms = which ? p.m : p.n, across = (p.k + 63) / 64;
+    const int i0 = block / across * 8, c0 = block % across * 64;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = c0 + lane;
+    const bool some = p.out[which] != nullptr, sum = which && p.db && c0 == 0;
+    const T* v = (const T*)p.v[which];
+    // two coefficients a thread, along the rows of dz: result row and term of each
+    const auto place = [&](int q, int& i, int& r) {
+        i = which ? threadIdx.x & 7 : (int)threadIdx.x / TERMS + 4 * q;
+        r = which ? (int)threadIdx.x / 8 + TERMS / 2 * q : threadIdx.x % TERMS;
+    };
+    const auto fetch = [&](int r0, float to[2]) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            int i, r;
+            place(q, i, r);
+            to[q] = 0.0f;
+            if (i0 + i < rows && r0 + r < terms) {
+                const long long y = which ? r0 + r : i0 + i;     // row and column of dz
+                const int x = which ? i0 + i : r0 + r;
+                const float dy = LinType<DT>::get(((const T*)p.dy)[y * p.dy_ld + x]);
+                float z[8] = {};
+                if constexpr (ACT != ODAMD_ACT_NONE) lin_load_z8<DT>(p.z, y * p.z_ld + x, 1, z);
+                to[q] = lin_grad<DT == ODAMD_DTYPE_BF16, ACT>(dy, z[0]);
+            }
+        }
+    };
+    float acc[8] = {};
+    double total = 0.0;
+    float next[2];
+    fetch(0, next);
+    for (int r0 = 0, turn = 0; r0 < terms; r0 += TERMS, turn ^= 1) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            int i, r;
+            place(q, i, r);
+            coef[turn][r][i] = next[q];
+        }
+        __syncthreads();                                         // one a round: the other buffer is written two rounds on
+        if (r0 + TERMS < terms) fetch(r0 + TERMS, next);
+        const int from = wave * SHARE;
+        if (some && c < p.k) {
+            // terms past the last one have zero coefficients, and the last one's row made zeros (it may hold no number)
+            float x[SHARE];
+#pragma unroll
+            for (int s = 0; s < SHARE; ++s) {
+                const float u = LinType<DT>::get(v[min(r0 + from + s, terms - 1) * p.v_ld[which] + c]);
+                x[s] = r0 + from + s < terms ? u : 0.0f;
+            }
+#pragma unroll
+            for (int s = 0; s < SHARE; ++s) {
+                const f32x4_t a = *(const f32x4_t*)coef[turn][from + s], b = *(const f32x4_t*)(coef[turn][from + s] + 4);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i] = fmaf(i < 4 ? a[i & 3] : b[i & 3], x[s], acc[i]);
+            }
+        }
+        if (sum) {
+#pragma unroll
+            for (int s = 0; s < SHARE / 8; ++s) total += coef[turn][from + (lane >> 3) * (SHARE / 8) + s][lane & 7];
+        }
+    }
+    // four waves at a time add their sums to what the ones before left
+#pragma unroll
+    for (int g = 0; g < WAVES / 4; ++g) {
+        if (wave / 4 == g)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float& at = joined[wave % 4][i][lane];
+                at = g == 0 ? acc[i] : at + acc[i];
+            }
+        __syncthreads();
+    }
+    if (sum) {
+#pragma unroll
+        for (int o = 8; o < 64; o <<= 1) total += __shfl_xor(total, o);
+        if (lane < 8) bias[wave][lane] = total;
+        __syncthreads();
+    }
+    const int i = threadIdx.x >> 6;
+    if (some && i < 8 && i0 + i < rows && c < p.k) {
+        float s = joined[0][i][lane];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) s += joined[w][i][lane];
+        ((T*)p.out[which])[(i0 + i) * p.out_ld[which] + c] = LinType<DT>::put(s);
+    }
+    if (sum && threadIdx.x < 8 && i0 + (int)threadIdx.x < rows) {
+        double s = bias[0][threadIdx.x];
+        for (int w = 1; w < WAVES; ++w) s += bias[w][threadIdx.x];
+        ((T*)p.db)[i0 + threadIdx.x] = LinType<DT>::put((float)s);
+    }
+}
+
 // ---- the products ----------------------------------------------------------------------------------------------------
 struct LinGemm {
     GemmOperand a, b;
@@ -624,7 +743,7 @@ struct LinSpace {
     }
 };
 
-struct LinPlan { int tile, longest; };   // longest: chunks a workgroup takes at most
+struct LinPlan { int tile, longest; double us; };   // longest: chunks a workgroup takes at most
 // Tile and length of the parts the reductions are cut into, by the estimated time of the launch (`count` products).  A larger
 // tile wins per product; but a 256 x 256 tile fills its compute unit, nothing runs beside its epilogue, and all units reach
 // theirs together: (25600, 1024, 4096) with bias, SiLU and residual in bf16 takes 285 us in 256, 300 in 128 and 383 us in
@@ -637,7 +756,7 @@ LinPlan lin_plan(const LinGemm* g, int count) {
         const int chunks = (g[q].k_len + lin_chunk<DT>() - 1) / lin_chunk<DT>();
         all = chunks > all ? chunks : all;
     }
-    LinPlan best = {64, all};
+    LinPlan best = {64, all, 0.0};
     if (count == 0) return best;
     double least = -1.0;
     for (int tile : {64, 128, 256})
@@ -653,7 +772,7 @@ LinPlan lin_plan(const LinGemm* g, int count) {
             }
             const double us = gemm_time_us(tile, load, DT == ODAMD_DTYPE_F32, DT == ODAMD_DTYPE_F32 ? 8.0 : 4.0) + extra;
             if (least < 0.0 || us < least) {
-                best = {tile, longest};
+                best = {tile, longest, us};
                 least = us;
             }
         }
@@ -938,8 +1057,51 @@ int lin_backward_f32(const odamd_linear_grad_desc& d, LinSpace& ws, bool go, hip
     return lin_products<DT, true>(t.launch, t.count, ws, go, s);
 }
 
+// Whether the backward pass goes that way: by its estimated time, measured as 2.4 us, 2 us (bfloat16: 3) for every step of 128
+// (256) terms of the longest sum, or 4.5 (9) ns for every step of any workgroup; products with what lies before them take
+// launches of 13.5 us in float32 (three more of them), of 6 us in bfloat16.  Small / products, us, rows x inputs x outputs: float32
+// 8 x 64 x 64 4.1 / 14.5, 512 x 64 x 64 10.4 / 21, 1024 x 64 x 64 18 / 23, 128 x 996 x 424 13 / 22, 256 x 1024 x 1024 41 / 33;
+// bfloat16 40 x 78 x 225 5.7 / 9.0, 256 x 256 x 256 6.4 / 8.7, 512 x 256 x 256 11.4 / 10.3, 8 x 996 x 424 13 / 9.3.
+template <int DT>
+bool lin_small(const odamd_linear_grad_desc& d) {
+    constexpr bool F32 = DT == ODAMD_DTYPE_F32;
+    constexpr int TERMS = lin_small_terms<DT>();
+    const double across = (d.k + 63) / 64;
+    double longest = 0.0, total = 0.0;
+    LinGemm g[2] = {};
+    int count = 0;
+    const auto add = [&](int rows, int terms, bool product) {
+        const double steps = (terms + TERMS - 1) / TERMS;
+        longest = steps > longest ? steps : longest;
+        total += (rows + 7) / 8 * across * steps;
+        if (!product) return;
+        g[count].m = rows;
+        g[count].n = d.k;
+        g[count++].k_len = terms;
+    };
+    if (d.dx) add(d.m, d.n, true);
+    if (d.dw || d.db) add(d.n, d.m, d.dw);
+    const double chain = (F32 ? 2.0 : 3.0) * longest, all = (F32 ? 2.0 : 3.0) + (F32 ? 4.5e-3 : 9e-3) * total;
+    return 2.4 + (chain > all ? chain : all) < lin_plan<DT>(g, count).us + (F32 ? 13.5 : 6.0);
+}
+template <int DT>
+int lin_small_backward(const odamd_linear_grad_desc& d, hipStream_t s) {
+    const long long across = (d.k + 63) / 64, block1 = d.dx ? (d.m + 7) / 8 * across : 0;
+    const long long blocks = block1 + (d.dw || d.db ? (d.n + 7) / 8 * across : 0);
+    if (!gemm_grid_ok(blocks, lin_small_threads<DT>())) return ODAMD_E_LIMIT;
+    const LinSmall p = {d.dy, d.z, {d.w, d.x}, {d.dx, d.dw}, d.db, d.dy_ld, d.z_ld, {d.w_ld, d.x_ld}, {d.dx_ld, d.dw_ld}, d.m, d.k, d.n, (int)block1};
+    lin_with_act(d.act, [&](auto act) { linear_small_backward_kernel<DT, act.value><<<(int)blocks, lin_small_threads<DT>(), 0, s>>>(p); });
+    return (int)hipGetLastError();
+}
+
+template <int DT>
 int lin_backward(const odamd_linear_grad_desc& d, LinSpace& ws, bool go, hipStream_t s) {
-    return d.dtype == ODAMD_DTYPE_F32 ? lin_backward_f32(d, ws, go, s) : lin_backward_bf16(d, ws, go, s);
+    if (lin_small<DT>(d)) return go ? lin_small_backward<DT>(d, s) : 0;
+    if constexpr (DT == ODAMD_DTYPE_F32) return lin_backward_f32(d, ws, go, s);
+    else return lin_backward_bf16(d, ws, go, s);
+}
+int lin_backward_any(const odamd_linear_grad_desc& d, LinSpace& ws, bool go, hipStream_t s) {
+    return d.dtype == ODAMD_DTYPE_F32 ? lin_backward<ODAMD_DTYPE_F32>(d, ws, go, s) : lin_backward<ODAMD_DTYPE_BF16>(d, ws, go, s);
 }
 
 constexpr long long LIN_MAX = 0x7fff0000LL;   // 2^31 less what an index passes its end by
@@ -977,7 +1139,7 @@ int odamd_linear_forward(const odamd_linear_desc* d, void* workspace, size_t wor
 size_t odamd_linear_backward_workspace_bytes(const odamd_linear_grad_desc* d) {
     if (!d || !lin_sizes_ok(d->m, d->k, d->n, d->act, d->dtype)) return 0;
     LinSpace ws = {nullptr};
-    lin_backward(*d, ws, false, nullptr);
+    lin_backward_any(*d, ws, false, nullptr);
     return (size_t)ws.at;
 }
 
@@ -993,7 +1155,7 @@ int odamd_linear_backward(const odamd_linear_grad_desc* d, void* workspace, size
     if (need && !workspace) return ODAMD_E_ARG;
     if (workspace_bytes < need) return ODAMD_E_WORKSPACE;
     LinSpace ws = {(char*)workspace};
-    return lin_backward(*d, ws, true, (hipStream_t)stream);
+    return lin_backward_any(*d, ws, true, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -103,7 +103,7 @@ def _linear_backward(dy, z, x, weight, act, want_dx, want_dw, want_db):
                             _ld(weight) if want_dx else 0, k, k, m, k, n, act, _DTYPES[dy.dtype])
     size = lib.odamd_linear_backward_workspace_bytes(d)
     ws = _workspace(size, dy.device)
-    check(_call(dy.device, lib.odamd_linear_backward, d, ws.data_ptr(), size), 'linear_backward')
+    check(_call(dy.device, lib.odamd_linear_backward, d, _ptr(ws), size), 'linear_backward')
     return dx, dw, db
 
 

@@ -56,7 +56,8 @@ def test_workspaces_are_asked_for_and_checked():
     assert lib.odamd_linear_forward(C.byref(d), P, need - 1, None) == E_WORKSPACE
     assert lib.odamd_linear_forward(C.byref(d), None, need, None) == E_ARG
     assert lib.odamd_linear_forward(C.byref(d), P + 64, need, None) == E_ALIGN
-    g = _grad_desc()
+    assert lib.odamd_linear_backward_workspace_bytes(C.byref(_grad_desc())) == 0   # a small layer takes none
+    g = _grad_desc(m=40000)
     need = lib.odamd_linear_backward_workspace_bytes(C.byref(g))
     assert lib.odamd_linear_backward(C.byref(g), P, need - 1, None) == E_WORKSPACE
     assert lib.odamd_linear_backward(C.byref(g), P + 8, need, None) == E_ALIGN
