@@ -144,7 +144,7 @@ def test_linear_long_reductions_backward(mx, m, k, n, dtype):
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
-@pytest.mark.parametrize('m', [4, 40])
+@pytest.mark.parametrize('m', [4, 40, 3000])
 def test_linear_strides_and_offsets(mx, m, dtype):
     """Slices of wider buffers, unaligned starts, transposed and expanded views."""
     k, n = 72, 48
@@ -211,6 +211,22 @@ def test_linear_only_wanted_gradients(mx):
         leaves = [t.detach().requires_grad_(i == q) for q, t in enumerate((x, w, b))]
         got, = torch.autograd.grad(mx.linear(*leaves, 'silu'), leaves[i], dy)
         assert torch.equal(got, full[i])
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('m, k, n', [(3000, 40, 72), (4100, 520, 264)])
+def test_linear_only_wanted_gradients_of_products(mx, m, k, n, dtype):
+    """Each gradient alone takes other paths than all of them together: within two roundings and 2^-16 of each other."""
+    tensors = [randn(m, k, dtype=dtype), randn(n, k, seed=1, dtype=dtype, scale=0.1), randn(n, seed=2, dtype=dtype)]
+    dy = randn(m, n, seed=3, dtype=dtype)
+    for act in (None, 'silu'):
+        leaves = [t.detach().requires_grad_() for t in tensors]
+        full = torch.autograd.grad(mx.linear(*leaves, act), leaves, dy)
+        for wanted in ([0], [1], [2], [0, 1], [0, 2], [1, 2]):
+            leaves = [t.detach().requires_grad_(i in wanted) for i, t in enumerate(tensors)]
+            got = torch.autograd.grad(mx.linear(*leaves, act), [leaves[i] for i in wanted], dy)
+            for i, g in zip(wanted, got):
+                assert float((g.double() - full[i].double()).norm()) <= (2 * HALF[dtype] + 2.0 ** -16) * float(full[i].double().norm())
 
 
 def test_linear_keeps_the_slope_of_large_values(mx):
@@ -584,7 +600,7 @@ def test_adam_over_ranges_equals_adam():
 # in use: streams, graphs, a training run
 # ---------------------------------------------------------------------------------------------
 def test_calls_on_two_streams_at_once(mx):
-    xs = [randn(40, 300, seed=i) for i in range(4)]
+    xs = [randn(m, 300, seed=i) for i, m in enumerate((40, 2500, 2501, 41))]
     w = randn(70, 300, seed=9)
     ref = [(mx.linear(x, w, None, 'silu'), mx.orthogonalize(x)) for x in xs]
     streams = [torch.cuda.Stream() for _ in range(2)]
@@ -598,11 +614,12 @@ def test_calls_on_two_streams_at_once(mx):
         assert torch.equal(a, c) and torch.equal(b, d)
 
 
+@pytest.mark.parametrize('rows', [30, 5000])
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
-def test_captured_and_replayed(mx, dtype):
+def test_captured_and_replayed(mx, dtype, rows):
     """Forward, backward, orthogonalisation and optimizer step in one graph; other inputs between the replays, eager work too."""
-    x, w, b, r = randn(30, 96, dtype=dtype), randn(64, 96, seed=1, dtype=dtype), randn(64, seed=2, dtype=dtype), randn(30, 64, seed=3, dtype=dtype)
-    dy = randn(30, 64, seed=4, dtype=dtype)
+    x, w, b, r = randn(rows, 96, dtype=dtype), randn(64, 96, seed=1, dtype=dtype), randn(64, seed=2, dtype=dtype), randn(rows, 64, seed=3, dtype=dtype)
+    dy = randn(rows, 64, seed=4, dtype=dtype)
     p, g, m = randn(2000), randn(2000, seed=5), torch.zeros(2000, device='cuda')
     table = mx.MatrixTable([(0, 16, 27), (500, 30, 50)])
 
@@ -624,7 +641,7 @@ def test_captured_and_replayed(mx, dtype):
         out = work(xs, ps, ms)
     pe, me = p.clone(), m.clone()
     for turn in range(4):
-        xs.copy_(randn(30, 96, seed=50 + turn, dtype=dtype))
+        xs.copy_(randn(rows, 96, seed=50 + turn, dtype=dtype))
         graph.replay()
         torch.cuda.synchronize()
         ref = work(xs.clone(), pe, me)
@@ -637,7 +654,7 @@ def test_two_graphs_at_once(mx):
     """Two captured graphs replayed on two streams at the same time: neither uses the other's workspace."""
     def work(x, w):
         return mx.linear(x, w, None, 'silu'), mx.orthogonalize(x)
-    cases = [(randn(100, 700, seed=i), randn(60, 700, seed=10 + i)) for i in range(2)]
+    cases = [(randn(5000, 300, seed=i), randn(60, 300, seed=10 + i)) for i in range(2)]
     refs = [work(*c) for c in cases]
     graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in cases]
     for c in cases:
