@@ -840,7 +840,10 @@ __global__ void __launch_bounds__(256) ns_join_kernel(NsTable t, int cuts, float
 using NsTile256 = GemmTile<2, true, 256, 256, 4, 2, 1, 2>;
 using NsTile128 = GemmTile<2, true, 128, 128, 2, 2, 1, 2>;
 using NsTile64 = GemmTile<2, true, 64, 64, 2, 2, 1, 2>;
-using NsTile64Few = GemmTile<2, true, 64, 64, 2, 2, 2, 3>;   // two wave groups: one tile, or less, for a compute unit
+// two wave groups, where a compute unit has one tile or two (78 matrices, 340 tiles: a step of 282 us instead of 295); with 528 tiles
+// of one length their third round costs more than it gains (2048 x 8192: 1173 instead of 1023 us)
+using NsTile64Few = GemmTile<2, true, 64, 64, 2, 2, 2, 3>;
+using NsTile64Two = GemmTile<2, true, 64, 64, 2, 2, 2, 2>;
 
 // Tiles of a stage over the whole table; -1: more than a launch of `threads` for each takes
 int ns_count(NsTable& t, int stage, int tile, int threads) {
@@ -867,8 +870,10 @@ template <int STAGE, bool MUON, int DT>
 int ns_launch64(NsTable& t, const NsIo& io, const NsJobs& jobs, hipStream_t s) {
     const int tiles = ns_count(t, STAGE, 64, NsTile64::THREADS * jobs.n);
     if (tiles < 0) return ODAMD_E_LIMIT;
-    return (long long)tiles * jobs.n > 256 ? ns_launch_tile<NsTile64, STAGE, MUON, DT>(t, io, jobs, s)
-                                           : ns_launch_tile<NsTile64Few, STAGE, MUON, DT>(t, io, jobs, s);
+    const long long all = (long long)tiles * jobs.n;
+    return all > 512 ? ns_launch_tile<NsTile64, STAGE, MUON, DT>(t, io, jobs, s)
+         : all > 256 ? ns_launch_tile<NsTile64Two, STAGE, MUON, DT>(t, io, jobs, s)
+                     : ns_launch_tile<NsTile64Few, STAGE, MUON, DT>(t, io, jobs, s);
 }
 
 template <int STAGE, bool MUON, int DT>
