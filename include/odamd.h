@@ -440,7 +440,8 @@ int odamd_linear_forward(const odamd_linear_desc* d, void* workspace, size_t wor
 
 /* Its backward pass: dz = dy act'(z);  dx = dz W (m x k),  dw = dz^T x (n x k),  db = column sums of dz (n values).  Outputs that
  * are NULL are not computed; w is needed for dx only, x for dw only, z with an activation only.  dz is rounded to `dtype`
- * between the two products (bfloat16: as an activation gradient in memory would be); db is summed before that rounding. */
+ * between the two products (bfloat16: as an activation gradient in memory would be; small layers keep it in float32); db is summed
+ * before that rounding. */
 typedef struct {
     const void* dy;
     const void* z;

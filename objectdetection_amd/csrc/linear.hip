@@ -250,17 +250,18 @@ struct LinRow {
     int m, k, n;
     LinEnd end;
 };
-// A workgroup takes four output columns of up to eight rows.  One row: a wave per column.  More rows: COLS columns a wave, which
-// share the x it loads, and COLS waves share a column's reduction, so that as many waves read W.  What bounds it: reading W
-// (1 x 4096 x 4096 bf16 7.5 us, 4.5 TB/s; 8 x 8192 x 8192 26 us, 5.1 TB/s), with many rows the x and W that come out of the
-// caches again.  8 x 4096 x 4096 bf16 with 1 / 2 / 4 columns a wave: 15.7 / 11.0 / 10.6 us, in float32 30 / 22 / 18 us.
-template <int DT, int MR, bool WIDE>
+// A workgroup takes four output columns of up to eight rows; its four waves hold all of them and share the reduction, so that x is
+// loaded once for four columns and as many waves read W as with a wave per column (8 x 4096 x 4096 bf16: 10.1 us, one column
+// a wave 15.7; 1 x 30000 x 64 float32 14.0 and 39.3).  Vectors are loaded from any element on: 1 x 1155 x 1001 float32 takes 3.7 us, by
+// single elements 7.9.  What bounds it: reading W (1 x 4096 x 4096 bf16 7.3 us, 4.6 TB/s; 8 x 8192 x 8192 26 us, 5.2 TB/s), with many
+// rows the x and W that come out of the caches again.
+template <int DT, int MR>
 __global__ void __launch_bounds__(256) linear_rows_kernel(LinRow p) {
     using T = typename LinType<DT>::T;
-    constexpr int V = WIDE ? 16 / (int)sizeof(T) : 1, COLS = MR < 4 ? MR : 4, N = MR * COLS;
+    constexpr int V = 16 / (int)sizeof(T), COLS = 4, N = MR * COLS;
     __shared__ float part[4][N];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col0 = blockIdx.x * 4 + wave / COLS * COLS, row0 = blockIdx.y * MR;
+    const int col0 = blockIdx.x * COLS, row0 = blockIdx.y * MR;
     // rows and columns past the last one are computed like the last one and not stored: all loads of a step go out together
     const T *x[MR], *w[COLS];
 #pragma unroll
@@ -270,16 +271,17 @@ __global__ void __launch_bounds__(256) linear_rows_kernel(LinRow p) {
     float acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = 0.0f;
-    for (int k = (wave % COLS * 64 + lane) * V; k < p.k; k += 64 * V * COLS) {
-        T wv[COLS][V], xv[MR][V];
+    const auto add = [&](auto width, int k) {
+        constexpr int W = width.value;
+        T wv[COLS][W], xv[MR][W];
 #pragma unroll
         for (int c = 0; c < COLS; ++c) {
-            if constexpr (WIDE) *(u32x4*)wv[c] = *(const u32x4*)(w[c] + k);
+            if constexpr (W > 1) *(u32x4*)wv[c] = *(const u32x4_any*)(w[c] + k);
             else wv[c][0] = w[c][k];
         }
 #pragma unroll
         for (int i = 0; i < MR; ++i) {
-            if constexpr (WIDE) *(u32x4*)xv[i] = *(const u32x4*)(x[i] + k);
+            if constexpr (W > 1) *(u32x4*)xv[i] = *(const u32x4_any*)(x[i] + k);
             else xv[i][0] = x[i][k];
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -288,8 +290,10 @@ __global__ void __launch_bounds__(256) linear_rows_kernel(LinRow p) {
 #pragma unroll
             for (int c = 0; c < COLS; ++c)
 #pragma unroll
-                for (int e = 0; e < V; ++e) acc[c * MR + i] = fmaf(LinType<DT>::get(xv[i][e]), LinType<DT>::get(wv[c][e]), acc[c * MR + i]);
-    }
+                for (int e = 0; e < W; ++e) acc[c * MR + i] = fmaf(LinType<DT>::get(xv[i][e]), LinType<DT>::get(wv[c][e]), acc[c * MR + i]);
+    };
+    for (int k = (wave * 64 + lane) * V; k + V <= p.k; k += 256 * V) add(std::integral_constant<int, V>{}, k);
+    if (wave == 0 && lane < p.k % V) add(std::integral_constant<int, 1>{}, p.k - p.k % V + lane);
     // sums over the lanes: while there are several values, a lane hands half of them on and keeps the other half
     int at = 0, o = 32;
 #pragma unroll
@@ -305,11 +309,11 @@ __global__ void __launch_bounds__(256) linear_rows_kernel(LinRow p) {
     for (; o; o >>= 1) acc[0] += __shfl_xor(acc[0], o);
     part[wave][at] = acc[0];                                // lanes of one value hold the same sum
     __syncthreads();
-    const int c = threadIdx.x / MR, i = threadIdx.x % MR, col = blockIdx.x * 4 + c;
-    if (c < 4 && row0 + i < p.m && col < p.n) {
+    const int c = threadIdx.x / MR, i = threadIdx.x % MR, col = col0 + c;
+    if (c < COLS && row0 + i < p.m && col < p.n) {
         float v[8] = {};
 #pragma unroll
-        for (int s = 0; s < COLS; ++s) v[0] += part[c / COLS * COLS + s][c % COLS * MR + i];
+        for (int s = 0; s < 4; ++s) v[0] += part[s][c * MR + i];
         lin_with_act(p.end.act, [&](auto act) { lin_finish8<DT, act.value>(p.end, row0 + i, col, 1, v); });
     }
 }
@@ -855,31 +859,29 @@ int lin_tiles(LinJobs& t, int unit_rows) {
     return gemm_grid_ok(at, 256) ? (int)at : -1;
 }
 
-// Whether a layer goes without matrix instructions: up to eight rows always (8 x 4096 x 4096 bf16 10.6 us, in products 13.7), more
+// Whether a layer goes without matrix instructions: up to eight rows always (8 x 4096 x 4096 bf16 10.1 us, in products 13.7), more
 // where its workgroups are few.  Products cost a launch or two for laying operands out, the rows a step per eight of them;
 // rows / products, us: float32 512 x 256 x 256 (4096 workgroups) 9.2 / 10.6, 1024 x 256 x 256 15.7 / 11.3, 128 x 1024 x 1024
 // 13.5 / 18.1, 256 x 1024 x 1024 22.5 / 19.9, 32 x 4096 x 4096 46 / 55; bfloat16 read in place 128 x 256 x 256 (1024) 4.2 / 4.5,
 // 256 x 256 x 256 6.8 / 4.5, 64 x 1024 x 1024 8.3 / 7.8; bfloat16 laid out 64 x 513 x 1024 (2048) 7.0 / 8.9, 128 x 513 x 1024
-// 11.0 / 9.0.
+// 11.0 / 9.0.  A long reduction in few workgroups is one chain of loads, which products cut: bfloat16 8 x 30000 x 64 17.9 / 18.4,
+// 8 x 100000 x 64 58 / 26 (float32, laid out first there, 86 / 252).
 template <int DT>
-bool lin_by_rows(int m, int n, bool direct) {
+bool lin_by_rows(int m, int k, int n, bool direct) {
     const long long blocks = ((m + 7LL) / 8) * ((n + 3LL) / 4);
+    if (DT == ODAMD_DTYPE_BF16 && direct && k > 32768 && blocks < 256) return false;
     return m <= 8 || blocks <= (DT == ODAMD_DTYPE_F32 ? 4096 : direct ? 1024 : 2048);
 }
 
 template <int DT>
 int lin_forward_rows(const odamd_linear_desc& d, const LinEnd& end, hipStream_t s) {
-    constexpr int V = DT == ODAMD_DTYPE_F32 ? 4 : 8;
-    const bool wide = (((uintptr_t)d.x | (uintptr_t)d.w) & 15) == 0 && d.x_ld % V == 0 && d.w_ld % V == 0 && d.k % V == 0;
     const LinRow p = {d.x, d.w, d.x_ld, d.w_ld, d.m, d.k, d.n, end};
     const dim3 blocks((d.n + 3) / 4, (d.m + 7) / 8);
     if (!gemm_grid_ok(blocks.x, 256)) return ODAMD_E_LIMIT;
-#define ODAMD_ROWS(MR) (wide ? linear_rows_kernel<DT, MR, true><<<blocks, 256, 0, s>>>(p) : linear_rows_kernel<DT, MR, false><<<blocks, 256, 0, s>>>(p))
-    if (d.m == 1) ODAMD_ROWS(1);
-    else if (d.m == 2) ODAMD_ROWS(2);
-    else if (d.m <= 4) ODAMD_ROWS(4);
-    else ODAMD_ROWS(8);
-#undef ODAMD_ROWS
+    if (d.m == 1) linear_rows_kernel<DT, 1><<<blocks, 256, 0, s>>>(p);
+    else if (d.m == 2) linear_rows_kernel<DT, 2><<<blocks, 256, 0, s>>>(p);
+    else if (d.m <= 4) linear_rows_kernel<DT, 4><<<blocks, 256, 0, s>>>(p);
+    else linear_rows_kernel<DT, 8><<<blocks, 256, 0, s>>>(p);
     return (int)hipGetLastError();
 }
 
@@ -889,7 +891,7 @@ int lin_forward(const odamd_linear_desc& d, LinSpace& ws, bool go, hipStream_t s
     const LinEnd end = {d.bias, d.residual, d.y, d.z, d.r_ld, d.y_ld, d.z_ld, d.act};
     // measuring, the pointers are not known: the workspace of products serves where only they may say
     const bool direct = !go || (lin_direct<DT>(d.x, d.x_ld, d.k) && lin_direct<DT>(d.w, d.w_ld, d.k));
-    if (lin_by_rows<DT>(d.m, d.n, direct)) return go ? lin_forward_rows<DT>(d, end, s) : 0;
+    if (lin_by_rows<DT>(d.m, d.k, d.n, direct)) return go ? lin_forward_rows<DT>(d, end, s) : 0;
     constexpr int SIZE = DT == ODAMD_DTYPE_F32 ? 4 : 2;
     LinLaunch launch = {};
     LinGemm& g = launch.g[0];

@@ -104,7 +104,8 @@ def check_linear(mx, x, w, b, act, r, backward=True):
 SIZES = [(1, 1, 1), (1, 64, 40), (2, 7, 3), (3, 130, 65), (7, 129, 9), (8, 256, 130), (9, 64, 64), (17, 33, 31), (33, 8, 200),
          (64, 64, 64), (65, 200, 63), (129, 72, 257), (300, 1000, 20), (1000, 24, 300)]
 # more than 4096 workgroups of eight rows and four columns: on matrix instructions in either type
-SIZES += [(600, 33, 257), (2000, 7, 80), (5000, 130, 29), (700, 64, 200), (10, 40, 9001), (40001, 1, 4), (513, 255, 256)]
+SIZES += [(600, 33, 257), (2000, 7, 80), (5000, 130, 29), (700, 64, 200), (10, 40, 9001), (40001, 1, 4), (513, 255, 256),
+          (1, 40001, 5), (2, 33000, 24), (9, 40000, 24)]
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
