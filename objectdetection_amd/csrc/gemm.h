@@ -5,10 +5,10 @@
 //   PL = 1: bf16 values, one v_mfma_f32_32x32x16_bf16 per 32 x 32 x 16 block;
 //   PL = 2: every value as a pair of fp16 numbers, v = (hi + lo) 2^-s; 32 hi and then their 32 lo lie side by side.  hi holds
 //           the upper 11 bits of v, lo the next 11, so hi_a hi_b + hi_a lo_b + lo_a hi_b (three v_mfma_f32_32x32x16_f16)
-//           carries a product to 2^-22, the dropped lo_a lo_b.  Float32 operands run at a third of the half-precision matrix rate this way, which is five
-//           times the rate of the float32 matrix instructions; 2^s is a power of two, so it costs no rounding.  fp16
-//           has no more exponents than its scale gives it: the caller's scale keeps the largest value under 65504, and the
-//           smallest step, 2^-24, lies 2^-39 or less under it.
+//           carries a product to 2^-22, the dropped lo_a lo_b.  Float32 operands run at a third of the half-precision matrix
+//           rate this way, which is five times the rate of the float32 matrix instructions; 2^s is a power of two, so it
+//           costs no rounding.  fp16 has no more exponents than its scale gives it: the caller's scale keeps the largest
+//           value under 65504, and the smallest step, 2^-24, lies 2^-39 or less under it.
 //
 // A workgroup holds a TM x TN tile of C in registers (WGM x WGN waves) and walks K in chunks of 128 bytes per row (64
 // bf16 values, or 32 pairs).  A chunk of A and B goes global -> LDS without passing registers
@@ -26,7 +26,8 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16v8_t;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 
-__device__ __attribute__((aligned(16))) const unsigned char g_gemm_zero[16] = {};   // 16 bytes of zeros: the source of pieces past the end of K
+// 16 bytes of zeros: the source of pieces past the end of K
+__device__ __attribute__((aligned(16))) const unsigned char g_gemm_zero[16] = {};
 
 __device__ __forceinline__ void gemm_dma16(const char* g, char* l) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
@@ -120,7 +121,7 @@ struct GemmTile {
     static constexpr int NI = (TM + TN) / 8 / NW;                   // DMA instructions per wave and chunk
     static_assert((TM + TN) % (8 * NW) == 0 && TM % 8 == 0, "whole DMA instructions");
     static_assert((KG - 1) * NW * FM * FN * 4096 <= RING, "the other groups' sums pass through the ring");
-    static_assert(NBUF >= 2 && NBUF <= 4 && LDS <= 160 * 1024, "LDS of a compute unit");
+    static_assert(NBUF >= 2 && NBUF <= 3 && LDS <= 160 * 1024, "LDS of a compute unit");
 
     f32x16_t acc[FM][FN];
 
@@ -262,8 +263,7 @@ struct GemmTile {
                 // this wave's pieces of round i have landed (those of up to NBUF - 2 later rounds may still be on their way)
                 // and its reads of round i - 1 have returned; behind the barrier that holds for every wave
                 const int ahead = min(NBUF - 2, rounds - 1 - i);
-                if (NBUF > 3 && ahead == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NBUF > 3 ? 2 * NI : 0) : "memory");
-                else if (NBUF > 2 && ahead == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NBUF > 2 ? NI : 0) : "memory");
+                if (NBUF > 2 && ahead == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NBUF > 2 ? NI : 0) : "memory");
                 else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                 gemm_barrier();
                 if (i + NBUF - 1 < rounds) issue(i + NBUF - 1);

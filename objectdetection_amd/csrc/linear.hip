@@ -3,13 +3,14 @@
 //   dz = dy act'(z),  z = x W^T + b;   dx = dz W,   dW = dz^T x,   db = column sums of dz   (dr = dy, the caller's own)
 // bfloat16 operands run on bf16 matrix instructions as they are; float32 operands as fp16 pairs (gemm.h) with a power of
 // two per row of each operand, so that a row's largest value sits just under 2^15: 22 bits per value down to 2^-17 of the row's
-// largest, and the same absolute step below.  Sums are float32; dz is kept in the operands' type, z in float32 or, beside bfloat16, in float16.
+// largest, and the same absolute step below.  Sums are float32; dz is kept in the operands' type, z in float32 or, beside
+// bfloat16, in float16.
 // dx reduces over the outputs and dW over the rows: in bfloat16 the products read W, x and dz with the reduction along their
 // rows, out of the caller's tensors; float32 pairs need a power of two per column there, so that W, x and dz are laid out
-// by columns first (one launch for all three).
+// by columns first (one launch for all three).  Few rows, and the backward pass of small layers, go without matrix instructions.
 // Times: (25600, 1024, 4096) bf16 with bias, SiLU and residual 285 us, 243 of them the product (a library product of that size
 // takes 206 us), the rest the epilogue's 420 MB; forward and backward of (8192, 1024, 4096) bf16 304 us; (4097, 1155, 1001)
-// float32 with GELU 66 us.  Few rows go without matrix instructions: (1, 1024, 1024) bf16 takes 3 us, a call of it 13 on the host.
+// float32 with GELU 66 us; (1, 1024, 1024) bf16 3 us, a call of it 13 on the host.
 #include "common.h"
 #include "odamd.h"
 
