@@ -79,10 +79,10 @@ static_assert(sizeof(NsTable) <= 3700, "kernel arguments are limited to 4 KiB");
 
 __host__ __device__ inline long long ns_up(long long v, int to) { return (v + to - 1) / to * to; }
 // Columns of an m x n matrix with few rows that a workgroup takes (t: m in 16-row tiles): all of them, or at least what its
-// waves have under way at once, and at most 32 parts.  Parts cost two launches more; one workgroup / parts, us: 16 x 1000 15.0 /
-// 16.4, 16 x 2000 22 / 17, 32 x 1000 35 / 32, 48 x 256 35 / 38, 48 x 512 44 / 40, 64 x 256 59 / 61, 64 x 512 75 / 64.
+// waves have under way at once, and at most 32 parts.  Parts cost two launches more; one workgroup / parts, us: 16 x 1000 12.3 /
+// 14, 16 x 2000 20 / 16, 32 x 1000 35 / 32, 48 x 256 35 / 38, 48 x 512 44 / 40, 64 x 256 59 / 61, 64 x 512 75 / 64.
 __host__ __device__ inline int ns_few_cols(int t, int n) {
-    return n <= 1024 / t ? (int)ns_up(n, 16) : (int)ns_up(ns_up(n, 32) / 32, t <= 2 ? 512 : 128);
+    return n <= (t == 1 ? 1536 : 1024 / t) ? (int)ns_up(n, 16) : (int)ns_up(ns_up(n, 32) / 32, t <= 2 ? 512 : 128);
 }
 // Workspace of a matrix then: Q and the partial sums of G G^T, in 64 bits
 __host__ __device__ inline long long ns_few_bytes(int t, int cols, int n) {
@@ -415,6 +415,42 @@ __device__ __forceinline__ double* ns_few_steps(double* lds, int steps, double e
     constexpr int EACH = (F::SUMS + F::THREADS - 1) / F::THREADS, LD = F::LD;
     double *a = lds, *p = lds + F::SQ, *q = lds + 2 * F::SQ;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, h = lane >> 4;
+    if constexpr (T == 1) {
+        // One tile: a lane's results, rows 4 e + h of column r, are by symmetry its operands of the next product, columns 4 e + h of
+        // row r, so that one wave takes all steps in registers (16 x 27: 7.4 us, through LDS 10.0).
+        if (wave == 0) {
+            const auto times = [](const f64x4_t& x, const f64x4_t& y) {
+                f64x4_t even = {}, odd = {};
+                even = ns_mma64(x[0], y[0], even);
+                odd = ns_mma64(x[1], y[1], odd);
+                even = ns_mma64(x[2], y[2], even);
+                odd = ns_mma64(x[3], y[3], odd);
+                return even + odd;
+            };
+            f64x4_t am, pm, qm = {};
+            double sum = 0.0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                am[e] = get(e * 64 + lane);
+                sum += r == 4 * e + h ? am[e] : 0.0;
+            }
+#pragma unroll
+            for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+            const double inv = 1.0 / (sqrt(sum) + eps);
+            am = am * inv * inv;
+            for (int step = 0; step < steps; ++step) {
+                const f64x4_t s = times(am, am);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) pm[e] = (r == 4 * e + h ? NS_A : 0.0) + NS_B * am[e] + NS_C * s[e];
+                qm = step == 0 ? pm : times(qm, pm);
+                am = times(pm, times(pm, am));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[(4 * e + h) * LD + r] = qm[e] * inv;
+        }
+        __syncthreads();
+        return q;
+    }
     double v[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
