@@ -44,7 +44,7 @@ def _ptr(t):
 
 
 def _workspace(size, device):
-    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    return torch.empty((size,), dtype=torch.uint8, device=device) if size else None
 
 
 def _check_tensor(name, t, dtype=None, device=None):
@@ -194,8 +194,9 @@ def orthogonalize(x, steps=5, eps=1e-7, out=None):
         raise ValueError(f'x must have rows and columns, not shape {tuple(x.shape)}')
     if not 1 <= int(steps) <= 32 or not eps >= 0:
         raise ValueError('steps must be 1 to 32, eps must not be negative')
-    rows, cols = x.shape[-2:]
-    if rows * cols > _MOST or x.shape[:-2].numel() > _MOST:
+    rows, cols = x.size(-2), x.size(-1)
+    batch = x.numel() // max(rows * cols, 1)
+    if rows * cols > _MOST or batch > _MOST:
         raise ValueError(f'at most {_MOST} elements of a matrix and matrices')
     if out is None:
         out = x.new_empty(x.shape)
@@ -203,10 +204,9 @@ def orthogonalize(x, steps=5, eps=1e-7, out=None):
         _check_tensor('out', out, x.dtype, x.device)
         if out.shape != x.shape or not out.is_contiguous():
             raise ValueError('out must be contiguous and have the shape of x')
-    if x.numel() == 0:
+    if batch == 0 or rows * cols == 0:
         return out
     src = x if x.is_contiguous() else x.detach().contiguous()
-    batch = src.numel() // (rows * cols)
     size = lib.odamd_orthogonalize_workspace_bytes(batch, rows, cols)
     ws = _workspace(size, x.device)
     check(_call(x.device, lib.odamd_orthogonalize, src.data_ptr(), out.data_ptr(), batch, rows, cols, int(steps), float(eps),

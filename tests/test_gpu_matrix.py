@@ -166,6 +166,64 @@ def test_linear_strides_and_offsets(mx, m, dtype):
     assert float((x.grad.double() - ref).norm() / ref.norm()) < 4 * HALF[dtype] + 1e-5
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('m, k, n', [(5, 40, 24), (33, 24, 41), (3000, 72, 200), (2100, 520, 1000)])
+def test_linear_entry_points_write_within_their_rows(mx, m, k, n, dtype):
+    """Rows of results further apart than they are long, the residual in the place of the result: what lies between stays."""
+    from objectdetection_amd import _lib
+    from objectdetection_amd._lib import lib, check
+    code, ztype = (0, torch.float32) if dtype == torch.float32 else (1, torch.float16)
+    st = torch.cuda.current_stream().cuda_stream
+    x, w, b = randn(m, k, dtype=dtype), randn(n, k, seed=1, dtype=dtype, scale=k ** -0.5), randn(n, seed=2, dtype=dtype)
+    r = randn(m, n, seed=3, dtype=dtype)
+    y = torch.full((m, n + 5), 7.0, dtype=dtype, device='cuda')
+    z = torch.full((m, n + 3), 7.0, dtype=ztype, device='cuda')
+    y[:, :n] = r
+    d = _lib.LinearDesc(x.data_ptr(), w.data_ptr(), b.data_ptr(), y.data_ptr(), y.data_ptr(), z.data_ptr(), k, k, n + 5, n + 5, n + 3,
+                        m, k, n, 1, code)
+    size = lib.odamd_linear_workspace_bytes(d)
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device='cuda')
+    check(lib.odamd_linear_forward(d, ws.data_ptr(), size, st))
+    z64, y64 = forward_reference(x, w, b, 'silu', r)
+    bound = forward_bound(x, w, b, 'silu', r, z64, dtype)
+    close(y[:, :n], y64, bound, dtype)
+    close(z[:, :n].float(), z64, bound + (2.0 ** -11 * z64.abs() + 2.0 ** -24 if dtype == torch.bfloat16 else 0), torch.float32)
+    assert bool((y[:, n:] == 7).all()) and bool((z[:, n:] == 7).all())
+    dy = randn(m, n, seed=4, dtype=dtype)
+    dx = torch.full((m, k + 3), 7.0, dtype=dtype, device='cuda')
+    dw = torch.full((n, k + 6), 7.0, dtype=dtype, device='cuda')
+    db = torch.full((n + 8,), 7.0, dtype=dtype, device='cuda')
+    g = _lib.LinearGradDesc(dy.data_ptr(), z.data_ptr(), x.data_ptr(), w.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
+                            n, n + 3, k, k, k + 3, k + 6, m, k, n, 1, code)
+    size = lib.odamd_linear_backward_workspace_bytes(g)
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device='cuda')
+    check(lib.odamd_linear_backward(g, ws.data_ptr(), size, st))
+    plain = mx._linear_backward(dy, z[:, :n].contiguous(), x, w, 1, True, True, True)
+    assert torch.equal(dx[:, :k], plain[0]) and torch.equal(dw[:, :k], plain[1]) and torch.equal(db[:n], plain[2])
+    assert bool((dx[:, k:] == 7).all()) and bool((dw[:, k:] == 7).all()) and bool((db[n:] == 7).all())
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('m, k, n', [(1, 72, 48), (7, 71, 45), (40, 72, 48), (3000, 72, 48), (3001, 71, 45), (2100, 520, 1000)])
+def test_linear_reads_nothing_beside_its_operands(mx, m, k, n, dtype):
+    """Operands in buffers that hold NaN everywhere else."""
+    def island(rows, cols, seed, scale=1.0):
+        sea = torch.full((rows + 4, cols + 24), float('nan'), dtype=dtype, device='cuda')
+        sea[2:rows + 2, 8:cols + 8] = randn(rows, cols, seed=seed, dtype=dtype, scale=scale)
+        return sea[2:rows + 2, 8:cols + 8].detach().requires_grad_()
+    x, w, r = island(m, k, 0), island(n, k, 1, k ** -0.5), island(m, n, 2)
+    b = island(1, n, 3)
+    for act in (None, 'gelu'):
+        y = mx.linear(x, w, b[0], act, r)
+        grads = torch.autograd.grad(y, (x, w, b, r), island(m, n, 4).detach())
+        copies = [t.detach().clone().requires_grad_() for t in (x, w, b, r)]
+        y2 = mx.linear(copies[0], copies[1], copies[2][0], act, copies[3])
+        grads2 = torch.autograd.grad(y2, copies, island(m, n, 4).detach().clone())
+        assert torch.isfinite(y).all() and float((y - y2).norm()) <= (HALF[dtype] + 1e-5) * float(y2.norm())
+        for g, h in zip(grads, grads2):
+            assert torch.isfinite(g).all() and float((g - h).norm()) <= (2 * HALF[dtype] + 1e-5) * float(h.norm())
+
+
 def test_linear_shapes_of_more_axes(mx):
     x, w, b = randn(2, 3, 5, 40), randn(24, 40, seed=1), randn(24, seed=2)
     y = mx.linear(x, w, b, 'silu')
@@ -600,6 +658,57 @@ def test_adam_over_ranges_equals_adam():
 # ---------------------------------------------------------------------------------------------
 # in use: streams, graphs, a training run
 # ---------------------------------------------------------------------------------------------
+def test_workspaces_hold_what_is_written(mx):
+    """Every entry point with a workspace of exactly the size asked for, in the middle of a larger buffer and full of NaN, none of
+    which reaches a result."""
+    from objectdetection_amd import _lib
+    from objectdetection_amd._lib import lib, check
+    st = torch.cuda.current_stream().cuda_stream
+    buf = torch.empty(200 << 20, dtype=torch.uint8, device='cuda')
+
+    def guarded(size, call, *results):
+        assert size + 8192 <= buf.numel()
+        end = 4096 + size
+        buf[4096:end] = 255
+        buf[:4096] = 165
+        buf[end:end + 4096] = 165
+        check(call(buf.data_ptr() + 4096))
+        assert all(bool(torch.isfinite(r).all()) for r in results if r is not None)
+        assert bool((buf[:4096] == 165).all()) and bool((buf[end:end + 4096] == 165).all())
+
+    for code, dtype in ((0, torch.float32), (1, torch.bfloat16)):
+        for batch, rows, cols in ((1, 1, 1), (3, 5, 4264), (2, 3000, 16), (1, 40, 7000), (4, 64, 2000), (1, 65, 66), (2, 130, 65),
+                                  (3, 129, 2049), (1, 700, 3000), (1, 1025, 1100)):
+            for steps in (5, 12):
+                g, out = randn(batch, rows, cols, dtype=dtype), torch.empty(batch, rows, cols, dtype=dtype, device='cuda')
+                size = lib.odamd_orthogonalize_workspace_bytes(batch, rows, cols)
+                guarded(size, lambda ws: lib.odamd_orthogonalize(g.data_ptr(), out.data_ptr(), batch, rows, cols, steps, 1e-7, code,
+                                                                 ws, size, st), out)
+        for m, k, n in ((9001, 33, 40), (3000, 1155, 101), (600, 2000, 700), (70, 1500, 3001), (10, 40, 9001)):
+            x, w, dy = randn(m, k, dtype=dtype), randn(n, k, seed=1, dtype=dtype), randn(m, n, seed=2, dtype=dtype)
+            y, z = torch.empty_like(dy), torch.empty(m, n, dtype=dtype if code == 0 else torch.float16, device='cuda')
+            dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty(n, dtype=dtype, device='cuda')
+            d = _lib.LinearDesc(x.data_ptr(), w.data_ptr(), None, None, y.data_ptr(), z.data_ptr(), k, k, 0, n, n, m, k, n, 2, code)
+            size = lib.odamd_linear_workspace_bytes(d)
+            guarded(size, lambda ws: lib.odamd_linear_forward(d, ws, size, st), y, z)
+            for outs in ((dx, dw, db), (dx, None, None), (None, dw, None), (None, None, db)):
+                g = _lib.LinearGradDesc(dy.data_ptr(), z.data_ptr(), x.data_ptr(), w.data_ptr(),
+                                        *(None if o is None else o.data_ptr() for o in outs), n, n, k, k, k, k, m, k, n, 2, code)
+                size = lib.odamd_linear_backward_workspace_bytes(g)
+                guarded(size, lambda ws: lib.odamd_linear_backward(g, ws, size, st), *outs)
+    for shapes in ([(16, 27), (5, 4000), (1, 1)], [(64, 64), (3, 9000), (1, 2)], [(64, 300), (65, 70), (300, 256)], [(8, 8)] * 130):
+        matrices, at = [], 0
+        for r, c in shapes:
+            matrices.append((at, r, c))
+            at += r * c
+        table = mx.MatrixTable(matrices)
+        p, g, m = randn(at), randn(at, seed=1), randn(at, seed=2)
+        for steps in (5, 12):
+            guarded(table.workspace_bytes, lambda ws: lib.odamd_muon_ema_step(
+                p.data_ptr(), g.data_ptr(), m.data_ptr(), None, table.table.ctypes.data, len(table), 0.01, 0.9, 1, 0.0, steps, 1e-7,
+                0.0, 1.0, ws, table.workspace_bytes, st), p, m)
+
+
 def test_calls_on_two_streams_at_once(mx):
     xs = [randn(m, 300, seed=i) for i, m in enumerate((40, 2500, 2501, 41))]
     w = randn(70, 300, seed=9)
