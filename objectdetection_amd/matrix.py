@@ -48,6 +48,9 @@ def _workspace(size, device):
 
 
 def _check_tensor(name, t, dtype=None, device=None):
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _DTYPES and (dtype is None or t.dtype is dtype) and (
+            device is None or t.device == device):
+        return
     if not torch.is_tensor(t) or not t.is_cuda:
         raise ValueError(f'{name} must be a CUDA tensor')
     if t.dtype not in _DTYPES:
@@ -70,10 +73,6 @@ def _rows(t):
     return t
 
 
-def _ld(t):
-    return max(t.stride(0), t.shape[1])
-
-
 # ---------------------------------------------------------------------------------------------
 # dense layer
 # ---------------------------------------------------------------------------------------------
@@ -81,29 +80,34 @@ def _linear_forward(x, weight, bias, residual, act, keep_z):
     """2-D operands as `_rows` leaves them -> (y, z or None)."""
     m, k = x.shape
     n = weight.shape[0]
+    dtype, device = x.dtype, x.device
     y = x.new_empty((m, n))
-    z = x.new_empty((m, n), dtype=_Z_DTYPES[x.dtype]) if keep_z else None
-    d = _lib.LinearDesc(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(z), _ld(x),
-                        _ld(weight), 0 if residual is None else _ld(residual), n, n, m, k, n, act, _DTYPES[x.dtype])
+    z = x.new_empty((m, n), dtype=_Z_DTYPES[dtype]) if keep_z else None
+    # a single row may have any stride: at least its length
+    d = _lib.LinearDesc(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(z), max(x.stride(0), k),
+                        max(weight.stride(0), k), 0 if residual is None else max(residual.stride(0), n), n, n, m, k, n, act,
+                        _DTYPES[dtype])
     size = lib.odamd_linear_workspace_bytes(d)
-    ws = _workspace(size, x.device)
-    check(_call(x.device, lib.odamd_linear_forward, d, _ptr(ws), size), 'linear_forward')
+    ws = _workspace(size, device)
+    check(_call(device, lib.odamd_linear_forward, d, _ptr(ws), size), 'linear_forward')
     return y, z
 
 
 def _linear_backward(dy, z, x, weight, act, want_dx, want_dw, want_db):
     """Gradients of `_linear_forward` from 2-D operands; x and weight may be None where they are not needed."""
     m, n = dy.shape
-    k = (weight if weight is not None else x).shape[1] if (want_dx or want_dw) else 1
+    k = weight.shape[1] if want_dx else x.shape[1] if want_dw else 1
+    device = dy.device
     dx = dy.new_empty((m, k)) if want_dx else None
     dw = dy.new_empty((n, k)) if want_dw else None
     db = dy.new_empty((n,)) if want_db else None
-    d = _lib.LinearGradDesc(dy.data_ptr(), _ptr(z), _ptr(x) if want_dw else None, _ptr(weight) if want_dx else None, _ptr(dx),
-                            _ptr(dw), _ptr(db), _ld(dy), 0 if z is None else _ld(z), _ld(x) if want_dw else 0,
-                            _ld(weight) if want_dx else 0, k, k, m, k, n, act, _DTYPES[dy.dtype])
+    d = _lib.LinearGradDesc(dy.data_ptr(), _ptr(z), x.data_ptr() if want_dw else None, weight.data_ptr() if want_dx else None,
+                            _ptr(dx), _ptr(dw), _ptr(db), max(dy.stride(0), n), n if z is None else max(z.stride(0), n),
+                            max(x.stride(0), k) if want_dw else 0, max(weight.stride(0), k) if want_dx else 0, k, k, m, k, n,
+                            act, _DTYPES[dy.dtype])
     size = lib.odamd_linear_backward_workspace_bytes(d)
-    ws = _workspace(size, dy.device)
-    check(_call(dy.device, lib.odamd_linear_backward, d, _ptr(ws), size), 'linear_backward')
+    ws = _workspace(size, device)
+    check(_call(device, lib.odamd_linear_backward, d, _ptr(ws), size), 'linear_backward')
     return dx, dw, db
 
 
@@ -143,26 +147,29 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     """act(x W^T + bias) + residual in one product.  x: (..., k); weight: (n, k); bias: (n,); residual: (..., n); all of one
     type, float32 or bfloat16.  activation: None, 'silu', 'gelu' (the erf form) or 'relu'.  Rows may be strided (a slice of a
     wider, concatenated buffer is read in place).  Differentiable once in all four tensors; in bfloat16 the pre-activation
-    that the backward pass keeps is float16 and the gradient at it bfloat16.  As with every differentiable torch operation, a backward
-    pass is captured into a graph on leaves that no eager graph holds any more (detached copies of them will do).  float32 products carry 22 bits per value, counted
-    from the largest magnitude of its row; a float32 row with an infinity gives NaN or infinity."""
+    that the backward pass keeps is float16 and the gradient at it bfloat16.  As with every differentiable torch operation,
+    a backward pass is captured into a graph on leaves that no eager graph holds any more (detached copies of them will do).
+    float32 products carry 22 bits per value, counted from the largest magnitude of its row; a float32 row with an infinity
+    gives NaN or infinity."""
     if activation not in ACTIVATIONS:
         raise ValueError(f'activation {activation!r}: one of {list(ACTIVATIONS)}')
     _check_tensor('x', x)
-    _check_tensor('weight', weight, x.dtype, x.device)
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or min(weight.shape) < 1:
+    dtype, device = x.dtype, x.device
+    _check_tensor('weight', weight, dtype, device)
+    k = x.shape[-1] if x.dim() else 0
+    if weight.dim() != 2 or weight.shape[1] != k or min(weight.shape) < 1:
         raise ValueError(f'x (..., k) and weight (n, k) do not fit: {tuple(x.shape)} and {tuple(weight.shape)}')
-    n = weight.shape[0]
+    n, flat = weight.shape[0], x.dim() == 2
     if bias is not None:
-        _check_tensor('bias', bias, x.dtype, x.device)
-        if tuple(bias.shape) != (n,):
+        _check_tensor('bias', bias, dtype, device)
+        if bias.shape != (n,):
             raise ValueError(f'bias must have shape ({n},), not {tuple(bias.shape)}')
     if residual is not None:
-        _check_tensor('residual', residual, x.dtype, x.device)
-        if residual.shape != x.shape[:-1] + (n,):
+        _check_tensor('residual', residual, dtype, device)
+        if residual.shape != ((x.shape[0], n) if flat else x.shape[:-1] + (n,)):
             raise ValueError(f'residual must have shape {tuple(x.shape[:-1]) + (n,)}, not {tuple(residual.shape)}')
     act = ACTIVATIONS[activation]
-    if max(x.numel() // x.shape[-1], *weight.shape) > _MOST:
+    if x.numel() // k > _MOST or k > _MOST or n > _MOST:
         raise ValueError(f'at most {_MOST} rows, inputs and outputs')
     if x.numel() == 0:
         # no rows: nothing to launch; the empty result stays connected to its inputs
@@ -172,11 +179,12 @@ def linear(x, weight, bias=None, activation=None, residual=None):
             y = y if bias is None else y + 0 * bias.sum()
             y = y if residual is None else y + residual
         return y
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, act)
     y, _ = _linear_forward(_rows(x), _rows(weight), bias if bias is None else bias.contiguous(),
                            None if residual is None else _rows(residual), act, False)
-    return y if x.dim() == 2 else y.view(x.shape[:-1] + (n,))
+    return y if flat else y.view(x.shape[:-1] + (n,))
 
 
 # ---------------------------------------------------------------------------------------------
