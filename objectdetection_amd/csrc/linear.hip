@@ -10,7 +10,7 @@
 // by columns first (one launch for all three).  Few rows, and the backward pass of small layers, go without matrix instructions.
 // Times: (25600, 1024, 4096) bf16 with bias, SiLU and residual 285 us, 243 of them the product (a library product of that size
 // takes 206 us), the rest the epilogue's 420 MB; forward and backward of (8192, 1024, 4096) bf16 304 us; (4097, 1155, 1001)
-// float32 with GELU 66 us; (1, 1024, 1024) bf16 3 us, a call of it 13 on the host.
+// float32 with GELU 66 us; (1, 1024, 1024) bf16 3 us, a call of it 12 on the host.
 #include "common.h"
 #include "odamd.h"
 
