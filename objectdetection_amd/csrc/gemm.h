@@ -153,7 +153,7 @@ struct GemmTile {
             constexpr int W = width.value, SLOTS = W / 8;           // 16-byte slots per row
             k = t * (64 / SLOTS) + lane / SLOTS;
             const int slot = lane % SLOTS, col = first + ((((slot >> 1) ^ gemm_turn<W>(k)) << 1) | (slot & 1)) * 8;
-            return o.p + (long long)k * o.ld + min(col, (o.cols - 1) & ~7) * 2;
+            return o.p + (long long)k * o.ld + column_at(col, o.cols);
         };
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
@@ -385,8 +385,6 @@ __device__ __forceinline__ void split_f16(float v, _Float16& hi, _Float16& lo) {
     const float rest = v - (float)hi;
     lo = fabsf(v) < 65504.0f ? (_Float16)rest : (_Float16)0.0f;
 }
-// Byte of value k's hi within its row; its lo lies 64 bytes on.
-__device__ __forceinline__ int split_at(int k) { return (k >> 5) * 128 + (k & 31) * 2; }
 // Eight of them, from a multiple of eight on.
 __device__ __forceinline__ void store_split8(char* hi_at, const float v[8], float scale) {
     f16x8_t hi, lo;

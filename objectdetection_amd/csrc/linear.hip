@@ -13,6 +13,7 @@
 // float32 with GELU 66 us; (1, 1024, 1024) bf16 3 us, a call of it 12 on the host.
 #include "common.h"
 #include "odamd.h"
+#include "offsets.h"
 
 #include <math.h>
 

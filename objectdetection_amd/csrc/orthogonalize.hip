@@ -31,6 +31,7 @@
 // 0.73 ms of norm and layout at the rate of a copy.
 #include "common.h"
 #include "odamd.h"
+#include "offsets.h"
 
 #include <math.h>
 
