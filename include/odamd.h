@@ -383,7 +383,8 @@ int odamd_adam_ema_ranges_step(float* param, const float* grad, float* exp_avg, 
  *   X = G / (|G|_F + eps), transposed while rows > cols;
  *   `steps` times (1 .. 32):  A = X X^T,  X = a X + (b A + c A A) X,  (a, b, c) = (3.4445, -4.7750, 2.0315);
  *   out = X, transposed back.
- * Matrices whose shorter side is at most 64 are computed in 64 bits and rounded once (steps over 10: as the others).  The
+ * Matrices whose shorter side is at most 64 are computed in 64 bits and rounded once (steps over 10: X is rounded to float32
+ * after every ten); their workspace is one float32 copy of the matrices and at most 0.7 MB for each matrix of over 256 columns.  The
  * others' products carry 22 bits per factor and sum in float32; out is rounded once.  With a float32 result a rounding grows by
  * 3.4445 per step in directions of small singular values, as in any float32 arithmetic of these formulas; with a bfloat16
  * result steps run in groups of five on A alone, which costs up to 1e-3 of the result's norm there, half a bfloat16 step.

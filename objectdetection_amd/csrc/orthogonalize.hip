@@ -11,7 +11,7 @@
 // with one product by X at the end of a phase of t steps: 1.5 m^2 n + (2 t - 1.5) m^3 multiply-adds for it (symmetric products
 // counted half) against t (1.5 m^2 n + 0.5 m^3).  What it costs is accuracy in the directions of small singular values: a
 // rounding of A grows by 3.4445^2 per step there, where a rounding of X grows by 3.4445.
-//   - At most 64 rows: A and all that follows in 64 bits, up to ten steps in one phase (further down: "at most 64 rows").
+//   - At most 64 rows: A and all that follows in 64 bits, phases of ten steps (further down: "at most 64 rows").
 //   - More rows, float32 results: phases of two steps, which keep float32's accuracy (error against 64 bits of 256 x 2304 noise
 //     with strong directions: 1.6e-6, one step a phase 1.9e-6), where n >= 2 m; one step a phase on squarer ones, which costs no
 //     more there.
@@ -42,7 +42,7 @@ namespace {
 constexpr double NS_A = 3.4445, NS_B = -4.7750, NS_C = 2.0315;
 constexpr float NS_SCALE = 4096.0f;
 constexpr int NS_GROUPS = 112;        // groups of one launch: their table travels in the kernel's arguments (4 KiB at most)
-constexpr int NS_FEW_STEPS = 10;      // steps that matrices of at most 64 rows run on A alone
+constexpr int NS_FEW_STEPS = 10;      // steps of a phase of matrices of at most 64 rows
 constexpr int NS_PARTS = 512;         // partial sums of squares per matrix, at most
 
 // stages: sums of squares, laying out, X X^T (whole, or a part of its reduction), P from A, products of square matrices, Q X,
@@ -85,7 +85,7 @@ __host__ __device__ inline long long ns_up(long long v, int to) { return (v + to
 __host__ __device__ inline int ns_few_cols(int t, int n) {
     return n <= (t == 1 ? 1536 : 1024 / t) ? (int)ns_up(n, 16) : (int)ns_up(ns_up(n, 32) / 32, t <= 2 ? 512 : 128);
 }
-// Workspace of a matrix then: Q and the partial sums of G G^T, in 64 bits
+// Workspace of a matrix that is taken in parts: Q and the partial sums of G G^T, in 64 bits
 __host__ __device__ inline long long ns_few_bytes(int t, int cols, int n) {
     return ns_up(8LL * (256 * t * t + ((long long)n + cols - 1) / cols * 128 * t * (t + 1)), 256);
 }
@@ -101,9 +101,6 @@ __host__ __device__ inline NsLayout ns_layout(int m, int n) {
     l.sq = l.xt1 + ns_up(n * mp * 4, 256);
     l.sq_size = ns_up(m * mp * 4, 256);
     l.end = l.sq + SQ_COUNT * l.sq_size;
-    const int rows = (m + 15) / 16;
-    const long long few = rows <= 4 ? ns_few_bytes(rows, ns_few_cols(rows, n), n) : 0;
-    l.end = few > l.end ? few : l.end;
     return l;
 }
 // Elements one workgroup of the norm pass takes: a multiple of eight that keeps the partial sums within NS_PARTS.
@@ -132,12 +129,14 @@ struct NsIo {
     float mu, grad_scale, decay, lr02, ema_keep, ema_take;   // decay: 1 - lr weight_decay, lr02: 0.2 lr
     int nesterov;
     double eps;
+    float* x;            // matrices of few rows: X between phases of steps, one matrix of the table behind the other
+    int scaled;          // and whether `in` is X already
 };
 
-struct NsPlace { int m, n, tall, tile; long long src; char* ws; };
+struct NsPlace { int m, n, tall, tile, group; long long src; char* ws; };
 
-// Which matrix a tile belongs to
-__device__ __forceinline__ NsPlace ns_find(const NsTable& t, int tile, int stage, int tile_size) {
+// Which matrix a tile belongs to.  few: workspaces are those of matrices of few rows, `few` 16-row tiles, in parts of tile_size columns
+__device__ __forceinline__ NsPlace ns_find(const NsTable& t, int tile, int stage, int tile_size, int few = 0) {
     // all groups at once: one latency, not one for every halving (78 matrices: 15 us launches are 0.5 us shorter)
     int lo = 0;
     if (t.n > 1) {
@@ -147,8 +146,8 @@ __device__ __forceinline__ NsPlace ns_find(const NsTable& t, int tile, int stage
     }
     const NsGroup& g = t.g[lo];
     const int each = ns_tiles(stage, tile_size, g.m, g.n), at = tile - g.tile0, which = at / each;
-    return {g.m, g.n, g.tall, at - which * each, g.src + (long long)which * g.m * g.n,
-            t.ws + (long long)g.ws * 256 + which * ns_layout(g.m, g.n).end};
+    return {g.m, g.n, g.tall, at - which * each, lo, g.src + (long long)which * g.m * g.n,
+            t.ws + (long long)g.ws * 256 + which * (few ? ns_few_bytes(few, tile_size, g.n) : ns_layout(g.m, g.n).end)};
 }
 
 // The optimizer's direction from the updated momentum
@@ -283,7 +282,8 @@ __global__ void __launch_bounds__(256) ns_split_kernel(NsTable t, NsIo io) {
 // ---- at most 64 rows -------------------------------------------------------------------------------------------------
 // All steps run on A = X X^T, in 64 bits (v_mfma_f64_16x16x4_f64, half the rate of the float32 instruction): a rounding of A, 2^-53,
 // grows to 2^-53 3.4445^18 = 5e-7 in ten steps, so the result has float32's accuracy, and the caller's matrix is read twice only,
-// for G G^T (whose trace is the norm) and for Q G.  What it costs is latency: 3 dependent products of m x m per step.
+// for G G^T (whose trace is the norm) and for Q G.  What it costs is latency: 3 dependent products of m x m per step.  More steps
+// start again from X every ten, which is held in float32 in between.
 // T: m in 16-row tiles.  Squares lie in LDS, rows LD doubles apart: sixteen rows at two neighbouring k touch all 64 banks.
 template <int T_> struct NsFew {
     static constexpr int T = T_, N = 16 * T, LD = N + 2, SQ = N * LD, TRI = T * (T + 1) / 2;
@@ -409,9 +409,9 @@ __device__ __forceinline__ double ns_few_sum(const double* sums, int u) {
     return s;
 }
 
-// Q / (|G| + eps) from G G^T: value u of it is get(u).  Left in the third square of `lds`.
+// Q / (|G| + eps) from G G^T (Q where G is X already): value u of it is get(u).  Left in the third square of `lds`.
 template <int T, typename GET>
-__device__ __forceinline__ double* ns_few_steps(double* lds, int steps, double eps, GET&& get) {
+__device__ __forceinline__ double* ns_few_steps(double* lds, int steps, const NsIo& io, GET&& get) {
     using F = NsFew<T>;
     constexpr int EACH = (F::SUMS + F::THREADS - 1) / F::THREADS, LD = F::LD;
     double *a = lds, *p = lds + F::SQ, *q = lds + 2 * F::SQ;
@@ -437,7 +437,7 @@ __device__ __forceinline__ double* ns_few_steps(double* lds, int steps, double e
             }
 #pragma unroll
             for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-            const double inv = 1.0 / (sqrt(sum) + eps);
+            const double inv = io.scaled ? 1.0 : 1.0 / (sqrt(sum) + io.eps);
             am = am * inv * inv;
             for (int step = 0; step < steps; ++step) {
                 const f64x4_t s = times(am, am);
@@ -474,7 +474,7 @@ __device__ __forceinline__ double* ns_few_steps(double* lds, int steps, double e
     double sum = lane < F::N ? a[lane * LD + lane] : 0.0;
 #pragma unroll
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    const double inv = 1.0 / (sqrt(sum) + eps);
+    const double inv = io.scaled ? 1.0 : 1.0 / (sqrt(sum) + io.eps);
     __syncthreads();
     for (int i = threadIdx.x; i < F::SQ; i += F::THREADS) a[i] = i % LD < F::N ? a[i] * inv * inv : 0.0;
     __syncthreads();
@@ -614,20 +614,20 @@ __global__ void __launch_bounds__(NsFew<T>::THREADS) ns_few_kernel(NsTable t, Ns
     using F = NsFew<T>;
     extern __shared__ __attribute__((aligned(16))) char space[];
     double* lds = (double*)space;
-    const NsPlace p = ns_find(t, blockIdx.x, STAGE, cols);
+    const NsPlace p = ns_find(t, blockIdx.x, STAGE, cols, T);
     double* q_at = (double*)p.ws;                             // Q, then the partial sums
     double* parts = q_at + F::N * F::N;
     const int from = p.tile * cols, to = from + min(p.n - from, cols);
     if constexpr (STAGE == ST_WHOLE) {
         ns_few_gram<T, MUON, DT>(io, p, 0, p.n, lds);
-        const double* q = ns_few_steps<T>(lds, steps, io.eps, [&](int u) { return ns_few_sum<T>(lds, u); });
+        const double* q = ns_few_steps<T>(lds, steps, io, [&](int u) { return ns_few_sum<T>(lds, u); });
         ns_few_out<T, MUON, DT>(io, p, 0, p.n, q);
     } else if constexpr (STAGE == ST_GRAM) {
         ns_few_gram<T, MUON, DT>(io, p, from, to, lds);
         for (int u = threadIdx.x; u < F::SUMS; u += F::THREADS) parts[(long long)p.tile * F::SUMS + u] = ns_few_sum<T>(lds, u);
     } else if constexpr (STAGE == ST_STEPS) {
         const int n_parts = ns_tiles(ST_GRAM, cols, p.m, p.n);
-        const double* q = ns_few_steps<T>(lds, steps, io.eps, [&](int u) {
+        const double* q = ns_few_steps<T>(lds, steps, io, [&](int u) {
             double s = parts[u];
 #pragma unroll 8
             for (int k = 1; k < n_parts; ++k) s += parts[(long long)k * F::SUMS + u];
@@ -638,6 +638,39 @@ __global__ void __launch_bounds__(NsFew<T>::THREADS) ns_few_kernel(NsTable t, Ns
         for (int i = threadIdx.x; i < F::N * F::N; i += F::THREADS) lds[i / F::N * F::LD + i % F::N] = q_at[i];
         __syncthreads();
         ns_few_out<T, MUON, DT>(io, p, from, to, lds);
+    }
+}
+
+// X before the first phase of many (what is left of a phase is float32, and the direction of the optimizer's step is made once), and
+// BACK: the result of the last one for the caller.
+template <bool MUON, int DT, bool BACK>
+__global__ void __launch_bounds__(256) ns_few_move_kernel(NsTable t, NsIo io) {
+    const NsPlace p = ns_find(t, blockIdx.x, ST_NORM, 0);
+    long long at_x = p.src - t.g[p.group].src;
+    for (int i = 0; i < p.group; ++i) at_x += (long long)t.g[i].m * t.g[i].n * t.g[i].count;
+    const long long total = (long long)p.m * p.n, share = ns_share(p.m, p.n), from = p.tile * share;
+    const long long to = from + share < total ? from + share : total;
+    const float step = MUON ? io.lr02 * sqrtf((float)p.n) : 0.0f;
+    for (long long i = from + threadIdx.x; i < to; i += 256) {
+        const long long at = p.src + i;
+        if constexpr (!BACK) {
+            float v[4], m[4];
+            ns_load4<DT>(io.in, at, 1, 1, v);
+            if constexpr (MUON) {
+                ns_load4<ODAMD_DTYPE_F32>(io.momentum, at, 1, 1, m);
+                m[0] = io.mu * m[0] + v[0] * io.grad_scale;
+                io.momentum[at] = m[0];
+                v[0] = ns_direction(io, v[0], m[0]);
+            }
+            io.x[at_x + i] = v[0];
+        } else if constexpr (MUON) {
+            const float w = io.param[at] * io.decay - step * io.x[at_x + i];
+            io.param[at] = w;
+            if (io.ema) io.ema[at] = io.ema_keep * io.ema[at] + io.ema_take * w;
+        } else {
+            const float v[4] = {io.x[at_x + i]};
+            ns_store4<DT>(io.out, at, 1, 1, v);
+        }
     }
 }
 
@@ -989,11 +1022,49 @@ int ns_few(NsTable& t, const NsIo& io, int steps, int n, hipStream_t s) {
 }
 
 template <bool MUON, int DT>
-int ns_run(NsTable& t, const NsIo& io, int steps, hipStream_t s) {
+int ns_few_phase(NsTable& t, const NsIo& io, int steps, hipStream_t s) {
     const int rows = ns_few_rows(t), cols = ns_longest(t);
-    if (rows <= 4 && steps <= NS_FEW_STEPS)
-        return rows == 1 ? ns_few<1, MUON, DT>(t, io, steps, cols, s) : rows == 2 ? ns_few<2, MUON, DT>(t, io, steps, cols, s)
-             : rows == 3 ? ns_few<3, MUON, DT>(t, io, steps, cols, s) : ns_few<4, MUON, DT>(t, io, steps, cols, s);
+    return rows == 1 ? ns_few<1, MUON, DT>(t, io, steps, cols, s) : rows == 2 ? ns_few<2, MUON, DT>(t, io, steps, cols, s)
+         : rows == 3 ? ns_few<3, MUON, DT>(t, io, steps, cols, s) : ns_few<4, MUON, DT>(t, io, steps, cols, s);
+}
+template <bool MUON, int DT, bool BACK>
+int ns_few_move(NsTable& t, const NsIo& io, hipStream_t s) {
+    if (ns_count(t, ST_NORM, 0, 256) < 0) return ODAMD_E_LIMIT;
+    ns_few_move_kernel<MUON, DT, BACK><<<t.tiles, 256, 0, s>>>(t, io);
+    return (int)hipGetLastError();
+}
+// More steps than a phase takes.  X lies in the caller's result where that is float32, else in the workspace.
+template <bool MUON, int DT>
+int ns_few_phases(NsTable& t, const NsIo& io, int steps, hipStream_t s) {
+    constexpr bool OWN = MUON || DT != ODAMD_DTYPE_F32;
+    NsTable x = t;
+    NsIo mid = {};
+    mid.eps = io.eps;
+    mid.in = io.in;
+    mid.out = io.out;
+    int rc = 0;
+    if constexpr (OWN) {
+        long long at = 0;
+        for (int i = 0; i < x.n; ++i) {
+            x.g[i].src = at;
+            at += (long long)x.g[i].m * x.g[i].n * x.g[i].count;
+        }
+        mid.in = mid.out = io.x;
+        rc = ns_few_move<MUON, DT, false>(t, io, s);
+    }
+    for (int done = 0; done < steps && rc == 0; done += NS_FEW_STEPS) {
+        rc = ns_few_phase<false, ODAMD_DTYPE_F32>(x, mid, steps - done < NS_FEW_STEPS ? steps - done : NS_FEW_STEPS, s);
+        mid.in = mid.out;
+        mid.scaled = 1;
+    }
+    if constexpr (OWN)
+        if (rc == 0) rc = ns_few_move<MUON, DT, true>(t, io, s);
+    return rc;
+}
+
+template <bool MUON, int DT>
+int ns_run(NsTable& t, const NsIo& io, int steps, hipStream_t s) {
+    if (ns_few_rows(t) <= 4) return steps <= NS_FEW_STEPS ? ns_few_phase<MUON, DT>(t, io, steps, s) : ns_few_phases<MUON, DT>(t, io, steps, s);
     constexpr bool LOOSE = MUON || DT == ODAMD_DTYPE_BF16;
     int phase = LOOSE ? 5 : 2;
     for (int i = 0; i < t.n; ++i)
@@ -1072,15 +1143,27 @@ void ns_fill(NsTable& t, const odamd_matrix* matrices, int from, int count) {
         t.g[to] = g;
     }
 }
-// Places their workspaces one behind the other; the bytes of all of them
-long long ns_place(NsTable& t, int steps) {
-    const int rows = ns_few_rows(t), n = ns_longest(t);
-    long long at = 0;
+// Places the workspaces of the table's matrices one behind the other; the bytes of all of them.  A table of few rows: X of all its
+// matrices (`x` bytes) lies before them, and only matrices that are taken in parts need more.
+size_t ns_place(NsTable& t, size_t& x) {
+    const int rows = ns_few_rows(t), n = ns_longest(t), cols = rows <= 4 ? ns_few_cols(rows, n) : 0;
+    size_t at = 0;
+    long long all = 0;
     for (int i = 0; i < t.n; ++i) {
+        const NsGroup& g = t.g[i];
         t.g[i].ws = (unsigned)(at / 256);
-        at += rows <= 4 && steps <= NS_FEW_STEPS ? ns_few_bytes(rows, ns_few_cols(rows, n), t.g[i].n) : ns_layout(t.g[i].m, t.g[i].n).end;
+        all += (long long)g.m * g.n * g.count;
+        at += (size_t)g.count * (rows > 4 ? ns_layout(g.m, g.n).end : cols < n ? ns_few_bytes(rows, cols, g.n) : 0);
     }
-    return at;
+    x = rows <= 4 ? (size_t)ns_up(all * 4, 256) : 0;
+    return x + at;
+}
+// One group
+void ns_single(NsTable& t, int batch, int rows, int cols) {
+    t.n = 1;
+    ns_orient(t.g[0], rows, cols);
+    t.g[0].src = 0;
+    t.g[0].count = batch;
 }
 
 }  // namespace
@@ -1089,9 +1172,10 @@ extern "C" {
 
 size_t odamd_orthogonalize_workspace_bytes(int batch, int rows, int cols) {
     if (batch < 1 || !ns_shape_ok(rows, cols)) return 0;
-    NsGroup g;
-    ns_orient(g, rows, cols);
-    return (size_t)batch * ns_layout(g.m, g.n).end;
+    NsTable t;
+    size_t x;
+    ns_single(t, batch, rows, cols);
+    return ns_place(t, x);
 }
 
 int odamd_orthogonalize(const void* x, void* out, int batch, int rows, int cols, int steps, double eps, int dtype, void* workspace,
@@ -1102,15 +1186,14 @@ int odamd_orthogonalize(const void* x, void* out, int batch, int rows, int cols,
     if ((uintptr_t)workspace & 255) return ODAMD_E_ALIGN;
     if (workspace_bytes < odamd_orthogonalize_workspace_bytes(batch, rows, cols)) return ODAMD_E_WORKSPACE;
     NsTable t;
-    t.n = 1;
-    t.ws = (char*)workspace;
-    ns_orient(t.g[0], rows, cols);
-    t.g[0].src = 0;
-    t.g[0].ws = 0;
-    t.g[0].count = batch;
+    size_t held;
+    ns_single(t, batch, rows, cols);
+    ns_place(t, held);
+    t.ws = (char*)workspace + held;
     NsIo io = {};
     io.in = x;
     io.out = out;
+    io.x = (float*)workspace;
     io.eps = eps;
     return dtype == ODAMD_DTYPE_F32 ? ns_run<false, ODAMD_DTYPE_F32>(t, io, steps, (hipStream_t)stream)
                                     : ns_run<false, ODAMD_DTYPE_BF16>(t, io, steps, (hipStream_t)stream);
@@ -1123,11 +1206,10 @@ size_t odamd_muon_workspace_bytes(const odamd_matrix* matrices_host, int n_matri
     size_t most = 0;
     for (int i = 0; i < n_matrices; i += NS_GROUPS) {
         NsTable t;
+        size_t x;
         ns_fill(t, matrices_host, i, n_matrices);
-        for (int steps : {1, NS_FEW_STEPS + 1}) {
-            const size_t need = (size_t)ns_place(t, steps);
-            most = need > most ? need : most;
-        }
+        const size_t need = ns_place(t, x);
+        most = need > most ? need : most;
     }
     return most;
 }
@@ -1158,9 +1240,11 @@ int odamd_muon_ema_step(float* param, const float* grad, float* momentum, float*
     io.eps = eps;
     for (int i = 0; i < n_matrices; i += NS_GROUPS) {
         NsTable t;
+        size_t held;
         ns_fill(t, matrices_host, i, n_matrices);
-        ns_place(t, steps);
-        t.ws = (char*)workspace;
+        ns_place(t, held);
+        t.ws = (char*)workspace + held;
+        io.x = (float*)workspace;
         const int rc = ns_run<true, ODAMD_DTYPE_F32>(t, io, steps, (hipStream_t)stream);
         if (rc != 0) return rc;
     }

@@ -194,7 +194,7 @@ def orthogonalize(x, steps=5, eps=1e-7, out=None):
     """Brings the singular values of every matrix of x (..., rows, cols) near one and keeps its singular vectors: `steps`
     Newton-Schulz products with the coefficients (3.4445, -4.7750, 2.0315) from x / (|x|_F + eps) on.  Five steps take
     singular values from 0.003 of the norm up to between 0.68 and 1.21.  float32 or bfloat16, rounded once.  Matrices with a side
-    of at most 64 are computed in 64 bits, others with products of 22 bits; bfloat16 results of those are off by up to 1e-3 of
+    of at most 64 are computed in 64 bits (over ten steps rounded to float32 after every ten), others with products of 22 bits; bfloat16 results of those are off by up to 1e-3 of
     their norm in directions of small singular values (half a bfloat16 step).  `out` may be x itself.  Not differentiable: the
     result belongs to no graph.  A matrix with a NaN or an infinity gives NaN."""
     _check_tensor('x', x)

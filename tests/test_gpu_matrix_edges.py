@@ -1,0 +1,89 @@
+"""GPU tests of the matrix operators at their edges, beside test_gpu_matrix.py, whose references and bounds they use."""
+import math
+
+import pytest
+import torch
+
+from .test_gpu_matrix import HALF, orth64, randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope='module')
+def mx():
+    from objectdetection_amd import matrix
+    return matrix
+
+
+# ---------------------------------------------------------------------------------------------
+# few rows, more than ten steps
+# ---------------------------------------------------------------------------------------------
+# X is rounded to float32 after every ten steps.  A step changes a difference of two X by at most the largest slope of
+# a s + b s^3 + c s^5 where singular values are, 4.25 at 1.21 (3.4445 at zero); norms lie between 0.68 and 1.21 times the root of
+# the rank, a factor of 1.78.
+def rounded_after_ten(steps):
+    return 1.78 * 4.25 ** (steps - 10) * (2.0 ** -24 + 1e-9)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('batch, rows, cols', [(3, 1, 7), (1, 16, 27), (5, 30, 50), (2, 40, 33), (2, 64, 200), (3, 2000, 16), (1, 33, 900), (2, 61, 1001)])
+def test_few_rows_more_than_ten_steps(mx, batch, rows, cols, dtype):
+    g = randn(batch, rows, cols, dtype=dtype, scale=1e-3)
+    for steps in (11, 13, 14):
+        got = mx.orthogonalize(g, steps=steps)
+        for i in range(batch):
+            ref = orth64(g[i], steps=steps)
+            assert float((got[i].double() - ref).norm()) <= (HALF[dtype] + rounded_after_ten(steps)) * float(ref.norm())
+        twin = g.clone()
+        assert torch.equal(mx.orthogonalize(twin, steps=steps, out=twin), got)
+    for steps in (20, 21, 32):
+        got = mx.orthogonalize(g, steps=steps).double().cpu()
+        for i in range(batch):
+            s = torch.linalg.svdvals(got[i])
+            assert 0.65 < float(s.min()) and float(s.max()) < 1.25
+
+
+def test_few_rows_more_than_ten_steps_and_no_numbers(mx):
+    g = randn(5, 40, 70)
+    g[1] = 0
+    g[2, 3, 4] = float('nan')
+    g[3, 39, 69] = float('inf')
+    for x in (g, g.bfloat16()):
+        y = mx.orthogonalize(x, steps=23)
+        assert float(y[1].abs().max()) == 0.0
+        assert bool(torch.isnan(y[2]).all()) and bool(torch.isnan(y[3]).all()) and bool(torch.isfinite(y[[0, 4]]).all())
+
+
+@pytest.mark.parametrize('top, long', [(16, 200), (33, 200), (64, 5000), (5, 40000)])
+def test_muon_step_of_few_rows_more_than_ten_steps(mx, top, long):
+    """Tables in one workgroup a matrix and in parts, tall and wide, at odd offsets; what lies between stays."""
+    shapes = [(top, top), (3, long), (long, top), (top - 3, 77), (1, 1), (5, 9), (long - 1, 2)]
+    matrices, at = [], 1
+    for r, c in shapes:
+        matrices.append((at, r, c))
+        at += r * c + 3
+    p, g, m, e = (randn(at, seed=i, scale=s) for i, s in enumerate((0.03, 1e-3, 1e-3, 0.03)))
+    steps = 12
+    for ema, nesterov in ((e, True), (None, False)):
+        rp, rm, re = p.double(), m.double(), e.double()
+        p1, m1, e1 = p.clone(), m.clone(), None if ema is None else ema.clone()
+        mx.muon_step(p1, g, m1, matrices, lr=0.01, nesterov=nesterov, weight_decay=0.1, ema=e1, ema_decay=0.7, grad_scale=0.5, steps=steps)
+        inside = torch.zeros_like(p, dtype=torch.bool)
+        for o, r, c in matrices:
+            s = slice(o, o + r * c)
+            inside[s] = True
+            gs = g[s].double() * 0.5
+            rm[s] = 0.95 * rm[s] + gs
+            u = gs + 0.95 * rm[s] if nesterov else rm[s]
+            o64 = orth64(u.view(r, c), steps=steps).reshape(-1)
+            rp[s] = rp[s] * (1 - 0.01 * 0.1) - 0.01 * 0.2 * math.sqrt(max(r, c)) * o64
+            re[s] = 0.7 * re[s] + (1 - 0.7) * rp[s]
+            # X's rounding, and the three of u, which singular values of these matrices carry to one within seven steps
+            step = 0.01 * 0.2 * math.sqrt(max(r, c)) * float(o64.norm())
+            allowed = step * (4 * rounded_after_ten(steps) + 3.4445 ** 7 * 3 * 2.0 ** -24) + 4 * 2.0 ** -24 * float(rp[s].norm())
+            assert float((p1[s].double() - rp[s]).norm()) <= allowed
+            assert float((m1[s].double() - rm[s]).abs().max()) <= 4 * 2.0 ** -24 * float(rm[s].abs().max())
+            if ema is not None:
+                assert float((e1[s].double() - re[s]).norm()) <= allowed + 4 * 2.0 ** -24 * float(re[s].norm())
+        for new, old in ((p1, p), (m1, m)) + (((e1, e),) if ema is not None else ()):
+            assert torch.equal(new[~inside], old[~inside])
