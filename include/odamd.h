@@ -419,7 +419,8 @@ int odamd_muon_ema_step(float* param, const float* grad, float* momentum, float*
  * number for a smaller one).  r may be y itself; no other operand may overlap an output.  Sums are float32 and y is rounded once; float32 products carry 22 bits
  * of each value, counted from the largest magnitude of its row of x or w down to 2^-17 of it and with the same absolute
  * step below.  A float32 row that holds an infinity gives NaN or infinity.  m, k and n are at most 2^31 - 2^16.
- * The workspace (256-byte aligned) may be NULL where the query returns 0. */
+ * The workspace (256-byte aligned) may be NULL where the query returns 0.  The queries go by the call's own descriptor, pointers
+ * included: bfloat16 operands on 16-byte boundaries whose rows are a multiple of eight long and apart are read in place. */
 #define ODAMD_ACT_NONE 0
 #define ODAMD_ACT_SILU 1
 #define ODAMD_ACT_GELU 2 /* z (1 + erf(z / sqrt 2)) / 2 */

@@ -848,8 +848,9 @@ int lin_products(LinLaunch& t, int count, LinSpace& ws, bool go, hipStream_t s) 
     return (int)hipGetLastError();
 }
 
+// Whether products read the caller's rows as they are: no workspace for these.  A query without the pointer counts on nothing.
 template <int DT> bool lin_direct(const void* p, long long ld, int k) {
-    return DT == ODAMD_DTYPE_BF16 && ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && k % 8 == 0;
+    return DT == ODAMD_DTYPE_BF16 && p && ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && k % 8 == 0;
 }
 // Blocks of a launch over the jobs: 64 x 64 tiles, or groups of rows; -1: more than a launch takes
 int lin_tiles(LinJobs& t, int unit_rows) {
@@ -891,8 +892,7 @@ int lin_forward_rows(const odamd_linear_desc& d, const LinEnd& end, hipStream_t 
 template <int DT>
 int lin_forward(const odamd_linear_desc& d, LinSpace& ws, bool go, hipStream_t s) {
     const LinEnd end = {d.bias, d.residual, d.y, d.z, d.r_ld, d.y_ld, d.z_ld, d.act};
-    // measuring, the pointers are not known: the workspace of products serves where only they may say
-    const bool direct = !go || (lin_direct<DT>(d.x, d.x_ld, d.k) && lin_direct<DT>(d.w, d.w_ld, d.k));
+    const bool direct = lin_direct<DT>(d.x, d.x_ld, d.k) && lin_direct<DT>(d.w, d.w_ld, d.k);
     if (lin_by_rows<DT>(d.m, d.k, d.n, direct)) return go ? lin_forward_rows<DT>(d, end, s) : 0;
     constexpr int SIZE = DT == ODAMD_DTYPE_F32 ? 4 : 2;
     LinLaunch launch = {};
@@ -904,8 +904,7 @@ int lin_forward(const odamd_linear_desc& d, LinSpace& ws, bool go, hipStream_t s
     LinJobs jobs = {};
     const long long kp = lin_up(d.k, lin_chunk<DT>());
     const auto operand = [&](const void* p, long long ld, int rows, GemmOperand& o, const unsigned*& max) {
-        // where the caller's rows can be read as they are, no workspace is used; measuring, the pointers are not known to be
-        if (go && lin_direct<DT>(p, ld, d.k)) {
+        if (lin_direct<DT>(p, ld, d.k)) {
             o = {(const char*)p, ld * SIZE, rows};
             return;
         }
@@ -986,13 +985,13 @@ int lin_backward_bf16(const odamd_linear_grad_desc& d, LinSpace& ws, bool go, hi
     const long long np = lin_up(d.n, 64), kp = lin_up(d.k, 64);
     // dz by rows serves both products; dy itself where there is no activation and its rows can be read as they are
     GemmOperand dz = {};
-    const bool direct = go && d.act == ODAMD_ACT_NONE && lin_direct<DT>(d.dy, d.dy_ld, d.n);
+    const bool direct = d.act == ODAMD_ACT_NONE && lin_direct<DT>(d.dy, d.dy_ld, d.n);
     if (t.count) {
         if (!direct) t.dz().rows = ws.take(d.m * np * 2);
         dz = direct ? GemmOperand{(const char*)d.dy, d.dy_ld * 2, d.m, d.n} : GemmOperand{t.dz().rows, np * 2, d.m, d.n};
     }
     const auto across = [&](const void* p, long long ld, int rows) {
-        if (go && lin_direct<DT>(p, ld, d.k)) return GemmOperand{(const char*)p, ld * 2, rows, d.k};
+        if (lin_direct<DT>(p, ld, d.k)) return GemmOperand{(const char*)p, ld * 2, rows, d.k};
         LinJob& j = t.add(p, ld, rows, d.k);
         j.rows = ws.take(rows * kp * 2);
         return GemmOperand{j.rows, kp * 2, rows, d.k};
