@@ -7,6 +7,7 @@ and takes its workspace from torch's allocator, so it can be captured into a gra
 """
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import lib, check
@@ -37,6 +38,21 @@ def _call(device, fn, *args):
         return fn(*args, _stream(device))
     with torch.cuda.device(device):
         return fn(*args, _stream(device))
+
+
+_tracing_state = torch._C._get_tracing_state
+
+
+def _watched():
+    """Whether something other than the backward pass follows operations on tensors: forward-mode differentiation or torch.jit.trace.
+    What is launched through raw pointers escapes both; an autograd function does not: it refuses a tangent, and a trace
+    records it."""
+    return forward_ad._current_level >= 0 or _tracing_state() is not None
+
+
+def _refuse_trace(name):
+    if _tracing_state() is not None:
+        raise RuntimeError(f'{name} writes to its arguments, which a trace does not record')
 
 
 def _ptr(t):
@@ -146,7 +162,7 @@ _Linear.gradients_once = staticmethod(torch.autograd.function.once_differentiabl
 def linear(x, weight, bias=None, activation=None, residual=None):
     """act(x W^T + bias) + residual in one product.  x: (..., k); weight: (n, k); bias: (n,); residual: (..., n); all of one
     type, float32 or bfloat16.  activation: None, 'silu', 'gelu' (the erf form) or 'relu'.  Rows may be strided (a slice of a
-    wider, concatenated buffer is read in place).  Differentiable once in all four tensors; in bfloat16 the pre-activation
+    wider, concatenated buffer is read in place).  Differentiable once in all four tensors, backward only; in bfloat16 the pre-activation
     that the backward pass keeps is float16 and the gradient at it bfloat16.  As with every differentiable torch operation,
     a backward pass is captured into a graph on leaves that no eager graph holds any more (detached copies of them will do).
     float32 products carry 22 bits per value, counted from the largest magnitude of its row; a float32 row with an infinity
@@ -179,8 +195,8 @@ def linear(x, weight, bias=None, activation=None, residual=None):
             y = y if bias is None else y + 0 * bias.sum()
             y = y if residual is None else y + residual
         return y
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+    if (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                     or (residual is not None and residual.requires_grad))) or _watched():
         return _Linear.apply(x, weight, bias, residual, act)
     y, _ = _linear_forward(_rows(x), _rows(weight), bias if bias is None else bias.contiguous(),
                            None if residual is None else _rows(residual), act, False)
@@ -190,36 +206,57 @@ def linear(x, weight, bias=None, activation=None, residual=None):
 # ---------------------------------------------------------------------------------------------
 # orthogonalisation and the optimizer step
 # ---------------------------------------------------------------------------------------------
+class _Orthogonalize(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, steps, eps):
+        return _orthogonalize(x, steps, eps, x.new_empty(x.shape))
+
+    @staticmethod
+    def backward(ctx, dy):
+        raise RuntimeError('orthogonalize has no backward pass: detach its argument or its result')
+
+
+def _orthogonalize(x, steps, eps, out):
+    rows, cols = x.size(-2), x.size(-1)
+    batch = x.numel() // max(rows * cols, 1)
+    if batch == 0 or rows * cols == 0:
+        return out
+    src = x if x.is_contiguous() else x.detach().contiguous()
+    size = lib.odamd_orthogonalize_workspace_bytes(batch, rows, cols)
+    ws = _workspace(size, x.device)
+    check(_call(x.device, lib.odamd_orthogonalize, src.data_ptr(), out.data_ptr(), batch, rows, cols, steps, eps,
+                _DTYPES[x.dtype], ws.data_ptr(), size), 'orthogonalize')
+    return out
+
+
 def orthogonalize(x, steps=5, eps=1e-7, out=None):
     """Brings the singular values of every matrix of x (..., rows, cols) near one and keeps its singular vectors: `steps`
     Newton-Schulz products with the coefficients (3.4445, -4.7750, 2.0315) from x / (|x|_F + eps) on.  Five steps take
-    singular values from 0.003 of the norm up to between 0.68 and 1.21.  float32 or bfloat16, rounded once.  Matrices with a side
-    of at most 64 are computed in 64 bits (over ten steps rounded to float32 after every ten), others with products of 22 bits; bfloat16 results of those are off by up to 1e-3 of
-    their norm in directions of small singular values (half a bfloat16 step).  `out` may be x itself.  Not differentiable: the
-    result belongs to no graph.  A matrix with a NaN or an infinity gives NaN."""
+    singular values from 0.003 of the norm up to between 0.68 and 1.21.  float32 or bfloat16, rounded once.  Matrices with a
+    side of at most 64 are computed in 64 bits (over ten steps rounded to float32 after every ten), others with products of 22
+    bits; bfloat16 results of those are off by up to 1e-3 of their norm in directions of small singular values (half a bfloat16
+    step).  A matrix with a NaN or an infinity gives NaN.  `out` may be x itself.  Not differentiable: a backward pass that
+    reaches the result raises, and `out` belongs to no graph."""
     _check_tensor('x', x)
     if x.dim() < 2:
         raise ValueError(f'x must have rows and columns, not shape {tuple(x.shape)}')
     if not 1 <= int(steps) <= 32 or not eps >= 0:
         raise ValueError('steps must be 1 to 32, eps must not be negative')
     rows, cols = x.size(-2), x.size(-1)
-    batch = x.numel() // max(rows * cols, 1)
-    if rows * cols > _MOST or batch > _MOST:
+    if rows * cols > _MOST or x.numel() // max(rows * cols, 1) > _MOST:
         raise ValueError(f'at most {_MOST} elements of a matrix and matrices')
+    steps, eps = int(steps), float(eps)
     if out is None:
-        out = x.new_empty(x.shape)
-    else:
-        _check_tensor('out', out, x.dtype, x.device)
-        if out.shape != x.shape or not out.is_contiguous():
-            raise ValueError('out must be contiguous and have the shape of x')
-    if batch == 0 or rows * cols == 0:
-        return out
-    src = x if x.is_contiguous() else x.detach().contiguous()
-    size = lib.odamd_orthogonalize_workspace_bytes(batch, rows, cols)
-    ws = _workspace(size, x.device)
-    check(_call(x.device, lib.odamd_orthogonalize, src.data_ptr(), out.data_ptr(), batch, rows, cols, int(steps), float(eps),
-                _DTYPES[x.dtype], ws.data_ptr(), size), 'orthogonalize')
-    return out
+        if (x.requires_grad and torch.is_grad_enabled()) or _watched():
+            return _Orthogonalize.apply(x, steps, eps)
+        return _orthogonalize(x, steps, eps, x.new_empty(x.shape))
+    _check_tensor('out', out, x.dtype, x.device)
+    if out.shape != x.shape or not out.is_contiguous():
+        raise ValueError('out must be contiguous and have the shape of x')
+    _refuse_trace('orthogonalize into `out`')
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise RuntimeError('orthogonalize into `out` has no tangent')
+    return _orthogonalize(x, steps, eps, out)
 
 
 class MatrixTable:
@@ -276,6 +313,7 @@ def muon_step(param, grad, momentum, matrices, lr, momentum_decay=0.95, nesterov
         raise ValueError(f'matrices end at {table.end}, the buffers at {param.numel()}')
     if not 1 <= int(steps) <= 32 or not eps >= 0:
         raise ValueError('steps must be 1 to 32, eps must not be negative')
+    _refuse_trace('muon_step')
     ws = _workspace(table.workspace_bytes, param.device)
     check(_call(param.device, lib.odamd_muon_ema_step, param.data_ptr(), grad.data_ptr(), momentum.data_ptr(), _ptr(ema),
                 table.table.ctypes.data, len(table), lr, momentum_decay, int(nesterov), weight_decay, int(steps), eps,

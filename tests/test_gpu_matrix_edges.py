@@ -87,3 +87,38 @@ def test_muon_step_of_few_rows_more_than_ten_steps(mx, top, long):
                 assert float((e1[s].double() - re[s]).norm()) <= allowed + 4 * 2.0 ** -24 * float(re[s].norm())
         for new, old in ((p1, p), (m1, m)) + (((e1, e),) if ema is not None else ()):
             assert torch.equal(new[~inside], old[~inside])
+
+
+# ---------------------------------------------------------------------------------------------
+# who else looks at the tensors
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.filterwarnings('ignore')
+def test_traced_calls_compute(mx):
+    x, w, b, r = randn(30, 40), randn(24, 40, seed=1), randn(24, seed=2), randn(30, 24, seed=3)
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad):
+            layer = torch.jit.trace(lambda t, u: mx.linear(t, w, b, 'silu', u), (x, r), check_trace=False)
+            orth = torch.jit.trace(lambda t: mx.orthogonalize(t), (x,), check_trace=False)
+            for seed in (10, 11):
+                other = randn(30, 40, seed=seed)
+                assert torch.equal(layer(other, r), mx.linear(other, w, b, 'silu', r))
+                assert torch.equal(orth(other), mx.orthogonalize(other))
+
+
+def test_forward_mode_is_refused(mx):
+    from torch.autograd import forward_ad
+    x, w = randn(30, 40), randn(24, 40, seed=1)
+    plain = mx.linear(x, w)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: mx.linear(dual, w), lambda: mx.orthogonalize(dual)):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert torch.equal(mx.linear(x, w), plain)
+
+
+def test_orthogonalize_is_no_part_of_a_backward_pass(mx):
+    x = randn(30, 40).requires_grad_()
+    with pytest.raises(RuntimeError, match='no backward pass'):
+        mx.orthogonalize(x).sum().backward()
+    assert torch.equal(mx.orthogonalize(x).detach(), mx.orthogonalize(x.detach()))

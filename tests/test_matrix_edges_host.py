@@ -1,6 +1,8 @@
 """Matrix operators at their edges, what the host decides: workspaces, refusals, and how they meet autograd."""
 import numpy as np
 import pytest
+import torch
+from torch.autograd import forward_ad
 
 from objectdetection_amd import matrix
 from objectdetection_amd._lib import lib
@@ -39,3 +41,63 @@ def test_a_dense_layer_asks_for_what_it_writes():
         assert back(act=act, dx=P, dw=None, w=P + 2) == sums + laid + n * k * 2
         assert back(act=act, dx=None, x=P + 2) == sums + laid + cut + m * k * 2
     assert back(act=0, dx=P, dw=None, dy=P + 2) == sums + dz
+
+
+# ---------------------------------------------------------------------------------------------
+# who else looks at the tensors: forward-mode differentiation, traces, a backward pass
+# ---------------------------------------------------------------------------------------------
+@pytest.fixture
+def on_host(monkeypatch):
+    """The Python layer over host arithmetic that, like the kernels, nothing of torch sees."""
+    def forward(x, weight, bias, residual, act, keep_z):
+        y = x.new_empty((x.shape[0], weight.shape[0]))
+        np.copyto(np.from_dlpack(y.detach()), np.from_dlpack(x.detach()) @ np.from_dlpack(weight.detach()).T)
+        return y, None
+
+    def orthogonal(x, steps, eps, out):
+        np.copyto(np.from_dlpack(out.detach()), 2 * np.from_dlpack(x.detach()))
+        return out
+    monkeypatch.setattr(matrix, '_check_tensor', lambda *a, **kw: None)
+    monkeypatch.setattr(matrix, '_linear_forward', forward)
+    monkeypatch.setattr(matrix, '_orthogonalize', orthogonal)
+
+
+@pytest.mark.parametrize('grad', [False, True])
+def test_a_tangent_is_refused_and_not_lost(on_host, grad):
+    x, w = torch.randn(3, 4), torch.randn(5, 4)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: matrix.linear(dual, w), lambda: matrix.linear(w, dual), lambda: matrix.orthogonalize(dual)):
+            with pytest.raises(NotImplementedError, match='forward mode'):
+                call()
+        with pytest.raises(RuntimeError, match='tangent'):
+            matrix.orthogonalize(dual, out=torch.empty(3, 4))
+        assert torch.allclose(matrix.linear(x, w), x @ w.t())           # without a tangent as ever
+        assert torch.equal(matrix.orthogonalize(x), 2 * x)
+        assert torch.equal(matrix.orthogonalize(x, out=torch.empty(3, 4)), 2 * x)
+
+
+@pytest.mark.filterwarnings('ignore')
+@pytest.mark.parametrize('grad', [False, True])
+def test_a_trace_holds_the_call(on_host, grad):
+    x, w = torch.randn(3, 4), torch.randn(5, 4)
+    with torch.set_grad_enabled(grad):
+        layer = torch.jit.trace(lambda t: matrix.linear(t, w), (x,), check_trace=False)
+        orth = torch.jit.trace(lambda t: matrix.orthogonalize(t), (x,), check_trace=False)
+        other = torch.randn(3, 4)
+        assert torch.allclose(layer(other), other @ w.t()) and torch.equal(orth(other), 2 * other)
+        flat = torch.zeros(12)
+        for write in (lambda t: matrix.orthogonalize(t, out=torch.empty(3, 4)),
+                      lambda t: matrix.muon_step(flat, t.view(12), torch.zeros(12), [(0, 3, 4)], 0.1)):
+            with pytest.raises(RuntimeError, match='trace does not record'):
+                torch.jit.trace(write, (x,), check_trace=False)
+
+
+def test_orthogonalize_raises_in_a_backward_pass(on_host):
+    x = torch.randn(3, 4, requires_grad=True)
+    with pytest.raises(RuntimeError, match='no backward pass'):
+        (matrix.orthogonalize(x).sum() + x.sum()).backward()
+    with torch.no_grad():
+        assert not matrix.orthogonalize(x).requires_grad
+    assert not matrix.orthogonalize(x.detach()).requires_grad
+    assert not matrix.orthogonalize(x, out=torch.empty(3, 4)).requires_grad
