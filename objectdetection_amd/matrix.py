@@ -32,8 +32,13 @@ def _stream(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+
+
 def _call(device, fn, *args):
     """fn(*args, current stream of `device`) with that device as the current one; its return code."""
+    if _dispatch_modes() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError('make_fx does not see a launch: the graph would hold an empty result')
     if _current_device() == device.index:
         return fn(*args, _stream(device))
     with torch.cuda.device(device):

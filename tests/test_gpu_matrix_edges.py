@@ -122,3 +122,18 @@ def test_orthogonalize_is_no_part_of_a_backward_pass(mx):
     with pytest.raises(RuntimeError, match='no backward pass'):
         mx.orthogonalize(x).sum().backward()
     assert torch.equal(mx.orthogonalize(x).detach(), mx.orthogonalize(x.detach()))
+
+
+def test_graphs_of_operations_are_refused(mx):
+    """make_fx records torch operations, and tensors without memory hold nothing: neither sees a launch."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w = randn(30, 40), randn(24, 40, seed=1)
+    for call in (lambda t: mx.linear(t, w), lambda t: mx.orthogonalize(t), lambda t: mx.orthogonalize(t, out=torch.empty_like(t))):
+        with pytest.raises(RuntimeError, match='make_fx'):
+            make_fx(call)(x)
+        with pytest.raises(RuntimeError):
+            make_fx(call, tracing_mode='fake')(x)
+    leaf = w.clone().requires_grad_()
+    y = mx.linear(x, leaf)
+    with pytest.raises(RuntimeError, match='make_fx'):
+        make_fx(lambda t: torch.autograd.grad(y, leaf, t))(torch.ones_like(y))
