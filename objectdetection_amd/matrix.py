@@ -9,7 +9,7 @@ import numpy as np
 import torch
 from torch.autograd import forward_ad
 
-from . import _lib
+from . import _lib, engine
 from ._lib import lib, check
 
 ACTIVATIONS = {None: 0, 'silu': 1, 'gelu': 2, 'relu': 3}
@@ -58,6 +58,13 @@ def _watched():
 def _refuse_trace(name):
     if _tracing_state() is not None:
         raise RuntimeError(f'{name} writes to its arguments, which a trace does not record')
+
+
+def _written(*tensors):
+    """Tensors of the caller's were written through raw pointers: a backward pass that saved one of them has to raise, plans that
+    hold folded weights have to fold them again."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+    engine.touch_weights()
 
 
 def _ptr(t):
@@ -261,7 +268,9 @@ def orthogonalize(x, steps=5, eps=1e-7, out=None):
     _refuse_trace('orthogonalize into `out`')
     if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
         raise RuntimeError('orthogonalize into `out` has no tangent')
-    return _orthogonalize(x, steps, eps, out)
+    _orthogonalize(x, steps, eps, out)
+    _written(out)
+    return out
 
 
 class MatrixTable:
@@ -323,3 +332,4 @@ def muon_step(param, grad, momentum, matrices, lr, momentum_decay=0.95, nesterov
     check(_call(param.device, lib.odamd_muon_ema_step, param.data_ptr(), grad.data_ptr(), momentum.data_ptr(), _ptr(ema),
                 table.table.ctypes.data, len(table), lr, momentum_decay, int(nesterov), weight_decay, int(steps), eps,
                 ema_decay, grad_scale, ws.data_ptr(), table.workspace_bytes), 'muon_ema_step')
+    _written(param, momentum, ema)

@@ -101,3 +101,29 @@ def test_orthogonalize_raises_in_a_backward_pass(on_host):
         assert not matrix.orthogonalize(x).requires_grad
     assert not matrix.orthogonalize(x.detach()).requires_grad
     assert not matrix.orthogonalize(x, out=torch.empty(3, 4)).requires_grad
+
+
+@pytest.mark.parametrize('with_ema', [False, True])
+def test_what_is_written_counts_as_written(on_host, monkeypatch, with_ema):
+    """A saved tensor that a call wrote makes the backward pass raise, and plans that folded a weight fold it again."""
+    from objectdetection_amd import engine
+    monkeypatch.setattr(matrix, '_call', lambda *a: 0)
+    generation = engine._weights_generation[0]
+    x = torch.randn(3, 4, requires_grad=True)
+    out = torch.randn(3, 4)
+    loss = (x * out).sum()
+    matrix.orthogonalize(torch.randn(3, 4), out=out)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+    assert engine._weights_generation[0] > generation
+    generation = engine._weights_generation[0]
+    buffers = [torch.randn(12) for _ in range(4)]
+    losses = [(x * b.view(3, 4)).sum() for b in buffers]
+    matrix.muon_step(*buffers[:3], [(0, 3, 4)], 0.1, ema=buffers[3] if with_ema else None)
+    for i, loss in enumerate(losses):
+        if i == 1 or (i == 3 and not with_ema):              # the gradient is read only
+            loss.backward()
+        else:
+            with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+                loss.backward()
+    assert engine._weights_generation[0] > generation
