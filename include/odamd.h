@@ -379,7 +379,7 @@ int odamd_adam_ema_ranges_step(float* param, const float* grad, float* exp_avg, 
  * Matrix operators (no counterpart in the reference).
  *
  * Orthogonalisation by Newton-Schulz products.  x: (batch, rows, cols), contiguous, `dtype`; out: the same shape and type,
- * may be x itself.  Per matrix G:
+ * may be x itself, and else shares no memory with it.  Per matrix G:
  *   X = G / (|G|_F + eps), transposed while rows > cols;
  *   `steps` times (1 .. 32):  A = X X^T,  X = a X + (b A + c A A) X,  (a, b, c) = (3.4445, -4.7750, 2.0315);
  *   out = X, transposed back.
@@ -401,7 +401,7 @@ int odamd_orthogonalize(const void* x, void* out, int batch, int rows, int cols,
  *   ema = ema_decay ema + (1 - ema_decay) p   where ema != NULL.
  * O is accurate to 1e-3 of its norm at least (the groups of five above; 64 bits where all matrices of up to 112 in a row have
  * a side of at most 64).  0.2 sqrt(max(rows, cols)) gives the update the root mean square of an Adam step, so that one learning rate and one weight
- * decay serve both.  Elements outside the matrices are neither read nor written; matrices must not overlap.  The workspace
+ * decay serve both.  Elements outside the matrices are neither read nor written; matrices must not overlap, buffers neither.  The workspace
  * is 256-byte aligned. */
 typedef struct {
     long long offset; /* >= 0 */

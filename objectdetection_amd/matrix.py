@@ -67,6 +67,12 @@ def _written(*tensors):
     engine.touch_weights()
 
 
+def _overlap(a, b):
+    """Whether two contiguous tensors share memory."""
+    first, second = a.data_ptr(), b.data_ptr()
+    return first < second + b.numel() * b.element_size() and second < first + a.numel() * a.element_size()
+
+
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 
@@ -265,6 +271,8 @@ def orthogonalize(x, steps=5, eps=1e-7, out=None):
     _check_tensor('out', out, x.dtype, x.device)
     if out.shape != x.shape or not out.is_contiguous():
         raise ValueError('out must be contiguous and have the shape of x')
+    if x.is_contiguous() and x.data_ptr() != out.data_ptr() and _overlap(x, out):
+        raise ValueError('out shares a part of the memory of x: it may be x itself or lie beside it')
     _refuse_trace('orthogonalize into `out`')
     if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
         raise RuntimeError('orthogonalize into `out` has no tangent')
@@ -323,6 +331,11 @@ def muon_step(param, grad, momentum, matrices, lr, momentum_decay=0.95, nesterov
         _check_tensor(name, t, device=param.device)
         if t.dtype != torch.float32 or t.dim() != 1 or not t.is_contiguous() or t.numel() != param.numel():
             raise ValueError(f'{name} must be a flat contiguous float32 buffer of the length of param')
+    buffers = [('param', param), ('grad', grad), ('momentum', momentum)] + ([] if ema is None else [('ema', ema)])
+    for i, (name, t) in enumerate(buffers):
+        for other, u in buffers[:i]:
+            if _overlap(t, u):
+                raise ValueError(f'{name} shares memory with {other}')
     if table.end > param.numel():
         raise ValueError(f'matrices end at {table.end}, the buffers at {param.numel()}')
     if not 1 <= int(steps) <= 32 or not eps >= 0:

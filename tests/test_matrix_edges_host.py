@@ -127,3 +127,28 @@ def test_what_is_written_counts_as_written(on_host, monkeypatch, with_ema):
             with pytest.raises(RuntimeError, match='modified by an inplace operation'):
                 loss.backward()
     assert engine._weights_generation[0] > generation
+
+
+def test_memory_shared_in_part_is_refused(on_host, monkeypatch):
+    monkeypatch.setattr(matrix, '_call', lambda *a: 0)
+    buf = torch.randn(200)
+    x = buf[:96].view(8, 12)
+    for start in (1, 4, 95):
+        with pytest.raises(ValueError, match='shares'):
+            matrix.orthogonalize(x, out=buf[start:start + 96].view(8, 12))
+        with pytest.raises(ValueError, match='shares'):
+            matrix.orthogonalize(buf[start:start + 96].view(8, 12), out=x)
+    for out in (x, x.view(8, 12), buf[:96].view(8, 12), buf[96:192].view(8, 12)):
+        assert matrix.orthogonalize(x, out=out) is out
+    # what is not contiguous is copied first
+    assert matrix.orthogonalize(buf[:192].view(8, 24)[:, :12], out=x) is x
+    flat = [torch.randn(100) for _ in range(4)]
+    for i in range(4):
+        for j in range(i):
+            args = list(flat)
+            args[i] = args[j]
+            with pytest.raises(ValueError, match='shares memory'):
+                matrix.muon_step(*args[:3], [(0, 8, 12)], 0.1, ema=args[3])
+    with pytest.raises(ValueError, match='momentum shares memory with param'):
+        matrix.muon_step(buf[:100], flat[1], buf[99:199], [(0, 8, 12)], 0.1)
+    matrix.muon_step(buf[:100], flat[1], buf[100:], [(0, 8, 12)], 0.1)
