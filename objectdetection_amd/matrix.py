@@ -285,10 +285,14 @@ class MatrixTable:
     """The matrices of a flat buffer, [(offset, rows, cols)], checked once: in the buffer, not overlapping."""
 
     def __init__(self, matrices):
-        a = np.asarray(list(matrices), dtype=np.int64).reshape(-1, 3)
+        given = np.asarray(list(matrices)).reshape(-1, 3)
+        with np.errstate(invalid='ignore'):
+            a = given.astype(np.int64) if given.dtype.kind in 'iuf' else np.zeros((0, 3), np.int64)
         size = a[:, 1] * a[:, 2]
-        if len(a) == 0 or (a[:, 0] < 0).any() or (a[:, 1:] < 1).any() or (a[:, 1:] >= 2 ** 31).any() or (size > _MOST).any():
-            raise ValueError(f'matrices: at least one (offset, rows, cols), offsets from 0, sizes from 1, at most {_MOST} elements each')
+        if (len(a) == 0 or (a != given).any() or (a[:, 0] < 0).any() or (a[:, 0] > 2 ** 62).any() or (a[:, 1:] < 1).any()
+                or (a[:, 1:] >= 2 ** 31).any() or (size > _MOST).any()):
+            raise ValueError(f'matrices: at least one (offset, rows, cols) of whole numbers, offsets from 0 to 2^62, sizes from 1, at '
+                             f'most {_MOST} elements each')
         order = np.argsort(a[:, 0], kind='stable')
         ends = (a[:, 0] + size)[order]
         if (a[order, 0][1:] < ends[:-1]).any():

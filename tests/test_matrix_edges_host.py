@@ -152,3 +152,15 @@ def test_memory_shared_in_part_is_refused(on_host, monkeypatch):
     with pytest.raises(ValueError, match='momentum shares memory with param'):
         matrix.muon_step(buf[:100], flat[1], buf[99:199], [(0, 8, 12)], 0.1)
     matrix.muon_step(buf[:100], flat[1], buf[100:], [(0, 8, 12)], 0.1)
+
+
+def test_a_table_of_matrices_ends_where_it_says():
+    """An end past 64 bits must not come out as one before the buffer's; sizes are whole numbers."""
+    for bad in ([(2 ** 63 - 10, 4, 4)], [(2 ** 62 + 1, 4, 4)], [(0, 4, 4), (2 ** 63 - 1, 1, 1)], [(2 ** 64, 4, 4)], [(2 ** 70, 4, 4)], [(0, 2.5, 4)],
+                [(0.5, 2, 4)], [(float('nan'), 2, 4)], [('0', '2', '4')], [(0, None, 4)]):
+        with pytest.raises(ValueError):
+            matrix.MatrixTable(bad)
+    t = matrix.MatrixTable([(2 ** 62, 4, 8), (0, 2 ** 15, 2 ** 16 - 2)])
+    assert t.end == 2 ** 62 + 32 and len(t.gaps(2 ** 62 + 40)) == 2
+    assert matrix.MatrixTable(np.array([[3, 2, 2]], np.int32)).end == 7
+    assert matrix.MatrixTable((np.int64(3), 2.0, 2) for _ in range(1)).end == 7
