@@ -169,3 +169,35 @@ def test_a_step_over_the_flat_buffers_reaches_cached_plans(mx):
     state.grad.copy_(randn(state.n))
     mx.muon_step(state.param, state.grad, state.exp_avg, te.muon_matrices(net, state), lr=0.1)
     assert not torch.equal(net(image), first)
+
+
+# ---------------------------------------------------------------------------------------------
+# activations, value by value: one input of weight one, z = x
+# ---------------------------------------------------------------------------------------------
+def value_and_slope(z, act):
+    """In 64 bits, by forms that keep their digits at negative z: 1 + erf would lose those of 64 bits too by z = -8."""
+    if act == 'silu':
+        p = 1 / (1 + torch.exp(-z))
+        return z * p, p * (1 + z * torch.exp(-z) * p)
+    p = 0.5 * torch.special.erfc(-z * math.sqrt(0.5))
+    return z * p, p + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('act', ['silu', 'gelu'])
+@pytest.mark.parametrize('m, n', [(4001, 1), (4001, 9), (40001, 8)])
+def test_activations_keep_their_tails(mx, act, dtype, m, n):
+    """Relative to the value, however small it is.  float32 products carry 22 bits of z, and a change of z by e changes the tails
+    by z z e of themselves (gelu) or z e (silu); bfloat16 values of z are exact, and the activation is good to 5e-5."""
+    x = torch.linspace(-12, 12, m, device='cuda').to(dtype)[:, None].requires_grad_()
+    w = torch.ones(n, 1, device='cuda', dtype=dtype)
+    z = x.detach().double()
+    y = mx.linear(x, w, None, act)
+    y64, s64 = value_and_slope(z, act)
+    rough = (z * z + 16) * 2.0 ** -21 if dtype == torch.float32 else 5e-5
+    assert bool(((y.detach().double() - y64).abs() <= (rough + HALF[dtype]) * y64.abs() + 1e-37).all())
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    s64 = n * s64
+    # slopes are sums that cross zero between -2 and 0; in bfloat16 they are rounded twice, before the product and after it
+    near = 2e-6 * n * (z.abs() < 2)
+    assert bool(((dx.double() - s64).abs() <= (rough + 2 * HALF[dtype]) * s64.abs() + near + 1e-37).all())
