@@ -126,7 +126,7 @@ struct NsIo {
     float* param;
     float* momentum;
     float* ema;
-    float mu, grad_scale, decay, lr02, ema_keep, ema_take;   // decay: 1 - lr weight_decay, lr02: 0.2 lr
+    float mu, grad_scale, shrink, lr02, ema_keep, ema_take;  // shrink: lr weight_decay, lr02: 0.2 lr
     int nesterov;
     double eps;
     float* x;            // matrices of few rows: X between phases of steps, one matrix of the table behind the other
@@ -164,6 +164,12 @@ __device__ __forceinline__ double ns_block_sum(double v, double* shared) {
     double s = 0.0;
     for (int i = 0; i < (int)(blockDim.x >> 6); ++i) s += shared[i];
     return s;
+}
+
+// A parameter after the step: w (1 - lr weight_decay) - step v, with one rounding against w.  1 - lr weight_decay is not a factor of
+// its own: it keeps eight bits of 5e-7, and none of 2e-8.
+__device__ __forceinline__ float ns_new_param(const NsIo& io, float w, float step, float v) {
+    return w - fmaf(io.shrink, w, step * v);
 }
 
 // Eight of the caller's values; zeros for those past the first `cnt`
@@ -592,7 +598,7 @@ __device__ __forceinline__ void ns_few_out(const NsIo& io, const NsPlace& p, int
                     float w[4], old[4];
                     ns_load4<DT>(io.param, at, sr, cnt, w);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = w[e] * io.decay - step * v[e];
+                    for (int e = 0; e < 4; ++e) w[e] = ns_new_param(io, w[e], step, v[e]);
                     ns_store4<DT>(io.param, at, sr, cnt, w);
                     if (io.ema) {
                         ns_load4<DT>(io.ema, at, sr, cnt, old);
@@ -664,7 +670,7 @@ __global__ void __launch_bounds__(256) ns_few_move_kernel(NsTable t, NsIo io) {
             }
             io.x[at_x + i] = v[0];
         } else if constexpr (MUON) {
-            const float w = io.param[at] * io.decay - step * io.x[at_x + i];
+            const float w = ns_new_param(io, io.param[at], step, io.x[at_x + i]);
             io.param[at] = w;
             if (io.ema) io.ema[at] = io.ema_keep * io.ema[at] + io.ema_take * w;
         } else {
@@ -705,7 +711,7 @@ __device__ __forceinline__ void ns_emit8(const NsIo& io, float step, long long a
         f32x4_t w[2], u[2];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            w[e >> 2][e & 3] = x.w[e >> 2][e & 3] * io.decay - step * v[e];
+            w[e >> 2][e & 3] = ns_new_param(io, x.w[e >> 2][e & 3], step, v[e]);
             u[e >> 2][e & 3] = io.ema_keep * x.e[e >> 2][e & 3] + io.ema_take * w[e >> 2][e & 3];
         }
         if (cnt == 8) {
@@ -1232,7 +1238,7 @@ int odamd_muon_ema_step(float* param, const float* grad, float* momentum, float*
     io.ema = ema;
     io.mu = (float)momentum_decay;
     io.grad_scale = (float)grad_scale;
-    io.decay = (float)(1.0 - lr * weight_decay);
+    io.shrink = (float)(lr * weight_decay);
     io.lr02 = (float)(0.2 * lr);
     io.ema_keep = (float)ema_decay;
     io.ema_take = (float)(1.0 - ema_decay);

@@ -201,3 +201,24 @@ def test_activations_keep_their_tails(mx, act, dtype, m, n):
     # slopes are sums that cross zero between -2 and 0; in bfloat16 they are rounded twice, before the product and after it
     near = 2e-6 * n * (z.abs() < 2)
     assert bool(((dx.double() - s64).abs() <= (rough + 2 * HALF[dtype]) * s64.abs() + near + 1e-37).all())
+
+
+# ---------------------------------------------------------------------------------------------
+# optimizer step
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('steps', [5, 12])
+@pytest.mark.parametrize('shapes', [[(16, 27), (30, 50)], [(16, 700), (3, 5000)], [(130, 129), (16, 27)], [(65, 700), (700, 65)]])
+def test_muon_step_decays_by_little(mx, shapes, steps):
+    """Without a gradient a step is the decay alone, rounded once: lr weight_decay from 2e-8 (under half a step of one) to 1e-3."""
+    matrices, at = [], 0
+    for r, c in shapes:
+        matrices.append((at, r, c))
+        at += r * c
+    p, zero = randn(at, scale=0.03), torch.zeros(at, device='cuda')
+    for weight_decay in (2e-5, 3e-5, 5e-4, 1.0):
+        got, ema = p.clone(), p.clone()
+        mx.muon_step(got, zero, zero.clone(), matrices, lr=1e-3, weight_decay=weight_decay, ema=ema, steps=steps)
+        ref = p.double() * (1 - 1e-3 * weight_decay)
+        # half a step, and the roundings of the decay itself
+        assert bool(((got.double() - ref).abs() <= 2.0 ** -24 * ref.abs() * (1 + 4e-3)).all())
+        assert torch.equal(ema, got)
