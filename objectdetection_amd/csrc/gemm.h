@@ -317,7 +317,8 @@ struct GemmTile {
     // cols(m, n, v[8], x) for C[m .. m+7][n], x = what load(m, n) of that kind gave before.  Every wave passes 32 rows at a time
     // through a slab of LDS of its own; BATCH of its loads are under way together, the first of them while the slab is
     // written (a load that waits for the store before it costs the epilogue a memory latency for every run).
-    template <bool ROWS, bool COLS, int BATCH, typename LR, typename FR, typename LC, typename FC>
+    // SYM: the tile lies on the diagonal of a symmetric result; runs of eight that cross it have their lower part from the upper one.
+    template <bool ROWS, bool COLS, int BATCH, bool SYM = false, typename LR, typename FR, typename LC, typename FC>
     __device__ __forceinline__ void hand_out(char* lds, LR&& load_row, FR&& rows, LC&& load_col, FC&& cols) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         if (KG > 1 && wave >= NW) return;                           // the first group holds the sums
@@ -358,6 +359,13 @@ struct GemmTile {
                     const float* at = slab + (p * RPP + lane / LPR) * SLAB_LD + lane % LPR * 8;
                     const f32x4_t u = *(const f32x4_t*)at, w = *(const f32x4_t*)(at + 4);
                     float v[8] = {u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]};
+                    if constexpr (SYM) {
+                        const int m = row_at(i, p);             // the block of eight rows and columns lies in this slab
+                        if (m >> 3 == row_n >> 3)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (row_n + e < m) v[e] = slab[(row_n + e - wm - i * 32) * SLAB_LD + m - wn];
+                    }
                     rows(row_at(i, p), row_n, v, xr[p % B]);
                 }
                 if constexpr (COLS) fetch_cols(0);
@@ -398,7 +406,6 @@ __device__ __forceinline__ void store_split8(char* hi_at, const float v[8], floa
     *(f16x8_t*)hi_at = hi;
     *(f16x8_t*)(hi_at + 64) = lo;
 }
-
 // ---- host ------------------------------------------------------------------------------------------------------------
 // A launch has fewer than 2^32 threads.
 inline bool gemm_grid_ok(long long blocks, int threads) { return blocks * threads <= 0xffffffffLL; }

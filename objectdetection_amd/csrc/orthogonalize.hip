@@ -22,8 +22,10 @@
 // The products of more rows run on fp16 pairs (gemm.h, PL = 2) scaled by 2^12 (Q, which grows to 3.4445^k, by less): the largest
 // entry becomes 14 300, the smallest step 2^-36.  bf16 products would leave a few percent in the result.
 // X is kept twice, by rows (X X^T reduces along n) and by columns (Q X reduces along m): both products then read their
-// operands along the reduction.  The m x m matrices are symmetric: tiles on and over the diagonal are computed, the rest
-// mirrored.  All matrices of a call share every launch.
+// operands along the reduction.  The m x m matrices are symmetric to the bit: what lies on and over the diagonal is computed, the
+// rest mirrored, within the tiles on the diagonal too.  Both halves of such a tile as they come differ by a rounding, and that
+// difference grows by 3.4445^2 a step where A has no singular value: five steps on a matrix of rank 3 were off by 1.5 to 2 % with
+// it, 2e-4 without; it costs 2 to 3 % of the time.  All matrices of a call share every launch.
 //
 // Eight 256 x 2304 in float32 take 195 us: 20 launches of 5 to 20 us, each a chain of a few latencies.  A step over the 94
 // matrices of the detector's largest preset takes 4.6 ms: 3.8 ms of products at 55 % of the matrix rate of a large library
@@ -167,7 +169,7 @@ __device__ __forceinline__ double ns_block_sum(double v, double* shared) {
 }
 
 // A parameter after the step: w (1 - lr weight_decay) - step v, with one rounding against w.  1 - lr weight_decay is not a factor of
-// its own: it keeps eight bits of 5e-7, and none of 2e-8.
+// its own: a float32 under one has steps of 6e-8, an eighth of 5e-7 and more than 2e-8.
 __device__ __forceinline__ float ns_new_param(const NsIo& io, float w, float step, float v) {
     return w - fmaf(io.shrink, w, step * v);
 }
@@ -450,7 +452,9 @@ __device__ __forceinline__ double* ns_few_steps(double* lds, int steps, const Ns
 #pragma unroll
                 for (int e = 0; e < 4; ++e) pm[e] = (r == 4 * e + h ? NS_A : 0.0) + NS_B * am[e] + NS_C * s[e];
                 qm = step == 0 ? pm : times(qm, pm);
-                am = times(pm, times(pm, am));
+                // P (P A) and its transpose, of the same products in the same order: their mean is symmetric to the bit
+                const f64x4_t t = times(pm, am);
+                am = (times(pm, t) + times(t, pm)) * 0.5;
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) q[(4 * e + h) * LD + r] = qm[e] * inv;
@@ -500,8 +504,7 @@ __device__ __forceinline__ double* ns_few_steps(double* lds, int steps, const Ns
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int row = ti * 16 + 4 * e + h, col = tj * 16 + r;
-            to[row * LD + col] = val[e] * scale;
-            to[col * LD + row] = val[e] * scale;
+            if (row <= col) to[row * LD + col] = to[col * LD + row] = val[e] * scale;      // symmetric to the bit
         }
     };
     constexpr int TURNS = (2 * F::TRI + F::WAVES - 1) / F::WAVES;
@@ -824,7 +827,10 @@ __global__ void __launch_bounds__(TILE::THREADS) ns_product_kernel(NsTable t, Ns
         const auto get_col = [&](int i, int j) { return get(j0 + j, i0 + i); };
         const auto rows = [&](int i, int j, float v[8], const Before& x) { put(i0 + i, j0 + j, v, x); };
         const auto cols = [&](int i, int j, float v[8], const Before& x) { put(j0 + j, i0 + i, v, x); };
-        if (ti == tj) tile.template hand_out<true, false, 4>(lds, get_row, rows, get_col, cols);
+        // a tile on the diagonal: the runs that reach it by rows, what lies under them by columns
+        const auto upper = [&](int i, int j, float v[8], const Before& x) { if (i < j + 8) rows(i, j, v, x); };
+        const auto lower = [&](int i, int j, float v[8], const Before& x) { if (i + 8 <= j) cols(i, j, v, x); };
+        if (ti == tj) tile.template hand_out<true, true, 4, true>(lds, get_row, upper, get_col, lower);
         else tile.template hand_out<true, true, 4>(lds, get_row, rows, get_col, cols);
     } else if constexpr (STAGE == ST_X) {
         char* xt = p.ws + (jobs.turn ? l.xt0 : l.xt1);
@@ -898,17 +904,17 @@ __global__ void __launch_bounds__(256) ns_join_kernel(NsTable t, int cuts, float
             v[e] = j + e < p.m ? s * scale : 0.0f;
             tile[r][c + e] = v[e];
         }
-        store_split8(out + (long long)i * mp * 4 + split_at(j), v, 1.0f);
+        if (ti != tj) store_split8(out + (long long)i * mp * 4 + split_at(j), v, 1.0f);
     }
-    if (ti == tj) return;
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         const int r = (threadIdx.x >> 3) + 32 * q;          // all rows of a tile over the diagonal exist
         float v[8];
-        if (j0 + r >= p.m) continue;
+        if (j0 + r >= p.m || i0 + c >= mp) continue;
+        // on the diagonal the whole tile, its lower half from the upper one
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = tile[c + e][r];
+        for (int e = 0; e < 8; ++e) v[e] = ti == tj && c + e >= r ? tile[r][c + e] : tile[c + e][r];
         store_split8(out + (long long)(j0 + r) * mp * 4 + split_at(i0 + c), v, 1.0f);
     }
 }

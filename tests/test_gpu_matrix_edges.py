@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from .test_gpu_matrix import HALF, orth64, randn
+from .test_gpu_matrix import HALF, LOOSE, orth64, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -222,3 +222,41 @@ def test_muon_step_decays_by_little(mx, shapes, steps):
         # half a step, and the roundings of the decay itself
         assert bool(((got.double() - ref).abs() <= 2.0 ** -24 * ref.abs() * (1 + 4e-3)).all())
         assert torch.equal(ema, got)
+
+
+# ---------------------------------------------------------------------------------------------
+# matrices with few directions
+# ---------------------------------------------------------------------------------------------
+def of_rank(rank, rows, cols, dtype=torch.float32):
+    """`rank` neighbouring columns, the rest zero: A has rows - rank singular values of zero, where every rounding that is not
+    symmetric would grow by 3.4445^2 a step and be seen by what lies in the other directions."""
+    g = torch.zeros(1, rows, cols, device='cuda', dtype=dtype)
+    g[0, :, 5:5 + rank] = randn(rows, rank, seed=rows, dtype=dtype)
+    return g
+
+
+@pytest.mark.parametrize('rank', [1, 3, 40])
+@pytest.mark.parametrize('rows, cols', [(65, 130), (130, 300), (130, 130), (128, 2048), (256, 2304), (257, 9001), (1025, 1100)])
+def test_orthogonalize_of_little_rank(mx, rows, cols, rank):
+    """Phases of five steps, of two and of one; the optimizer step shows the phases of five before they are rounded to bfloat16."""
+    low, g = of_rank(rank, rows, cols, torch.bfloat16), of_rank(rank, rows, cols)
+    for x, tol in ((low, LOOSE + HALF[torch.bfloat16]), (g, 3.4445 ** 5 * 2.0 ** -24)):
+        for y in (x, x.transpose(1, 2).contiguous()):
+            ref = orth64(y[0])
+            assert float((mx.orthogonalize(y)[0].double() - ref).norm()) <= tol * float(ref.norm())
+    flat = g.reshape(-1).contiguous()
+    p, m = torch.zeros_like(flat), torch.zeros_like(flat)
+    mx.muon_step(p, flat, m, [(0, rows, cols)], lr=-5 / math.sqrt(max(rows, cols)), momentum_decay=0.0, nesterov=False)
+    ref = orth64(g[0])
+    assert float((p.view(rows, cols).double() - ref).norm()) <= LOOSE * float(ref.norm())
+
+
+@pytest.mark.parametrize('rank', [1, 2])
+@pytest.mark.parametrize('rows, cols', [(12, 300), (16, 300), (16, 4000), (30, 300), (48, 4000), (64, 300)])
+def test_orthogonalize_of_few_rows_and_little_rank(mx, rows, cols, rank):
+    """64 bits: a rounding of Q, 2^-53 of 3.4445^10 at most, over up to 64 directions, is under 1e-9."""
+    g = of_rank(rank, rows, cols)
+    for steps in range(5, 11):
+        for x in (g, g.transpose(1, 2).contiguous()):
+            ref = orth64(x[0], steps=steps)
+            assert float((mx.orthogonalize(x, steps=steps)[0].double() - ref).norm()) <= (2.0 ** -24 + 1e-9) * float(ref.norm())
