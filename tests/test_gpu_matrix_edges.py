@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from .test_gpu_matrix import HALF, LOOSE, orth64, randn
+from .test_gpu_matrix import HALF, LOOSE, SIZES, orth64, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -260,3 +260,50 @@ def test_orthogonalize_of_few_rows_and_little_rank(mx, rows, cols, rank):
         for x in (g, g.transpose(1, 2).contiguous()):
             ref = orth64(x[0], steps=steps)
             assert float((mx.orthogonalize(x, steps=steps)[0].double() - ref).norm()) <= (2.0 ** -24 + 1e-9) * float(ref.norm())
+
+
+# ---------------------------------------------------------------------------------------------
+# nothing is left out: sums that are exact
+# ---------------------------------------------------------------------------------------------
+LONG = [(2100, 264, 2050), (4000, 96, 4100), (50, 4000, 72), (4097, 300, 1001), (2056, 520, 2000), (9000, 136, 520), (5001, 129, 131),
+        (2100, 263, 2049), (70, 1500, 3001), (2500, 1030, 1033), (30001, 40, 56), (64, 9001, 64), (520, 33, 20001), (257, 2049, 129)]
+
+
+def whole(*shape, seed, dtype):
+    """-3 .. 3 without 0: no product is zero, sums of up to 2^20 of them are exact in float32, whatever their order."""
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    v = torch.randint(1, 4, shape, generator=g, device='cuda') * (2 * torch.randint(0, 2, shape, generator=g, device='cuda') - 1)
+    return v.to(dtype)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('m, k, n', SIZES + LONG)
+def test_linear_sums_every_term(mx, m, k, n, dtype):
+    """Whole numbers: the result and all gradients are exact, rounded once."""
+    x, w, b, r = (whole(*s, seed=i, dtype=dtype) for i, s in enumerate(((m, k), (n, k), (n,), (m, n))))
+    dy = whole(m, n, seed=9, dtype=dtype)
+    z = x.double() @ w.double().t() + b.double()
+    for act in (None, 'relu'):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        y = mx.linear(*leaves[:3], act, leaves[3])
+        assert torch.equal(y.detach(), ((z.clamp(min=0) if act else z) + r.double()).to(dtype))
+        dz = dy.double() * (z > 0) if act else dy.double()
+        dx, dw, db, dr = torch.autograd.grad(y, leaves, dy)
+        assert torch.equal(dx, (dz @ w.double()).to(dtype))
+        assert torch.equal(dw, (dz.t().contiguous() @ x.double()).to(dtype))
+        assert torch.equal(db, dz.sum(0).to(dtype)) and torch.equal(dr, dy)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('rows, cols', [(5, 1025), (16, 1537), (33, 1001), (64, 513), (3, 70001), (65, 130), (130, 2049), (256, 2304),
+                                        (257, 9001), (1025, 1100), (70, 4001)])
+def test_orthogonalize_reads_every_column(mx, rows, cols, dtype):
+    """All but three neighbouring columns are zero, at the ends and where the reduction may be cut: a column left out is an error of
+    order one.  A rounding of X to 22 bits grows by 3.4445 a step in the directions that have no singular value."""
+    tol = 1.41 * 3.4445 ** 5 * 3 * 2.0 ** -22 + HALF[dtype]
+    for at in sorted({0, 31, cols // 3 - 1, cols // 2 - 1, cols * 3 // 4 - 1, cols - 4, cols - 3}):
+        g = torch.zeros(1, rows, cols, device='cuda', dtype=dtype)
+        g[0, :, at:at + 3] = randn(rows, 3, seed=at, dtype=dtype)
+        for x in (g, g.transpose(1, 2).contiguous()):
+            got, ref = mx.orthogonalize(x)[0].double(), orth64(x[0])
+            assert float((got - ref).norm()) <= tol * float(ref.norm())
