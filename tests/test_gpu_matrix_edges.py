@@ -307,3 +307,94 @@ def test_orthogonalize_reads_every_column(mx, rows, cols, dtype):
         for x in (g, g.transpose(1, 2).contiguous()):
             got, ref = mx.orthogonalize(x)[0].double(), orth64(x[0])
             assert float((got - ref).norm()) <= tol * float(ref.norm())
+
+
+# ---------------------------------------------------------------------------------------------
+# operands and results of more than 2^31 elements
+# ---------------------------------------------------------------------------------------------
+@pytest.fixture
+def room():
+    """100 GB of the card's memory, given back afterwards."""
+    if torch.cuda.get_device_properties(0).total_memory < 200 << 30:
+        pytest.skip('a card of less memory')
+    torch.cuda.empty_cache()
+    yield
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('m, k, n', [(4, 64, 4), (40, 72, 64), (3000, 64, 56), (3001, 71, 45)])
+def test_linear_of_rows_far_apart(mx, room, m, k, n, dtype):
+    """The last rows of x, the residual and the gradient begin past element 2^31: the same bits as close together."""
+    apart = (2 ** 31 // (m - 1) // 8 + 100) * 8
+    far = torch.empty((m - 1) * apart + 4096, dtype=dtype, device='cuda')
+    x, r, dy = (far.as_strided((m, c), (apart, 1), at) for c, at in ((k, 0), (n, 256), (n, 512)))
+    w, b = randn(n, k, seed=1, dtype=dtype, scale=k ** -0.5), randn(n, seed=2, dtype=dtype)
+    for seed, t in enumerate((x, r, dy)):
+        t.copy_(randn(*t.shape, seed=10 + seed, dtype=dtype))
+    # close together on rows of the same alignment: the same way through the kernels
+    near = torch.empty(m * 1024, dtype=dtype, device='cuda')
+    copies = [near.as_strided((m, t.shape[1]), (1024, 1), at).copy_(t) for t, at in ((x, 0), (r, 256), (dy, 512))]
+    results = []
+    for x, r, dy in ((x, r, dy), copies):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        y = mx.linear(*leaves[:3], 'silu', leaves[3])
+        results.append((y.detach(), *torch.autograd.grad(y, leaves, dy)))
+    assert all(torch.equal(a, c) for a, c in zip(*results))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+def test_linear_of_large_results(mx, room, dtype):
+    m, k, n = 2 ** 20 + 77, 16, 2056
+    x, w = whole(m, k, seed=0, dtype=dtype).requires_grad_(), whole(n, k, seed=1, dtype=dtype).requires_grad_()
+    y = mx.linear(x, w, None, 'relu')
+    z = x[-300:].detach().double() @ w.detach().double().t()
+    assert torch.equal(y[-300:].detach(), z.clamp(min=0).to(dtype))
+    # exact: sums of -1 and 1 times 0 .. 3
+    dy = torch.ones(1, device='cuda', dtype=dtype).expand(m, n)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert torch.equal(dx[-300:], ((z > 0).double() @ w.detach().double()).to(dtype))
+    last = torch.zeros(k, dtype=torch.float64, device='cuda')
+    for at in range(0, m, 2 ** 18):
+        part = x[at:at + 2 ** 18].detach().double()
+        last += ((part @ w[-1].detach().double()) > 0).double() @ part
+    assert torch.equal(dw[-1], last.to(dtype))
+
+
+@pytest.mark.parametrize('steps', [5, 12])
+@pytest.mark.parametrize('shapes', [[(16, 27), (64, 300), (3, 9000)], [(130, 257), (16, 27), (700, 66)]])
+def test_muon_step_far_into_the_buffers(mx, room, shapes, steps):
+    """Matrices past element 2^31, and Adam over ranges there: the same bits as at the start of short buffers."""
+    from objectdetection_amd._lib import lib, check
+    import numpy as np
+    matrices, at = [], 1
+    for r, c in shapes:
+        matrices.append((at, r, c))
+        at += r * c + 3
+    length = at + 100
+    start = 2 ** 31 + 5
+    near = [randn(length, seed=i, scale=0.01).abs() for i in range(4)]
+    far = [torch.empty(start + length, device='cuda') for _ in range(4)]
+    for f, t in zip(far, near):
+        f[start:].copy_(t)
+    mx.muon_step(*near[:3], matrices, lr=0.01, weight_decay=0.1, ema=near[3], ema_decay=0.9, steps=steps)
+    mx.muon_step(*far[:3], [(o + start, r, c) for o, r, c in matrices], lr=0.01, weight_decay=0.1, ema=far[3], ema_decay=0.9, steps=steps)
+    assert all(torch.equal(f[start:], t) for f, t in zip(far, near))
+    stream = torch.cuda.current_stream().cuda_stream
+    for bufs, o in ((near, 0), (far, start)):
+        a = np.array([(o + 3, 1000), (o + length - 50, 50)], dtype=mx.RANGE_DTYPE)
+        check(lib.odamd_adam_ema_ranges_step(*(t.data_ptr() for t in bufs), None, a.ctypes.data, len(a), 0.01, 0.937, 0.999, 1e-8, 5e-4, 3,
+                                             0.0, 1.0, stream))
+    # by their bits: the third buffer has negative values, whose root is no number
+    assert all(torch.equal(f[start:].view(torch.int32), t.view(torch.int32)) for f, t in zip(far, near))
+
+
+@pytest.mark.parametrize('batch, rows, cols, dtype', [(2 ** 22 + 3, 16, 32, torch.float32), (2 ** 15 + 9, 256, 256, torch.bfloat16)])
+def test_orthogonalize_of_a_large_batch(mx, room, batch, rows, cols, dtype):
+    g = torch.zeros(batch, rows, cols, dtype=dtype, device='cuda')
+    g[:5], g[-9:] = randn(5, rows, cols, dtype=dtype), randn(9, rows, cols, seed=1, dtype=dtype)
+    got = mx.orthogonalize(g)
+    for i in (0, 4, batch - 9, batch - 1):
+        ref = orth64(g[i])
+        assert float((got[i].double() - ref).norm()) <= (LOOSE + HALF[dtype]) * float(ref.norm())
+    assert float(got[5:8].abs().max()) == 0.0 and float(got[-12:-9].abs().max()) == 0.0
