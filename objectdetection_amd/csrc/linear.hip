@@ -325,8 +325,8 @@ __global__ void __launch_bounds__(256) linear_rows_kernel(LinRow p) {
 }
 
 // ---- laying operands out ---------------------------------------------------------------------------------------------
-// One matrix (m x n) of the caller's, optionally dz = src act'(z): written by rows and / or by columns with the reduction
-// padded with zeros to whole chunks.
+// One matrix (m x n) of the caller's, optionally dz = src act'(z): written by rows and / or (float32) by columns with the
+// reduction padded with zeros to whole chunks.
 struct LinJob {
     const void* src;
     const void* z;
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(256) linear_lay_kernel(LinJobs t) {
     const LinJob& p = lin_job(t, blockIdx.x);
     const int at = blockIdx.x - p.tile0, nt = (p.n + 63) / 64, i0 = at / nt * 64, j0 = at % nt * 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int np = (int)lin_up(p.n, lin_chunk<DT>()), mp = (int)lin_up(p.m, lin_chunk<DT>()), c = (threadIdx.x & 7) * 8;
+    const int np = (int)lin_up(p.n, lin_chunk<DT>()), c = (threadIdx.x & 7) * 8;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         const int r = (threadIdx.x >> 3) + 32 * q;
@@ -458,15 +458,18 @@ __global__ void __launch_bounds__(256) linear_lay_kernel(LinJobs t) {
         for (int q = 0; q < 64; ++q) s += tile[q][lane];
         p.sums[(long long)(i0 / 64) * p.n + j0 + lane] = s;
     }
-    if (!p.cols) return;
+    if constexpr (DT == ODAMD_DTYPE_F32) {
+        const int mp = (int)lin_up(p.m, lin_chunk<DT>());
+        if (!p.cols) return;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int r = (threadIdx.x >> 3) + 32 * q;
-        float v[8];
-        if (j0 + r < p.n && i0 + c < mp) {
+        for (int q = 0; q < 2; ++q) {
+            const int r = (threadIdx.x >> 3) + 32 * q;
+            float v[8];
+            if (j0 + r < p.n && i0 + c < mp) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = tile[c + e][r];
-            lin_lay8<DT>(p.cols, j0 + r, mp, i0 + c, v, DT == ODAMD_DTYPE_F32 ? lin_shift(p.col_max[j0 + r]) : 0);
+                for (int e = 0; e < 8; ++e) v[e] = tile[c + e][r];
+                lin_lay8<DT>(p.cols, j0 + r, mp, i0 + c, v, lin_shift(p.col_max[j0 + r]));
+            }
         }
     }
 }

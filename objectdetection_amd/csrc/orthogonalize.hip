@@ -27,7 +27,7 @@
 // difference grows by 3.4445^2 a step where A has no singular value: five steps on a matrix of rank 3 were off by 1.5 to 2 % with
 // it, 2e-4 without; it costs 2 to 3 % of the time.  All matrices of a call share every launch.
 //
-// Eight 256 x 2304 in float32 take 195 us: 20 launches of 5 to 20 us, each a chain of a few latencies.  A step over the 94
+// Eight 256 x 2304 in float32 take 207 us: 22 launches of 5 to 20 us, each a chain of a few latencies.  A step over the 94
 // matrices of the detector's largest preset takes 4.6 ms: 3.8 ms of products at 55 % of the matrix rate of a large library
 // product (tiles on the diagonal compute both halves; 128 x 128 tiles are bound by LDS reads and matrix instructions alike) and
 // 0.73 ms of norm and layout at the rate of a copy.
