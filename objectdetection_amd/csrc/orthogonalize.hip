@@ -15,7 +15,7 @@
 //   - More rows, float32 results: phases of two steps, which keep float32's accuracy (error against 64 bits of 256 x 2304 noise
 //     with strong directions: 1.6e-6, one step a phase 1.9e-6), where n >= 2 m; one step a phase on squarer ones, which costs no
 //     more there.
-//   - More rows, bfloat16 results and the optimizer step: phases of five.  3e-6 to 8e-5 on such matrices, under 8e-4
+//   - More rows, bfloat16 results and the optimizer step: phases of five.  1e-6 to 6e-5 on such matrices, under 7e-4
 //     (3.4445^8 2^-24 = 1.2e-3) where the singular values fall like 1 / i^2 or vanish; a bfloat16 result is rounded by 2e-3,
 //     and the step multiplies by the learning rate.
 //
@@ -28,9 +28,9 @@
 // it, 2e-4 without; it costs 2 to 3 % of the time.  All matrices of a call share every launch.
 //
 // Eight 256 x 2304 in float32 take 207 us: 22 launches of 5 to 20 us, each a chain of a few latencies.  A step over the 94
-// matrices of the detector's largest preset takes 4.6 ms: 3.8 ms of products at 55 % of the matrix rate of a large library
+// matrices of the detector's largest preset takes 4.7 ms: 4.0 ms of products at 53 % of the matrix rate of a large library
 // product (tiles on the diagonal compute both halves; 128 x 128 tiles are bound by LDS reads and matrix instructions alike) and
-// 0.73 ms of norm and layout at the rate of a copy.
+// 0.7 ms of norm and layout at the rate of a copy.
 #include "common.h"
 #include "odamd.h"
 #include "offsets.h"
@@ -426,7 +426,7 @@ __device__ __forceinline__ double* ns_few_steps(double* lds, int steps, const Ns
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, h = lane >> 4;
     if constexpr (T == 1) {
         // One tile: a lane's results, rows 4 e + h of column r, are by symmetry its operands of the next product, columns 4 e + h of
-        // row r, so that one wave takes all steps in registers (16 x 27: 7.4 us, through LDS 10.0).
+        // row r, so that one wave takes all steps in registers (16 x 27: 8.1 us, through LDS over 10).
         if (wave == 0) {
             const auto times = [](const f64x4_t& x, const f64x4_t& y) {
                 f64x4_t even = {}, odd = {};

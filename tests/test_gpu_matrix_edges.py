@@ -398,3 +398,47 @@ def test_orthogonalize_of_a_large_batch(mx, room, batch, rows, cols, dtype):
         ref = orth64(g[i])
         assert float((got[i].double() - ref).norm()) <= (LOOSE + HALF[dtype]) * float(ref.norm())
     assert float(got[5:8].abs().max()) == 0.0 and float(got[-12:-9].abs().max()) == 0.0
+
+
+# ---------------------------------------------------------------------------------------------
+# in use
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('rows, cols', [(30, 50), (16, 4000), (130, 300)])
+def test_many_steps_captured_and_replayed(mx, rows, cols):
+    """Several phases of steps in a graph, other inputs and eager work between its replays."""
+    table = mx.MatrixTable([(3, rows, cols), (rows * cols + 7, 16, 27)])
+    length = table.end + 2
+    g, p, m = randn(length), randn(length, seed=1), torch.zeros(length, device='cuda')
+    low = randn(2, rows, cols, seed=2, dtype=torch.bfloat16)
+
+    def work(low, p, m):
+        mx.muon_step(p, g, m, table, lr=0.01, steps=12)
+        return mx.orthogonalize(low, steps=12), mx.orthogonalize(low.float(), steps=23)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work(low.clone(), p.clone(), m.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    xs, ps, ms = low.clone(), p.clone(), m.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work(xs, ps, ms)
+    for turn in range(4):
+        xs.copy_(randn(2, rows, cols, seed=60 + turn, dtype=torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref = work(xs.clone(), p, m)
+        assert all(torch.equal(a, c) for a, c in zip(out, ref))
+        assert torch.equal(ps, p) and torch.equal(ms, m)
+
+
+def test_compiled_callers_leave_the_calls_alone(mx):
+    x, w = randn(30, 40), randn(24, 40, seed=1)
+    call = torch.compile(lambda t: mx.linear(t, w, None, 'gelu') * 2, backend='eager')
+    assert torch.equal(call(x), mx.linear(x, w, None, 'gelu') * 2)
+    leaf, twin = (w.clone().requires_grad_() for _ in range(2))
+    call = torch.compile(lambda t: (mx.linear(t, leaf, None, 'silu') * t[:, :24]).sum(), backend='eager')
+    call(x).backward()
+    (mx.linear(x, twin, None, 'silu') * x[:, :24]).sum().backward()
+    assert torch.equal(leaf.grad, twin.grad)
